@@ -205,6 +205,22 @@ int vc_layernorm_bwd_add(int dtype, const void* x, const void* dout, const float
                          const float* rstd, const void* add, void* dx, float* dgamma, float* dbeta, int M, int C,
                          vc_stream_t stream);
 
+/* ---- group normalisation with its activation -----------------------------------------------------------
+ * No counterpart in the reference, whose encoders normalise over the batch.  x, residual (nullable), y, dy, dx,
+ * dresidual: channels-last [N][S][C] in `dtype`; any C with C % G == 0 (16-byte vectors when C is a multiple of 8 and
+ * the pointers are 16-byte aligned).  y = act((x - mean) * rstd * gamma + beta + residual) with one mean / rstd
+ * [N][G] per sample and group; gamma / beta nullable (1 / 0).  act: 0 none, 1 ReLU, 2 SiLU, 3 GELU (erf).  Backward takes
+ * the forward call's mean / rstd, writes dx and dresidual (both nullable) and ACCUMULATES dgamma / dbeta (nullable).
+ * workspace: vc_group_norm_workspace_floats() floats, 8-byte aligned, contents irrelevant before and after; every sum
+ * has a fixed order. */
+int64_t vc_group_norm_workspace_floats(int N, int S, int C, int G);
+int vc_group_norm_fwd(int dtype, const void* x, const void* residual, const float* gamma, const float* beta, void* y,
+                      float* mean, float* rstd, float* workspace, int N, int S, int C, int G, float eps, int act,
+                      vc_stream_t stream);
+int vc_group_norm_bwd(int dtype, const void* x, const void* dy, const void* residual, const float* gamma,
+                      const float* beta, const float* mean, const float* rstd, void* dx, void* dresidual, float* dgamma,
+                      float* dbeta, float* workspace, int N, int S, int C, int G, int act, vc_stream_t stream);
+
 /* ---- layout, pooling, elementwise ------------------------------------------------------------------ */
 /* x_3d[:, t] slicing + NCHW->channels-last (model_components.py:127, 176, 285, 460; Conv3D input
  * [B,1,T,H,W] from utils/common/data_loaders.py:56).  time_major: frame = t*B + b. */

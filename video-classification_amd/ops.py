@@ -9,6 +9,7 @@ into libvc_hip.  Parameter gradients are accumulated by the kernels directly int
 import os
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 
@@ -1584,6 +1585,140 @@ class _LayerNorm(torch.autograd.Function):
 def layer_norm(x, ln):
     """ln: nn.LayerNorm holding weight / bias / eps; normalises the last dimension."""
     return _LayerNorm.apply(x, ln.weight, ln.bias, ln.eps)
+
+
+# ----------------------------------------------------------------------------------------------
+# operators whose parameters never enter the autograd graph
+# ----------------------------------------------------------------------------------------------
+def _anchor(inputs, params):
+    """None, or a fresh empty leaf that makes autograd call the backward pass when only parameters need gradients.
+    Parameter gradients are written by the kernels, so the parameters themselves stay out of the graph: a leaf's
+    gradient node belongs to the stream it was made on, and one that an eager step made cannot be used in a capture."""
+    if not torch.is_grad_enabled() or any(t is not None and t.requires_grad for t in inputs):
+        return None
+    for p in params:
+        if p is not None and p.requires_grad:
+            return torch.empty(0, device=p.device, requires_grad=True)
+    return None
+
+
+def _capturing(t):
+    return t.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
+def _leaf_guard(what, *inputs):
+    """Raises when a graph capture is about to use a leaf whose gradient node a live eager graph owns: that node runs
+    on the eager stream, and the backward pass would tie this stream into the capture and end the process."""
+    if not torch.is_grad_enabled():
+        return
+    for t in inputs:
+        if t is None or not (t.requires_grad and t.is_leaf):
+            continue
+        meta = torch.autograd.graph.get_gradient_edge(t).node.metadata  # lives exactly as long as the node does
+        if not _capturing(t):
+            meta["vc_eager"] = True
+        elif meta.get("vc_eager"):
+            raise RuntimeError(f"{what}: a graph capture meets an input whose eager graph is still alive; drop the eager "
+                               "result (or its loss) first, or capture on a detached copy of the input")
+
+
+def _same_device(what, first, *rest):
+    for t in rest:
+        if t is not None and t.device != first.device:
+            raise RuntimeError(f"{what}: tensors on {first.device} and {t.device}")
+
+
+# ----------------------------------------------------------------------------------------------
+# group normalisation
+# ----------------------------------------------------------------------------------------------
+GN_ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
+
+
+def _f32_param(what, p):
+    """Detached contiguous fp32 storage of a parameter (None stays None)."""
+    if p is None:
+        return None
+    if p.dtype != torch.float32:
+        raise TypeError(f"{what}: parameters must be float32, not {p.dtype}")
+    return p.detach().contiguous()
+
+
+def _add_grad(p, g):
+    """Accumulates g into p.grad unless the kernels wrote p.grad itself."""
+    if g is not p.grad:
+        p.grad.add_(g.view(p.shape))
+
+
+def _grad_target(p):
+    """A dense fp32 tensor the kernels may accumulate p's gradient into: p.grad where it is dense, else a zeroed stand-in
+    that _add_grad folds in.  None where p needs no gradient."""
+    if p is None or not p.requires_grad:
+        return None
+    g = _grad_buf(p)
+    return g if g.is_contiguous() and g.dtype == torch.float32 else torch.zeros(p.shape, device=p.device)
+
+
+class _GroupNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, anchor, gn, act):
+        N, C, G = x.shape[0], x.shape[-1], gn.num_groups
+        S = x.numel() // (N * C)
+        x = x.contiguous()
+        res = residual.contiguous() if residual is not None else None
+        gamma, beta = _f32_param("group_norm", gn.weight), _f32_param("group_norm", gn.bias)
+        y = torch.empty_like(x)
+        stat = torch.empty(2, N, G, device=x.device, dtype=torch.float32)
+        ws = torch.empty(L.query("vc_group_norm_workspace_floats", N, S, C, G), device=x.device, dtype=torch.float32)
+        L.call("vc_group_norm_fwd", L.dtype_code(x.dtype), L.ptr(x), L.ptr(res), L.ptr(gamma), L.ptr(beta), L.ptr(y),
+               L.ptr(stat[0]), L.ptr(stat[1]), L.ptr(ws), N, S, C, G, float(gn.eps), act, L.stream())
+        ctx.dims, ctx.act, ctx.weight, ctx.bias = (N, S, C, G), act, gn.weight, gn.bias
+        ctx.save_for_backward(x, res if act else None, stat, gamma, beta)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, res, stat, gamma, beta = ctx.saved_tensors
+        N, S, C, G = ctx.dims
+        dy = cast(dy.contiguous(), x.dtype)
+        need_dx, need_dres = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        dx = torch.empty_like(x) if need_dx else None
+        # without an activation the shortcut's gradient is the incoming one
+        dres = (torch.empty_like(x) if ctx.act else dy) if need_dres else None
+        dw, db = _grad_target(ctx.weight), _grad_target(ctx.bias)
+        if need_dx or dw is not None or db is not None or (need_dres and ctx.act):
+            ws = torch.empty(L.query("vc_group_norm_workspace_floats", N, S, C, G), device=x.device, dtype=torch.float32)
+            L.call("vc_group_norm_bwd", L.dtype_code(x.dtype), L.ptr(x), L.ptr(dy), L.ptr(res), L.ptr(gamma), L.ptr(beta),
+                   L.ptr(stat[0]), L.ptr(stat[1]), L.ptr(dx), L.ptr(dres if ctx.act else None), L.ptr(dw), L.ptr(db),
+                   L.ptr(ws), N, S, C, G, ctx.act, L.stream())
+            for p, g in ((ctx.weight, dw), (ctx.bias, db)):
+                if g is not None:
+                    _add_grad(p, g)
+        _ready(ctx.weight, ctx.bias)
+        return dx, dres, None, None, None
+
+
+def group_norm(x, gn, act="none", residual=None):
+    """act(GroupNorm(x) + residual) on a channels-last map: x [N, ..., C], each sample's channels normalised in
+    ``gn.num_groups`` groups over all its positions (a frame of [F,1,H,W,C], a whole clip of [B,D,H,W,C], a row of [M,C]).
+    gn: an nn.GroupNorm holding num_groups / eps / weight / bias (its own forward is not used); act: "none", "relu",
+    "silu" or "gelu"; residual: same shape and type as x.  x is float32 or bfloat16; statistics, sums and the parameters'
+    gradients (accumulated into .grad) are float32."""
+    _require_cuda(x, "group_norm")
+    if act not in GN_ACTS:
+        raise ValueError(f"group_norm: act must be one of {sorted(GN_ACTS)}, not {act!r}")
+    L.dtype_code(x.dtype)
+    if x.dim() < 2 or x.shape[-1] != gn.num_channels:
+        raise RuntimeError(f"group_norm: input of shape {tuple(x.shape)} does not end in {gn.num_channels} channels")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise RuntimeError(f"group_norm: residual {tuple(residual.shape)} {residual.dtype} does not match the input "
+                           f"{tuple(x.shape)} {x.dtype}")
+    _same_device("group_norm", x, residual, gn.weight, gn.bias)
+    if x.numel() == 0:
+        return x.clone()
+    with torch.cuda.device(x.device):
+        _leaf_guard("group_norm", x, residual)
+        return _GroupNorm.apply(x, residual, _anchor((x, residual), (gn.weight, gn.bias)), gn, GN_ACTS[act])
 
 
 class _LayerNormFork(torch.autograd.Function):
