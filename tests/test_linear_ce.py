@@ -1,0 +1,381 @@
+"""ops.linear_cross_entropy against the definition in 64 bits, its masks and refusals.
+
+Tolerances.  A logit is a sum of K products in fp32, joined 32 at a time (a unit in the last place, 2^-23, per join and
+three joins per 32 products of two-term operands): dz = ((3K/32 + 4) 2^-23 + 2^-21) S with S = sum |x||w| + |b|; the 2^-21
+is the two-term form itself.  exp(z - lse) is then off by 2 dz + 2^-20 relative.  A gradient sums d = p - onehot over
+rows or classes: the error of p, plus the rounding of d to its terms (2^-12 or 2^-22 of the value) and the joins of that
+sum, each weighted by |W| or |x|.  The result's own type adds half a step."""
+import pytest
+import torch
+import torch.nn as nn
+
+U = 2.0 ** -24
+TYPES = {"f32": (torch.float32, torch.float32), "mixed": (torch.bfloat16, torch.float32),
+         "bf16": (torch.bfloat16, torch.bfloat16)}
+
+
+def half(dt):
+    return torch.finfo(dt).eps / 2
+
+
+def make(N, K, V, types, seed=0, bias=True, ignored=0.0, spread=2.0, dev="cuda"):
+    xd, wd = TYPES[types]
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(N, K, generator=g).to(xd)
+    w = (torch.randn(V, K, generator=g) * spread / K ** 0.5).to(xd).to(wd)
+    b = torch.randn(V, generator=g).to(wd) if bias else None
+    t = torch.randint(0, V, (N,), generator=g)
+    if ignored:
+        t[torch.rand(N, generator=g) < ignored] = -100
+    par = lambda p: nn.Parameter(p.to(dev)) if p is not None else None
+    return x.to(dev), par(w), par(b), t.to(dev)
+
+
+def reference(x, w, b, t, eps, weight):
+    """Row losses, gradients for the row weights `weight`, and error bounds, all in float64 on the tensors' device."""
+    x, w = x.detach().double(), w.detach().double()
+    bias = b.detach().double() if b is not None else torch.zeros(w.shape[0], device=x.device, dtype=torch.float64)
+    N, K, V = x.shape[0], x.shape[1], w.shape[0]
+    keep = t != -100
+    x = torch.where(keep[:, None], x, torch.zeros_like(x))
+    z = x @ w.t() + bias
+    lse = torch.logsumexp(z, dim=1)
+    tt = torch.where(keep, t, torch.zeros_like(t))
+    rows = lse - (1 - eps) * z.gather(1, tt[:, None])[:, 0]
+    if eps:
+        rows = rows - eps * z.mean(1)
+    rows = torch.where(keep, rows, torch.zeros_like(rows))
+    p = torch.exp(z - lse[:, None])
+    d = p - eps / V
+    d[torch.arange(N, device=x.device), tt] -= 1 - eps
+    r = torch.where(keep, weight.double(), torch.zeros_like(rows))
+    d, p = d * r[:, None], p * r.abs()[:, None]
+    S = x.abs() @ w.abs().t() + bias.abs().clamp_max(1e30)
+    dz = ((3 * K / 32 + 4) * 2.0 ** -23 + 2.0 ** -21) * float(S.max())
+    return dict(rows=rows, lse=lse, z=z, d=d, p=p, dz=dz, dx=d @ w, dw=d.t() @ x, db=d.sum(0), x=x, w=w)
+
+
+def check(ref, types, rows=None, dx=None, dw=None, db=None, extra=0.0):
+    xd, wd = TYPES[types]
+    dz = ref["dz"] + extra
+    N, V = ref["d"].shape
+    if rows is not None:
+        err = (rows.double() - ref["rows"]).abs()
+        assert (err <= 4 * dz + 2.0 ** -20 * (1 + ref["lse"].abs().clamp_max(1e30))).all(), float(err.max())
+    ep = 2 * dz + 2.0 ** -20
+    for got, want, A, P, M, dt, length in ((dx, ref["dx"], ref["d"].abs(), ref["p"], ref["w"].abs(), xd, V),
+                                           (dw, ref["dw"], ref["d"].abs().t(), ref["p"].t(), ref["x"].abs(), wd, N)):
+        if got is None:
+            continue
+        term = 2.0 ** -22 if dt == torch.float32 else 2.0 ** -12
+        tol = (term + 2.0 ** -21 + (3 * length / 32 + 8) * 2.0 ** -23) * (A @ M) + ep * (P @ M)
+        if got is dx and extra:
+            tol = tol + 2.0 ** -12 * (A @ M)  # the weight's own single term
+        err = (got.double() - want).abs()
+        assert (err <= tol + half(dt) * want.abs() + 1e-37).all(), float((err - tol - half(dt) * want.abs()).max())
+    if db is not None:
+        tol = ep * ref["p"].sum(0) + (N / 16 + 16) * U * ref["d"].abs().sum(0)
+        err = (db.double() - ref["db"]).abs()
+        assert (err <= tol + half(wd) * ref["db"].abs() + 1e-37).all(), float((err - tol).max())
+
+
+SHAPES = [(1, 8, 2), (1, 1, 1), (3, 5, 7), (32, 256, 101), (130, 64, 129), (257, 100, 300), (64, 72, 2001), (1000, 40, 130),
+          (128, 128, 128), (129, 65, 1), (5, 520, 4099), (700, 33, 1025)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("types", list(TYPES))
+@pytest.mark.parametrize("bias,eps,ignored", [(True, 0.0, 0.0), (False, 0.1, 0.3)])
+@pytest.mark.parametrize("N,K,V", SHAPES)
+def test_mean(cuda, types, bias, eps, ignored, N, K, V):
+    from video_classification_amd import ops
+    x, w, b, t = make(N, K, V, types, bias=bias, ignored=ignored)
+    xg = x.clone().requires_grad_(True)
+    stats = {}
+    loss = ops.linear_cross_entropy(xg, w, b, t, label_smoothing=eps, stats=stats)
+    loss.backward()
+    count = max(1, int((t != -100).sum()))
+    ref = reference(x, w, b, t, eps, torch.full((N,), 1.0 / count, device=x.device))
+    want = float(ref["rows"].sum() / count)
+    assert abs(loss.item() - want) <= 4 * ref["dz"] + 2.0 ** -20 * (1 + float(ref["lse"].abs().max()))
+    check(ref, types, None, xg.grad, w.grad, b.grad if bias else None)
+    assert xg.grad.dtype == x.dtype and w.grad.dtype == w.dtype
+    assert (xg.grad[t == -100] == 0).all()
+    top = ref["z"].max(1).values
+    picked = ref["z"].gather(1, stats["pred"][:, None])[:, 0]
+    assert (top - picked <= 2 * ref["dz"]).all()
+    assert int(stats["correct"]) == int(((stats["pred"] == t) & (t != -100)).sum())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("types", list(TYPES))
+def test_rows_and_sum(cuda, types):
+    from video_classification_amd import ops
+    x, w, b, t = make(150, 96, 333, types, ignored=0.2)
+    g = torch.randn(150, generator=torch.Generator().manual_seed(5)).cuda() * 3e-3
+    xg = x.clone().requires_grad_(True)
+    rows = ops.linear_cross_entropy(xg, w, b, t, reduction="none")
+    assert rows.shape == (150,) and (rows[t == -100] == 0).all()
+    rows.backward(g)
+    ref = reference(x, w, b, t, 0.0, g)
+    check(ref, types, rows.detach(), xg.grad, w.grad, b.grad)
+    w.grad = b.grad = xg.grad = None
+    loss = ops.linear_cross_entropy(xg.view(10, 15, 96), w, b, t.view(10, 15), reduction="sum")
+    (loss * 0.25).backward()
+    ref = reference(x, w, b, t, 0.0, torch.full((150,), 0.25, device=x.device))
+    assert abs(loss.item() - float(ref["rows"].sum())) <= 150 * (4 * ref["dz"] + 2.0 ** -20 * (1 + float(ref["lse"].abs().max())))
+    check(ref, types, None, xg.grad, w.grad, b.grad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("types,N,K,V", [("bf16", 4096, 64, 13001), ("mixed", 3000, 48, 13000), ("f32", 2000, 40, 13100)])
+def test_pieces_of_the_classes(cuda, types, N, K, V):
+    from video_classification_amd import ops
+    x, w, b, t = make(N, K, V, types)
+    xg = x.clone().requires_grad_(True)
+    loss = ops.linear_cross_entropy(xg, w, b, t)
+    loss.backward()
+    ref = reference(x, w, b, t, 0.0, torch.full((N,), 1.0 / N, device=x.device))
+    assert abs(loss.item() - float(ref["rows"].mean())) <= 4 * ref["dz"] + 2.0 ** -20 * (1 + float(ref["lse"].abs().max()))
+    check(ref, types, None, xg.grad, w.grad, b.grad)
+
+
+@pytest.mark.gpu
+def test_master_weights_beyond_bf16(cuda):
+    """bf16 rows against fp32 weights that bf16 cannot hold: the weight's single fp16 term is off by 2^-12 of the value."""
+    from video_classification_amd import ops
+    x, w, b, t = make(200, 128, 500, "mixed")
+    with torch.no_grad():
+        w.mul_(1.2345)
+    xg = x.clone().requires_grad_(True)
+    ops.linear_cross_entropy(xg, w, b, t, reduction="sum").backward()
+    ref = reference(x, w, b, t, 0.0, torch.ones(200, device=x.device))
+    check(ref, "mixed", None, xg.grad, w.grad, b.grad, extra=2.0 ** -12 * float((ref["x"].abs() @ ref["w"].abs().t()).max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("types", list(TYPES))
+@pytest.mark.parametrize("xs,ws", [(1e-6, 1e3), (1e8, 1e-9), (1e-20, 1e20)])
+def test_magnitudes(cuda, types, xs, ws):
+    """Operands far from 1: the scales follow their magnitudes."""
+    from video_classification_amd import ops
+    x, w, b, t = make(70, 64, 150, types)
+    x = (x.float() * xs).to(x.dtype)
+    with torch.no_grad():
+        w.copy_((w.float() * ws).to(TYPES[types][0]).to(w.dtype))
+    xg = x.clone().requires_grad_(True)
+    ops.linear_cross_entropy(xg, w, b, t).backward()
+    ref = reference(x, w, b, t, 0.0, torch.full((70,), 1 / 70, device=x.device))
+    check(ref, types, None, xg.grad, w.grad, b.grad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("types", list(TYPES))
+def test_ignored_rows_may_hold_anything(cuda, types):
+    from video_classification_amd import ops
+    x, w, b, t = make(200, 64, 150, types, ignored=0.4)
+    bad = x.clone()
+    drop = (t == -100).nonzero()[:, 0]
+    bad[drop[0]], bad[drop[1]], bad[drop[2]] = float("nan"), float("inf"), torch.finfo(x.dtype).min
+    outs = []
+    for src in (x, bad):
+        w.grad = b.grad = None
+        xg = src.clone().requires_grad_(True)
+        loss = ops.linear_cross_entropy(xg, w, b, t, label_smoothing=0.1)
+        loss.backward()
+        outs.append((loss.detach(), xg.grad, w.grad, b.grad))
+    for a, c in zip(*outs):
+        assert torch.isfinite(a).all() and torch.equal(a, c)
+    # nothing counts: loss 0, gradients 0
+    w.grad = b.grad = None
+    xg = bad.clone().requires_grad_(True)
+    loss = ops.linear_cross_entropy(xg, w, b, torch.full_like(t, -100))
+    loss.backward()
+    assert loss.item() == 0 and not xg.grad.any() and not w.grad.any() and not b.grad.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("types", list(TYPES))
+@pytest.mark.parametrize("low", [float("-inf"), "lowest"])
+def test_classes_masked_by_the_bias(cuda, types, low):
+    from video_classification_amd import ops
+    x, w, b, t = make(150, 64, 400, types)
+    low = float(torch.finfo(b.dtype).min) if low == "lowest" else low
+    with torch.no_grad():
+        b[128:300] = low
+    t = torch.where((t >= 128) & (t < 300), t % 128, t)  # targets are live classes
+    xg = x.clone().requires_grad_(True)
+    rows = ops.linear_cross_entropy(xg, w, b, t, reduction="none")
+    rows.sum().backward()
+    live = torch.cat([torch.arange(128), torch.arange(300, 400)]).cuda()
+    tl = torch.where(t >= 300, t - 172, t)
+    ref = reference(x, w[live], b[live], tl, 0.0, torch.ones(150, device=x.device))
+    check(ref, types, rows.detach(), xg.grad, w.grad[live], b.grad[live])
+    assert not w.grad[128:300].any() and not b.grad[128:300].any()
+
+
+@pytest.mark.gpu
+def test_bad_values_show(cuda):
+    """A target outside the classes and a NaN in a row that counts make the loss NaN and touch nothing out of bounds."""
+    from video_classification_amd import ops
+    x, w, b, t = make(64, 32, 40, "f32")
+    for v in (40, -1, 2 ** 40, -2 ** 40):
+        bad = t.clone()
+        bad[5] = v
+        rows = ops.linear_cross_entropy(x, w, b, bad, reduction="none")
+        assert torch.isnan(rows[5]) and torch.isfinite(rows[:5]).all() and torch.isfinite(rows[6:]).all()
+        xg = x.clone().requires_grad_(True)
+        ops.linear_cross_entropy(xg, w, b, bad).backward()
+        assert torch.isnan(xg.grad[5]).all() and torch.isfinite(xg.grad[6:]).all()
+    x[7, 3] = float("nan")
+    rows = ops.linear_cross_entropy(x, w, b, t, reduction="none")
+    assert torch.isnan(rows[7]) and torch.isfinite(rows[:7]).all() and torch.isfinite(rows[8:]).all()
+
+
+@pytest.mark.gpu
+def test_gradient_against_differences(cuda):
+    from video_classification_amd import ops
+    x, w, b, t = make(40, 24, 60, "f32", ignored=0.2)
+    g = torch.Generator().manual_seed(1)
+    vx, vw, vb = (torch.randn(s.shape, generator=g).cuda().double() for s in (x, w, b))
+    one = torch.ones(40, device=x.device)
+    f = lambda h: reference_sum(x.double() + h * vx, w.detach().double() + h * vw, b.detach().double() + h * vb, t)
+    h = 1e-5
+    want = (f(h) - f(-h)) / (2 * h)
+    xg = x.clone().requires_grad_(True)
+    ops.linear_cross_entropy(xg, w, b, t, label_smoothing=0.1, reduction="sum").backward()
+    parts = [(xg.grad.double() * vx).sum(), (w.grad.double() * vw).sum(), (b.grad.double() * vb).sum()]
+    scale = sum(float((p.grad.double() * v).abs().sum()) for p, v in ((xg, vx), (w, vw), (b, vb)))
+    assert abs(float(sum(parts)) - want) <= 1e-5 * scale and one.numel() == 40
+
+
+def reference_sum(x, w, b, t, eps=0.1):
+    return float(reference(x, w, b, t, eps, torch.ones(x.shape[0], device=x.device))["rows"].sum())
+
+
+@pytest.mark.gpu
+def test_views_accumulation_repeatability_and_stream(cuda):
+    from video_classification_amd import ops
+    x, w, b, t = make(100, 64, 300, "mixed")
+    want = ops.linear_cross_entropy(x, w, b, t).detach()
+    wide = torch.zeros(100, 130, device=cuda, dtype=x.dtype)
+    wide[:, 1:65] = x
+    assert torch.equal(ops.linear_cross_entropy(wide[:, 1:65], w, b, t).detach(), want)
+    wt = w.detach().t().contiguous().t()
+    assert not wt.is_contiguous() and torch.equal(ops.linear_cross_entropy(x, wt, b, t), want)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        other = ops.linear_cross_entropy(x, w, b, t).detach()
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(other, want)
+    ops.linear_cross_entropy(x, w, b, t).backward()  # x needs no gradient: only the parameters'
+    once = w.grad.clone(), b.grad.clone()
+    ops.linear_cross_entropy(x, w, b, t).backward()
+    assert torch.equal(w.grad, 2 * once[0]) and torch.equal(b.grad, 2 * once[1])
+    # agrees with the operators it stands in for (a linear layer in bf16 and the loss of its logits)
+    lin = nn.Linear(64, 300).cuda()
+    with torch.no_grad():
+        lin.weight.copy_(w)
+        lin.bias.copy_(b)
+    z = ops.linear(x, lin.weight, lin.bias, out_f32=True)[:, :300]
+    assert abs(ops.cross_entropy(z, t).item() - want.item()) < 1e-3
+
+
+@pytest.mark.gpu
+def test_captured_step_replays(cuda):
+    from video_classification_amd import ops
+    x, w, b, t = make(300, 96, 500, "mixed", ignored=0.1)
+    w.grad, b.grad = torch.zeros_like(w), torch.zeros_like(b)
+
+    def step():
+        w.grad.zero_()
+        b.grad.zero_()
+        xi = x.detach().requires_grad_(True)
+        loss = ops.linear_cross_entropy(xi, w, b, t)
+        return [loss.detach(), torch.autograd.grad(loss, xi)[0]]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for k in range(3):
+        nx, _, _, nt = make(300, 96, 500, "mixed", ignored=0.3 * k, seed=20 + k)
+        x.copy_(nx)
+        t.copy_(nt)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [v.clone() for v in out] + [w.grad.clone(), b.grad.clone()]
+        want = step() + [w.grad.clone(), b.grad.clone()]
+        for a, c in zip(got, want):
+            assert torch.equal(a, c)
+
+
+@pytest.mark.gpu
+def test_refusals(cuda):
+    from video_classification_amd import ops
+    x, w, b, t = make(6, 16, 20, "f32")
+    ce = ops.linear_cross_entropy
+    with pytest.raises(TypeError, match="float32 weights"):
+        ce(x, w.detach().bfloat16(), None, t)
+    with pytest.raises(TypeError):
+        ce(x.half(), w, b, t)
+    with pytest.raises(RuntimeError, match="bias"):
+        ce(x, w, b[:5], t)
+    with pytest.raises(RuntimeError, match="bias"):
+        ce(x, w, b.detach().bfloat16(), t)
+    with pytest.raises(RuntimeError, match="rows"):
+        ce(x[:, :8], w, b, t)
+    with pytest.raises(RuntimeError, match="target"):
+        ce(x, w, b, t[:5])
+    with pytest.raises(RuntimeError, match="target"):
+        ce(x, w, b, t.int())
+    with pytest.raises(ValueError, match="label_smoothing"):
+        ce(x, w, b, t, label_smoothing=1.5)
+    with pytest.raises(ValueError, match="reduction"):
+        ce(x, w, b, t, reduction="max")
+    with pytest.raises(RuntimeError, match="tensors on"):
+        ce(x, w, b, t.cpu())
+    xe = x[:0].requires_grad_(True)
+    empty = ce(xe, w, b, t[:0])
+    assert empty.item() == 0
+    empty.backward()
+    assert xe.grad.shape == (0, 16) and w.grad is None
+
+
+def test_refuses_cpu_and_bad_abi_arguments():
+    from video_classification_amd import _lib as L
+    from video_classification_amd import ops
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        ops.linear_cross_entropy(torch.zeros(2, 8), torch.zeros(4, 8), None, torch.zeros(2, dtype=torch.int64))
+    assert L.query("vc_linear_ce_bytes", 0, 1, 1, 0, 4, 8) == -1
+    assert L.query("vc_linear_ce_bytes", 0, 0, 1, 2, 4, 8) == -1
+    assert L.query("vc_linear_ce_bytes", 3, 1, 1, 2, 4, 8) == -1
+    for what in (0, 1, 2):
+        assert L.query("vc_linear_ce_bytes", what, 1, 0, 2, 4, 8) > 0
+    null = L.ptr(None)
+
+    def fwd(xd, wd, n, v, k, smooth=0.0):
+        L.call("vc_linear_ce_fwd", xd, wd, null, null, null, null, L.i64(-100), float(smooth), 1, null, null, null, null, null,
+               null, n, v, k, null)
+
+    for args, code in (((0, 1, 2, 4, 8), -4), ((5, 1, 2, 4, 8), -2), ((1, 1, 0, 4, 8), -1), ((1, 1, 2, 4, 1 << 21), -1),
+                       ((1, 1, 2, 4, 8), -4), ((1, 1, 2, 4, 8, 2.0), -4)):
+        with pytest.raises(RuntimeError, match=f"status {code}"):
+            fwd(*args)
+
+
+def test_plan_covers_every_size():
+    """Workspace sizes are positive and grow with the sizes (the pieces keep the gradient buffers bounded)."""
+    from video_classification_amd import _lib as L
+    for n, v, k in ((1, 1, 1), (16384, 65536, 2048), (4096, 13001, 64), (1 << 22, 7, 8), (3, 1 << 22, 8)):
+        sizes = [L.query("vc_linear_ce_bytes", what, 1, 1, n, v, k) for what in (0, 1, 2)]
+        assert all(s > 0 for s in sizes)
+        assert sizes[0] >= 2 * (n + v) * k
+    small = L.query("vc_linear_ce_bytes", 2, 1, 1, 8192, 65536, 64)
+    assert small < (8192 + 65536) * 64 * 2 + (400 << 20)

@@ -77,7 +77,7 @@ def query(name, *args):
     """Call an entry point that returns a value (not a status code); ints are passed as C int."""
     fn = getattr(lib(), name)
     if name in ("vc_lstm_persist_xchg_bytes", "vc_lstm_persist_bwd_xchg_bytes", "vc_cbam_workspace_floats",
-                "vc_group_norm_workspace_floats"):
+                "vc_group_norm_workspace_floats", "vc_linear_ce_bytes"):
         fn.restype = ctypes.c_longlong
     return fn(*[ctypes.c_int(int(a)) if isinstance(a, (bool, int)) else a for a in args])
 

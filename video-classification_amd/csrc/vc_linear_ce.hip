@@ -1,0 +1,801 @@
+// Softmax cross entropy of a linear classifier, z = x W^T + b over V classes, without the logit matrix: forward keeps a
+// running maximum and sum per row and tile of classes, backward recomputes the logits of a piece of the classes at a time.
+//
+//   lse_n = log sum_v exp(z_nv),  loss_n = lse_n - (1 - eps) z_{n,t_n} - eps / V sum_v z_nv
+//   d_nv = (exp(z_nv - lse_n) - (1 - eps) [v = t_n] - eps / V) r_n          (r_n the row's weight in the loss)
+//   dx = d W,  dW += d^T x,  db += sum_n d
+// Rows whose target is ignore_index have r_n = 0 and are read as zeros, whatever they hold.
+//
+// 2 N V K operations forward, 6 N V K backward (the logits once more, dx, dW): bound by the matrix pipes for the sizes where
+// time matters, which is why the logits are recomputed rather than kept: N x V fp32 logits written and read cost as much
+// as the product at K = 1024 and gigabytes of memory.
+//
+// All products run on fp16 terms (vc_gemm16.h).  x and W are scaled by one power of two each (from their largest finite
+// magnitude): bf16 values are exact in one term over 29 binades and within 2^-40 of the largest magnitude below that, fp32
+// values take two terms (22 bits).  An fp32 master weight next to bf16 activations takes one term (11 bits, against the
+// 8 of a bf16 copy).  d is at most 1 in magnitude and is scaled by 2^15: one term (2^-12 of the value) where the gradient
+// it makes is bf16, two where it is fp32.
+#include "vc_gemm16.h"
+
+namespace {
+
+constexpr int AMAX_BLOCKS = 256;  // partial maxima per operand
+
+// ---- scales ----------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float finite_mag(float v) {
+  const float a = fabsf(v);
+  return a <= 3.4028235e38f ? a : 0.f;  // NaN and infinities do not set the scale
+}
+
+template <typename T>
+__device__ __forceinline__ float amax_part(const T* p, int64_t rows, int K, const int64_t* target, int64_t ignore, int block,
+                                           int nblocks) {
+  float m = 0.f;
+  if (!target) {
+    const int64_t total = rows * K, head = ((uintptr_t)p & 15) ? 0 : total / 8 * 8;
+    for (int64_t i = ((int64_t)block * 256 + threadIdx.x) * 8; i < head; i += (int64_t)nblocks * 256 * 8) {
+      const F8 v = load8(p + i);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m = fmaxf(m, finite_mag(v.v[e]));
+    }
+    for (int64_t i = head + (int64_t)block * 256 + threadIdx.x; i < total; i += (int64_t)nblocks * 256)
+      m = fmaxf(m, finite_mag(to_f32(p[i])));
+  } else {
+    for (int64_t r = block * 4 + (threadIdx.x >> 6); r < rows; r += nblocks * 4) {
+      if (target[r] == ignore) continue;
+      for (int k = threadIdx.x & 63; k < K; k += 64) m = fmaxf(m, finite_mag(to_f32(p[r * K + k])));
+    }
+  }
+  return m;
+}
+
+// amax[0 .. 255] / [256 .. 511] = largest finite magnitudes met by the blocks of x / W
+template <typename TX, typename TW>
+__global__ __launch_bounds__(256) void ce_amax_kernel(const TX* __restrict__ x, const TW* __restrict__ w, int N, int V,
+                                                      int K, const int64_t* __restrict__ target, int64_t ignore,
+                                                      float* __restrict__ amax) {
+  __shared__ float sm[4];
+  const int b = blockIdx.x & (AMAX_BLOCKS - 1);
+  float m = blockIdx.x < AMAX_BLOCKS ? amax_part(x, N, K, target, ignore, b, AMAX_BLOCKS)
+                                     : amax_part(w, V, K, (const int64_t*)nullptr, 0, b, AMAX_BLOCKS);
+  m = wave_max(m);
+  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) amax[blockIdx.x] = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+}
+
+// exponent e with 2^14 <= amax 2^e < 2^15 (0 for an operand without a finite value other than zero)
+__device__ __forceinline__ int scale_exp(const float* amax, float* sm) {
+  float m = wave_max(amax[threadIdx.x & (AMAX_BLOCKS - 1)]);
+  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  return m > 0.f ? 14 - ilogbf(m) : 0;
+}
+
+// ---- packing -----------------------------------------------------------------------------------------------------
+// dst[plane][row][ld] = terms of src[row][k] 2^e, zeros behind K; ignored rows are zeros.  A wave per row and 512 columns.
+template <typename T>
+__device__ __forceinline__ void pack_rows(const T* __restrict__ src, f16* __restrict__ dst, int64_t plane, int rows, int K,
+                                          int ld, int planes, int e, const int64_t* target, int64_t ignore, int64_t unit) {
+  const int per = (ld + 511) / 512;
+  const int64_t row = unit / per;
+  if (row >= rows) return;
+  const int c0 = (int)(unit - row * per) * 512 + (threadIdx.x & 63) * 8;
+  if (c0 >= ld) return;
+  const bool drop = target && target[row] == ignore;
+  const T* s = src + row * K;
+  float v[8];
+  if (!drop && c0 + 8 <= K && ((uintptr_t)(s + c0) & 15) == 0) {
+    const F8 t = load8(s + c0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = t.v[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = !drop && c0 + i < K ? to_f32(s[c0 + i]) : 0.f;
+  }
+  f16x8 hi, lo;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    f16 h, l;
+    f16_split(ldexpf(v[i], e), h, l);
+    hi[i] = h;
+    lo[i] = l;
+  }
+  *reinterpret_cast<f16x8*>(dst + row * ld + c0) = hi;
+  if (planes == 2) *reinterpret_cast<f16x8*>(dst + plane + row * ld + c0) = lo;
+}
+
+// exps[0] / [1] = scale exponents of x / W; the first `xblocks` workgroups pack x, the others W
+template <typename TX, typename TW>
+__global__ __launch_bounds__(256) void ce_pack_kernel(const TX* __restrict__ x, const TW* __restrict__ w, int N, int V,
+                                                      int K, int ld, int px, int pw, const int64_t* __restrict__ target,
+                                                      int64_t ignore, const float* __restrict__ amax, f16* __restrict__ xp,
+                                                      f16* __restrict__ wp, int* __restrict__ exps, int xblocks) {
+  __shared__ float sm[4];
+  const bool isx = (int)blockIdx.x < xblocks;
+  const int e = scale_exp(isx ? amax : amax + AMAX_BLOCKS, sm);
+  if (threadIdx.x == 0 && ((int)blockIdx.x == 0 || (int)blockIdx.x == xblocks)) exps[isx ? 0 : 1] = e;
+  const int64_t unit = (int64_t)(isx ? blockIdx.x : blockIdx.x - xblocks) * 4 + (threadIdx.x >> 6);
+  if (isx) pack_rows(x, xp, (int64_t)N * ld, N, K, ld, px, e, target, ignore, unit);
+  else pack_rows(w, wp, (int64_t)V * ld, V, K, ld, pw, e, (const int64_t*)nullptr, 0, unit);
+}
+
+// dst[c][ldd] = src[r][c] for both operands and all planes: 64 x 64 tiles through LDS, zeros behind the last row
+struct TransArgs {
+  const f16* src[2];
+  f16* dst[2];
+  int rows[2], lds[2], ldd[2], planes[2], tiles[2];  // tiles of one plane
+  int cols;
+};
+__global__ __launch_bounds__(256) void ce_transpose_kernel(TransArgs t) {
+  __shared__ f16 sm[64][72];
+  int id = blockIdx.x;
+  const int which = id < t.tiles[0] * t.planes[0] ? 0 : 1;
+  if (which) id -= t.tiles[0] * t.planes[0];
+  const int plane = id / t.tiles[which];
+  id -= plane * t.tiles[which];
+  const int rows = t.rows[which], lds = t.lds[which], ldd = t.ldd[which];
+  const int tc = lds / 64, r0 = id / tc * 64, c0 = id % tc * 64;
+  const f16* s = t.src[which] + (int64_t)plane * rows * lds;
+  f16* d = t.dst[which] + (int64_t)plane * t.cols * ldd;
+  for (int i = threadIdx.x; i < 512; i += 256) {
+    const int r = i >> 3, c = (i & 7) * 8;
+    f16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (r0 + r < rows) v = *reinterpret_cast<const f16x8*>(s + (int64_t)(r0 + r) * lds + c0 + c);
+    *reinterpret_cast<f16x8*>(&sm[r][c]) = v;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 512; i += 256) {
+    const int c = i >> 3, r = (i & 7) * 8;
+    if (c0 + c >= t.cols) continue;
+    f16x8 v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = sm[r + e][c];
+    *reinterpret_cast<f16x8*>(d + (int64_t)(c0 + c) * ldd + r0 + r) = v;
+  }
+}
+
+// ---- forward: statistics of a 128-class tile ---------------------------------------------------------------------
+struct Stat {
+  float m, s, z;  // running maximum, sum of exp(z - m), sum of z
+  int arg;        // lowest class that attains m
+};
+__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * 1.4426950408889634f); }
+__device__ __forceinline__ void stat_join(Stat& a, const Stat& b) {
+  if (b.m > a.m || (b.m == a.m && b.arg < a.arg)) a.arg = b.arg;
+  const float m = fmaxf(a.m, b.m);
+  const float ref = m == -INFINITY ? 0.f : m;  // nothing but -inf so far: exp(-inf - 0) = 0
+  a.s = a.s * exp_of(a.m - ref) + b.s * exp_of(b.m - ref);
+  a.m = m;
+  a.z += b.z;
+}
+__device__ __forceinline__ Stat stat_shfl(const Stat& a, int o) {
+  return Stat{__shfl_xor(a.m, o, 64), __shfl_xor(a.s, o, 64), __shfl_xor(a.z, o, 64), __shfl_xor(a.arg, o, 64)};
+}
+
+struct CeArgs {
+  const f16* w;      // [pw][V][ld]
+  const f16* x;      // [px][N][ld]
+  const void* bias;  // nullable, float or bf16
+  const int64_t* target;
+  const int* exps;
+  int N, V, ld, bias_bf16;
+  int tiles_v, tiles_n;
+};
+
+// logits of the tile from the accumulators: z = acc 2^-(ex + ew) + bias, -inf behind the last class
+__device__ __forceinline__ void tile_bias(const CeArgs& a, int v0, float (&bias)[4][4]) {
+  const int lane = threadIdx.x & 63, q = lane >> 4, wm = threadIdx.x >> 7;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int v = v0 + wm * 64 + i * 16 + q * 4 + r;
+      float b = 0.f;
+      if (v >= a.V) b = -INFINITY;
+      else if (a.bias) b = a.bias_bf16 ? (float)((const bf16*)a.bias)[v] : ((const float*)a.bias)[v];
+      bias[i][r] = b;
+    }
+}
+
+// part[vt][n] = (max, sum, sum z, arg) of the tile, zt[n] = the target's logit
+template <int PW, int PX>
+__global__ __launch_bounds__(G_THREADS, 2) void ce_stats_kernel(CeArgs a, float4* __restrict__ part,
+                                                                float* __restrict__ zt) {
+  typedef G16<PW, PX> G;
+  __shared__ __attribute__((aligned(1024))) f16 smem[G::LDS];
+  int tv, tn;
+  g16_tile(blockIdx.x, gridDim.x, a.tiles_v, a.tiles_n, tv, tn);
+  const int v0 = tv * GM, n0 = tn * GM;
+  f32x4 acc[4][4];
+  G::zero(acc);
+  G::run(acc, a.w + (int64_t)v0 * a.ld, (int64_t)a.V * a.ld, a.ld, a.V - v0, a.x + (int64_t)n0 * a.ld,
+         (int64_t)a.N * a.ld, a.ld, a.N - n0, 0, a.ld, smem);
+  const int lane = threadIdx.x & 63, q = lane >> 4, l15 = lane & 15;
+  const int wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
+  const int es = -(a.exps[0] + a.exps[1]);
+  float bias[4][4];
+  tile_bias(a, v0, bias);
+  float4* xch = reinterpret_cast<float4*>(smem);
+  Stat st[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int n = n0 + wn * 64 + j * 16 + l15;
+    const int t = n < a.N ? (int)min(max(a.target[n], (int64_t)-1), (int64_t)a.V) : -1;
+    Stat s{-INFINITY, 0.f, 0.f, a.V};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int v = v0 + wm * 64 + i * 16 + q * 4 + r;
+        const float z = ldexpf(acc[i][j][r], es) + bias[i][r];
+        acc[i][j][r] = z;
+        if (z > s.m) {
+          s.m = z;
+          s.arg = v;
+        }
+        if (v < a.V) s.z += z;
+        if (v == t) zt[n] = z;
+      }
+    const float ref = s.m == -INFINITY ? 0.f : s.m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s.s += exp_of(acc[i][j][r] - ref);
+    stat_join(s, stat_shfl(s, 16));
+    stat_join(s, stat_shfl(s, 32));
+    st[j] = s;
+    if (wm == 1 && q == 0) xch[wn * 64 + j * 16 + l15] = make_float4(s.m, s.s, s.z, __int_as_float(s.arg));
+  }
+  __syncthreads();
+  if (wm == 0 && q == 0)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = wn * 64 + j * 16 + l15;
+      const float4 o = xch[c];
+      stat_join(st[j], Stat{o.x, o.y, o.z, __float_as_int(o.w)});
+      if (n0 + c < a.N)
+        part[(int64_t)tv * a.N + n0 + c] = make_float4(st[j].m, st[j].s, st[j].z, __int_as_float(st[j].arg));
+    }
+}
+
+// Per row: lse, loss (0 for ignored rows, NaN for a target outside [0, V)), arg-max.  32 rows x 8 runs of tiles per block.
+__global__ __launch_bounds__(256) void ce_join_kernel(const float4* __restrict__ part, const float* __restrict__ zt,
+                                                      const int64_t* __restrict__ target, int64_t ignore, int N, int V,
+                                                      int tiles_v, float smooth, float* __restrict__ lse,
+                                                      float* __restrict__ rowloss, int64_t* __restrict__ pred) {
+  __shared__ Stat sm[8][32];
+  const int e = threadIdx.x & 31, run = threadIdx.x >> 5;
+  const int n = blockIdx.x * 32 + e;
+  Stat s{-INFINITY, 0.f, 0.f, V};
+  if (n < N) {
+    const int per = (tiles_v + 7) / 8, t1 = min(tiles_v, (run + 1) * per);
+#pragma unroll 4
+    for (int t = run * per; t < t1; ++t) {
+      const float4 o = part[(int64_t)t * N + n];
+      stat_join(s, Stat{o.x, o.y, o.z, __float_as_int(o.w)});
+    }
+  }
+  sm[run][e] = s;
+  __syncthreads();
+  if (run == 0 && n < N) {
+#pragma unroll
+    for (int r = 1; r < 8; ++r) stat_join(s, sm[r][e]);
+    const float l = (s.m == -INFINITY ? 0.f : s.m) + logf(s.s);
+    lse[n] = l;
+    const int64_t t = target[n];
+    float loss = 0.f;
+    if (t != ignore) {
+      if (t < 0 || t >= V) loss = NAN;
+      else {
+        const float d = l - zt[n];
+        loss = smooth > 0.f ? (1.f - smooth) * d + smooth * (l - s.z / (float)V) : d;
+      }
+    }
+    rowloss[n] = loss;
+    if (pred) pred[n] = s.arg < V ? s.arg : 0;
+  }
+}
+
+// loss (nullable) = sum of the row losses (mean: divided by the counted rows, or by 1 if there are none), total[0] = that
+// count; correct (nullable) = counted rows whose arg-max is the target.  One block.
+__global__ __launch_bounds__(1024) void ce_total_kernel(const float* __restrict__ rowloss, const int64_t* __restrict__ target,
+                                                        const int64_t* __restrict__ pred, int64_t ignore, int N, int mean,
+                                                        float* __restrict__ loss, float* __restrict__ total,
+                                                        int* __restrict__ correct) {
+  __shared__ double sd[16];
+  __shared__ int sc[16], sk[16];
+  double a = 0.0;
+  int c = 0, k = 0;
+  for (int n = threadIdx.x; n < N; n += 1024) {
+    const int64_t t = target[n];
+    if (t != ignore) {
+      a += (double)rowloss[n];
+      ++c;
+      if (pred && pred[n] == t) ++k;
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    a += __shfl_xor(a, o, 64);
+    c += __shfl_xor(c, o, 64);
+    k += __shfl_xor(k, o, 64);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    sd[threadIdx.x >> 6] = a;
+    sc[threadIdx.x >> 6] = c;
+    sk[threadIdx.x >> 6] = k;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 16; ++i) {
+      a += sd[i];
+      c += sc[i];
+      k += sk[i];
+    }
+    if (loss) *loss = (float)(mean ? a / (double)max(c, 1) : a);
+    total[0] = (float)c;
+    if (correct) *correct = k;
+  }
+}
+
+// ---- backward ------------------------------------------------------------------------------------------------------
+// rs[n] = weight of row n relative to the largest one (0 for ignored rows), fac[0] = that largest weight.
+// per_row: g[N], else g[0] (divided by the counted rows for the mean).
+__global__ __launch_bounds__(1024) void ce_weights_kernel(const float* __restrict__ g, const float* __restrict__ total,
+                                                          const int64_t* __restrict__ target, int64_t ignore, int N,
+                                                          int mean, int per_row, float* __restrict__ rs,
+                                                          float* __restrict__ fac) {
+  __shared__ float sm[16];
+  float big = 1.f;
+  if (per_row) {
+    big = 0.f;
+    for (int n = threadIdx.x; n < N; n += 1024)
+      if (target[n] != ignore) big = fmaxf(big, finite_mag(g[n]));
+    big = wave_max(big);
+    if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = big;
+    __syncthreads();
+    big = sm[0];
+    for (int i = 1; i < 16; ++i) big = fmaxf(big, sm[i]);
+    if (!(big > 0.f)) big = 1.f;
+  }
+  for (int n = threadIdx.x; n < N; n += 1024) rs[n] = target[n] == ignore ? 0.f : per_row ? g[n] / big : 1.f;
+  if (threadIdx.x == 0) fac[0] = per_row ? big : mean ? g[0] / fmaxf(total[0], 1.f) : g[0];
+}
+
+constexpr float D_SCALE = 32768.f;  // of the scaled gradient terms
+
+// One 128 x 128 tile of d for the classes [vbeg, vbeg + vcols): dT[v - vbeg][ldn] and dn[n][ldv], PD terms each, and the
+// column sums dbpart[tile n][v].
+template <int PW, int PX, int PD>
+__global__ __launch_bounds__(G_THREADS, 2) void ce_grad_kernel(CeArgs a, const float* __restrict__ lse,
+                                                               const float* __restrict__ rs, float smooth, int vbeg,
+                                                               int vcols, f16* __restrict__ dT, int ldn,
+                                                               f16* __restrict__ dn, int ldv, int pdn,
+                                                               float* __restrict__ dbpart) {
+  typedef G16<PW, PX> G;
+  __shared__ __attribute__((aligned(1024))) f16 smem[G::LDS];
+  __shared__ float sb[2][GM];
+  int tv, tn;
+  g16_tile(blockIdx.x, gridDim.x, a.tiles_v, a.tiles_n, tv, tn);
+  const int v0 = vbeg + tv * GM, n0 = tn * GM;
+  f32x4 acc[4][4];
+  G::zero(acc);
+  G::run(acc, a.w + (int64_t)v0 * a.ld, (int64_t)a.V * a.ld, a.ld, a.V - v0, a.x + (int64_t)n0 * a.ld,
+         (int64_t)a.N * a.ld, a.ld, a.N - n0, 0, a.ld, smem);
+  const int lane = threadIdx.x & 63, q = lane >> 4, l15 = lane & 15;
+  const int wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
+  const int es = -(a.exps[0] + a.exps[1]);
+  const float each = smooth / (float)a.V;
+  float bias[4][4];
+  tile_bias(a, v0, bias);
+  float col[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) col[i][r] = 0.f;
+  const int64_t planeT = (int64_t)vcols * ldn, planeN = (int64_t)a.N * ldv;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int n = n0 + wn * 64 + j * 16 + l15;
+    const bool row = n < a.N;
+    const float w = row ? rs[n] : 0.f, l = row ? lse[n] : 0.f;
+    const int t = row ? (int)min(max(a.target[n], (int64_t)-1), (int64_t)a.V) : -1;
+    const bool bad = row && w != 0.f && (t < 0 || t >= a.V);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int vr = wm * 64 + i * 16 + q * 4, vl = v0 - vbeg + vr;
+      f16x4 hi, lo;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int v = v0 + vr + r;
+        float d = exp_of(ldexpf(acc[i][j][r], es) + bias[i][r] - l) - each;
+        if (v == t) d -= 1.f - smooth;
+        if (bad) d = NAN;
+        d = w == 0.f || v >= a.V ? 0.f : d * w;  // ignored rows vanish whatever they hold
+        col[i][r] += d;
+        f16 h, o;
+        f16_split(d * D_SCALE, h, o);
+        hi[r] = h;
+        lo[r] = o;
+        if (vl + r < vcols && n < ldn) {
+          dT[(int64_t)(vl + r) * ldn + n] = h;
+          if (PD == 2) dT[planeT + (int64_t)(vl + r) * ldn + n] = o;
+        }
+      }
+      if (row && vl < ldv) {
+        *reinterpret_cast<f16x4*>(dn + (int64_t)n * ldv + vl) = hi;
+        if (pdn == 2) *reinterpret_cast<f16x4*>(dn + planeN + (int64_t)n * ldv + vl) = lo;
+      }
+    }
+  }
+  if (dbpart) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float s = col[i][r];
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+        if (l15 == 0) sb[wn][wm * 64 + i * 16 + q * 4 + r] = s;
+      }
+    __syncthreads();
+    if (threadIdx.x < GM && v0 + (int)threadIdx.x < a.V)
+      dbpart[(int64_t)tn * a.V + v0 + threadIdx.x] = sb[0][threadIdx.x] + sb[1][threadIdx.x];
+  }
+}
+
+// db[v] += fac sum over the row tiles of dbpart[tile][v]
+template <typename T>
+__global__ __launch_bounds__(256) void ce_bias_kernel(const float* __restrict__ dbpart, int tiles, int V,
+                                                      const float* __restrict__ fac, T* __restrict__ db) {
+  const int v = blockIdx.x * 256 + threadIdx.x;
+  if (v >= V) return;
+  float s = 0.f;
+#pragma unroll 4
+  for (int t = 0; t < tiles; ++t) s += dbpart[(int64_t)t * V + v];
+  db[v] = from_f32<T>(to_f32(db[v]) + s * fac[0]);
+}
+
+struct MmArgs {
+  const f16* a;
+  const f16* b;
+  int64_t aplane, bplane;
+  int lda, ldb, M, Nn, k;      // k = padded reduction length, a multiple of 64
+  int tiles_m, tiles_n, splits, kper;
+  float* part;                 // [splits][M][Nn], or null: write out
+  int add;                     // add to what part / out hold
+  void* out;                   // [M][Nn]
+  const float* fac;
+  const int* exps;
+  int which;                   // operand b's scale exponent
+};
+
+__device__ __forceinline__ float mm_factor(const float* fac, const int* exps, int which) {
+  return ldexpf(fac[0], -15 - exps[which]);
+}
+
+// out[m][n] (+)= fac 2^-(scales) sum_k a[m][k] b[n][k], or raw fp32 partial sums of a slice of k
+template <int PA, int PB, typename T>
+__global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
+  typedef G16<PA, PB> G;
+  __shared__ __attribute__((aligned(1024))) f16 smem[G::LDS];
+  const int tiles = g.tiles_m * g.tiles_n;
+  const int split = blockIdx.x / tiles;
+  int tm, tn;
+  g16_tile(blockIdx.x - split * tiles, tiles, g.tiles_m, g.tiles_n, tm, tn);
+  const int m0 = tm * GM, n0 = tn * GM;
+  f32x4 acc[4][4];
+  G::zero(acc);
+  const int k0 = split * g.kper, k1 = min(g.k, k0 + g.kper);
+  G::run(acc, g.a + (int64_t)m0 * g.lda, g.aplane, g.lda, g.M - m0, g.b + (int64_t)n0 * g.ldb, g.bplane, g.ldb, g.Nn - n0,
+         k0, k1, smem);
+  const int lane = threadIdx.x & 63, q = lane >> 4, l15 = lane & 15;
+  const int wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
+  const float f = g.part ? 1.f : mm_factor(g.fac, g.exps, g.which);
+  float* part = g.part ? g.part + (int64_t)split * g.M * g.Nn : nullptr;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int m = m0 + wm * 64 + i * 16 + q * 4 + r;
+      if (m >= g.M) continue;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int n = n0 + wn * 64 + j * 16 + l15;
+        if (n >= g.Nn) continue;
+        const int64_t o = (int64_t)m * g.Nn + n;
+        float v = acc[i][j][r];
+        if (part) part[o] = g.add ? part[o] + v : v;
+        else {
+          T* out = (T*)g.out;
+          v *= f;
+          out[o] = from_f32<T>(g.add ? to_f32(out[o]) + v : v);
+        }
+      }
+    }
+}
+
+// out (+)= factor * sum over the slices, in order
+template <typename T>
+__global__ __launch_bounds__(256) void ce_reduce_kernel(const float* __restrict__ part, int slices, int64_t n,
+                                                        const float* __restrict__ fac, const int* __restrict__ exps,
+                                                        int which, int add, T* __restrict__ out) {
+  const float f = mm_factor(fac, exps, which);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    float s = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < slices; ++k) s += part[k * n + i];
+    s *= f;
+    out[i] = from_f32<T>(add ? to_f32(out[i]) + s : s);
+  }
+}
+
+// ---- host side: shapes and workspaces ---------------------------------------------------------------------------------
+int pad64(int v) { return (v + 63) / 64 * 64; }
+int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
+
+struct Plan {
+  int ld, px, pw;              // row length and terms of the packed operands
+  int pdx, pdw;                // terms of d for dx and dW
+  int ldn, piece, pieces;      // padded rows, classes of a piece
+  int sx, kx, sw, kw;          // slices of the reductions of dx (per piece) and dW, and their lengths
+  // forward workspace (saved for backward): packed x, packed W, exponents, lse, total
+  int64_t o_xp, o_wp, o_exps, o_lse, o_total, saved;
+  // forward scratch
+  int64_t f_amax, f_part, f_zt, fwd;
+  // backward scratch
+  int64_t b_xt, b_wt, b_rs, b_fac, b_dT, b_dn, b_db, b_px, b_pw, bwd;
+};
+
+// slices of a reduction of length k (a multiple of 64) over `tiles` output tiles: enough to give every CU two workgroups,
+// of at least 512 elements, and not more than 16
+void slices(int tiles, int k, int& s, int& per) {
+  int want = (2 * 256) / (tiles < 1 ? 1 : tiles);
+  const int most = k / 512 < 16 ? k / 512 : 16;
+  if (want > most) want = most;
+  if (want < 1) want = 1;
+  per = pad64((k + want - 1) / want);
+  s = (k + per - 1) / per;
+}
+
+Plan make_plan(int xf32, int wf32, int N, int V, int K) {
+  Plan p;
+  p.ld = pad64(K);
+  p.px = xf32 ? 2 : 1;
+  p.pw = xf32 ? 2 : 1;
+  p.pdx = xf32 ? 2 : 1;
+  p.pdw = wf32 ? 2 : 1;
+  p.ldn = pad64(N);
+  // a piece of d (both orders, all terms) stays below 192 MiB, inside the last-level cache
+  const int64_t per_class = (int64_t)p.ldn * 2 * (p.pdx + p.pdw);
+  int64_t cols = (192ll << 20) / per_class / GM * GM;
+  if (cols < GM) cols = GM;
+  const int all = (V + GM - 1) / GM * GM;
+  p.pieces = (int)((all + cols - 1) / cols);
+  p.piece = (int)(((all / GM + p.pieces - 1) / p.pieces) * GM);
+  p.pieces = (all + p.piece - 1) / p.piece;
+  const int tn = ceil_div(N, GM), tk = ceil_div(K, GM);
+  slices(tn * tk, p.piece, p.sx, p.kx);
+  slices((p.piece / GM) * tk, p.ldn, p.sw, p.kw);
+  int64_t o = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t at = o;
+    o += up256(bytes);
+    return at;
+  };
+  p.o_xp = take((int64_t)p.px * N * p.ld * 2);
+  p.o_wp = take((int64_t)p.pw * V * p.ld * 2);
+  p.o_exps = take(16);
+  p.o_lse = take((int64_t)N * 4);
+  p.o_total = take(16);
+  p.saved = o;
+  o = 0;
+  p.f_amax = take(2 * AMAX_BLOCKS * 4);
+  p.f_part = take((int64_t)ceil_div(V, GM) * N * 16);
+  p.f_zt = take((int64_t)N * 4);
+  p.fwd = o;
+  o = 0;
+  p.b_xt = take((int64_t)p.px * K * p.ldn * 2);
+  p.b_wt = take((int64_t)p.pw * K * pad64(V) * 2);
+  p.b_rs = take((int64_t)N * 4);
+  p.b_fac = take(16);
+  p.b_dT = take((int64_t)p.pdw * p.piece * p.ldn * 2);
+  p.b_dn = take((int64_t)p.pdx * N * p.piece * 2);
+  p.b_db = take((int64_t)tn * V * 4);
+  p.b_px = (p.pieces > 1 || p.sx > 1) ? take((int64_t)p.sx * N * K * 4) : -1;
+  p.b_pw = p.sw > 1 ? take((int64_t)p.sw * p.piece * K * 4) : -1;
+  p.bwd = o;
+  return p;
+}
+
+int check_ce(const char* who, int xdtype, int wdtype, int N, int V, int K, float smooth) {
+  for (int d : {xdtype, wdtype})
+    if (d != VC_F32 && d != VC_BF16) {
+      vc_set_error("%s: unsupported dtype %d", who, d);
+      return VC_ERR_DTYPE;
+    }
+  VC_CHECK_ARG(xdtype == VC_BF16 || wdtype == VC_F32, "%s: fp32 rows need fp32 weights", who);
+  VC_CHECK_SHAPE(N > 0 && V > 0 && K > 0, "%s: empty shape N=%d V=%d K=%d", who, N, V, K);
+  // 128 rows of an operand have to fit a 32-bit buffer descriptor, tiles a grid
+  VC_CHECK_SHAPE(K <= (1 << 20) && N <= (1 << 22) && V <= (1 << 22), "%s: N, V or K too large (at most 2^22, 2^22, 2^20)",
+                 who);
+  VC_CHECK_SHAPE((int64_t)ceil_div(N, GM) * ceil_div(V, GM) < (1ll << 31) - 1, "%s: too many tiles", who);
+  VC_CHECK_ARG(smooth >= 0.f && smooth <= 1.f, "%s: label smoothing %g outside [0, 1]", who, (double)smooth);
+  return VC_OK;
+}
+
+template <typename TX, typename TW>
+void pack_go(const Plan& p, const void* x, const void* w, int N, int V, int K, const int64_t* target, int64_t ignore,
+             char* saved, char* ws, hipStream_t st) {
+  float* amax = (float*)(ws + p.f_amax);
+  const int per = ceil_div(p.ld, 512);
+  const int xb = (int)ceil_div64((int64_t)N * per, 4), wb = (int)ceil_div64((int64_t)V * per, 4);
+  hipLaunchKernelGGL((ce_amax_kernel<TX, TW>), dim3(2 * AMAX_BLOCKS), dim3(256), 0, st, (const TX*)x, (const TW*)w, N, V, K,
+                     target, ignore, amax);
+  hipLaunchKernelGGL((ce_pack_kernel<TX, TW>), dim3(xb + wb), dim3(256), 0, st, (const TX*)x, (const TW*)w, N, V, K, p.ld,
+                     p.px, p.pw, target, ignore, amax, (f16*)(saved + p.o_xp), (f16*)(saved + p.o_wp),
+                     (int*)(saved + p.o_exps), xb);
+}
+
+template <int PA, int PB>
+void mm_go(const MmArgs& g, int out_bf16, hipStream_t st) {
+  const dim3 grid(g.tiles_m * g.tiles_n * g.splits);
+  if (out_bf16) hipLaunchKernelGGL((ce_mm_kernel<PA, PB, bf16>), grid, dim3(G_THREADS), 0, st, g);
+  else hipLaunchKernelGGL((ce_mm_kernel<PA, PB, float>), grid, dim3(G_THREADS), 0, st, g);
+}
+void mm_terms(int pa, int pb, const MmArgs& g, int out_bf16, hipStream_t st) {
+  if (pa == 1 && pb == 1) mm_go<1, 1>(g, out_bf16, st);
+  else if (pa == 2 && pb == 1) mm_go<2, 1>(g, out_bf16, st);
+  else mm_go<2, 2>(g, out_bf16, st);
+}
+void reduce_go(const float* part, int slices, int64_t n, const float* fac, const int* exps, int which, int add, void* out,
+               int out_bf16, hipStream_t st) {
+  const int grid = (int)(ceil_div64(n, 256) < 4096 ? ceil_div64(n, 256) : 4096);
+  if (out_bf16)
+    hipLaunchKernelGGL((ce_reduce_kernel<bf16>), dim3(grid), dim3(256), 0, st, part, slices, n, fac, exps, which, add, (bf16*)out);
+  else
+    hipLaunchKernelGGL((ce_reduce_kernel<float>), dim3(grid), dim3(256), 0, st, part, slices, n, fac, exps, which, add, (float*)out);
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t vc_linear_ce_bytes(int what, int xdtype, int wdtype, int N, int V, int K) {
+  if (check_ce("vc_linear_ce_bytes", xdtype, wdtype, N, V, K, 0.f) != VC_OK) return -1;
+  const Plan p = make_plan(xdtype == VC_F32, wdtype == VC_F32, N, V, K);
+  return what == 0 ? p.saved : what == 1 ? p.fwd : what == 2 ? p.bwd : -1;
+}
+
+int vc_linear_ce_fwd(int xdtype, int wdtype, const void* x, const void* w, const void* bias, const int64_t* target,
+                     int64_t ignore_index, float smoothing, int mean, float* row_loss, float* loss, int64_t* pred,
+                     int* correct, void* saved, void* workspace, int N, int V, int K, hipStream_t stream) {
+  const int rc = check_ce("vc_linear_ce_fwd", xdtype, wdtype, N, V, K, smoothing);
+  if (rc != VC_OK) return rc;
+  VC_CHECK_ARG(x && w && target && row_loss && saved && workspace, "vc_linear_ce_fwd: null pointer");
+  VC_CHECK_ARG(!correct || pred, "vc_linear_ce_fwd: the count of correct rows needs pred");
+  VC_CHECK_ARG((((uintptr_t)saved | (uintptr_t)workspace) & 255) == 0, "vc_linear_ce_fwd: buffers must be 256-byte aligned");
+  const Plan p = make_plan(xdtype == VC_F32, wdtype == VC_F32, N, V, K);
+  char *sv = (char*)saved, *ws = (char*)workspace;
+  if (xdtype == VC_F32) pack_go<float, float>(p, x, w, N, V, K, target, ignore_index, sv, ws, stream);
+  else if (wdtype == VC_F32) pack_go<bf16, float>(p, x, w, N, V, K, target, ignore_index, sv, ws, stream);
+  else pack_go<bf16, bf16>(p, x, w, N, V, K, target, ignore_index, sv, ws, stream);
+  CeArgs a{(const f16*)(sv + p.o_wp), (const f16*)(sv + p.o_xp), bias, target, (const int*)(sv + p.o_exps), N, V, p.ld,
+           wdtype == VC_BF16, ceil_div(V, GM), ceil_div(N, GM)};
+  float4* part = (float4*)(ws + p.f_part);
+  float* zt = (float*)(ws + p.f_zt);
+  const dim3 grid(a.tiles_v * a.tiles_n);
+  if (p.pw == 2) hipLaunchKernelGGL((ce_stats_kernel<2, 2>), grid, dim3(G_THREADS), 0, stream, a, part, zt);
+  else hipLaunchKernelGGL((ce_stats_kernel<1, 1>), grid, dim3(G_THREADS), 0, stream, a, part, zt);
+  hipLaunchKernelGGL(ce_join_kernel, dim3(ceil_div(N, 32)), dim3(256), 0, stream, part, zt, target, ignore_index, N, V,
+                     a.tiles_v, smoothing, (float*)(sv + p.o_lse), row_loss, pred);
+  hipLaunchKernelGGL(ce_total_kernel, dim3(1), dim3(1024), 0, stream, row_loss, target, pred, ignore_index, N, mean, loss,
+                     (float*)(sv + p.o_total), correct);
+  VC_LAUNCH_CHECK("vc_linear_ce_fwd");
+  return VC_OK;
+}
+
+int vc_linear_ce_bwd(int xdtype, int wdtype, const void* bias, const int64_t* target, int64_t ignore_index, float smoothing,
+                     int mean, int per_row, const float* dloss, const void* saved, void* dx, void* dw, void* db,
+                     void* workspace, int N, int V, int K, hipStream_t stream) {
+  const int rc = check_ce("vc_linear_ce_bwd", xdtype, wdtype, N, V, K, smoothing);
+  if (rc != VC_OK) return rc;
+  VC_CHECK_ARG(target && dloss && saved && workspace, "vc_linear_ce_bwd: null pointer");
+  VC_CHECK_ARG(!(mean && per_row), "vc_linear_ce_bwd: a mean has one upstream gradient");
+  VC_CHECK_ARG((((uintptr_t)saved | (uintptr_t)workspace) & 255) == 0, "vc_linear_ce_bwd: buffers must be 256-byte aligned");
+  if (!dx && !dw && !db) return VC_OK;
+  const Plan p = make_plan(xdtype == VC_F32, wdtype == VC_F32, N, V, K);
+  const char* sv = (const char*)saved;
+  char* ws = (char*)workspace;
+  const f16 *xp = (const f16*)(sv + p.o_xp), *wp = (const f16*)(sv + p.o_wp);
+  f16 *xt = (f16*)(ws + p.b_xt), *wt = (f16*)(ws + p.b_wt), *dT = (f16*)(ws + p.b_dT), *dn = (f16*)(ws + p.b_dn);
+  const int* exps = (const int*)(sv + p.o_exps);
+  const float* lse = (const float*)(sv + p.o_lse);
+  float *rs = (float*)(ws + p.b_rs), *fac = (float*)(ws + p.b_fac), *dbp = (float*)(ws + p.b_db);
+  const int vp = pad64(V), tn = ceil_div(N, GM), tk = ceil_div(K, GM);
+  hipLaunchKernelGGL(ce_weights_kernel, dim3(1), dim3(1024), 0, stream, dloss, (const float*)(sv + p.o_total), target,
+                     ignore_index, N, mean, per_row, rs, fac);
+  TransArgs t{{xp, wp}, {xt, wt}, {N, V}, {p.ld, p.ld}, {p.ldn, vp}, {dw ? p.px : 0, dx ? p.pw : 0},
+              {(p.ldn / 64) * (p.ld / 64), (vp / 64) * (p.ld / 64)}, K};
+  const int tblocks = t.tiles[0] * t.planes[0] + t.tiles[1] * t.planes[1];
+  if (tblocks) hipLaunchKernelGGL(ce_transpose_kernel, dim3(tblocks), dim3(256), 0, stream, t);
+  for (int c = 0; c < p.pieces; ++c) {
+    const int vbeg = c * p.piece;
+    const int vcols = p.piece < ceil_div(V - vbeg, GM) * GM ? p.piece : ceil_div(V - vbeg, GM) * GM;
+    CeArgs a{wp, xp, bias, target, exps, N, V, p.ld, wdtype == VC_BF16, vcols / GM, tn};
+    const dim3 grid(a.tiles_v * tn);
+    float* dbq = db ? dbp : nullptr;
+    if (p.pw == 2)
+      hipLaunchKernelGGL((ce_grad_kernel<2, 2, 2>), grid, dim3(G_THREADS), 0, stream, a, lse, rs, smoothing, vbeg, vcols, dT,
+                         p.ldn, dn, vcols, p.pdx, dbq);
+    else if (p.pdw == 2)
+      hipLaunchKernelGGL((ce_grad_kernel<1, 1, 2>), grid, dim3(G_THREADS), 0, stream, a, lse, rs, smoothing, vbeg, vcols, dT,
+                         p.ldn, dn, vcols, p.pdx, dbq);
+    else
+      hipLaunchKernelGGL((ce_grad_kernel<1, 1, 1>), grid, dim3(G_THREADS), 0, stream, a, lse, rs, smoothing, vbeg, vcols, dT,
+                         p.ldn, dn, vcols, p.pdx, dbq);
+    if (dx) {
+      MmArgs g{};
+      g.a = dn;
+      g.aplane = (int64_t)N * vcols;
+      g.lda = vcols;
+      g.M = N;
+      g.b = wt + vbeg;
+      g.bplane = (int64_t)K * vp;
+      g.ldb = vp;
+      g.Nn = K;
+      g.k = vcols < vp - vbeg ? vcols : vp - vbeg;
+      g.tiles_m = tn;
+      g.tiles_n = tk;
+      g.splits = p.sx;
+      g.kper = p.kx;
+      g.part = p.b_px >= 0 ? (float*)(ws + p.b_px) : nullptr;
+      g.add = c > 0;
+      g.out = dx;
+      g.fac = fac;
+      g.exps = exps;
+      g.which = 1;
+      mm_terms(p.pdx, p.pw, g, xdtype == VC_BF16, stream);
+    }
+    if (dw) {
+      const int rows = vcols < V - vbeg ? vcols : V - vbeg;
+      char* out = (char*)dw + (int64_t)vbeg * K * (wdtype == VC_BF16 ? 2 : 4);
+      MmArgs g{};
+      g.a = dT;
+      g.aplane = (int64_t)vcols * p.ldn;
+      g.lda = p.ldn;
+      g.M = rows;
+      g.b = xt;
+      g.bplane = (int64_t)K * p.ldn;
+      g.ldb = p.ldn;
+      g.Nn = K;
+      g.k = p.ldn;
+      g.tiles_m = ceil_div(rows, GM);
+      g.tiles_n = tk;
+      g.splits = p.sw;
+      g.kper = p.kw;
+      g.part = p.b_pw >= 0 ? (float*)(ws + p.b_pw) : nullptr;
+      g.add = g.part ? 0 : 1;
+      g.out = out;
+      g.fac = fac;
+      g.exps = exps;
+      g.which = 0;
+      mm_terms(p.pdw, p.px, g, wdtype == VC_BF16, stream);
+      if (g.part) reduce_go(g.part, p.sw, (int64_t)rows * K, fac, exps, 0, 1, out, wdtype == VC_BF16, stream);
+    }
+  }
+  if (dx && p.b_px >= 0)
+    reduce_go((const float*)(ws + p.b_px), p.sx, (int64_t)N * K, fac, exps, 1, 0, dx, xdtype == VC_BF16, stream);
+  if (db) {
+    if (wdtype == VC_BF16)
+      hipLaunchKernelGGL((ce_bias_kernel<bf16>), dim3(ceil_div(V, 256)), dim3(256), 0, stream, dbp, tn, V, fac, (bf16*)db);
+    else
+      hipLaunchKernelGGL((ce_bias_kernel<float>), dim3(ceil_div(V, 256)), dim3(256), 0, stream, dbp, tn, V, fac, (float*)db);
+  }
+  VC_LAUNCH_CHECK("vc_linear_ce_bwd");
+  return VC_OK;
+}
+
+}  // extern "C"

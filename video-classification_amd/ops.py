@@ -1359,6 +1359,101 @@ def cross_entropy(logits, target, stats=None):
 
 
 # ----------------------------------------------------------------------------------------------
+# linear classifier + cross entropy without the logits
+# ----------------------------------------------------------------------------------------------
+CE_REDUCTIONS = ("mean", "sum", "none")
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, anchor, params, target, ignore_index, smoothing, reduction, want_pred):
+        weight, bias = params  # in a tuple, so that autograd does not see them
+        N, K = x.shape
+        V = weight.shape[0]
+        xd, wd = L.dtype_code(x.dtype), L.dtype_code(weight.dtype)
+        w = weight.detach().contiguous()
+        b = bias.detach().contiguous() if bias is not None else None
+        dev = x.device
+        saved = torch.empty(L.query("vc_linear_ce_bytes", 0, xd, wd, N, V, K), device=dev, dtype=torch.uint8)
+        ws = torch.empty(L.query("vc_linear_ce_bytes", 1, xd, wd, N, V, K), device=dev, dtype=torch.uint8)
+        rows = torch.empty(N, device=dev, dtype=torch.float32)
+        loss = torch.empty((), device=dev, dtype=torch.float32) if reduction != "none" else None
+        pred = torch.empty(N, device=dev, dtype=torch.int64) if want_pred else None
+        correct = torch.empty(1, device=dev, dtype=torch.int32) if want_pred else None
+        L.call("vc_linear_ce_fwd", xd, wd, L.ptr(x), L.ptr(w), L.ptr(b), L.ptr(target), L.i64(ignore_index),
+               float(smoothing), int(reduction == "mean"), L.ptr(rows), L.ptr(loss), L.ptr(pred), L.ptr(correct),
+               L.ptr(saved), L.ptr(ws), N, V, K, L.stream())
+        ctx.dims, ctx.codes, ctx.opts = (N, V, K), (xd, wd), (ignore_index, smoothing, reduction)
+        ctx.weight, ctx.bias, ctx.xdtype = weight, bias, x.dtype
+        ctx.save_for_backward(saved, target, b)
+        out = rows if loss is None else loss
+        if want_pred:
+            ctx.mark_non_differentiable(pred, correct)
+        return out, pred, correct
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, _dpred, _dcorrect):
+        saved, target, b = ctx.saved_tensors
+        (N, V, K), (xd, wd), (ignore_index, smoothing, reduction) = ctx.dims, ctx.codes, ctx.opts
+        g = g.contiguous().float()
+        dx = torch.empty(N, K, device=saved.device, dtype=ctx.xdtype) if ctx.needs_input_grad[0] else None
+        dw, db = _grad_target(ctx.weight), _grad_target(ctx.bias)
+        ws = torch.empty(L.query("vc_linear_ce_bytes", 2, xd, wd, N, V, K), device=saved.device, dtype=torch.uint8)
+        L.call("vc_linear_ce_bwd", xd, wd, L.ptr(b), L.ptr(target), L.i64(ignore_index), float(smoothing),
+               int(reduction == "mean"), int(reduction == "none"), L.ptr(g), L.ptr(saved), L.ptr(dx), L.ptr(dw), L.ptr(db),
+               L.ptr(ws), N, V, K, L.stream())
+        for p, t in ((ctx.weight, dw), (ctx.bias, db)):
+            if t is not None:
+                _add_grad(p, t)
+        _ready(ctx.weight, ctx.bias)
+        return (dx,) + (None,) * 7
+
+
+def linear_cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoothing=0.0, reduction="mean", stats=None):
+    """Cross entropy of the classifier ``x @ weight.T + bias`` against `target`, without keeping the logits: what
+    ``cross_entropy(linear(x, weight, bias, out_f32=True), target)`` computes, in pieces of the classes.
+
+    x [..., K] float32 or bfloat16, weight [V, K] and bias [V] (or None) float32, or bfloat16 next to bfloat16 x, target
+    int64 of x's leading shape.  Rows whose target is `ignore_index` count for nothing; any other target outside [0, V)
+    makes the loss NaN.  reduction: "mean" over the rows that count (0 if there are none), "sum", or "none" (a loss per row,
+    0 where ignored).  The loss is float32; gradients of weight and bias are accumulated into .grad.  stats: a dict that
+    receives "pred" (arg-max per row) and "correct" (rows that count and are right)."""
+    _require_cuda(x, "linear_cross_entropy")
+    xd, wd = L.dtype_code(x.dtype), L.dtype_code(weight.dtype)
+    if xd == L.VC_F32 and wd != L.VC_F32:
+        raise TypeError("linear_cross_entropy: float32 rows need float32 weights")
+    if bias is not None and (bias.dtype != weight.dtype or tuple(bias.shape) != (weight.shape[0],)):
+        raise RuntimeError(f"linear_cross_entropy: bias {tuple(bias.shape)} {bias.dtype} does not match the weight "
+                           f"{tuple(weight.shape)} {weight.dtype}")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or weight.numel() == 0:
+        raise RuntimeError(f"linear_cross_entropy: rows {tuple(x.shape)} against a weight {tuple(weight.shape)}")
+    if target.dtype != torch.int64 or target.shape != x.shape[:-1]:
+        raise RuntimeError(f"linear_cross_entropy: target must be int64 {tuple(x.shape[:-1])}, got {target.dtype} "
+                           f"{tuple(target.shape)}")
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError(f"linear_cross_entropy: label_smoothing {label_smoothing} outside [0, 1]")
+    if reduction not in CE_REDUCTIONS:
+        raise ValueError(f"linear_cross_entropy: reduction must be one of {CE_REDUCTIONS}, not {reduction!r}")
+    _same_device("linear_cross_entropy", x, weight, bias, target)
+    if target.numel() == 0:
+        loss = x.float().sum(-1) if reduction == "none" else x.float().sum()
+        if stats is not None:
+            stats["pred"] = target.reshape(-1)
+            stats["correct"] = torch.zeros(1, device=x.device, dtype=torch.int32)
+        return loss
+    with torch.cuda.device(x.device):
+        _leaf_guard("linear_cross_entropy", x)
+        x2 = x.reshape(-1, x.shape[-1]).contiguous()
+        out, pred, correct = _LinearCrossEntropy.apply(x2, _anchor((x,), (weight, bias)), (weight, bias),
+                                                       target.reshape(-1).contiguous(), int(ignore_index),
+                                                       float(label_smoothing), reduction, stats is not None)
+    if stats is not None:
+        stats["pred"], stats["correct"] = pred, correct
+    return out.view(target.shape) if reduction == "none" else out
+
+
+# ----------------------------------------------------------------------------------------------
 # dropout
 # ----------------------------------------------------------------------------------------------
 _dropout_seed = [0x5EED]
@@ -1650,12 +1745,12 @@ def _add_grad(p, g):
 
 
 def _grad_target(p):
-    """A dense fp32 tensor the kernels may accumulate p's gradient into: p.grad where it is dense, else a zeroed stand-in
+    """A dense tensor of p's type the kernels may accumulate p's gradient into: p.grad where it is dense, else a zeroed stand-in
     that _add_grad folds in.  None where p needs no gradient."""
     if p is None or not p.requires_grad:
         return None
     g = _grad_buf(p)
-    return g if g.is_contiguous() and g.dtype == torch.float32 else torch.zeros(p.shape, device=p.device)
+    return g if g.is_contiguous() else torch.zeros(p.shape, device=p.device, dtype=p.dtype)
 
 
 class _GroupNorm(torch.autograd.Function):
