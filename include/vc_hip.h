@@ -372,6 +372,17 @@ int vc_linear_ce_bwd(int xdtype, int wdtype, const void* bias, const int64_t* ta
 int vc_optim_step(int mode, float* p, const float* g, float* m, float* v, int64_t n, float lr, float b1, float b2,
                   float eps, float wd, int step, float grad_scale, const float* lr_dev, const int64_t* step_dev,
                   vc_stream_t stream);
+/* Orthogonalised updates (the Muon optimizer's step; no counterpart in the reference): every matrix g[i] [rows][cols], dense,
+ * becomes out[i] = p_steps(... p_1(g / (|g|_F + eps))) with p_k(X) = a X + b (X X^T) X + c (X X^T)^2 X, coeffs = steps
+ * triples (a, b, c).  g, out, rows, cols, coeffs are HOST arrays, their pointers DEVICE matrices of `dtype`; out[i] may
+ * be g[i].  The caller bounds the iterates over singular values in [0, 1]: cap = the largest |value| any iterate takes,
+ * gain = the largest ratio of an iterate to its start, pmax = the largest |b l + c l^2| for l in [0, cap^2].
+ * workspace: vc_newton_schulz_bytes() bytes, 256-byte aligned, contents irrelevant; all matrices share each launch (64 at a
+ * time).  Products are as accurate as fp32's; a zero matrix stays zero. */
+int64_t vc_newton_schulz_bytes(int count, const int* rows, const int* cols);
+int vc_newton_schulz(int dtype, int count, const void* const* g, void* const* out, const int* rows, const int* cols,
+                     int steps, const float* coeffs, double eps, float cap, float gain, float pmax, void* workspace,
+                     vc_stream_t stream);
 /* *counter += inc on the stream: the device-resident step counter that lr_dev/step_dev/seed_dev users read, so
  * that a hipGraph of the whole training step replays with current values */
 int vc_counter_add(int64_t* counter, int64_t inc, vc_stream_t stream);

@@ -77,7 +77,8 @@ def query(name, *args):
     """Call an entry point that returns a value (not a status code); ints are passed as C int."""
     fn = getattr(lib(), name)
     if name in ("vc_lstm_persist_xchg_bytes", "vc_lstm_persist_bwd_xchg_bytes", "vc_cbam_workspace_floats",
-                "vc_group_norm_workspace_floats", "vc_linear_ce_bytes"):
+                "vc_group_norm_workspace_floats", "vc_linear_ce_bytes",
+                "vc_newton_schulz_bytes"):
         fn.restype = ctypes.c_longlong
     return fn(*[ctypes.c_int(int(a)) if isinstance(a, (bool, int)) else a for a in args])
 
@@ -88,3 +89,19 @@ def i64(v):
 
 def int_array(vals):
     return (ctypes.c_int * len(vals))(*[int(v) for v in vals])
+
+
+def float_array(vals):
+    return (ctypes.c_float * len(vals))(*[float(v) for v in vals])
+
+
+def ptr_array(addresses):
+    return (ctypes.c_void_p * len(addresses))(*addresses)
+
+
+def f64(v):
+    return ctypes.c_double(float(v))
+
+
+def last_error():
+    return lib().vc_last_error().decode("utf-8", "replace")

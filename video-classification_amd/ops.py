@@ -6,6 +6,7 @@ of 8.  PyTorch only owns the memory and the autograd graph; every arithmetic ste
 into libvc_hip.  Parameter gradients are accumulated by the kernels directly into ``param.grad``
 (fp32), so the autograd functions return ``None`` for parameter inputs.
 """
+import functools
 import os
 
 import torch
@@ -1933,3 +1934,82 @@ class _PatchMerge(torch.autograd.Function):
 def patch_merge(x):
     """[B,H,W,C] -> [B,H/2,W/2,4C] with timm's PatchMerging channel order."""
     return _PatchMerge.apply(x)
+
+
+# ----------------------------------------------------------------------------------------------
+# orthogonalised updates
+# ----------------------------------------------------------------------------------------------
+NS_COEFFS = (3.4445, -4.7750, 2.0315)
+
+
+@functools.lru_cache(maxsize=64)
+def _ns_bounds(coeffs):
+    """(cap, gain, pmax) of the polynomials over singular values in [0, 1]: the largest value any iterate takes, the
+    largest ratio of an iterate to its start, and the largest |b l + c l^2| for l up to cap^2, each with 2 % to spare."""
+    s = torch.cat([torch.logspace(-8, 0, 20001, dtype=torch.float64), torch.linspace(0, 1, 20001, dtype=torch.float64)[1:]])
+    x, cap, gain = s, 1.0, 1.0
+    for a, b, c in coeffs:
+        x = x * (a + x * x * (b + c * x * x))
+        cap, gain = max(cap, float(x.abs().max())), max(gain, float((x / s).abs().max()))
+    cap, gain = 1.02 * cap, 1.02 * gain
+    lam = torch.linspace(0, cap * cap, 20001, dtype=torch.float64)
+    pmax = max([float((b * lam + c * lam * lam).abs().max()) for _, b, c in coeffs] + [1e-3])
+    return cap, gain, 1.02 * pmax
+
+
+def newton_schulz(g, steps=5, coeffs=NS_COEFFS, eps=1e-7):
+    """Orthogonalises matrices by `steps` Newton-Schulz products: X = G / (|G|_F + eps), then X <- a X + b (X X^T) X +
+    c (X X^T)^2 X, which drives every singular value towards 1 (the update of the Muon optimizer).
+
+    g: a tensor [..., m, n], or a list or tuple of such tensors of any shapes (all of one type, float32 or bfloat16, on one
+    device); all their matrices go through the same launches.  coeffs: (a, b, c), or `steps` such triples.  Returns new
+    tensors of g's structure, shapes and type; products are carried at float32 accuracy whatever the type.  Not
+    differentiable: gradients are its input."""
+    single = isinstance(g, torch.Tensor)
+    items = [g] if single else list(g)
+    if not items:
+        return []
+    steps = int(steps)
+    if not 0 <= steps <= 64:
+        raise ValueError(f"newton_schulz: steps {steps} outside [0, 64]")
+    if eps < 0:
+        raise ValueError(f"newton_schulz: eps {eps} is negative")
+    per_step = [tuple(map(float, c)) for c in coeffs] if isinstance(coeffs[0], (tuple, list)) else \
+        [tuple(map(float, coeffs))] * steps
+    if len(per_step) != steps or any(len(c) != 3 for c in per_step):
+        raise ValueError(f"newton_schulz: coeffs must be (a, b, c) or {steps} such triples")
+    cap, gain, pmax = _ns_bounds(tuple(per_step))
+    if not (cap <= 16 and gain <= 8192 and pmax <= 8192):
+        raise ValueError(f"newton_schulz: these coefficients let singular values grow to {cap:.3g} (by a factor of "
+                         f"{gain:.3g}); at most 16 (8192) is supported")
+    first = items[0]
+    for t in items:
+        _require_cuda(t, "newton_schulz")
+        if t.dim() < 2:
+            raise RuntimeError(f"newton_schulz: a matrix needs two dimensions, got {tuple(t.shape)}")
+        if t.dtype != first.dtype:
+            raise TypeError(f"newton_schulz: matrices of {first.dtype} and {t.dtype} in one call")
+    code = L.dtype_code(first.dtype)
+    _same_device("newton_schulz", first, *items)
+    with torch.cuda.device(first.device), torch.no_grad():
+        srcs = [t.detach().contiguous() for t in items]
+        outs = [torch.empty_like(t) for t in srcs]
+        gp, op, rows, cols = [], [], [], []
+        for s, o in zip(srcs, outs):
+            m, n = s.shape[-2:]
+            step = m * n * s.element_size()
+            for k in range(s.numel() // (m * n) if m * n else 0):
+                gp.append(s.data_ptr() + k * step)
+                op.append(o.data_ptr() + k * step)
+                rows.append(m)
+                cols.append(n)
+        if gp:
+            count, r, c = len(gp), L.int_array(rows), L.int_array(cols)
+            nbytes = L.query("vc_newton_schulz_bytes", count, r, c)
+            if nbytes < 0:
+                raise RuntimeError("newton_schulz: " + L.last_error())
+            ws = torch.empty(nbytes, device=first.device, dtype=torch.uint8)
+            L.call("vc_newton_schulz", code, count, L.ptr_array(gp), L.ptr_array(op), r, c, steps,
+                   L.float_array([v for t in per_step for v in t]), L.f64(eps), float(cap), float(gain), float(pmax),
+                   L.ptr(ws), L.stream())
+    return outs[0] if single else (tuple(outs) if isinstance(g, tuple) else outs)
