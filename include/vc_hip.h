@@ -383,6 +383,13 @@ int64_t vc_newton_schulz_bytes(int count, const int* rows, const int* cols);
 int vc_newton_schulz(int dtype, int count, const void* const* g, void* const* out, const int* rows, const int* cols,
                      int steps, const float* coeffs, double eps, float cap, float gain, float pmax, void* workspace,
                      vc_stream_t stream);
+/* The elementwise halves of that optimizer over a flat fp32 buffer whose parameters start on 64-element boundaries (n a
+ * multiple of 64): m <- mu m + grad_scale g with u = the (Nesterov) update, and, after u's matrices were orthogonalised,
+ * p <- (1 - lr wd) p - lr scale[i / 64] u with lr read from the device. */
+int vc_muon_momentum(const float* g, float* m, float* u, int64_t n, float mu, int nesterov, float grad_scale,
+                     vc_stream_t stream);
+int vc_muon_apply(float* p, const float* u, const float* scale, int64_t n, const float* lr_dev, float wd,
+                  vc_stream_t stream);
 /* *counter += inc on the stream: the device-resident step counter that lr_dev/step_dev/seed_dev users read, so
  * that a hipGraph of the whole training step replays with current values */
 int vc_counter_add(int64_t* counter, int64_t inc, vc_stream_t stream);

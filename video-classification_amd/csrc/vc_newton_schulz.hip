@@ -37,6 +37,39 @@ struct NsArgs {
   int count;
 };
 
+// m <- mu m + f g;  u = f g + mu m (nesterov) or m
+__global__ __launch_bounds__(256) void muon_momentum_kernel(const float* __restrict__ g, float* __restrict__ m,
+                                                            float* __restrict__ u, int64_t n, float mu, int nesterov,
+                                                            float f) {
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
+    const f32x4 gv = *reinterpret_cast<const f32x4*>(g + i);
+    f32x4 mv = *reinterpret_cast<const f32x4*>(m + i), uv;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float e = gv[k] * f;
+      mv[k] = fmaf(mu, mv[k], e);
+      uv[k] = nesterov ? fmaf(mu, mv[k], e) : mv[k];
+    }
+    *reinterpret_cast<f32x4*>(m + i) = mv;
+    *reinterpret_cast<f32x4*>(u + i) = uv;
+  }
+}
+
+// p <- (1 - lr wd) p - lr scale u, one scale per 64 elements (parameters start on 64-element boundaries)
+__global__ __launch_bounds__(256) void muon_apply_kernel(float* __restrict__ p, const float* __restrict__ u,
+                                                         const float* __restrict__ scale, int64_t n,
+                                                         const float* __restrict__ lr_dev, float wd) {
+  const float lr = *lr_dev, keep = 1.f - lr * wd;
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
+    f32x4 pv = *reinterpret_cast<const f32x4*>(p + i);
+    const f32x4 uv = *reinterpret_cast<const f32x4*>(u + i);
+    const float s = lr * scale[i >> 6];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) pv[k] = fmaf(keep, pv[k], -s * uv[k]);
+    *reinterpret_cast<f32x4*>(p + i) = pv;
+  }
+}
+
 __host__ __device__ inline int up64(int v) { return (v + 63) / 64 * 64; }
 __host__ __device__ inline int64_t up128(int64_t v) { return (v + 127) / 128 * 128; }
 
@@ -440,6 +473,30 @@ int vc_newton_schulz(int dtype, int count, const void* const* g, void* const* ou
     }
     VC_LAUNCH_CHECK("vc_newton_schulz");
   }
+  return VC_OK;
+}
+
+int vc_muon_momentum(const float* g, float* m, float* u, int64_t n, float mu, int nesterov, float grad_scale,
+                     hipStream_t stream) {
+  VC_CHECK_ARG(g && m && u, "vc_muon_momentum: null pointer");
+  VC_CHECK_SHAPE(n > 0 && n % 64 == 0, "vc_muon_momentum: n = %lld is not a positive multiple of 64", (long long)n);
+  VC_CHECK_ARG((((uintptr_t)g | (uintptr_t)m | (uintptr_t)u) & 15) == 0, "vc_muon_momentum: buffers must be 16-byte aligned");
+  const int64_t b = ceil_div64(n, 1024);
+  hipLaunchKernelGGL(muon_momentum_kernel, dim3((unsigned)(b < 4096 ? b : 4096)), dim3(256), 0, stream, g, m, u, n, mu,
+                     nesterov, grad_scale);
+  VC_LAUNCH_CHECK("vc_muon_momentum");
+  return VC_OK;
+}
+
+int vc_muon_apply(float* p, const float* u, const float* scale, int64_t n, const float* lr_dev, float wd,
+                  hipStream_t stream) {
+  VC_CHECK_ARG(p && u && scale && lr_dev, "vc_muon_apply: null pointer");
+  VC_CHECK_SHAPE(n > 0 && n % 64 == 0, "vc_muon_apply: n = %lld is not a positive multiple of 64", (long long)n);
+  VC_CHECK_ARG((((uintptr_t)p | (uintptr_t)u) & 15) == 0, "vc_muon_apply: buffers must be 16-byte aligned");
+  const int64_t b = ceil_div64(n, 1024);
+  hipLaunchKernelGGL(muon_apply_kernel, dim3((unsigned)(b < 4096 ? b : 4096)), dim3(256), 0, stream, p, u, scale, n, lr_dev,
+                     wd);
+  VC_LAUNCH_CHECK("vc_muon_apply");
   return VC_OK;
 }
 

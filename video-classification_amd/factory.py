@@ -33,15 +33,20 @@ def create_model(model_name, config):
     model = cfg.get("model", {}) or {}
     ckpt = cfg.get("checkpoint", {}) or {}
     num_classes = int(data.get("num_classes", 101))
+    # not a key of the reference: "group" puts GroupNorm in BatchNorm's place (Conv3D, CRNN, ResNetCRNN)
+    norm = model.get("norm", "batch")
+    if norm != "batch" and model_name not in ("Conv3D", "CRNN", "ResNetCRNN"):
+        raise ValueError(f"model.norm = {norm!r}: {model_name} has no BatchNorm trunk to replace")
 
     if model_name == "Conv3D":  # train.py:86-117
-        return M.Conv3DModel(types.SimpleNamespace(dropout_p=0.5, num_classes=num_classes))
+        return M.Conv3DModel(types.SimpleNamespace(dropout_p=0.5, num_classes=num_classes, norm=norm))
 
     if model_name == "CRNN":  # train.py:119-160
         size = int(data.get("frame_size", 224))
         c = types.SimpleNamespace(img_x=size, img_y=size, CNN_fc_hidden1=1024, CNN_fc_hidden2=768, CNN_embed_dim=512,
                                   dropout_p=0.0, use_pretrained=bool(ckpt.get("pretrained", False)),
-                                  RNN_hidden_layers=3, RNN_hidden_nodes=512, RNN_FC_dim=256, num_classes=num_classes)
+                                  RNN_hidden_layers=3, RNN_hidden_nodes=512, RNN_FC_dim=256, num_classes=num_classes,
+                                  norm=norm)
         if c.use_pretrained:
             raise NotImplementedError("CRNN with checkpoint.pretrained selects the VGG16 branch of EncoderCNN "
                                       "(model_components.py:72-79), which needs torchvision's weights")
@@ -56,7 +61,7 @@ def create_model(model_name, config):
                                   RNN_hidden_layers=int(model.get("hidden_layers", 3)),
                                   RNN_hidden_nodes=int(model.get("hidden_nodes", 512)),
                                   RNN_FC_dim=int(model.get("fc_dim", 256)), num_classes=num_classes,
-                                  arch="resnet152")  # model_components.py:159-162 builds resnet152 whatever the YAML says
+                                  norm=norm, arch="resnet152")  # model_components.py:159-162 builds resnet152 whatever the YAML says
         return M.ResNetCRNNModel(c)
 
     if model_name == "swintransformer-RNN":  # train.py:256-278 with Config / create_model of UCF101_SwinCRNN_fixed.py

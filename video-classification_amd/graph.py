@@ -19,6 +19,7 @@ import torch
 import torch.distributed as dist
 
 from . import ops
+from .trainer import forward_for
 
 
 class GraphedTrainStep:
@@ -52,7 +53,7 @@ class GraphedTrainStep:
             g0 = torch.cuda.CUDAGraph()
             with torch.cuda.graph(g0):
                 self.opt.flat.zero_grad()
-                out = model(self.x)
+                out = forward_for(model, criterion, self.x)
                 self.loss = criterion(out, self.y)
                 # the tensors the captured loss kernel writes: an eager call of the same criterion (validation, a
                 # short last batch) rebinds criterion.stats to fresh tensors, so replays must hand out THESE
@@ -102,7 +103,7 @@ class GraphedTrainStep:
 
     def _eager(self):
         self.opt.zero_grad()
-        loss = self.crit(self.model(self.x), self.y)
+        loss = self.crit(forward_for(self.model, self.crit, self.x), self.y)
         loss.backward()
         self.opt.step()
         return loss

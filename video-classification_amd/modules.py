@@ -18,6 +18,8 @@ statistics per time step (``groups = T``) and applying the T running-statistic u
 ``compute_dtype`` is ``torch.bfloat16`` (MFMA path, fp32 accumulation, fp32 master weights) or
 ``torch.float32`` (exact path used by the parity tests).
 """
+import math
+
 import torch
 import torch.nn as nn
 
@@ -44,6 +46,42 @@ class _HipModule(nn.Module):
         ops.bump_weights_epoch()
 
 
+NORMS = ("batch", "group")
+
+
+def _norm_layer(kind, channels, dims, momentum=0.1):
+    """The parameter container of a normalisation: BatchNorm{dims}d, or GroupNorm with 32 groups (fewer where 32 does not
+    divide the channels)."""
+    if kind not in NORMS:
+        raise ValueError(f"norm must be one of {NORMS}, not {kind!r}")
+    if kind == "group":
+        return nn.GroupNorm(math.gcd(32, channels), channels)
+    return {1: nn.BatchNorm1d, 2: nn.BatchNorm2d, 3: nn.BatchNorm3d}[dims](channels, momentum=momentum)
+
+
+def _conv_norm(x, weight, norm, T, bias=None, kernel=1, stride=1, padding=0, relu=False, residual=None, **bn_kw):
+    """relu(norm(conv(x)) + residual); `bn_kw` are ops.conv_bn's hints, which only BatchNorm's batch statistics need."""
+    if isinstance(norm, nn.GroupNorm):
+        y = ops.conv(x, weight, bias, kernel, stride, padding)
+        return ops.group_norm(y, norm, "relu" if relu else "none", residual)
+    return ops.conv_bn(x, weight, norm, T, bias, kernel, stride, padding, relu=relu, residual=residual, **bn_kw)
+
+
+def _input_conv_norm(x, weight, norm, T, bias, kernel, stride, padding, layout, dtype, pool=None):
+    """The first layer from the raw clip: convolution, normalisation, ReLU and, with `pool` = (k, s, p), the max-pool."""
+    if isinstance(norm, nn.GroupNorm):
+        a = ops.group_norm(ops.input_conv(x, weight, bias, kernel, stride, padding, layout, dtype), norm, "relu")
+        return _pool_frames(a, *pool) if pool is not None else a
+    return ops.input_conv(x, weight, bias, kernel, stride, padding, layout, dtype, bn=norm, groups=T, relu=True, pool=pool)
+
+
+def _pool_frames(a, k, s, p):
+    """2-D max-pool of every frame of [N, D, H, W, C]."""
+    N, D, H, W, C = a.shape
+    y = ops.max_pool2d(a.view(N * D, H, W, C), k, s, p)
+    return y.view(N, D, *y.shape[1:])
+
+
 def _frames_to_seq(y, T, B):
     """[T*B, E] time-major rows -> [B, T, E] (a view; the memory stays time-major)."""
     return y.view(T, B, y.shape[-1]).transpose(0, 1)
@@ -54,7 +92,7 @@ def _frames_to_seq(y, T, B):
 # --------------------------------------------------------------------------------------
 class EncoderCNN(_HipModule):
     def __init__(self, img_x=224, img_y=224, fc_hidden1=512, fc_hidden2=512, drop_p=0.3, CNN_embed_dim=300,
-                 use_pretrained=False):
+                 use_pretrained=False, norm="batch"):
         super().__init__()
         if use_pretrained:
             raise NotImplementedError("EncoderCNN(use_pretrained=True) needs torchvision's VGG16 weights "
@@ -68,7 +106,7 @@ class EncoderCNN(_HipModule):
         for i, k in enumerate(self.kernels):
             setattr(self, f"conv{i + 1}", nn.Sequential(
                 nn.Conv2d(chans[i], chans[i + 1], kernel_size=k, stride=2, padding=0),
-                nn.BatchNorm2d(chans[i + 1], momentum=0.01), nn.ReLU(inplace=True)))
+                _norm_layer(norm, chans[i + 1], 2, momentum=0.01), nn.ReLU(inplace=True)))
             h, w = conv_out(h, k, 2), conv_out(w, k, 2)
         self.feat_hw = (h, w)
         self.feature_dim = chans[-1] * h * w
@@ -82,10 +120,10 @@ class EncoderCNN(_HipModule):
         for i, k in enumerate(self.kernels):
             blk = getattr(self, f"conv{i + 1}")
             if i == 0:  # 3-channel layer: taps along W folded into the channel axis by the layout kernel
-                a = ops.input_conv(x_3d, blk[0].weight, blk[0].bias, (1, k, k), (1, 2, 2), 0, "clip",
-                                   self.compute_dtype, bn=blk[1], groups=T, relu=True)
+                a = _input_conv_norm(x_3d, blk[0].weight, blk[1], T, blk[0].bias, (1, k, k), (1, 2, 2), 0, "clip",
+                                     self.compute_dtype)
             else:
-                a = ops.conv_bn(a, blk[0].weight, blk[1], T, blk[0].bias, (1, k, k), (1, 2, 2), 0, relu=True)
+                a = _conv_norm(a, blk[0].weight, blk[1], T, blk[0].bias, (1, k, k), (1, 2, 2), 0, relu=True)
         a = ops.mark_cut(a)  # fc1 below holds four fifths of the model's parameters: its gradient bucket completes here
         # flatten(NCHW) + fc1 == a convolution whose kernel covers the whole feature map
         hf, wf = self.feat_hw
@@ -103,20 +141,27 @@ class EncoderCNN(_HipModule):
 class Bottleneck(nn.Module):
     expansion = 4
 
-    def __init__(self, inplanes, planes, stride=1, downsample=None):
+    def __init__(self, inplanes, planes, stride=1, downsample=None, norm="batch"):
         super().__init__()
         self.conv1 = nn.Conv2d(inplanes, planes, 1, bias=False)
-        self.bn1 = nn.BatchNorm2d(planes)
+        self.bn1 = _norm_layer(norm, planes, 2)
         self.conv2 = nn.Conv2d(planes, planes, 3, stride=stride, padding=1, bias=False)
-        self.bn2 = nn.BatchNorm2d(planes)
+        self.bn2 = _norm_layer(norm, planes, 2)
         self.conv3 = nn.Conv2d(planes, planes * 4, 1, bias=False)
-        self.bn3 = nn.BatchNorm2d(planes * 4)
+        self.bn3 = _norm_layer(norm, planes * 4, 2)
         self.relu = nn.ReLU(inplace=True)
         self.downsample = downsample
         self.stride = stride
 
     def run(self, x, T):
         s = self.stride
+        if isinstance(self.bn1, nn.GroupNorm):
+            idt = x
+            if self.downsample is not None:
+                idt = _conv_norm(x, self.downsample[0].weight, self.downsample[1], T, None, 1, (1, s, s), 0)
+            a = _conv_norm(x, self.conv1.weight, self.bn1, T, relu=True)
+            a = _conv_norm(a, self.conv2.weight, self.bn2, T, None, (1, 3, 3), (1, s, s), (0, 1, 1), relu=True)
+            return _conv_norm(a, self.conv3.weight, self.bn3, T, relu=True, residual=idt)
         # x feeds conv1 and the shortcut: both backward paths add into one gradient buffer (no add pass)
         join = ops.GradJoin(2, getattr(x, "_vc_bn_tail", None)) if (x.requires_grad and torch.is_grad_enabled()) else None
         idt = None
@@ -139,10 +184,10 @@ class Bottleneck(nn.Module):
 RESNET_LAYERS = {"resnet50": (3, 4, 6, 3), "resnet101": (3, 4, 23, 3), "resnet152": (3, 8, 36, 3)}
 
 
-def make_resnet_trunk(arch="resnet152", width=64):
+def make_resnet_trunk(arch="resnet152", width=64, norm="batch"):
     """Children 0..8 = conv1, bn1, relu, maxpool, layer1..4, avgpool, i.e. the layout of
     ``nn.Sequential(*list(resnet.children())[:-1])`` (reference model_components.py:164-165).  `width` = channels of
-    the stem (64 in torchvision's networks; a multiple of 8)."""
+    the stem (64 in torchvision's networks; a multiple of 8).  `norm`: "batch", or "group" for GroupNorm in its place."""
     inplanes = width
     stages = []
     for i, (planes, n) in enumerate(zip((width, 2 * width, 4 * width, 8 * width), RESNET_LAYERS[arch])):
@@ -151,11 +196,12 @@ def make_resnet_trunk(arch="resnet152", width=64):
             s = (1 if i == 0 else 2) if b == 0 else 1
             ds = None
             if b == 0 and (s != 1 or inplanes != planes * 4):
-                ds = nn.Sequential(nn.Conv2d(inplanes, planes * 4, 1, stride=s, bias=False), nn.BatchNorm2d(planes * 4))
-            blocks.append(Bottleneck(inplanes, planes, s, ds))
+                ds = nn.Sequential(nn.Conv2d(inplanes, planes * 4, 1, stride=s, bias=False),
+                                   _norm_layer(norm, planes * 4, 2))
+            blocks.append(Bottleneck(inplanes, planes, s, ds, norm))
             inplanes = planes * 4
         stages.append(nn.Sequential(*blocks))
-    trunk = nn.Sequential(nn.Conv2d(3, width, 7, stride=2, padding=3, bias=False), nn.BatchNorm2d(width),
+    trunk = nn.Sequential(nn.Conv2d(3, width, 7, stride=2, padding=3, bias=False), _norm_layer(norm, width, 2),
                           nn.ReLU(inplace=True), nn.MaxPool2d(3, stride=2, padding=1), *stages,
                           nn.AdaptiveAvgPool2d((1, 1)))
     for m in trunk.modules():
@@ -167,8 +213,8 @@ def make_resnet_trunk(arch="resnet152", width=64):
 def run_resnet_trunk(trunk, x_3d, T, dtype):
     """x_3d: raw fp32 clip [B,T,3,H,W] -> pooled features [T*B, 2048] (frames time-major)."""
     # conv1 -> bn1 -> relu -> maxpool(3, 2, 1): the last three are one pass (the 112 x 112 activation is never written)
-    a = ops.input_conv(x_3d, trunk[0].weight, None, (1, 7, 7), (1, 2, 2), (0, 3, 3), "clip", dtype, bn=trunk[1],
-                       groups=T, relu=True, pool=(3, 2, 1))
+    a = _input_conv_norm(x_3d, trunk[0].weight, trunk[1], T, None, (1, 7, 7), (1, 2, 2), (0, 3, 3), "clip", dtype,
+                         pool=(3, 2, 1))
     for li in range(4, 8):
         for blk in trunk[li]:
             a = blk.run(a, T)
@@ -179,33 +225,39 @@ def run_resnet_trunk(trunk, x_3d, T, dtype):
 
 
 class _HeadBN(_HipModule):
-    def _make_head(self, feat, h1, h2, embed):
+    def _make_head(self, feat, h1, h2, embed, norm="batch"):
         self.fc1 = nn.Linear(feat, h1)
-        self.bn1 = nn.BatchNorm1d(h1, momentum=0.01)
+        self.bn1 = _norm_layer(norm, h1, 1, momentum=0.01)
         self.fc2 = nn.Linear(h1, h2)
-        self.bn2 = nn.BatchNorm1d(h2, momentum=0.01)
+        self.bn2 = _norm_layer(norm, h2, 1, momentum=0.01)
         self.fc3 = nn.Linear(h2, embed)
         self._embed = embed
 
+    @staticmethod
+    def _head_norm(y, norm, T):
+        if isinstance(norm, nn.GroupNorm):
+            return ops.group_norm(y, norm, "relu")
+        return ops.batch_norm(y, norm, T, relu=True)
+
     def _head(self, f, T, drop_after_first):
-        y = ops.batch_norm(ops.linear(f, self.fc1.weight, self.fc1.bias), self.bn1, T, relu=True)
+        y = self._head_norm(ops.linear(f, self.fc1.weight, self.fc1.bias), self.bn1, T)
         if drop_after_first:
             y = ops.dropout(y, self.drop_p, self.training)
-        y = ops.batch_norm(ops.linear(y, self.fc2.weight, self.fc2.bias), self.bn2, T, relu=True)
+        y = self._head_norm(ops.linear(y, self.fc2.weight, self.fc2.bias), self.bn2, T)
         y = ops.dropout(y, self.drop_p, self.training)
         return ops.linear(y, self.fc3.weight, self.fc3.bias, out_f32=True)[:, :self._embed]
 
 
 class ResCNNEncoder(_HeadBN):
     def __init__(self, fc_hidden1=512, fc_hidden2=512, drop_p=0.3, CNN_embed_dim=300, use_pretrained=True,
-                 arch="resnet152", width=64):
+                 arch="resnet152", width=64, norm="batch"):
         super().__init__()
         # The reference downloads ImageNet weights when use_pretrained is set (model_components.py:157-162);
         # here the trunk always starts from torchvision's random initialisation and pretrained weights, if
         # wanted, arrive through load_state_dict (same keys).
         self.fc_hidden1, self.fc_hidden2, self.drop_p = fc_hidden1, fc_hidden2, drop_p
-        self.resnet = make_resnet_trunk(arch, width)
-        self._make_head(32 * width, fc_hidden1, fc_hidden2, CNN_embed_dim)
+        self.resnet = make_resnet_trunk(arch, width, norm)
+        self._make_head(32 * width, fc_hidden1, fc_hidden2, CNN_embed_dim, norm)
 
     def forward(self, x_3d):
         B, T = x_3d.shape[0], x_3d.shape[1]
@@ -225,11 +277,19 @@ class DecoderRNN(_HipModule):
         self.fc1 = nn.Linear(h_RNN, h_FC_dim)
         self.fc2 = nn.Linear(h_FC_dim, num_classes)
 
-    def forward(self, x_RNN):
+    @property
+    def classifier(self):
+        return self.fc2
+
+    def forward_features(self, x_RNN):
+        """The rows the last layer classifies."""
         x_tm = ops.cast_ag(x_RNN.transpose(0, 1).contiguous(), self.compute_dtype)   # [T,B,E]
         seq = ops.lstm(x_tm, self.LSTM)                                              # [T,B,H]
         y = ops.linear(seq[-1], self.fc1.weight, self.fc1.bias, relu=True)
-        y = ops.dropout(y, self.drop_p, self.training)
+        return ops.dropout(y, self.drop_p, self.training)
+
+    def forward(self, x_RNN):
+        y = self.forward_features(x_RNN)
         return ops.linear(y, self.fc2.weight, self.fc2.bias, out_f32=True)[:, :self.num_classes]
 
 
@@ -246,13 +306,20 @@ class TCG_LSTM(_HipModule):
         self.fc = nn.Sequential(nn.Linear(2 * hidden, 256), nn.ReLU(True), nn.Dropout(drop),
                                 nn.Linear(256, num_classes))
 
-    def forward(self, g, c):
+    @property
+    def classifier(self):
+        return self.fc[3]
+
+    def forward_features(self, g, c):
         s_in, l_in = ops.tcg_inputs(g, c, self.down, self.compute_dtype)
         h_s = ops.lstm(s_in, self.lstm_short)          # [T,B,2H]
         h_l = ops.lstm(l_in, self.lstm_long)           # [Tl,B,H]
         clip = ops.tcg_fuse(h_s, h_l, self.gate[0])    # [B,2H]
         y = ops.linear(clip, self.fc[0].weight, self.fc[0].bias, relu=True)
-        y = ops.dropout(y, self.drop, self.training)
+        return ops.dropout(y, self.drop, self.training)
+
+    def forward(self, g, c):
+        y = self.forward_features(g, c)
         return ops.linear(y, self.fc[3].weight, self.fc[3].bias, out_f32=True)[:, :self.num_classes]
 
 
@@ -262,9 +329,10 @@ class TCG_LSTM(_HipModule):
 class Conv3DModel(_HipModule):
     def __init__(self, config):
         super().__init__()
+        norm = getattr(config, "norm", "batch")
         mods, cin = [], 1
         for cout in (32, 64, 128, 256):
-            mods += [nn.Conv3d(cin, cout, kernel_size=(3, 3, 3), padding=(1, 1, 1)), nn.BatchNorm3d(cout),
+            mods += [nn.Conv3d(cin, cout, kernel_size=(3, 3, 3), padding=(1, 1, 1)), _norm_layer(norm, cout, 3),
                      nn.ReLU(inplace=True), nn.MaxPool3d(kernel_size=(1, 2, 2))]
             cin = cout
         mods.append(nn.AdaptiveAvgPool3d((1, 1, 1)))
@@ -273,21 +341,29 @@ class Conv3DModel(_HipModule):
         self.fc = nn.Sequential(nn.Dropout(config.dropout_p), nn.Linear(256, 512), nn.ReLU(),
                                 nn.Dropout(config.dropout_p), nn.Linear(512, config.num_classes))
 
-    def forward(self, x):
+    @property
+    def classifier(self):
+        return self.fc[4]
+
+    def forward_features(self, x):
         a = None
         for i in range(4):
             cv, bn = self.conv3d[4 * i], self.conv3d[4 * i + 1]
             # BatchNorm3d + ReLU + MaxPool3d((1,2,2)) as one pass: the pool never crosses the depth axis
             if i == 0:  # 1-channel layer straight from the fp32 volume (W taps folded into the channel axis)
-                a = ops.input_conv(x, cv.weight, cv.bias, 3, 1, 1, "volume", self.compute_dtype, bn=bn, groups=1,
-                                   relu=True, pool=(2, 2, 0))
+                a = _input_conv_norm(x, cv.weight, bn, 1, cv.bias, 3, 1, 1, "volume", self.compute_dtype, pool=(2, 2, 0))
+            elif isinstance(bn, nn.GroupNorm):
+                a = _pool_frames(_conv_norm(a, cv.weight, bn, 1, cv.bias, 3, 1, 1, relu=True), 2, 2, 0)
             else:
                 a = ops.conv_bn(a, cv.weight, bn, 1, cv.bias, 3, 1, 1, relu=True, pool=(2, 2, 0))
         B, D, H, W, C = a.shape
         f = ops.global_avg_pool(a.view(B, D * H * W, C))
         f = ops.dropout(f, self.dropout_p, self.training)
         y = ops.linear(f, self.fc[1].weight, self.fc[1].bias, relu=True)
-        y = ops.dropout(y, self.dropout_p, self.training)
+        return ops.dropout(y, self.dropout_p, self.training)
+
+    def forward(self, x):
+        y = self.forward_features(x)
         return ops.linear(y, self.fc[4].weight, self.fc[4].bias, out_f32=True)[:, :self.num_classes]
 
 
@@ -303,13 +379,22 @@ class _EncDec(_HipModule):
         out = self.encoder(x)
         return self.decoder(*out) if isinstance(out, tuple) else self.decoder(out)
 
+    @property
+    def classifier(self):
+        return self.decoder.classifier
+
+    def forward_features(self, x):
+        """What the classifier takes: everything but the last linear layer."""
+        out = self.encoder(x)
+        return self.decoder.forward_features(*out) if isinstance(out, tuple) else self.decoder.forward_features(out)
+
 
 class CRNNModel(_EncDec):
     def __init__(self, config):
         super().__init__(
             EncoderCNN(img_x=config.img_x, img_y=config.img_y, fc_hidden1=config.CNN_fc_hidden1,
                        fc_hidden2=config.CNN_fc_hidden2, drop_p=config.dropout_p, CNN_embed_dim=config.CNN_embed_dim,
-                       use_pretrained=getattr(config, "use_pretrained", False)),
+                       use_pretrained=getattr(config, "use_pretrained", False), norm=getattr(config, "norm", "batch")),
             DecoderRNN(CNN_embed_dim=config.CNN_embed_dim, h_RNN_layers=config.RNN_hidden_layers,
                        h_RNN=config.RNN_hidden_nodes, h_FC_dim=config.RNN_FC_dim, drop_p=config.dropout_p,
                        num_classes=config.num_classes))
@@ -320,7 +405,7 @@ class ResNetCRNNModel(_EncDec):
         super().__init__(
             ResCNNEncoder(fc_hidden1=config.CNN_fc_hidden1, fc_hidden2=config.CNN_fc_hidden2, drop_p=config.dropout_p,
                           CNN_embed_dim=config.CNN_embed_dim, use_pretrained=getattr(config, "use_pretrained", True),
-                          arch=getattr(config, "arch", "resnet152")),
+                          arch=getattr(config, "arch", "resnet152"), norm=getattr(config, "norm", "batch")),
             DecoderRNN(CNN_embed_dim=config.CNN_embed_dim, h_RNN_layers=config.RNN_hidden_layers,
                        h_RNN=config.RNN_hidden_nodes, h_FC_dim=config.RNN_FC_dim, drop_p=config.dropout_p,
                        num_classes=config.num_classes))

@@ -1957,14 +1957,14 @@ def _ns_bounds(coeffs):
     return cap, gain, 1.02 * pmax
 
 
-def newton_schulz(g, steps=5, coeffs=NS_COEFFS, eps=1e-7):
+def newton_schulz(g, steps=5, coeffs=NS_COEFFS, eps=1e-7, inplace=False):
     """Orthogonalises matrices by `steps` Newton-Schulz products: X = G / (|G|_F + eps), then X <- a X + b (X X^T) X +
     c (X X^T)^2 X, which drives every singular value towards 1 (the update of the Muon optimizer).
 
     g: a tensor [..., m, n], or a list or tuple of such tensors of any shapes (all of one type, float32 or bfloat16, on one
     device); all their matrices go through the same launches.  coeffs: (a, b, c), or `steps` such triples.  Returns new
-    tensors of g's structure, shapes and type; products are carried at float32 accuracy whatever the type.  Not
-    differentiable: gradients are its input."""
+    tensors of g's structure, shapes and type, or with `inplace` the (dense) tensors of g themselves; products are carried
+    at float32 accuracy whatever the type.  Not differentiable: gradients are its input."""
     single = isinstance(g, torch.Tensor)
     items = [g] if single else list(g)
     if not items:
@@ -1989,11 +1989,13 @@ def newton_schulz(g, steps=5, coeffs=NS_COEFFS, eps=1e-7):
             raise RuntimeError(f"newton_schulz: a matrix needs two dimensions, got {tuple(t.shape)}")
         if t.dtype != first.dtype:
             raise TypeError(f"newton_schulz: matrices of {first.dtype} and {t.dtype} in one call")
+        if inplace and (not t.is_contiguous() or (t.requires_grad and torch.is_grad_enabled())):
+            raise RuntimeError("newton_schulz: in place needs dense tensors outside the autograd graph")
     code = L.dtype_code(first.dtype)
     _same_device("newton_schulz", first, *items)
     with torch.cuda.device(first.device), torch.no_grad():
         srcs = [t.detach().contiguous() for t in items]
-        outs = [torch.empty_like(t) for t in srcs]
+        outs = items if inplace else [torch.empty_like(t) for t in srcs]
         gp, op, rows, cols = [], [], [], []
         for s, o in zip(srcs, outs):
             m, n = s.shape[-2:]

@@ -28,8 +28,9 @@ class FlatParams:
 
     ALIGN = 64  # elements: every parameter starts on a 256-byte boundary
 
-    def __init__(self, model):
-        params = [p for p in model.parameters() if p.requires_grad]
+    def __init__(self, model, params=None):
+        """params: the model's trainable parameters in the order they are to have (default: registration order)."""
+        params = list(params) if params is not None else [p for p in model.parameters() if p.requires_grad]
         if not params:
             raise ValueError("model has no trainable parameters")
         dev = params[0].device
@@ -187,6 +188,113 @@ class FusedOptimizer(torch.optim.Optimizer):
         self.sync_lr()
 
 
+class MuonOptimizer(FusedOptimizer):
+    """Muon: momentum whose matrices are orthogonalised by Newton-Schulz products (ops.newton_schulz) before they become the
+    update, so that every direction of a weight moves alike; AdamW for everything that is not a matrix.
+
+    A parameter of two or more dimensions is a matrix [shape[0], rest] unless it has a single row or column, its name
+    contains one of `adam_names`, or it belongs to the model's ``classifier`` (the last layer's rows are classes, not
+    directions).  The update is lr * 0.2 * sqrt(max(rows, cols)) * orthogonalised momentum, whose entries have the size
+    of an AdamW update, so one learning rate serves both; weight decay is decoupled.  Matrices come first in the flat
+    buffers: [matrices | the rest], each part updated by its own launches."""
+
+    def __init__(self, model, lr=1e-3, weight_decay=1e-2, betas=(0.9, 0.999), eps=1e-8, momentum=0.95, nesterov=True,
+                 steps=5, adam_names=("relative_position_bias_table",)):
+        if not 0.0 <= momentum < 1.0 or int(steps) < 0:
+            raise ValueError(f"MuonOptimizer: momentum {momentum} outside [0, 1) or steps {steps} negative")
+        head = getattr(model, "classifier", None)
+        skip = {id(p) for p in head.parameters()} if isinstance(head, nn.Module) else set()
+        named = [(n, p) for n, p in model.named_parameters() if p.requires_grad]
+
+        def matrix(n, p):
+            return p.dim() >= 2 and min(p.shape[0], p.numel() // p.shape[0]) > 1 and id(p) not in skip and \
+                not any(a in n for a in adam_names)
+
+        mats = [p for n, p in named if matrix(n, p)]
+        rest = [p for n, p in named if not matrix(n, p)]
+        self.flat = FlatParams(model, mats + rest)
+        self.mode, self.n_mats = None, len(mats)
+        defaults = dict(lr=lr, weight_decay=1e-2 if weight_decay is None else weight_decay, betas=betas, eps=eps,
+                        momentum=momentum, nesterov=bool(nesterov), ns_steps=int(steps))
+        torch.optim.Optimizer.__init__(self, self.flat.params, defaults)
+        dev = self.flat.data.device
+        self.split = self.flat.offsets[len(mats)] if rest else self.flat.total  # first element of the rest
+        self.m = torch.zeros_like(self.flat.data)
+        self.v = torch.zeros(self.flat.total - self.split, device=dev)
+        self.update = torch.zeros(self.split, device=dev)
+        self.update_mats = [self.flat.view_of(self.update, i).view(p.shape[0], -1) for i, p in enumerate(mats)]
+        scale = torch.zeros(self.split // FlatParams.ALIGN)
+        for i, u in enumerate(self.update_mats):
+            o = self.flat.offsets[i] // FlatParams.ALIGN
+            scale[o:o + (u.numel() + FlatParams.ALIGN - 1) // FlatParams.ALIGN] = 0.2 * max(u.shape) ** 0.5
+        self.scale = scale.to(dev)
+        self.steps = 0
+        self.grad_scale = 1.0
+        self.bucketer = None
+        self.step_dev = torch.zeros(1, device=dev, dtype=torch.int64)
+        self.lr_dev = torch.full((1,), float(lr), device=dev, dtype=torch.float32)
+        self._lr_host = float(lr)
+        self._bind_state()
+
+    def _v_of(self, i):
+        o, p = self.flat.offsets[i] - self.split, self.flat.params[i]
+        return self.v[o:o + p.numel()].view(p.shape)
+
+    def _bind_state(self):
+        for i, p in enumerate(self.flat.params):
+            if i < self.n_mats:
+                self.state[p] = {"momentum_buffer": self.flat.view_of(self.m, i)}
+            else:
+                self.state[p] = {"step": torch.tensor(float(self.steps)), "exp_avg": self.flat.view_of(self.m, i),
+                                 "exp_avg_sq": self._v_of(i)}
+
+    def launch(self):
+        g = self.param_groups[0]
+        flat, k = self.flat, self.split
+        b1, b2 = g["betas"]
+        L.call("vc_counter_add", L.ptr(self.step_dev), L.i64(1), L.stream())
+        if k:
+            L.call("vc_muon_momentum", L.ptr(flat.grad), L.ptr(self.m), L.ptr(self.update), L.i64(k), float(g["momentum"]),
+                   int(g["nesterov"]), float(self.grad_scale), L.stream())
+            ops.newton_schulz(self.update_mats, steps=g["ns_steps"], inplace=True)
+            L.call("vc_muon_apply", L.ptr(flat.data), L.ptr(self.update), L.ptr(self.scale), L.i64(k), L.ptr(self.lr_dev),
+                   float(g["weight_decay"]), L.stream())
+        if k < flat.total:
+            L.call("vc_optim_step", 1, L.ptr(flat.data[k:]), L.ptr(flat.grad[k:]), L.ptr(self.m[k:]), L.ptr(self.v),
+                   L.i64(flat.total - k), float(g["lr"]), float(b1), float(b2), float(g["eps"]), float(g["weight_decay"]), 0,
+                   float(self.grad_scale), L.ptr(self.lr_dev), L.ptr(self.step_dev), L.stream())
+        ops.advance_seed_counter(flat.data.device)
+
+    def after_step(self):
+        self.steps += 1
+        for p in self.flat.params[self.n_mats:]:
+            self.state[p]["step"] += 1
+        ops.bump_weights_epoch()
+
+    def state_dict(self):
+        sd = super().state_dict()
+        sd["muon_steps"] = self.steps  # there may be no AdamW parameter to carry it
+        return sd
+
+    def load_state_dict(self, state_dict):
+        state_dict = dict(state_dict)
+        steps = state_dict.pop("muon_steps", None)
+        torch.optim.Optimizer.load_state_dict(self, state_dict)
+        seen = 0
+        for i, p in enumerate(self.flat.params):
+            st = self.state[p]
+            pairs = [("momentum_buffer", self.flat.view_of(self.m, i))] if i < self.n_mats else \
+                [("exp_avg", self.flat.view_of(self.m, i)), ("exp_avg_sq", self._v_of(i))]
+            for key, view in pairs:
+                view.copy_(st[key]) if key in st else view.zero_()
+            seen = max(seen, int(st["step"])) if "step" in st else seen
+        self.steps = int(steps) if steps is not None else seen
+        self._bind_state()
+        self.step_dev.fill_(self.steps)
+        self._lr_host = None
+        self.sync_lr()
+
+
 def set_deterministic(seed=42):
     """Seeds Python, numpy and torch and makes every step repeat bit for bit on the device (reference:
     utils/common/training_utils.py:27-35, whose cudnn.deterministic = True is ops.set_deterministic here)."""
@@ -202,7 +310,10 @@ def set_deterministic(seed=42):
 
 
 def get_optimizer(model, optimizer_name="adam", lr=0.001, weight_decay=1e-4):
-    """Same factory signature as the reference (training_utils.py:311-331)."""
+    """Same factory signature as the reference (training_utils.py:311-331); besides its "adam", "adamw" and "sgd" also
+    "muon" (MuonOptimizer)."""
+    if optimizer_name.lower() == "muon":
+        return MuonOptimizer(model, lr=lr, weight_decay=weight_decay)
     return FusedOptimizer(model, optimizer_name, lr=lr, weight_decay=weight_decay)
 
 
@@ -381,8 +492,34 @@ class FusedCrossEntropyLoss(nn.Module):
         return ops.cross_entropy(output, target, self.stats)
 
 
+class LinearCrossEntropyLoss(FusedCrossEntropyLoss):
+    """Cross entropy with the model's last linear layer inside it (ops.linear_cross_entropy), for label sets whose logits
+    should not be kept: takes ``model.forward_features(x)`` instead of ``model(x)``, which the epoch loops and the graphed
+    step hand it.  `model` needs ``forward_features`` and ``classifier`` (an nn.Linear), as the models of this package
+    have."""
+
+    takes_features = True
+
+    def __init__(self, model, ignore_index=-100, label_smoothing=0.0):
+        super().__init__()
+        if not isinstance(getattr(model, "classifier", None), nn.Linear) or not hasattr(model, "forward_features"):
+            raise TypeError("LinearCrossEntropyLoss: the model has no classifier layer / forward_features")
+        object.__setattr__(self, "_model", model)  # not a child: the layer stays the model's
+        self.ignore_index, self.label_smoothing = ignore_index, label_smoothing
+
+    def forward(self, features, target):
+        lin = self._model.classifier
+        return ops.linear_cross_entropy(features[..., :lin.in_features], lin.weight, lin.bias, target.reshape(features.shape[:-1]),
+                                        self.ignore_index, self.label_smoothing, stats=self.stats)
+
+
+def forward_for(model, criterion, x):
+    """What `criterion` takes of the model: its logits, or the features in front of the last layer."""
+    return model.forward_features(x) if getattr(criterion, "takes_features", False) else model(x)
+
+
 def _run_batch(model, data, target, criterion):
-    output = model(data)
+    output = forward_for(model, criterion, data)
     loss = criterion(output, target.squeeze())
     if isinstance(criterion, FusedCrossEntropyLoss):
         correct = criterion.stats["correct"]
