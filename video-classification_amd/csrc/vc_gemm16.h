@@ -5,12 +5,17 @@
 // bits in all (an absolute floor of 2^-25 of the scaled unit), and the product is hi*hi + hi*lo + lo*hi: three MFMA of
 // the 2.5 PFLOP/s kind per product against the 157 TFLOP/s of the fp32 matrix instructions, at fp32's accuracy.
 //
-// Layout: rows of `ld` elements, ld a multiple of 64 with zeros behind the last column, the second term one `plane`
-// behind the first.  Four waves in a 2 x 2 grid own 64 x 64 each.  Two LDS stages of (PA + PB) x 128 rows x BK elements
-// (BK = 64 for single terms, 32 otherwise, so at most 32 KiB a stage and two workgroups per CU); a stage's rows hold
-// their 16-byte chunks permuted so that the 16 rows of a fragment read fall into 16 different 16-byte slots of the 256-byte
-// bank row.  Stages are filled by LDS-DMA requests in opaque assembly (with the builtin the compiler waits for every
-// outstanding request before each LDS read); rows beyond the matrix lie outside the buffer descriptor and read as zero.
+// An operand is stored with the reduction along its rows (ROW: [tile side][k], rows of `ld` elements, ld a multiple of
+// 64 with zeros behind the last column) or across them (COL: [k][tile side], ld a multiple of 8; it is then read from LDS
+// with the transposing ds_read_b64_tr_b16, so no operand is ever copied into the other order).  The second term lies one
+// `plane` behind the first.
+//
+// Four waves in a 2 x 2 grid own 64 x 64 each.  Two LDS stages of (PA + PB) x 128 x BK elements (BK = 64 for single terms,
+// 32 otherwise, so at most 32 KiB a stage and two workgroups per CU).  ROW stages permute the 16-byte chunks of a row so
+// that the 16 rows of a fragment read fall into 16 different slots of the 256-byte bank row; COL stages permute the
+// 32-byte blocks of a row so that the eight rows of a transposing read fall on different groups of banks.  Stages are
+// filled by LDS-DMA requests in opaque assembly (with the builtin the compiler waits for every outstanding request
+// before each LDS read); what lies behind the operand's last row falls outside its buffer descriptor and reads as zero.
 #pragma once
 #include "vc_common.h"
 
@@ -33,16 +38,26 @@ __device__ __forceinline__ void g16_dma(const i32x4_t& rs, unsigned lds_byte, un
 __device__ __forceinline__ unsigned g16_lds(const void* p) {
   return (unsigned)(size_t)(__attribute__((address_space(3))) const void*)p;
 }
-// buffer descriptor of `rows` rows of ld elements at p (wave-uniform); the range check yields zeros behind them
-__device__ __forceinline__ i32x4_t g16_desc(const f16* p, int rows, int ld) {
+// buffer descriptor of `bytes` bytes at p (wave-uniform); reads behind them yield zero
+__device__ __forceinline__ i32x4_t g16_desc(const f16* p, unsigned bytes) {
   const uint64_t u = (uint64_t)p;
   i32x4_t d;
   d[0] = __builtin_amdgcn_readfirstlane((int)u);
   d[1] = __builtin_amdgcn_readfirstlane((int)(u >> 32));
-  d[2] = __builtin_amdgcn_readfirstlane((int)((unsigned)(rows < GM ? rows : GM) * (unsigned)ld * 2u));
+  d[2] = __builtin_amdgcn_readfirstlane((int)bytes);
   d[3] = 0x00020000;
   return d;
 }
+
+enum { ROW = 0, COL = 1 };
+
+// One operand of a tile.  ROW: p = the tile's first row, n = rows from there on.  COL: p = row 0 of the matrix, side = the
+// tile's first column, n = rows (the true length of the reduction).
+struct Op16 {
+  const f16* p;
+  int64_t plane;
+  int ld, n, side;
+};
 
 // A value of 22 bits in two fp16 terms.
 __device__ __forceinline__ void f16_split(float v, f16& hi, f16& lo) {
@@ -50,50 +65,85 @@ __device__ __forceinline__ void f16_split(float v, f16& hi, f16& lo) {
   lo = (f16)(v - (float)hi);
 }
 
-template <int PA, int PB>
+template <int PA, int PB, int KA = ROW, int KB = ROW>
 struct G16 {
   static constexpr int BK = PA + PB == 2 ? 64 : 32;
   static constexpr int PLANE = GM * BK;              // elements of one plane of a stage
   static constexpr int STAGE = (PA + PB) * PLANE;
   static constexpr int LDS = 2 * STAGE;              // elements of shared memory
-  static constexpr int CH = BK / 8;                  // 16-byte chunks of a row
-  static constexpr int RPI = 64 / CH;                // rows one wave request fills
-  static constexpr int REQ = GM / RPI / 4;           // requests per wave, plane and stage
+  static constexpr int CH = BK / 8;                  // 16-byte chunks of a ROW stage's row
+  static constexpr int RPI = 64 / CH;                // rows of it that one wave request fills
+  static constexpr int REQ = BK / 16;                // requests per wave, plane and stage (1 KiB each)
 
-  __device__ static __forceinline__ int swz(int row) { return BK == 64 ? (row >> 1) & 7 : (row >> 2) & 3; }
+  __device__ static __forceinline__ int rswz(int row) { return BK == 64 ? (row >> 1) & 7 : (row >> 2) & 3; }
+  __device__ static __forceinline__ int cswz(int row) { return (row & 3) | ((row >> 1) & 4); }
 
-  // acc[i][j][r] += sum over k in [k0, k1) for A row wm*64 + i*16 + (lane>>4)*4 + r and B row wn*64 + j*16 + (lane&15)
-  // of the tile whose first rows a and b point at, `ar` / `br` rows of them present.  k0, k1 multiples of BK.  The LDS is
-  // free again for the caller when the function returns.
-  __device__ static __forceinline__ void run(f32x4 (&acc)[4][4], const f16* a, int64_t aplane, int lda, int ar,
-                                             const f16* b, int64_t bplane, int ldb, int br, int k0, int k1, f16* smem) {
+  // byte offset of this lane's 16 bytes of request t, relative to the tile's corner of the k-step
+  template <int KIND>
+  __device__ static __forceinline__ unsigned src_off(int t, int wave, int lane, int ld) {
+    if (KIND == ROW) {
+      const int row = (t * 4 + wave) * RPI + lane / CH;
+      return (unsigned)row * (unsigned)ld * 2u + (unsigned)((lane % CH) ^ rswz(row)) * 16u;
+    }
+    const int row = (t * 4 + wave) * 4 + (lane >> 4), pos = lane & 15;
+    return (unsigned)row * (unsigned)ld * 2u + (unsigned)((((pos >> 1) ^ cswz(row)) << 1) | (pos & 1)) * 16u;
+  }
+
+  template <int KIND>
+  __device__ static __forceinline__ void stage_op(const Op16& o, int plane, unsigned lds, const unsigned (&v)[REQ], int k) {
+    if (KIND == ROW) {
+      const i32x4_t d = g16_desc(o.p + plane * o.plane, (unsigned)(o.n < GM ? o.n : GM) * (unsigned)o.ld * 2u);
+#pragma unroll
+      for (int t = 0; t < REQ; ++t) g16_dma(d, lds + t * 4096, v[t], k * 2);
+    } else {
+      const int rows = o.n - k < BK ? o.n - k : BK;
+      const i32x4_t d = g16_desc(o.p + plane * o.plane + (int64_t)k * o.ld + o.side,
+                                 rows > 0 ? (unsigned)rows * (unsigned)o.ld * 2u - (unsigned)o.side * 2u : 0u);
+#pragma unroll
+      for (int t = 0; t < REQ; ++t) g16_dma(d, lds + t * 4096, v[t], 0);
+    }
+  }
+
+  // fragment of the 16 tile rows (ROW) or columns (COL) of block `blk` (0..7), 32 reduction elements from kk * 32
+  template <int KIND>
+  __device__ static __forceinline__ f16x8 frag(const f16* st, int blk, int kk, int lane) {
+    const int l15 = lane & 15, q = lane >> 4;
+    if (KIND == ROW) {
+      const int row = blk * 16 + l15;
+      return *reinterpret_cast<const f16x8*>(st + row * BK + (((kk * 4 + q) ^ rswz(row)) << 3));
+    }
+    typedef short s16x4_t __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4_t lds4;
+    const int r0 = 8 * q + ((lane >> 2) & 3);  // this lane supplies row r0, columns 4 (lane & 3) .. + 3, then row r0 + 4
+    const f16* p = st + (kk * 32 + r0) * GM + ((blk ^ cswz(r0)) << 4) + (lane & 3) * 4;
+    union {
+      s16x4_t h[2];
+      f16x8 v;
+    } u;
+    u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p));
+    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 4 * GM));
+    return u.v;
+  }
+
+  // acc[i][j][r] += sum over k in [k0, k1) of A's tile row wm*64 + i*16 + (lane>>4)*4 + r and B's tile row wn*64 + j*16 +
+  // (lane&15).  k0, k1 multiples of BK.  The LDS is free again for the caller when the function returns.
+  __device__ static __forceinline__ void run(f32x4 (&acc)[4][4], const Op16& a, const Op16& b, int k0, int k1, f16* smem) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wm = wave >> 1, wn = wave & 1, l15 = lane & 15, q = lane >> 4;
-    i32x4_t da[PA], db[PB];
-#pragma unroll
-    for (int p = 0; p < PA; ++p) da[p] = g16_desc(a + p * aplane, ar, lda);
-#pragma unroll
-    for (int p = 0; p < PB; ++p) db[p] = g16_desc(b + p * bplane, br, ldb);
+    const int wm = wave >> 1, wn = wave & 1;
     unsigned va[REQ], vb[REQ];
 #pragma unroll
     for (int t = 0; t < REQ; ++t) {
-      const int row = (t * 4 + wave) * RPI + lane / CH, c = (lane % CH) ^ swz(row);
-      va[t] = (unsigned)row * (unsigned)lda * 2u + c * 16u;
-      vb[t] = (unsigned)row * (unsigned)ldb * 2u + c * 16u;
+      va[t] = src_off<KA>(t, wave, lane, a.ld);
+      vb[t] = src_off<KB>(t, wave, lane, b.ld);
     }
     auto stage = [&](int s, int k) {
-      f16* base = smem + s * STAGE + wave * RPI * BK;
+      const unsigned base = g16_lds(smem + s * STAGE) + wave * 1024;
 #pragma unroll
-      for (int p = 0; p < PA; ++p)
+      for (int p = 0; p < PA; ++p) stage_op<KA>(a, p, base + p * PLANE * 2, va, k);
 #pragma unroll
-        for (int t = 0; t < REQ; ++t) g16_dma(da[p], g16_lds(base + p * PLANE + t * 4 * RPI * BK), va[t], k * 2);
-#pragma unroll
-      for (int p = 0; p < PB; ++p)
-#pragma unroll
-        for (int t = 0; t < REQ; ++t) g16_dma(db[p], g16_lds(base + (PA + p) * PLANE + t * 4 * RPI * BK), vb[t], k * 2);
+      for (int p = 0; p < PB; ++p) stage_op<KB>(b, p, base + (PA + p) * PLANE * 2, vb, k);
     };
-    const int arow = wm * 64 + l15, brow = wn * 64 + l15;
     k0 = __builtin_amdgcn_readfirstlane(k0);
     k1 = __builtin_amdgcn_readfirstlane(k1);
     int s = 0;
@@ -109,13 +159,10 @@ struct G16 {
         f16x8 fa[PA][4], fb[PB][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int ra = arow + i * 16, rb = brow + i * 16;
 #pragma unroll
-          for (int p = 0; p < PA; ++p)
-            fa[p][i] = *reinterpret_cast<const f16x8*>(st + p * PLANE + ra * BK + (((kk * 4 + q) ^ swz(ra)) << 3));
+          for (int p = 0; p < PA; ++p) fa[p][i] = frag<KA>(st + p * PLANE, wm * 4 + i, kk, lane);
 #pragma unroll
-          for (int p = 0; p < PB; ++p)
-            fb[p][i] = *reinterpret_cast<const f16x8*>(st + (PA + p) * PLANE + rb * BK + (((kk * 4 + q) ^ swz(rb)) << 3));
+          for (int p = 0; p < PB; ++p) fb[p][i] = frag<KB>(st + (PA + p) * PLANE, wn * 4 + i, kk, lane);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)

@@ -19,7 +19,7 @@
 
 namespace {
 
-constexpr int AMAX_BLOCKS = 256;  // partial maxima per operand
+constexpr int AMAX_MOST = 1024;  // partial maxima per operand, at most
 
 // ---- scales ----------------------------------------------------------------------------------------------------
 __device__ __forceinline__ float finite_mag(float v) {
@@ -49,24 +49,26 @@ __device__ __forceinline__ float amax_part(const T* p, int64_t rows, int K, cons
   return m;
 }
 
-// amax[0 .. 255] / [256 .. 511] = largest finite magnitudes met by the blocks of x / W
+// amax[0 .. xb) / [AMAX_MOST ..] = largest finite magnitudes met by the xb blocks of x / the others' of W
 template <typename TX, typename TW>
 __global__ __launch_bounds__(256) void ce_amax_kernel(const TX* __restrict__ x, const TW* __restrict__ w, int N, int V,
                                                       int K, const int64_t* __restrict__ target, int64_t ignore,
-                                                      float* __restrict__ amax) {
+                                                      float* __restrict__ amax, int xb) {
   __shared__ float sm[4];
-  const int b = blockIdx.x & (AMAX_BLOCKS - 1);
-  float m = blockIdx.x < AMAX_BLOCKS ? amax_part(x, N, K, target, ignore, b, AMAX_BLOCKS)
-                                     : amax_part(w, V, K, (const int64_t*)nullptr, 0, b, AMAX_BLOCKS);
+  const int b = blockIdx.x;
+  float m = b < xb ? amax_part(x, N, K, target, ignore, b, xb)
+                   : amax_part(w, V, K, (const int64_t*)nullptr, 0, b - xb, (int)gridDim.x - xb);
   m = wave_max(m);
   if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
   __syncthreads();
-  if (threadIdx.x == 0) amax[blockIdx.x] = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  if (threadIdx.x == 0) amax[b < xb ? b : AMAX_MOST + b - xb] = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
 }
 
 // exponent e with 2^14 <= amax 2^e < 2^15 (0 for an operand without a finite value other than zero)
-__device__ __forceinline__ int scale_exp(const float* amax, float* sm) {
-  float m = wave_max(amax[threadIdx.x & (AMAX_BLOCKS - 1)]);
+__device__ __forceinline__ int scale_exp(const float* amax, int parts, float* sm) {
+  float m = 0.f;
+  for (int i = threadIdx.x; i < parts; i += 256) m = fmaxf(m, amax[i]);
+  m = wave_max(m);
   if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
   __syncthreads();
   m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
@@ -111,68 +113,20 @@ template <typename TX, typename TW>
 __global__ __launch_bounds__(256) void ce_pack_kernel(const TX* __restrict__ x, const TW* __restrict__ w, int N, int V,
                                                       int K, int ld, int px, int pw, const int64_t* __restrict__ target,
                                                       int64_t ignore, const float* __restrict__ amax, f16* __restrict__ xp,
-                                                      f16* __restrict__ wp, int* __restrict__ exps, int xblocks) {
+                                                      f16* __restrict__ wp, int* __restrict__ exps, int xblocks, int xb,
+                                                      int wb) {
   __shared__ float sm[4];
   const bool isx = (int)blockIdx.x < xblocks;
-  const int e = scale_exp(isx ? amax : amax + AMAX_BLOCKS, sm);
+  const int e = scale_exp(isx ? amax : amax + AMAX_MOST, isx ? xb : wb, sm);
   if (threadIdx.x == 0 && ((int)blockIdx.x == 0 || (int)blockIdx.x == xblocks)) exps[isx ? 0 : 1] = e;
   const int64_t unit = (int64_t)(isx ? blockIdx.x : blockIdx.x - xblocks) * 4 + (threadIdx.x >> 6);
   if (isx) pack_rows(x, xp, (int64_t)N * ld, N, K, ld, px, e, target, ignore, unit);
   else pack_rows(w, wp, (int64_t)V * ld, V, K, ld, pw, e, (const int64_t*)nullptr, 0, unit);
 }
 
-// dst[c][ldd] = src[r][c] for both operands and all planes: 64 x 64 tiles through LDS, zeros behind the last row
-struct TransArgs {
-  const f16* src[2];
-  f16* dst[2];
-  int rows[2], lds[2], ldd[2], planes[2], tiles[2];  // tiles of one plane
-  int cols;
-};
-__global__ __launch_bounds__(256) void ce_transpose_kernel(TransArgs t) {
-  __shared__ f16 sm[64][72];
-  int id = blockIdx.x;
-  const int which = id < t.tiles[0] * t.planes[0] ? 0 : 1;
-  if (which) id -= t.tiles[0] * t.planes[0];
-  const int plane = id / t.tiles[which];
-  id -= plane * t.tiles[which];
-  const int rows = t.rows[which], lds = t.lds[which], ldd = t.ldd[which];
-  const int tc = lds / 64, r0 = id / tc * 64, c0 = id % tc * 64;
-  const f16* s = t.src[which] + (int64_t)plane * rows * lds;
-  f16* d = t.dst[which] + (int64_t)plane * t.cols * ldd;
-  for (int i = threadIdx.x; i < 512; i += 256) {
-    const int r = i >> 3, c = (i & 7) * 8;
-    f16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (r0 + r < rows) v = *reinterpret_cast<const f16x8*>(s + (int64_t)(r0 + r) * lds + c0 + c);
-    *reinterpret_cast<f16x8*>(&sm[r][c]) = v;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < 512; i += 256) {
-    const int c = i >> 3, r = (i & 7) * 8;
-    if (c0 + c >= t.cols) continue;
-    f16x8 v;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = sm[r + e][c];
-    *reinterpret_cast<f16x8*>(d + (int64_t)(c0 + c) * ldd + r0 + r) = v;
-  }
-}
-
-// ---- forward: statistics of a 128-class tile ---------------------------------------------------------------------
-struct Stat {
-  float m, s, z;  // running maximum, sum of exp(z - m), sum of z
-  int arg;        // lowest class that attains m
-};
-__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * 1.4426950408889634f); }
-__device__ __forceinline__ void stat_join(Stat& a, const Stat& b) {
-  if (b.m > a.m || (b.m == a.m && b.arg < a.arg)) a.arg = b.arg;
-  const float m = fmaxf(a.m, b.m);
-  const float ref = m == -INFINITY ? 0.f : m;  // nothing but -inf so far: exp(-inf - 0) = 0
-  a.s = a.s * exp_of(a.m - ref) + b.s * exp_of(b.m - ref);
-  a.m = m;
-  a.z += b.z;
-}
-__device__ __forceinline__ Stat stat_shfl(const Stat& a, int o) {
-  return Stat{__shfl_xor(a.m, o, 64), __shfl_xor(a.s, o, 64), __shfl_xor(a.z, o, 64), __shfl_xor(a.arg, o, 64)};
-}
+// ---- logits of a 128-class x 128-row tile ---------------------------------------------------------------------------
+// Everything behind the products works on z log2(e): the exponentials are then one subtraction and one v_exp_f32.
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 struct CeArgs {
   const f16* w;      // [pw][V][ld]
@@ -184,8 +138,14 @@ struct CeArgs {
   int tiles_v, tiles_n;
 };
 
-// logits of the tile from the accumulators: z = acc 2^-(ex + ew) + bias, -inf behind the last class
-__device__ __forceinline__ void tile_bias(const CeArgs& a, int v0, float (&bias)[4][4]) {
+// acc = z log2(e) without the bias, which follows in `bias` (-inf behind the last class): rows v0 + .., columns n0 + ..
+template <int PW, int PX>
+__device__ __forceinline__ void logit_tile(const CeArgs& a, int v0, int n0, f16* smem, f32x4 (&acc)[4][4],
+                                           float (&bias)[4][4], float& scale) {
+  typedef G16<PW, PX> G;
+  G::zero(acc);
+  G::run(acc, Op16{a.w + (int64_t)v0 * a.ld, (int64_t)a.V * a.ld, a.ld, a.V - v0, 0},
+         Op16{a.x + (int64_t)n0 * a.ld, (int64_t)a.N * a.ld, a.ld, a.N - n0, 0}, 0, a.ld, smem);
   const int lane = threadIdx.x & 63, q = lane >> 4, wm = threadIdx.x >> 7;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -194,55 +154,96 @@ __device__ __forceinline__ void tile_bias(const CeArgs& a, int v0, float (&bias)
       const int v = v0 + wm * 64 + i * 16 + q * 4 + r;
       float b = 0.f;
       if (v >= a.V) b = -INFINITY;
-      else if (a.bias) b = a.bias_bf16 ? (float)((const bf16*)a.bias)[v] : ((const float*)a.bias)[v];
+      else if (a.bias) b = (a.bias_bf16 ? (float)((const bf16*)a.bias)[v] : ((const float*)a.bias)[v]) * LOG2E;
       bias[i][r] = b;
     }
+  int es = -(a.exps[0] + a.exps[1]);
+  if (es < -120 || es > 120) {  // operands of extreme magnitude: two factors
+    const float f = ldexpf(1.f, es / 2);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] *= f;
+    es -= es / 2;
+  }
+  scale = ldexpf(LOG2E, es);
 }
 
-// part[vt][n] = (max, sum, sum z, arg) of the tile, zt[n] = the target's logit
-template <int PW, int PX>
+// position of class t among this lane's 16 of a tile column (i * 4 + r), or -1
+__device__ __forceinline__ int lane_class(int t, int v0) {
+  const int lane = threadIdx.x & 63, d = t - (v0 + (threadIdx.x >> 7) * 64 + (lane >> 4) * 4);
+  return (unsigned)d < 64u && (d & 12) == 0 ? (d >> 4) * 4 + (d & 3) : -1;
+}
+__device__ __forceinline__ int row_target(const CeArgs& a, int n) {
+  return n < a.N ? (int)min(max(a.target[n], (int64_t)-1), (int64_t)a.V) : -1;
+}
+
+// ---- forward: statistics of a tile -----------------------------------------------------------------------------------
+struct Stat {
+  float m, s, z;  // running maximum, sum of 2^(z - m), sum of z (all in units of log2)
+  int arg;        // lowest class that attains m
+};
+__device__ __forceinline__ void stat_join(Stat& a, const Stat& b) {
+  if (b.m > a.m || (b.m == a.m && b.arg < a.arg)) a.arg = b.arg;
+  const float m = fmaxf(a.m, b.m);
+  const float ref = m == -INFINITY ? 0.f : m;  // nothing but -inf so far: 2^(-inf - 0) = 0
+  a.s = a.s * __builtin_amdgcn_exp2f(a.m - ref) + b.s * __builtin_amdgcn_exp2f(b.m - ref);
+  a.m = m;
+  a.z += b.z;
+}
+__device__ __forceinline__ Stat stat_shfl(const Stat& a, int o) {
+  return Stat{__shfl_xor(a.m, o, 64), __shfl_xor(a.s, o, 64), __shfl_xor(a.z, o, 64), __shfl_xor(a.arg, o, 64)};
+}
+
+// part[vt][n] = (max, sum, sum z, arg) of the tile, zt[n] = the target's logit.  MORE: also sum z and arg (label smoothing,
+// predictions), which cost four operations more per logit.
+template <int PW, int PX, bool MORE>
 __global__ __launch_bounds__(G_THREADS, 2) void ce_stats_kernel(CeArgs a, float4* __restrict__ part,
                                                                 float* __restrict__ zt) {
-  typedef G16<PW, PX> G;
-  __shared__ __attribute__((aligned(1024))) f16 smem[G::LDS];
+  __shared__ __attribute__((aligned(1024))) f16 smem[G16<PW, PX>::LDS];
   int tv, tn;
   g16_tile(blockIdx.x, gridDim.x, a.tiles_v, a.tiles_n, tv, tn);
   const int v0 = tv * GM, n0 = tn * GM;
   f32x4 acc[4][4];
-  G::zero(acc);
-  G::run(acc, a.w + (int64_t)v0 * a.ld, (int64_t)a.V * a.ld, a.ld, a.V - v0, a.x + (int64_t)n0 * a.ld,
-         (int64_t)a.N * a.ld, a.ld, a.N - n0, 0, a.ld, smem);
+  float bias[4][4], scale;
+  logit_tile<PW, PX>(a, v0, n0, smem, acc, bias, scale);
   const int lane = threadIdx.x & 63, q = lane >> 4, l15 = lane & 15;
   const int wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
-  const int es = -(a.exps[0] + a.exps[1]);
-  float bias[4][4];
-  tile_bias(a, v0, bias);
   float4* xch = reinterpret_cast<float4*>(smem);
   Stat st[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int n = n0 + wn * 64 + j * 16 + l15;
-    const int t = n < a.N ? (int)min(max(a.target[n], (int64_t)-1), (int64_t)a.V) : -1;
     Stat s{-INFINITY, 0.f, 0.f, a.V};
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int v = v0 + wm * 64 + i * 16 + q * 4 + r;
-        const float z = ldexpf(acc[i][j][r], es) + bias[i][r];
-        acc[i][j][r] = z;
-        if (z > s.m) {
-          s.m = z;
-          s.arg = v;
-        }
-        if (v < a.V) s.z += z;
-        if (v == t) zt[n] = z;
+        acc[i][j][r] = fmaf(acc[i][j][r], scale, bias[i][r]);
+        s.m = fmaxf(s.m, acc[i][j][r]);
       }
+    if (MORE) {
+#pragma unroll
+      for (int e = 15; e >= 0; --e) {
+        const int v = v0 + wm * 64 + (e >> 2) * 16 + q * 4 + (e & 3);
+        const float z = acc[e >> 2][j][e & 3];
+        if (z == s.m) s.arg = v;
+        if (v < a.V) s.z += z;
+      }
+    }
+    const int hit = lane_class(row_target(a, n), v0);
+    if (hit >= 0) {
+      float z = 0.f;
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (e == hit) z = acc[e >> 2][j][e & 3];
+      if (n < a.N && v0 + wm * 64 + (hit >> 2) * 16 + q * 4 + (hit & 3) < a.V) zt[n] = z;
+    }
     const float ref = s.m == -INFINITY ? 0.f : s.m;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) s.s += exp_of(acc[i][j][r] - ref);
+      for (int r = 0; r < 4; ++r) s.s += __builtin_amdgcn_exp2f(acc[i][j][r] - ref);
     stat_join(s, stat_shfl(s, 16));
     stat_join(s, stat_shfl(s, 32));
     st[j] = s;
@@ -260,7 +261,7 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_stats_kernel(CeArgs a, float4
     }
 }
 
-// Per row: lse, loss (0 for ignored rows, NaN for a target outside [0, V)), arg-max.  32 rows x 8 runs of tiles per block.
+// Per row: lse (in units of log2), loss (0 for ignored rows, NaN for a target outside [0, V)), arg-max.  32 rows x 8 runs of tiles per block.
 __global__ __launch_bounds__(256) void ce_join_kernel(const float4* __restrict__ part, const float* __restrict__ zt,
                                                       const int64_t* __restrict__ target, int64_t ignore, int N, int V,
                                                       int tiles_v, float smooth, float* __restrict__ lse,
@@ -282,7 +283,7 @@ __global__ __launch_bounds__(256) void ce_join_kernel(const float4* __restrict__
   if (run == 0 && n < N) {
 #pragma unroll
     for (int r = 1; r < 8; ++r) stat_join(s, sm[r][e]);
-    const float l = (s.m == -INFINITY ? 0.f : s.m) + logf(s.s);
+    const float l = (s.m == -INFINITY ? 0.f : s.m) + log2f(s.s);
     lse[n] = l;
     const int64_t t = target[n];
     float loss = 0.f;
@@ -290,7 +291,7 @@ __global__ __launch_bounds__(256) void ce_join_kernel(const float4* __restrict__
       if (t < 0 || t >= V) loss = NAN;
       else {
         const float d = l - zt[n];
-        loss = smooth > 0.f ? (1.f - smooth) * d + smooth * (l - s.z / (float)V) : d;
+        loss = LN2 * (smooth > 0.f ? (1.f - smooth) * d + smooth * (l - s.z / (float)V) : d);
       }
     }
     rowloss[n] = loss;
@@ -364,69 +365,80 @@ __global__ __launch_bounds__(1024) void ce_weights_kernel(const float* __restric
   if (threadIdx.x == 0) fac[0] = per_row ? big : mean ? g[0] / fmaxf(total[0], 1.f) : g[0];
 }
 
-constexpr float D_SCALE = 32768.f;  // of the scaled gradient terms
+constexpr float D_SCALE = 32768.f;  // of d's fp16 terms, and of dbpart
 
-// One 128 x 128 tile of d for the classes [vbeg, vbeg + vcols): dT[v - vbeg][ldn] and dn[n][ldv], PD terms each, and the
-// column sums dbpart[tile n][v].
+__device__ __forceinline__ float row16_sum(float v) {  // over the 16 lanes of a DPP row
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, true));
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x124, 0xf, 0xf, true));
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x122, 0xf, 0xf, true));
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x121, 0xf, 0xf, true));
+  return v;
+}
+
+// One 128 x 128 tile of d for the classes [vbeg, vbeg + vcols), as dn[n][vcols] in PD terms scaled by 2^15, and its column
+// sums dbpart[tile n][v].
 template <int PW, int PX, int PD>
 __global__ __launch_bounds__(G_THREADS, 2) void ce_grad_kernel(CeArgs a, const float* __restrict__ lse,
                                                                const float* __restrict__ rs, float smooth, int vbeg,
-                                                               int vcols, f16* __restrict__ dT, int ldn,
-                                                               f16* __restrict__ dn, int ldv, int pdn,
+                                                               int vcols, f16* __restrict__ dn,
                                                                float* __restrict__ dbpart) {
-  typedef G16<PW, PX> G;
-  __shared__ __attribute__((aligned(1024))) f16 smem[G::LDS];
+  __shared__ __attribute__((aligned(1024))) f16 smem[G16<PW, PX>::LDS];
   __shared__ float sb[2][GM];
   int tv, tn;
   g16_tile(blockIdx.x, gridDim.x, a.tiles_v, a.tiles_n, tv, tn);
   const int v0 = vbeg + tv * GM, n0 = tn * GM;
   f32x4 acc[4][4];
-  G::zero(acc);
-  G::run(acc, a.w + (int64_t)v0 * a.ld, (int64_t)a.V * a.ld, a.ld, a.V - v0, a.x + (int64_t)n0 * a.ld,
-         (int64_t)a.N * a.ld, a.ld, a.N - n0, 0, a.ld, smem);
+  float bias[4][4], scale;
+  logit_tile<PW, PX>(a, v0, n0, smem, acc, bias, scale);
   const int lane = threadIdx.x & 63, q = lane >> 4, l15 = lane & 15;
   const int wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
-  const int es = -(a.exps[0] + a.exps[1]);
-  const float each = smooth / (float)a.V;
-  float bias[4][4];
-  tile_bias(a, v0, bias);
+  const float each = smooth / (float)a.V * D_SCALE;
   float col[4][4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r) col[i][r] = 0.f;
-  const int64_t planeT = (int64_t)vcols * ldn, planeN = (int64_t)a.N * ldv;
+  const int64_t plane = (int64_t)a.N * vcols;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int n = n0 + wn * 64 + j * 16 + l15;
-    const bool row = n < a.N;
-    const float w = row ? rs[n] : 0.f, l = row ? lse[n] : 0.f;
-    const int t = row ? (int)min(max(a.target[n], (int64_t)-1), (int64_t)a.V) : -1;
-    const bool bad = row && w != 0.f && (t < 0 || t >= a.V);
+    const float w = n < a.N ? rs[n] : 0.f;
+    const int t = row_target(a, n);
+    float l = w != 0.f ? lse[n] - 15.f : 0.f;  // 2^(z - l) is the scaled probability
+    if (w != 0.f && (t < 0 || t >= a.V)) l = NAN;
+    const int hit = lane_class(t, v0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        acc[i][j][r] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], scale, bias[i][r]) - l);
+    if (smooth > 0.f)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (v0 + wm * 64 + i * 16 + q * 4 + r < a.V) acc[i][j][r] -= each;
+    if (hit >= 0)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (e == hit) acc[e >> 2][j][e & 3] -= (1.f - smooth) * D_SCALE;
+    const bool live = w != 0.f;  // rows that do not count vanish whatever they hold
+    f16* o = dn + (int64_t)n * vcols + (v0 - vbeg + wm * 64 + q * 4);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int vr = wm * 64 + i * 16 + q * 4, vl = v0 - vbeg + vr;
       f16x4 hi, lo;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int v = v0 + vr + r;
-        float d = exp_of(ldexpf(acc[i][j][r], es) + bias[i][r] - l) - each;
-        if (v == t) d -= 1.f - smooth;
-        if (bad) d = NAN;
-        d = w == 0.f || v >= a.V ? 0.f : d * w;  // ignored rows vanish whatever they hold
+        const float d = live ? acc[i][j][r] * w : 0.f;
         col[i][r] += d;
-        f16 h, o;
-        f16_split(d * D_SCALE, h, o);
+        f16 h, e;
+        f16_split(d, h, e);
         hi[r] = h;
-        lo[r] = o;
-        if (vl + r < vcols && n < ldn) {
-          dT[(int64_t)(vl + r) * ldn + n] = h;
-          if (PD == 2) dT[planeT + (int64_t)(vl + r) * ldn + n] = o;
-        }
+        lo[r] = e;
       }
-      if (row && vl < ldv) {
-        *reinterpret_cast<f16x4*>(dn + (int64_t)n * ldv + vl) = hi;
-        if (pdn == 2) *reinterpret_cast<f16x4*>(dn + planeN + (int64_t)n * ldv + vl) = lo;
+      if (n < a.N) {
+        *reinterpret_cast<f16x4*>(o + i * 16) = hi;
+        if (PD == 2) *reinterpret_cast<f16x4*>(o + plane + i * 16) = lo;
       }
     }
   }
@@ -435,9 +447,7 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_grad_kernel(CeArgs a, const f
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float s = col[i][r];
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+        const float s = row16_sum(col[i][r]);
         if (l15 == 0) sb[wn][wm * 64 + i * 16 + q * 4 + r] = s;
       }
     __syncthreads();
@@ -455,31 +465,30 @@ __global__ __launch_bounds__(256) void ce_bias_kernel(const float* __restrict__ 
   float s = 0.f;
 #pragma unroll 4
   for (int t = 0; t < tiles; ++t) s += dbpart[(int64_t)t * V + v];
-  db[v] = from_f32<T>(to_f32(db[v]) + s * fac[0]);
+  db[v] = from_f32<T>(to_f32(db[v]) + s * (fac[0] / D_SCALE));
 }
 
+// out[m][c] = factor * sum over the reduction of (row side)[m] (column side)[c]: dx = d W and dW = d^T x
 struct MmArgs {
-  const f16* a;
-  const f16* b;
-  int64_t aplane, bplane;
-  int lda, ldb, M, Nn, k;      // k = padded reduction length, a multiple of 64
+  Op16 c, m;                   // column side (W or x, COL) and row side (d: ROW for dx, COL for dW), at their corners
+  int M, Nn, k;                // rows and columns of the result, reduction length (a multiple of 64)
   int tiles_m, tiles_n, splits, kper;
   float* part;                 // [splits][M][Nn], or null: write out
   int add;                     // add to what part / out hold
   void* out;                   // [M][Nn]
   const float* fac;
   const int* exps;
-  int which;                   // operand b's scale exponent
+  int which;                   // whose scale exponent the column side carries
+  int vec;                     // rows of the result start on 16-byte (fp32) / 8-byte (bf16) boundaries
 };
 
 __device__ __forceinline__ float mm_factor(const float* fac, const int* exps, int which) {
   return ldexpf(fac[0], -15 - exps[which]);
 }
 
-// out[m][n] (+)= fac 2^-(scales) sum_k a[m][k] b[n][k], or raw fp32 partial sums of a slice of k
-template <int PA, int PB, typename T>
+template <int PC, int PM, int KM, typename T>
 __global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
-  typedef G16<PA, PB> G;
+  typedef G16<PC, PM, COL, KM> G;
   __shared__ __attribute__((aligned(1024))) f16 smem[G::LDS];
   const int tiles = g.tiles_m * g.tiles_n;
   const int split = blockIdx.x / tiles;
@@ -489,32 +498,60 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
   f32x4 acc[4][4];
   G::zero(acc);
   const int k0 = split * g.kper, k1 = min(g.k, k0 + g.kper);
-  G::run(acc, g.a + (int64_t)m0 * g.lda, g.aplane, g.lda, g.M - m0, g.b + (int64_t)n0 * g.ldb, g.bplane, g.ldb, g.Nn - n0,
-         k0, k1, smem);
+  Op16 c = g.c, m = g.m;
+  c.side = n0;
+  if (KM == ROW) {
+    m.p += (int64_t)m0 * m.ld;
+    m.n = g.M - m0;
+  } else
+    m.side = m0;
+  G::run(acc, c, m, k0, k1, smem);
   const int lane = threadIdx.x & 63, q = lane >> 4, l15 = lane & 15;
-  const int wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
+  const int wave = threadIdx.x >> 6, wc = wave >> 1, wr = wave & 1;
   const float f = g.part ? 1.f : mm_factor(g.fac, g.exps, g.which);
   float* part = g.part ? g.part + (int64_t)split * g.M * g.Nn : nullptr;
+  const bool vec = g.vec;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int j = 0; j < 4; ++j) {
+    const int row = m0 + wr * 64 + j * 16 + l15;
+    if (row >= g.M) continue;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int m = m0 + wm * 64 + i * 16 + q * 4 + r;
-      if (m >= g.M) continue;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int n = n0 + wn * 64 + j * 16 + l15;
-        if (n >= g.Nn) continue;
-        const int64_t o = (int64_t)m * g.Nn + n;
-        float v = acc[i][j][r];
-        if (part) part[o] = g.add ? part[o] + v : v;
-        else {
-          T* out = (T*)g.out;
+    for (int i = 0; i < 4; ++i) {
+      const int col = n0 + wc * 64 + i * 16 + q * 4;  // four results of one row
+      const int64_t o = (int64_t)row * g.Nn + col;
+      f32x4 v = acc[i][j];
+      if (vec) {
+        if (col >= g.Nn) continue;
+        if (part) {
+          if (g.add) v += *reinterpret_cast<const f32x4*>(part + o);
+          *reinterpret_cast<f32x4*>(part + o) = v;
+        } else if constexpr (sizeof(T) == 4) {
+          float* out = (float*)g.out + o;
           v *= f;
-          out[o] = from_f32<T>(g.add ? to_f32(out[o]) + v : v);
+          if (g.add) v += *reinterpret_cast<const f32x4*>(out);
+          *reinterpret_cast<f32x4*>(out) = v;
+        } else {
+          bf16* out = (bf16*)g.out + o;
+          v *= f;
+          bf16x4 r = {0, 0, 0, 0};
+          if (g.add) r = *reinterpret_cast<const bf16x4*>(out);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) r[e] = (bf16)((float)r[e] + v[e]);
+          *reinterpret_cast<bf16x4*>(out) = r;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (col + e >= g.Nn) break;
+          if (part) part[o + e] = g.add ? part[o + e] + v[e] : v[e];
+          else {
+            T* out = (T*)g.out + o + e;
+            *out = from_f32<T>(g.add ? to_f32(*out) + v[e] * f : v[e] * f);
+          }
         }
       }
     }
+  }
 }
 
 // out (+)= factor * sum over the slices, in order
@@ -538,15 +575,15 @@ int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
 struct Plan {
   int ld, px, pw;              // row length and terms of the packed operands
-  int pdx, pdw;                // terms of d for dx and dW
-  int ldn, piece, pieces;      // padded rows, classes of a piece
+  int pdx, pdw, pd;            // terms of d for dx and dW, and the larger of the two
+  int piece, pieces;           // classes of a piece
   int sx, kx, sw, kw;          // slices of the reductions of dx (per piece) and dW, and their lengths
   // forward workspace (saved for backward): packed x, packed W, exponents, lse, total
   int64_t o_xp, o_wp, o_exps, o_lse, o_total, saved;
   // forward scratch
   int64_t f_amax, f_part, f_zt, fwd;
   // backward scratch
-  int64_t b_xt, b_wt, b_rs, b_fac, b_dT, b_dn, b_db, b_px, b_pw, bwd;
+  int64_t b_rs, b_fac, b_dn, b_db, b_px, b_pw, bwd;
 };
 
 // slices of a reduction of length k (a multiple of 64) over `tiles` output tiles: enough to give every CU two workgroups,
@@ -567,10 +604,9 @@ Plan make_plan(int xf32, int wf32, int N, int V, int K) {
   p.pw = xf32 ? 2 : 1;
   p.pdx = xf32 ? 2 : 1;
   p.pdw = wf32 ? 2 : 1;
-  p.ldn = pad64(N);
-  // a piece of d (both orders, all terms) stays below 192 MiB, inside the last-level cache
-  const int64_t per_class = (int64_t)p.ldn * 2 * (p.pdx + p.pdw);
-  int64_t cols = (192ll << 20) / per_class / GM * GM;
+  p.pd = p.pdx > p.pdw ? p.pdx : p.pdw;
+  // a piece of d stays below 128 MiB, half of the last-level cache
+  int64_t cols = (128ll << 20) / ((int64_t)N * 2 * p.pd) / GM * GM;
   if (cols < GM) cols = GM;
   const int all = (V + GM - 1) / GM * GM;
   p.pieces = (int)((all + cols - 1) / cols);
@@ -578,7 +614,7 @@ Plan make_plan(int xf32, int wf32, int N, int V, int K) {
   p.pieces = (all + p.piece - 1) / p.piece;
   const int tn = ceil_div(N, GM), tk = ceil_div(K, GM);
   slices(tn * tk, p.piece, p.sx, p.kx);
-  slices((p.piece / GM) * tk, p.ldn, p.sw, p.kw);
+  slices((p.piece / GM) * tk, pad64(N), p.sw, p.kw);
   int64_t o = 0;
   auto take = [&](int64_t bytes) {
     const int64_t at = o;
@@ -592,17 +628,14 @@ Plan make_plan(int xf32, int wf32, int N, int V, int K) {
   p.o_total = take(16);
   p.saved = o;
   o = 0;
-  p.f_amax = take(2 * AMAX_BLOCKS * 4);
+  p.f_amax = take(2 * AMAX_MOST * 4);
   p.f_part = take((int64_t)ceil_div(V, GM) * N * 16);
   p.f_zt = take((int64_t)N * 4);
   p.fwd = o;
   o = 0;
-  p.b_xt = take((int64_t)p.px * K * p.ldn * 2);
-  p.b_wt = take((int64_t)p.pw * K * pad64(V) * 2);
   p.b_rs = take((int64_t)N * 4);
   p.b_fac = take(16);
-  p.b_dT = take((int64_t)p.pdw * p.piece * p.ldn * 2);
-  p.b_dn = take((int64_t)p.pdx * N * p.piece * 2);
+  p.b_dn = take((int64_t)p.pd * N * p.piece * 2);
   p.b_db = take((int64_t)tn * V * 4);
   p.b_px = (p.pieces > 1 || p.sx > 1) ? take((int64_t)p.sx * N * K * 4) : -1;
   p.b_pw = p.sw > 1 ? take((int64_t)p.sw * p.piece * K * 4) : -1;
@@ -632,23 +665,29 @@ void pack_go(const Plan& p, const void* x, const void* w, int N, int V, int K, c
   float* amax = (float*)(ws + p.f_amax);
   const int per = ceil_div(p.ld, 512);
   const int xb = (int)ceil_div64((int64_t)N * per, 4), wb = (int)ceil_div64((int64_t)V * per, 4);
-  hipLaunchKernelGGL((ce_amax_kernel<TX, TW>), dim3(2 * AMAX_BLOCKS), dim3(256), 0, st, (const TX*)x, (const TW*)w, N, V, K,
-                     target, ignore, amax);
+  auto blocks = [](int64_t elems) {  // of about 8 K elements
+    const int64_t b = ceil_div64(elems, 8192);
+    return (int)(b < AMAX_MOST ? b : AMAX_MOST);
+  };
+  const int xa = blocks((int64_t)N * K), wa = blocks((int64_t)V * K);
+  hipLaunchKernelGGL((ce_amax_kernel<TX, TW>), dim3(xa + wa), dim3(256), 0, st, (const TX*)x, (const TW*)w, N, V, K, target,
+                     ignore, amax, xa);
   hipLaunchKernelGGL((ce_pack_kernel<TX, TW>), dim3(xb + wb), dim3(256), 0, st, (const TX*)x, (const TW*)w, N, V, K, p.ld,
                      p.px, p.pw, target, ignore, amax, (f16*)(saved + p.o_xp), (f16*)(saved + p.o_wp),
-                     (int*)(saved + p.o_exps), xb);
+                     (int*)(saved + p.o_exps), xb, xa, wa);
 }
 
-template <int PA, int PB>
+template <int PC, int PM, int KM>
 void mm_go(const MmArgs& g, int out_bf16, hipStream_t st) {
   const dim3 grid(g.tiles_m * g.tiles_n * g.splits);
-  if (out_bf16) hipLaunchKernelGGL((ce_mm_kernel<PA, PB, bf16>), grid, dim3(G_THREADS), 0, st, g);
-  else hipLaunchKernelGGL((ce_mm_kernel<PA, PB, float>), grid, dim3(G_THREADS), 0, st, g);
+  if (out_bf16) hipLaunchKernelGGL((ce_mm_kernel<PC, PM, KM, bf16>), grid, dim3(G_THREADS), 0, st, g);
+  else hipLaunchKernelGGL((ce_mm_kernel<PC, PM, KM, float>), grid, dim3(G_THREADS), 0, st, g);
 }
-void mm_terms(int pa, int pb, const MmArgs& g, int out_bf16, hipStream_t st) {
-  if (pa == 1 && pb == 1) mm_go<1, 1>(g, out_bf16, st);
-  else if (pa == 2 && pb == 1) mm_go<2, 1>(g, out_bf16, st);
-  else mm_go<2, 2>(g, out_bf16, st);
+template <int KM>
+void mm_terms(int pc, int pm, const MmArgs& g, int out_bf16, hipStream_t st) {
+  if (pm == 1) mm_go<1, 1, KM>(g, out_bf16, st);
+  else if (pc == 1) mm_go<1, 2, KM>(g, out_bf16, st);
+  else mm_go<2, 2, KM>(g, out_bf16, st);
 }
 void reduce_go(const float* part, int slices, int64_t n, const float* fac, const int* exps, int which, int add, void* out,
                int out_bf16, hipStream_t st) {
@@ -687,8 +726,11 @@ int vc_linear_ce_fwd(int xdtype, int wdtype, const void* x, const void* w, const
   float4* part = (float4*)(ws + p.f_part);
   float* zt = (float*)(ws + p.f_zt);
   const dim3 grid(a.tiles_v * a.tiles_n);
-  if (p.pw == 2) hipLaunchKernelGGL((ce_stats_kernel<2, 2>), grid, dim3(G_THREADS), 0, stream, a, part, zt);
-  else hipLaunchKernelGGL((ce_stats_kernel<1, 1>), grid, dim3(G_THREADS), 0, stream, a, part, zt);
+  const bool more = smoothing > 0.f || pred;
+  if (p.pw == 2 && more) hipLaunchKernelGGL((ce_stats_kernel<2, 2, true>), grid, dim3(G_THREADS), 0, stream, a, part, zt);
+  else if (p.pw == 2) hipLaunchKernelGGL((ce_stats_kernel<2, 2, false>), grid, dim3(G_THREADS), 0, stream, a, part, zt);
+  else if (more) hipLaunchKernelGGL((ce_stats_kernel<1, 1, true>), grid, dim3(G_THREADS), 0, stream, a, part, zt);
+  else hipLaunchKernelGGL((ce_stats_kernel<1, 1, false>), grid, dim3(G_THREADS), 0, stream, a, part, zt);
   hipLaunchKernelGGL(ce_join_kernel, dim3(ceil_div(N, 32)), dim3(256), 0, stream, part, zt, target, ignore_index, N, V,
                      a.tiles_v, smoothing, (float*)(sv + p.o_lse), row_loss, pred);
   hipLaunchKernelGGL(ce_total_kernel, dim3(1), dim3(1024), 0, stream, row_loss, target, pred, ignore_index, N, mean, loss,
@@ -710,17 +752,13 @@ int vc_linear_ce_bwd(int xdtype, int wdtype, const void* bias, const int64_t* ta
   const char* sv = (const char*)saved;
   char* ws = (char*)workspace;
   const f16 *xp = (const f16*)(sv + p.o_xp), *wp = (const f16*)(sv + p.o_wp);
-  f16 *xt = (f16*)(ws + p.b_xt), *wt = (f16*)(ws + p.b_wt), *dT = (f16*)(ws + p.b_dT), *dn = (f16*)(ws + p.b_dn);
+  f16* dn = (f16*)(ws + p.b_dn);
   const int* exps = (const int*)(sv + p.o_exps);
   const float* lse = (const float*)(sv + p.o_lse);
   float *rs = (float*)(ws + p.b_rs), *fac = (float*)(ws + p.b_fac), *dbp = (float*)(ws + p.b_db);
-  const int vp = pad64(V), tn = ceil_div(N, GM), tk = ceil_div(K, GM);
+  const int tn = ceil_div(N, GM), tk = ceil_div(K, GM);
   hipLaunchKernelGGL(ce_weights_kernel, dim3(1), dim3(1024), 0, stream, dloss, (const float*)(sv + p.o_total), target,
                      ignore_index, N, mean, per_row, rs, fac);
-  TransArgs t{{xp, wp}, {xt, wt}, {N, V}, {p.ld, p.ld}, {p.ldn, vp}, {dw ? p.px : 0, dx ? p.pw : 0},
-              {(p.ldn / 64) * (p.ld / 64), (vp / 64) * (p.ld / 64)}, K};
-  const int tblocks = t.tiles[0] * t.planes[0] + t.tiles[1] * t.planes[1];
-  if (tblocks) hipLaunchKernelGGL(ce_transpose_kernel, dim3(tblocks), dim3(256), 0, stream, t);
   for (int c = 0; c < p.pieces; ++c) {
     const int vbeg = c * p.piece;
     const int vcols = p.piece < ceil_div(V - vbeg, GM) * GM ? p.piece : ceil_div(V - vbeg, GM) * GM;
@@ -728,61 +766,50 @@ int vc_linear_ce_bwd(int xdtype, int wdtype, const void* bias, const int64_t* ta
     const dim3 grid(a.tiles_v * tn);
     float* dbq = db ? dbp : nullptr;
     if (p.pw == 2)
-      hipLaunchKernelGGL((ce_grad_kernel<2, 2, 2>), grid, dim3(G_THREADS), 0, stream, a, lse, rs, smoothing, vbeg, vcols, dT,
-                         p.ldn, dn, vcols, p.pdx, dbq);
-    else if (p.pdw == 2)
-      hipLaunchKernelGGL((ce_grad_kernel<1, 1, 2>), grid, dim3(G_THREADS), 0, stream, a, lse, rs, smoothing, vbeg, vcols, dT,
-                         p.ldn, dn, vcols, p.pdx, dbq);
+      hipLaunchKernelGGL((ce_grad_kernel<2, 2, 2>), grid, dim3(G_THREADS), 0, stream, a, lse, rs, smoothing, vbeg, vcols, dn,
+                         dbq);
+    else if (p.pd == 2)
+      hipLaunchKernelGGL((ce_grad_kernel<1, 1, 2>), grid, dim3(G_THREADS), 0, stream, a, lse, rs, smoothing, vbeg, vcols, dn,
+                         dbq);
     else
-      hipLaunchKernelGGL((ce_grad_kernel<1, 1, 1>), grid, dim3(G_THREADS), 0, stream, a, lse, rs, smoothing, vbeg, vcols, dT,
-                         p.ldn, dn, vcols, p.pdx, dbq);
+      hipLaunchKernelGGL((ce_grad_kernel<1, 1, 1>), grid, dim3(G_THREADS), 0, stream, a, lse, rs, smoothing, vbeg, vcols, dn,
+                         dbq);
+    const int rows = vcols < V - vbeg ? vcols : V - vbeg;
+    MmArgs g{};
+    g.Nn = K;
+    g.tiles_n = tk;
+    g.fac = fac;
+    g.exps = exps;
     if (dx) {
-      MmArgs g{};
-      g.a = dn;
-      g.aplane = (int64_t)N * vcols;
-      g.lda = vcols;
+      g.c = Op16{wp + (int64_t)vbeg * p.ld, (int64_t)V * p.ld, p.ld, rows, 0};
+      g.m = Op16{dn, (int64_t)N * vcols, vcols, N, 0};
       g.M = N;
-      g.b = wt + vbeg;
-      g.bplane = (int64_t)K * vp;
-      g.ldb = vp;
-      g.Nn = K;
-      g.k = vcols < vp - vbeg ? vcols : vp - vbeg;
+      g.k = pad64(rows);
       g.tiles_m = tn;
-      g.tiles_n = tk;
       g.splits = p.sx;
       g.kper = p.kx;
       g.part = p.b_px >= 0 ? (float*)(ws + p.b_px) : nullptr;
       g.add = c > 0;
       g.out = dx;
-      g.fac = fac;
-      g.exps = exps;
       g.which = 1;
-      mm_terms(p.pdx, p.pw, g, xdtype == VC_BF16, stream);
+      g.vec = K % 4 == 0 && ((uintptr_t)dx & 15) == 0;
+      mm_terms<ROW>(p.pw, p.pdx, g, xdtype == VC_BF16, stream);
     }
     if (dw) {
-      const int rows = vcols < V - vbeg ? vcols : V - vbeg;
       char* out = (char*)dw + (int64_t)vbeg * K * (wdtype == VC_BF16 ? 2 : 4);
-      MmArgs g{};
-      g.a = dT;
-      g.aplane = (int64_t)vcols * p.ldn;
-      g.lda = p.ldn;
+      g.c = Op16{xp, (int64_t)N * p.ld, p.ld, N, 0};
+      g.m = Op16{dn, (int64_t)N * vcols, vcols, N, 0};
       g.M = rows;
-      g.b = xt;
-      g.bplane = (int64_t)K * p.ldn;
-      g.ldb = p.ldn;
-      g.Nn = K;
-      g.k = p.ldn;
+      g.k = pad64(N);
       g.tiles_m = ceil_div(rows, GM);
-      g.tiles_n = tk;
       g.splits = p.sw;
       g.kper = p.kw;
       g.part = p.b_pw >= 0 ? (float*)(ws + p.b_pw) : nullptr;
       g.add = g.part ? 0 : 1;
       g.out = out;
-      g.fac = fac;
-      g.exps = exps;
       g.which = 0;
-      mm_terms(p.pdw, p.px, g, wdtype == VC_BF16, stream);
+      g.vec = K % 4 == 0 && ((uintptr_t)dw & 15) == 0;
+      mm_terms<COL>(p.px, p.pdw, g, wdtype == VC_BF16, stream);
       if (g.part) reduce_go(g.part, p.sw, (int64_t)rows * K, fac, exps, 0, 1, out, wdtype == VC_BF16, stream);
     }
   }

@@ -31,6 +31,9 @@ struct NsMat {
   int m, n;
   int tall;    // G is [n][m]
   int t0;      // first workgroup of this matrix in the launch
+  // symmetric products: tiles [0, direct) are worked by one workgroup each, the others in `slices` runs of the reduction
+  // whose partial tiles start at p0 and are joined by the workgroups from f0 on of a second launch
+  int direct, slices, p0, f0;
 };
 struct NsArgs {
   NsMat mat[NS_MAX];
@@ -73,20 +76,17 @@ __global__ __launch_bounds__(256) void muon_apply_kernel(float* __restrict__ p, 
 __host__ __device__ inline int up64(int v) { return (v + 63) / 64 * 64; }
 __host__ __device__ inline int64_t up128(int64_t v) { return (v + 127) / 128 * 128; }
 
-// Buffers of one matrix, two planes each: X [m][ldn] and X^T [n][ldm] twice (read and written in turn), S and P [m][ldm].
+// Buffers of one matrix, two planes each: X [m][ldn] twice (read and written in turn), S and P [m][ldm].
 struct NsView {
   int ldm, ldn;
-  int64_t x, xt, xo, xto, s, p, end;
+  int64_t x, xo, s, p, end;
   __host__ __device__ NsView(const NsMat& t, int parity) {
     ldm = up64(t.m);
     ldn = up64(t.n);
-    const int64_t ex = up128(2ll * t.m * ldn), et = up128(2ll * t.n * ldm), es = up128(2ll * t.m * ldm);
-    const int64_t half = ex + et;
-    x = t.at + (parity ? half : 0);
-    xo = t.at + (parity ? 0 : half);
-    xt = x + ex;
-    xto = xo + ex;
-    s = t.at + 2 * half;
+    const int64_t ex = up128(2ll * t.m * ldn), es = up128(2ll * t.m * ldm);
+    x = t.at + (parity ? ex : 0);
+    xo = t.at + (parity ? 0 : ex);
+    s = t.at + 2 * ex;
     p = s + es;
     end = p + es;
   }
@@ -163,7 +163,7 @@ __global__ __launch_bounds__(64) void ns_scale_kernel(NsArgs a, int blocks, cons
   }
 }
 
-// Y_0 in both orders: 64 x 64 tiles of the wide orientation through LDS, zeros in the padding
+// Y_0: 64 x 64 tiles of the wide orientation, through LDS where G is tall; zeros in the padding
 template <typename T>
 __global__ __launch_bounds__(256) void ns_init_kernel(NsArgs a, f16* __restrict__ ws, const NsScale* __restrict__ sc) {
   __shared__ float sm[64][65];
@@ -184,31 +184,18 @@ __global__ __launch_bounds__(256) void ns_init_kernel(NsArgs a, f16* __restrict_
   __syncthreads();
   for (int e = threadIdx.x; e < 512; e += 256) {
     const int hi = e >> 3, lo = (e & 7) * 8;
+    if (r0 + hi >= t.m) continue;
     f16x8 h, l;
-    if (r0 + hi < t.m) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        f16 u, v;
-        f16_split(sm[hi][lo + k], u, v);
-        h[k] = u;
-        l[k] = v;
-      }
-      f16* d = ws + w.x + (int64_t)(r0 + hi) * w.ldn + c0 + lo;
-      *reinterpret_cast<f16x8*>(d) = h;
-      *reinterpret_cast<f16x8*>(d + (int64_t)t.m * w.ldn) = l;
+    for (int k = 0; k < 8; ++k) {
+      f16 u, v;
+      f16_split(sm[hi][lo + k], u, v);
+      h[k] = u;
+      l[k] = v;
     }
-    if (c0 + hi < t.n) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        f16 u, v;
-        f16_split(sm[lo + k][hi], u, v);
-        h[k] = u;
-        l[k] = v;
-      }
-      f16* d = ws + w.xt + (int64_t)(c0 + hi) * w.ldm + r0 + lo;
-      *reinterpret_cast<f16x8*>(d) = h;
-      *reinterpret_cast<f16x8*>(d + (int64_t)t.n * w.ldm) = l;
-    }
+    f16* d = ws + w.x + (int64_t)(r0 + hi) * w.ldn + c0 + lo;
+    *reinterpret_cast<f16x8*>(d) = h;
+    *reinterpret_cast<f16x8*>(d + (int64_t)t.m * w.ldn) = l;
   }
 }
 
@@ -218,127 +205,227 @@ struct NsStep {
   int last;
 };
 
-// The symmetric products.  SQUARE false: S = rho^2 Y Y^T; true: P = b S + c S S.  Tiles on and below the diagonal; the mirror
-// of an off-diagonal tile is stored with it.
+// Tile `id` of the lower triangle of tm x tm tiles, in bands of eight tile rows walked column by column.
+__device__ __forceinline__ void tri_tile(int id, int tiles, int& m, int& n) {
+  int b = 0;
+  while (32 * (b + 1) * (b + 1) + 4 * (b + 1) <= id) ++b;  // 64 b + 36 tiles in a whole band b
+  int w = id - (32 * b * b + 4 * b);
+  const int rows = tiles - 8 * b < 8 ? tiles - 8 * b : 8;
+  if (w < rows * 8 * b) {
+    n = w / rows;
+    m = 8 * b + w % rows;
+  } else {
+    w -= rows * 8 * b;
+    int j = 0;
+    while (w >= rows - j) {
+      w -= rows - j;
+      ++j;
+    }
+    n = 8 * b + j;
+    m = n + w;
+  }
+  m = __builtin_amdgcn_readfirstlane(m);
+  n = __builtin_amdgcn_readfirstlane(n);
+}
+// workgroups of one XCD (every eighth) take a contiguous run of [0, total)
+__device__ __forceinline__ int xcd_run(int id, int total) {
+  const int q = total >> 3, r = total & 7, xcd = id & 7, idx = id >> 3;
+  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + idx;
+}
+
+// What becomes of an accumulated tile (rows m0 + .. in registers, columns n0 + .. across lanes) of a symmetric product:
+// S = rho^2 Y Y^T, or P = b S + c S S (SQUARE), stored at (column, row) straight from the registers and, off the
+// diagonal, at (row, column) through LDS.
 template <bool SQUARE>
-__global__ __launch_bounds__(G_THREADS, 2) void ns_sym_kernel(NsArgs a, f16* __restrict__ ws,
-                                                              const NsScale* __restrict__ sc, NsStep st, int parity) {
-  typedef G16<2, 2> G;
-  __shared__ __attribute__((aligned(1024))) f16 smem[G::LDS];
-  const int i = find_mat(a, blockIdx.x);
-  const NsMat& t = a.mat[i];
-  const NsView w(t, parity);
-  const int id = blockIdx.x - t.t0;
-  int tm = (int)((sqrtf(8.f * id + 1.f) - 1.f) * 0.5f);  // id = tm (tm + 1) / 2 + tn, tn <= tm
-  while ((tm + 1) * (tm + 2) / 2 <= id) ++tm;
-  while (tm * (tm + 1) / 2 > id) --tm;
-  tm = __builtin_amdgcn_readfirstlane(tm);
-  const int tn = id - tm * (tm + 1) / 2;
-  const int m0 = tm * GM, n0 = tn * GM;
-  const f16* src = ws + (SQUARE ? w.s : w.x);
-  const int ld = SQUARE ? w.ldm : w.ldn;
-  const int64_t plane = (int64_t)t.m * ld;
-  f32x4 acc[4][4];
-  G::zero(acc);
-  G::run(acc, src + (int64_t)m0 * ld, plane, ld, t.m - m0, src + (int64_t)n0 * ld, plane, ld, t.m - n0, 0, ld, smem);
+__device__ __forceinline__ void sym_store(f32x4 (&acc)[4][4], const NsMat& t, const NsView& w, f16* ws, const NsScale& sc,
+                                          const NsStep& st, int m0, int n0, f16* smem) {
   const int lane = threadIdx.x & 63, q = lane >> 4, l15 = lane & 15;
   const int wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
   const f16* s = ws + w.s;
   f16* dst = ws + (SQUARE ? w.p : w.s);
   const int64_t pl = (int64_t)t.m * w.ldm;
-  const float rho2 = sc[i].rho2;
-  const int e = SQUARE ? st.ep - 2 * st.es : st.es - 2 * sc[i].ey;
+  const float f = SQUARE ? ldexpf(st.c, st.ep - 2 * st.es) : ldexpf(sc.rho2, st.es - 2 * sc.ey);
   const float sb = ldexpf(st.b, st.ep - st.es);
+  constexpr int STR = GM + 8;
+  f16x4 lo[4][4];
 #pragma unroll
-  for (int ii = 0; ii < 4; ++ii)
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int r = m0 + wm * 64 + ii * 16 + q * 4, c = n0 + wn * 64 + j * 16 + l15;
-      f16x4 hi, lo;
+      const int r = m0 + wm * 64 + i * 16 + q * 4, c = n0 + wn * 64 + j * 16 + l15;
+      const bool in = c < t.m && r < w.ldm;
+      const int64_t o = (int64_t)c * w.ldm + r;
+      f16x4 sh = {0, 0, 0, 0}, sl = {0, 0, 0, 0}, h;
+      if (SQUARE && in) {
+        sh = *reinterpret_cast<const f16x4*>(s + o);
+        sl = *reinterpret_cast<const f16x4*>(s + o + pl);
+      }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        float v;
-        if (SQUARE) {
-          v = st.c * ldexpf(acc[ii][j][k], e);
-          if (r + k < t.m && c < t.m) {
-            const int64_t o = (int64_t)(r + k) * w.ldm + c;
-            v = fmaf(sb, (float)s[o] + (float)s[o + pl], v);
-          }
-        } else
-          v = rho2 * ldexpf(acc[ii][j][k], e);
-        f16 h, l;
-        f16_split(v, h, l);
-        hi[k] = h;
-        lo[k] = l;
-        if (r + k < t.m && c < w.ldm) {
-          const int64_t o = (int64_t)(r + k) * w.ldm + c;
-          dst[o] = h;
-          dst[o + pl] = l;
-        }
+        float v = acc[i][j][k] * f;
+        if (SQUARE) v = fmaf(sb, (float)sh[k] + (float)sl[k], v);
+        f16 u, e;
+        f16_split(v, u, e);
+        h[k] = u;
+        lo[i][j][k] = e;
+        if (m0 != n0) smem[(r - m0 + k) * STR + c - n0] = u;
       }
-      if (tm != tn && c < t.m && r < w.ldm) {
-        const int64_t o = (int64_t)c * w.ldm + r;
-        *reinterpret_cast<f16x4*>(dst + o) = hi;
-        *reinterpret_cast<f16x4*>(dst + o + pl) = lo;
+      if (in) {
+        *reinterpret_cast<f16x4*>(dst + o) = h;
+        *reinterpret_cast<f16x4*>(dst + o + pl) = lo[i][j];
       }
     }
+  if (m0 == n0) return;
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    if (p) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            smem[(wm * 64 + i * 16 + q * 4 + k) * STR + wn * 64 + j * 16 + l15] = lo[i][j][k];
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < GM * 16; e += G_THREADS) {
+      const int r = e >> 4, c = (e & 15) * 8;  // below the diagonal every column of the tile is inside
+      if (m0 + r < t.m)
+        *reinterpret_cast<f16x8*>(dst + p * pl + (int64_t)(m0 + r) * w.ldm + n0 + c) =
+            *reinterpret_cast<const f16x8*>(smem + r * STR + c);
+    }
+    __syncthreads();
+  }
 }
 
-// X <- a X + P X, into the other pair of buffers, or the result in G's orientation after the last step
-template <typename T>
-__global__ __launch_bounds__(G_THREADS, 2) void ns_update_kernel(NsArgs a, f16* __restrict__ ws,
-                                                                 const NsScale* __restrict__ sc, NsStep st, int parity) {
+// A tile, or a slice of the reduction of one, of a symmetric product; tiles on and below the diagonal only.
+template <bool SQUARE>
+__global__ __launch_bounds__(G_THREADS, 2) void ns_sym_kernel(NsArgs a, f16* __restrict__ ws,
+                                                              const NsScale* __restrict__ sc, NsStep st, int parity,
+                                                              float* __restrict__ part) {
   typedef G16<2, 2> G;
   __shared__ __attribute__((aligned(1024))) f16 smem[G::LDS];
   const int i = find_mat(a, blockIdx.x);
   const NsMat& t = a.mat[i];
   const NsView w(t, parity);
-  const int tiles_m = (t.m + GM - 1) / GM;
-  const int id = blockIdx.x - t.t0;
-  const int tn = id / tiles_m, tm = id - tn * tiles_m;
+  const int tiles = (t.m + GM - 1) / GM, count = tiles * (tiles + 1) / 2;
+  const int units = t.direct + (count - t.direct) * t.slices;
+  const int id = xcd_run(blockIdx.x - t.t0, units);
+  const int ld = SQUARE ? w.ldm : w.ldn;
+  int tile = id, k0 = 0, k1 = ld, slot = -1;
+  if (id >= t.direct) {
+    slot = id - t.direct;
+    tile = t.direct + slot / t.slices;
+    const int per = (ld / G::BK + t.slices - 1) / t.slices * G::BK, s = slot % t.slices;
+    k0 = s * per;
+    k1 = min(ld, k0 + per);
+  }
+  int tm, tn;
+  tri_tile(tile, tiles, tm, tn);
   const int m0 = tm * GM, n0 = tn * GM;
-  const int64_t pp = (int64_t)t.m * w.ldm, px = (int64_t)t.m * w.ldn, pt = (int64_t)t.n * w.ldm;
-  const f16 *x = ws + w.x, *xt = ws + w.xt;
+  const f16* src = ws + (SQUARE ? w.s : w.x);
+  const int64_t plane = (int64_t)t.m * ld;
   f32x4 acc[4][4];
   G::zero(acc);
-  G::run(acc, ws + w.p + (int64_t)m0 * w.ldm, pp, w.ldm, t.m - m0, xt + (int64_t)n0 * w.ldm, pt, w.ldm, t.n - n0, 0, w.ldm,
-         smem);
+  G::run(acc, Op16{src + (int64_t)m0 * ld, plane, ld, t.m - m0, 0}, Op16{src + (int64_t)n0 * ld, plane, ld, t.m - n0, 0}, k0,
+         k1, smem);
+  if (slot >= 0) {
+    f32x4* o = reinterpret_cast<f32x4*>(part + ((int64_t)t.p0 + slot) * GM * GM) + threadIdx.x;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[e * G_THREADS] = acc[e >> 2][e & 3];
+    return;
+  }
+  sym_store<SQUARE>(acc, t, w, ws, sc[i], st, m0, n0, smem);
+}
+
+// joins the slices of a tile in order
+template <bool SQUARE>
+__global__ __launch_bounds__(G_THREADS, 2) void ns_sym_join_kernel(NsArgs a, f16* __restrict__ ws,
+                                                                   const NsScale* __restrict__ sc, NsStep st, int parity,
+                                                                   const float* __restrict__ part) {
+  __shared__ __attribute__((aligned(1024))) f16 smem[GM * (GM + 8)];
+  int i = 0;
+  while (i + 1 < a.count && a.mat[i + 1].f0 <= (int)blockIdx.x) ++i;
+  i = __builtin_amdgcn_readfirstlane(i);
+  const NsMat& t = a.mat[i];
+  const NsView w(t, parity);
+  const int e0 = blockIdx.x - t.f0;
+  int tm, tn;
+  tri_tile(t.direct + e0, (t.m + GM - 1) / GM, tm, tn);
+  f32x4 acc[4][4];
+  G16<2, 2>::zero(acc);
+  const f32x4* p = reinterpret_cast<const f32x4*>(part + ((int64_t)t.p0 + (int64_t)e0 * t.slices) * GM * GM) + threadIdx.x;
+  for (int s = 0; s < t.slices; ++s, p += GM * GM / 4)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e >> 2][e & 3] += p[e * G_THREADS];
+  sym_store<SQUARE>(acc, t, w, ws, sc[i], st, tm * GM, tn * GM, smem);
+}
+
+// X <- a X + P X, into the other buffer, or the result in G's orientation after the last step.  The columns of X run along
+// the registers, so X is read and written in groups of four.
+template <typename T>
+__global__ __launch_bounds__(G_THREADS, 2) void ns_update_kernel(NsArgs a, f16* __restrict__ ws,
+                                                                 const NsScale* __restrict__ sc, NsStep st, int parity) {
+  typedef G16<2, 2, COL, ROW> G;
+  __shared__ __attribute__((aligned(1024))) f16 smem[G::LDS];
+  const int i = find_mat(a, blockIdx.x);
+  const NsMat& t = a.mat[i];
+  const NsView w(t, parity);
+  const int tiles_m = (t.m + GM - 1) / GM, tiles_n = (t.n + GM - 1) / GM;
+  int tm, tn;
+  g16_tile(blockIdx.x - t.t0, tiles_m * tiles_n, tiles_m, tiles_n, tm, tn);
+  const int m0 = tm * GM, n0 = tn * GM;
+  const int64_t pp = (int64_t)t.m * w.ldm, px = (int64_t)t.m * w.ldn;
+  const f16* x = ws + w.x;
+  f32x4 acc[4][4];
+  G::zero(acc);
+  G::run(acc, Op16{x, px, w.ldn, t.m, n0}, Op16{ws + w.p + (int64_t)m0 * w.ldm, pp, w.ldm, t.m - m0, 0}, 0, w.ldm, smem);
   const int lane = threadIdx.x & 63, q = lane >> 4, l15 = lane & 15;
-  const int wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
-  f16 *xo = ws + w.xo, *xto = ws + w.xto;
-  const float rho = sc[i].rho;
+  const int wave = threadIdx.x >> 6, wc = wave >> 1, wr = wave & 1;
+  f16* xo = ws + w.xo;
+  const float f = ldexpf(1.f, -st.ep), fo = sc[i].rho;
   const int ey = sc[i].ey;
+  T* out = (T*)t.out;
+  const bool vec = !t.tall && t.n % 4 == 0 && ((uintptr_t)out & 15) == 0;
 #pragma unroll
-  for (int ii = 0; ii < 4; ++ii)
+  for (int j = 0; j < 4; ++j) {
+    const int r = m0 + wr * 64 + j * 16 + l15;
+    if (r >= t.m) continue;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int r = m0 + wm * 64 + ii * 16 + q * 4, c = n0 + wn * 64 + j * 16 + l15;
-      f16x4 hi, lo;
+    for (int ii = 0; ii < 4; ++ii) {
+      const int c = n0 + wc * 64 + ii * 16 + q * 4;
+      if (c >= w.ldn) continue;
+      const int64_t o = (int64_t)r * w.ldn + c;
+      const f16x4 xh = *reinterpret_cast<const f16x4*>(x + o), xl = *reinterpret_cast<const f16x4*>(x + o + px);
+      float v[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float v = ldexpf(acc[ii][j][k], -st.ep);
-        const int64_t o = (int64_t)(r + k) * w.ldn + c;
-        if (r + k < t.m && c < t.n) v = fmaf(st.a, (float)x[o] + (float)x[o + px], v);
-        if (st.last) {
-          if (r + k < t.m && c < t.n)
-            ((T*)t.out)[t.tall ? (int64_t)c * t.m + r + k : (int64_t)(r + k) * t.n + c] = from_f32<T>(rho * ldexpf(v, -ey));
-          continue;
+      for (int k = 0; k < 4; ++k) v[k] = fmaf(st.a, (float)xh[k] + (float)xl[k], acc[ii][j][k] * f);
+      if (!st.last) {
+        f16x4 h, l;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          f16 u, e;
+          f16_split(v[k], u, e);
+          h[k] = u;
+          l[k] = e;
         }
-        f16 h, l;
-        f16_split(v, h, l);
-        hi[k] = h;
-        lo[k] = l;
-        if (r + k < t.m && c < w.ldn) {
-          xo[o] = h;
-          xo[o + px] = l;
-        }
+        *reinterpret_cast<f16x4*>(xo + o) = h;
+        *reinterpret_cast<f16x4*>(xo + o + px) = l;
+        continue;
       }
-      if (!st.last && c < t.n && r < w.ldm) {
-        const int64_t o = (int64_t)c * w.ldm + r;
-        *reinterpret_cast<f16x4*>(xto + o) = hi;
-        *reinterpret_cast<f16x4*>(xto + o + pt) = lo;
-      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = fo * ldexpf(v[k], -ey);
+      if (vec) {
+        if (c >= t.n) continue;
+        T* d = out + (int64_t)r * t.n + c;
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4*>(d) = f32x4{v[0], v[1], v[2], v[3]};
+        else *reinterpret_cast<bf16x4*>(d) = bf16x4{(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
+      } else
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (c + k < t.n) out[t.tall ? (int64_t)(c + k) * t.m + r : (int64_t)r * t.n + c + k] = from_f32<T>(v[k]);
     }
+  }
 }
 
 // steps = 0: the normalised matrix itself
@@ -355,6 +442,52 @@ __global__ __launch_bounds__(256) void ns_copy_kernel(NsArgs a, const NsScale* _
 
 int64_t norm_blocks(int64_t m, int64_t n) { return ceil_div64(m * n, NORM_CHUNK); }
 
+// How the symmetric products of a launch are cut.  `slots` workgroups (two per CU) run at once.
+//  - Fewer tiles than slots: every reduction is cut into runs of about equal length so that the runs fill the slots.
+//  - One matrix with a little more than whole rounds of tiles: the tiles of the last round are cut instead of leaving
+//    most of the chip idle for it (4096 x 4096: 528 tiles on 512 slots).
+// Returns the partial tiles; fills direct / slices / p0 / f0 of every matrix.  len(t) = its reduction in k-steps of 32.
+template <typename F>
+int64_t cut_sym(NsArgs& a, F len, int& joins) {
+  const int slots = 512;
+  int64_t tiles = 0, work = 0, parts = 0;
+  joins = 0;
+  auto count = [](const NsMat& t) {
+    const int n = ceil_div(t.m, GM);
+    return n * (n + 1) / 2;
+  };
+  for (int i = 0; i < a.count; ++i) {
+    tiles += count(a.mat[i]);
+    work += (int64_t)count(a.mat[i]) * len(a.mat[i]);
+  }
+  for (int i = 0; i < a.count; ++i) {
+    NsMat& t = a.mat[i];
+    const int n = count(t);
+    t.direct = n;
+    t.slices = 1;
+    if (tiles < slots) {
+      const int64_t run = ceil_div64(work, slots) > 8 ? ceil_div64(work, slots) : 8;
+      const int64_t s = len(t) / run;
+      if (s > 1) {
+        t.slices = (int)(s < 32 ? s : 32);
+        t.direct = 0;
+      }
+    } else if (a.count == 1 && tiles % slots && tiles % slots <= slots / 2) {
+      const int tail = (int)(tiles % slots);
+      const int s = slots / tail < len(t) / 4 ? slots / tail : len(t) / 4;
+      if (s > 1) {
+        t.slices = s < 32 ? s : 32;
+        t.direct = n - tail;
+      }
+    }
+    t.p0 = (int)parts;
+    t.f0 = joins;
+    parts += (int64_t)(n - t.direct) * (t.slices > 1 ? t.slices : 0);
+    joins += n - t.direct;
+  }
+  return parts;
+}
+
 int check_ns(const char* who, int dtype, int count, const int* rows, const int* cols) {
   if (dtype != VC_F32 && dtype != VC_BF16) {
     vc_set_error("%s: unsupported dtype %d", who, dtype);
@@ -369,6 +502,34 @@ int check_ns(const char* who, int dtype, int count, const int* rows, const int* 
   return VC_OK;
 }
 
+// Sizes of a launch's matrices and where everything lies in the workspace:
+// [NsScale per matrix | partial norms | partial tiles | fp16 buffers]
+struct NsLayout {
+  int64_t norm_blocks, init_tiles, upd_tiles, part, mats, bytes;
+};
+NsLayout layout(NsArgs& a, const int* rows, const int* cols) {
+  NsLayout l{};
+  int64_t at = 0;
+  for (int i = 0; i < a.count; ++i) {
+    NsMat& t = a.mat[i];
+    t.tall = rows[i] > cols[i];
+    t.m = t.tall ? cols[i] : rows[i];
+    t.n = t.tall ? rows[i] : cols[i];
+    t.at = at;
+    at = NsView(t, 0).end;
+    l.norm_blocks += norm_blocks(t.m, t.n);
+    l.init_tiles += (int64_t)(up64(t.m) / 64) * (up64(t.n) / 64);
+    l.upd_tiles += (int64_t)ceil_div(t.m, GM) * ceil_div(t.n, GM);
+  }
+  int joins;
+  const int64_t p1 = cut_sym(a, [](const NsMat& t) { return up64(t.n) / 32; }, joins);
+  const int64_t p2 = cut_sym(a, [](const NsMat& t) { return up64(t.m) / 32; }, joins);
+  l.part = NS_MAX * (int64_t)sizeof(NsScale) + up128(l.norm_blocks * 8);
+  l.mats = l.part + (p1 > p2 ? p1 : p2) * GM * GM * 4;
+  l.bytes = l.mats + at * 2;
+  return l;
+}
+
 }  // namespace
 
 extern "C" {
@@ -377,16 +538,9 @@ int64_t vc_newton_schulz_bytes(int count, const int* rows, const int* cols) {
   if (check_ns("vc_newton_schulz_bytes", VC_F32, count, rows, cols) != VC_OK) return -1;
   int64_t most = 0;
   for (int b = 0; b < count; b += NS_MAX) {
-    int64_t elems = 0, blocks = 0;
-    for (int i = b; i < count && i < b + NS_MAX; ++i) {
-      const int m = rows[i] < cols[i] ? rows[i] : cols[i], n = rows[i] < cols[i] ? cols[i] : rows[i];
-      NsMat t{};
-      t.m = m;
-      t.n = n;
-      elems += NsView(t, 0).end;
-      blocks += norm_blocks(m, n);
-    }
-    const int64_t bytes = NS_MAX * (int64_t)sizeof(NsScale) + up128(blocks * 8) + elems * 2;
+    NsArgs a{};
+    a.count = count - b < NS_MAX ? count - b : NS_MAX;
+    const int64_t bytes = layout(a, rows + b, cols + b).bytes;
     if (bytes > most) most = bytes;
   }
   return most;
@@ -405,71 +559,57 @@ int vc_newton_schulz(int dtype, int count, const void* const* g, void* const* ou
                (double)gain, (double)pmax);
   for (int i = 0; i < count; ++i) VC_CHECK_ARG(g[i] && out[i], "vc_newton_schulz: null matrix %d", i);
   NsScale* sc = (NsScale*)workspace;
-  double* part = (double*)((char*)workspace + NS_MAX * sizeof(NsScale));
+  double* norms = (double*)((char*)workspace + NS_MAX * sizeof(NsScale));
   NsStep st;
   st.es = (int)floorf(log2f(60000.f / (cap * cap)));
   st.ep = (int)floorf(log2f(60000.f / pmax));
+  const bool bf = dtype == VC_BF16;
   for (int b = 0; b < count; b += NS_MAX) {
-    NsArgs a;
+    NsArgs a{};
     a.count = count - b < NS_MAX ? count - b : NS_MAX;
-    int64_t blocks = 0, t_init = 0, t_sym = 0, t_upd = 0;
-    for (int i = 0; i < a.count; ++i) blocks += norm_blocks(rows[b + i], cols[b + i]);
-    int64_t at = 0;
-    int tn[NS_MAX], ti[NS_MAX], ts[NS_MAX], tu[NS_MAX];
-    f16* ws = (f16*)((char*)part + up128(blocks * 8));
-    blocks = 0;
-    for (int i = 0; i < a.count; ++i) {
-      NsMat& t = a.mat[i];
-      const int r = rows[b + i], c = cols[b + i];
-      t.g = g[b + i];
-      t.out = out[b + i];
-      t.tall = r > c;
-      t.m = t.tall ? c : r;
-      t.n = t.tall ? r : c;
-      t.at = at;
-      at = NsView(t, 0).end;
-      tn[i] = (int)blocks;
-      ti[i] = (int)t_init;
-      ts[i] = (int)t_sym;
-      tu[i] = (int)t_upd;
-      blocks += norm_blocks(t.m, t.n);
-      t_init += (int64_t)(up64(t.m) / 64) * (up64(t.n) / 64);
-      const int64_t tm = ceil_div(t.m, GM), tnn = ceil_div(t.n, GM);
-      t_sym += tm * (tm + 1) / 2;
-      t_upd += tm * tnn;
-    }
-    VC_CHECK_SHAPE(blocks < (1ll << 31) && t_init < (1ll << 31) && t_sym < (1ll << 31) && t_upd < (1ll << 31),
+    const NsLayout l = layout(a, rows + b, cols + b);
+    VC_CHECK_SHAPE(l.norm_blocks < (1ll << 31) && l.init_tiles < (1ll << 31) && l.upd_tiles < (1ll << 31),
                    "vc_newton_schulz: too many tiles");
-    auto with = [&](const int* first) {
-      for (int i = 0; i < a.count; ++i) a.mat[i].t0 = first[i];
+    float* part = (float*)((char*)workspace + l.part);
+    f16* ws = (f16*)((char*)workspace + l.mats);
+    for (int i = 0; i < a.count; ++i) {
+      a.mat[i].g = g[b + i];
+      a.mat[i].out = out[b + i];
+    }
+    auto launch = [&](auto blocks_of, auto kernel, int threads, auto... args) {  // blocks in the order of the matrices
+      int64_t at = 0;
+      for (int i = 0; i < a.count; ++i) {
+        a.mat[i].t0 = (int)at;
+        at += blocks_of(a.mat[i]);
+      }
+      hipLaunchKernelGGL(kernel, dim3((unsigned)at), dim3(threads), 0, stream, a, args...);
     };
-    const bool bf = dtype == VC_BF16;
-    with(tn);
-    if (bf) hipLaunchKernelGGL((ns_norm_kernel<bf16>), dim3((unsigned)blocks), dim3(256), 0, stream, a, part);
-    else hipLaunchKernelGGL((ns_norm_kernel<float>), dim3((unsigned)blocks), dim3(256), 0, stream, a, part);
-    hipLaunchKernelGGL(ns_scale_kernel, dim3(a.count), dim3(64), 0, stream, a, (int)blocks, part, eps, cap, gain, sc);
-    if (steps == 0) {
-      if (bf) hipLaunchKernelGGL((ns_copy_kernel<bf16>), dim3((unsigned)blocks), dim3(256), 0, stream, a, sc);
-      else hipLaunchKernelGGL((ns_copy_kernel<float>), dim3((unsigned)blocks), dim3(256), 0, stream, a, sc);
-    }
-    with(ti);
-    if (steps) {
-      if (bf) hipLaunchKernelGGL((ns_init_kernel<bf16>), dim3((unsigned)t_init), dim3(256), 0, stream, a, ws, sc);
-      else hipLaunchKernelGGL((ns_init_kernel<float>), dim3((unsigned)t_init), dim3(256), 0, stream, a, ws, sc);
-    }
+    auto by_norm = [](const NsMat& t) { return norm_blocks(t.m, t.n); };
+    auto by_init = [](const NsMat& t) { return (int64_t)(up64(t.m) / 64) * (up64(t.n) / 64); };
+    auto by_upd = [](const NsMat& t) { return (int64_t)ceil_div(t.m, GM) * ceil_div(t.n, GM); };
+    auto by_sym = [](const NsMat& t) {
+      const int64_t n = ceil_div(t.m, GM);
+      return t.direct + (n * (n + 1) / 2 - t.direct) * t.slices;
+    };
+    launch(by_norm, bf ? ns_norm_kernel<bf16> : ns_norm_kernel<float>, 256, norms);
+    hipLaunchKernelGGL(ns_scale_kernel, dim3(a.count), dim3(64), 0, stream, a, (int)l.norm_blocks, norms, eps, cap, gain, sc);
+    if (steps == 0) launch(by_norm, bf ? ns_copy_kernel<bf16> : ns_copy_kernel<float>, 256, sc);
+    else launch(by_init, bf ? ns_init_kernel<bf16> : ns_init_kernel<float>, 256, ws, sc);
     for (int k = 0; k < steps; ++k) {
       st.a = coeffs[3 * k];
       st.b = coeffs[3 * k + 1];
       st.c = coeffs[3 * k + 2];
       st.last = k == steps - 1;
-      with(ts);
-      hipLaunchKernelGGL((ns_sym_kernel<false>), dim3((unsigned)t_sym), dim3(G_THREADS), 0, stream, a, ws, sc, st, k & 1);
-      hipLaunchKernelGGL((ns_sym_kernel<true>), dim3((unsigned)t_sym), dim3(G_THREADS), 0, stream, a, ws, sc, st, k & 1);
-      with(tu);
-      if (bf)
-        hipLaunchKernelGGL((ns_update_kernel<bf16>), dim3((unsigned)t_upd), dim3(G_THREADS), 0, stream, a, ws, sc, st, k & 1);
-      else
-        hipLaunchKernelGGL((ns_update_kernel<float>), dim3((unsigned)t_upd), dim3(G_THREADS), 0, stream, a, ws, sc, st, k & 1);
+      int joins = 0;
+      cut_sym(a, [](const NsMat& t) { return up64(t.n) / 32; }, joins);
+      launch(by_sym, ns_sym_kernel<false>, G_THREADS, ws, sc, st, k & 1, part);
+      if (joins)
+        hipLaunchKernelGGL(ns_sym_join_kernel<false>, dim3(joins), dim3(G_THREADS), 0, stream, a, ws, sc, st, k & 1, part);
+      cut_sym(a, [](const NsMat& t) { return up64(t.m) / 32; }, joins);
+      launch(by_sym, ns_sym_kernel<true>, G_THREADS, ws, sc, st, k & 1, part);
+      if (joins)
+        hipLaunchKernelGGL(ns_sym_join_kernel<true>, dim3(joins), dim3(G_THREADS), 0, stream, a, ws, sc, st, k & 1, part);
+      launch(by_upd, bf ? ns_update_kernel<bf16> : ns_update_kernel<float>, G_THREADS, ws, sc, st, k & 1);
     }
     VC_LAUNCH_CHECK("vc_newton_schulz");
   }
