@@ -89,20 +89,43 @@ struct G16 {
     return (unsigned)row * (unsigned)ld * 2u + (unsigned)((((pos >> 1) ^ cswz(row)) << 1) | (pos & 1)) * 16u;
   }
 
+  // A staged operand plane: its descriptor, moved along the reduction by a scalar offset (ROW) or by its base (COL).
   template <int KIND>
-  __device__ static __forceinline__ void stage_op(const Op16& o, int plane, unsigned lds, const unsigned (&v)[REQ], int k) {
-    if (KIND == ROW) {
-      const i32x4_t d = g16_desc(o.p + plane * o.plane, (unsigned)(o.n < GM ? o.n : GM) * (unsigned)o.ld * 2u);
+  struct Stream {
+    i32x4_t d;
+    uint64_t at;     // COL: address of the k-step's corner
+    uint64_t step;   // COL: bytes of a k-step
+    int left, ld2, side2;
+    __device__ __forceinline__ void open(const Op16& o, int plane, int k0) {
+      if (KIND == ROW) {
+        d = g16_desc(o.p + plane * o.plane, (unsigned)(o.n < GM ? o.n : GM) * (unsigned)o.ld * 2u);
+        return;
+      }
+      const uint64_t u = (uint64_t)(o.p + plane * o.plane + (int64_t)k0 * o.ld + o.side);
+      at = (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)u) |
+           ((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(u >> 32)) << 32);
+      ld2 = __builtin_amdgcn_readfirstlane(o.ld * 2);
+      side2 = __builtin_amdgcn_readfirstlane(o.side * 2);
+      left = __builtin_amdgcn_readfirstlane(o.n - k0);
+      step = (uint64_t)BK * (unsigned)ld2;
+      d[3] = 0x00020000;
+    }
+    __device__ __forceinline__ void stage(unsigned lds, const unsigned (&v)[REQ], int k) {
+      if (KIND == ROW) {
 #pragma unroll
-      for (int t = 0; t < REQ; ++t) g16_dma(d, lds + t * 4096, v[t], k * 2);
-    } else {
-      const int rows = o.n - k < BK ? o.n - k : BK;
-      const i32x4_t d = g16_desc(o.p + plane * o.plane + (int64_t)k * o.ld + o.side,
-                                 rows > 0 ? (unsigned)rows * (unsigned)o.ld * 2u - (unsigned)o.side * 2u : 0u);
+        for (int t = 0; t < REQ; ++t) g16_dma(d, lds + t * 4096, v[t], k * 2);
+        return;
+      }
+      const int rows = left < BK ? left : BK;
+      d[0] = (int)at;
+      d[1] = (int)(at >> 32);
+      d[2] = rows > 0 ? rows * ld2 - side2 : 0;
 #pragma unroll
       for (int t = 0; t < REQ; ++t) g16_dma(d, lds + t * 4096, v[t], 0);
+      at += step;
+      left -= BK;
     }
-  }
+  };
 
   // fragment of the 16 tile rows (ROW) or columns (COL) of block `blk` (0..7), 32 reduction elements from kk * 32
   template <int KIND>
@@ -137,15 +160,21 @@ struct G16 {
       va[t] = src_off<KA>(t, wave, lane, a.ld);
       vb[t] = src_off<KB>(t, wave, lane, b.ld);
     }
+    k0 = __builtin_amdgcn_readfirstlane(k0);
+    k1 = __builtin_amdgcn_readfirstlane(k1);
+    Stream<KA> sa[PA];
+    Stream<KB> sb[PB];
+#pragma unroll
+    for (int p = 0; p < PA; ++p) sa[p].open(a, p, k0);
+#pragma unroll
+    for (int p = 0; p < PB; ++p) sb[p].open(b, p, k0);
     auto stage = [&](int s, int k) {
       const unsigned base = g16_lds(smem + s * STAGE) + wave * 1024;
 #pragma unroll
-      for (int p = 0; p < PA; ++p) stage_op<KA>(a, p, base + p * PLANE * 2, va, k);
+      for (int p = 0; p < PA; ++p) sa[p].stage(base + p * PLANE * 2, va, k);
 #pragma unroll
-      for (int p = 0; p < PB; ++p) stage_op<KB>(b, p, base + (PA + p) * PLANE * 2, vb, k);
+      for (int p = 0; p < PB; ++p) sb[p].stage(base + (PA + p) * PLANE * 2, vb, k);
     };
-    k0 = __builtin_amdgcn_readfirstlane(k0);
-    k1 = __builtin_amdgcn_readfirstlane(k1);
     int s = 0;
     if (k0 < k1) stage(0, k0);
     for (int k = k0; k < k1; k += BK, s ^= 1) {

@@ -43,7 +43,18 @@ __device__ __forceinline__ float amax_part(const T* p, int64_t rows, int K, cons
   } else {
     for (int64_t r = block * 4 + (threadIdx.x >> 6); r < rows; r += nblocks * 4) {
       if (target[r] == ignore) continue;
-      for (int k = threadIdx.x & 63; k < K; k += 64) m = fmaxf(m, finite_mag(to_f32(p[r * K + k])));
+      const T* row = p + r * K;
+      int k = threadIdx.x & 63;
+      if (K % 8 == 0 && ((uintptr_t)p & 15) == 0) {
+        for (k *= 8; k < K; k += 512) {
+          const F8 v = load8(row + k);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) m = fmaxf(m, finite_mag(v.v[e]));
+        }
+      } else {
+#pragma unroll 4
+        for (; k < K; k += 64) m = fmaxf(m, finite_mag(to_f32(row[k])));
+      }
     }
   }
   return m;
@@ -261,17 +272,17 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_stats_kernel(CeArgs a, float4
     }
 }
 
-// Per row: lse (in units of log2), loss (0 for ignored rows, NaN for a target outside [0, V)), arg-max.  32 rows x 8 runs of tiles per block.
+// Per row: lse (in units of log2), loss (0 for ignored rows, NaN for a target outside [0, V)), arg-max.  8 rows x 32 runs of tiles per block.
 __global__ __launch_bounds__(256) void ce_join_kernel(const float4* __restrict__ part, const float* __restrict__ zt,
                                                       const int64_t* __restrict__ target, int64_t ignore, int N, int V,
                                                       int tiles_v, float smooth, float* __restrict__ lse,
                                                       float* __restrict__ rowloss, int64_t* __restrict__ pred) {
-  __shared__ Stat sm[8][32];
-  const int e = threadIdx.x & 31, run = threadIdx.x >> 5;
-  const int n = blockIdx.x * 32 + e;
+  __shared__ Stat sm[32][8];
+  const int e = threadIdx.x & 7, run = threadIdx.x >> 3;
+  const int n = blockIdx.x * 8 + e;
   Stat s{-INFINITY, 0.f, 0.f, V};
   if (n < N) {
-    const int per = (tiles_v + 7) / 8, t1 = min(tiles_v, (run + 1) * per);
+    const int per = (tiles_v + 31) / 32, t1 = min(tiles_v, (run + 1) * per);
 #pragma unroll 4
     for (int t = run * per; t < t1; ++t) {
       const float4 o = part[(int64_t)t * N + n];
@@ -280,9 +291,16 @@ __global__ __launch_bounds__(256) void ce_join_kernel(const float4* __restrict__
   }
   sm[run][e] = s;
   __syncthreads();
-  if (run == 0 && n < N) {
 #pragma unroll
-    for (int r = 1; r < 8; ++r) stat_join(s, sm[r][e]);
+  for (int w = 16; w > 1; w >>= 1) {
+    if (run < w) {
+      stat_join(s, sm[run + w][e]);
+      sm[run][e] = s;
+    }
+    __syncthreads();
+  }
+  if (run == 0 && n < N) {
+    stat_join(s, sm[1][e]);
     const float l = (s.m == -INFINITY ? 0.f : s.m) + log2f(s.s);
     lse[n] = l;
     const int64_t t = target[n];
@@ -511,6 +529,27 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
   const float f = g.part ? 1.f : mm_factor(g.fac, g.exps, g.which);
   float* part = g.part ? g.part + (int64_t)split * g.M * g.Nn : nullptr;
   const bool vec = g.vec;
+  if (!part)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] *= f;
+  // what is added to comes first: the stores could alias these loads and would hold them back
+  if (vec && g.add) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t o = (int64_t)min(m0 + wr * 64 + j * 16 + l15, g.M - 1) * g.Nn + min(n0 + wc * 64 + i * 16 + q * 4, g.Nn - 4);
+        if (part) acc[i][j] += *reinterpret_cast<const f32x4*>(part + o);
+        else if constexpr (sizeof(T) == 4) acc[i][j] += *reinterpret_cast<const f32x4*>((const float*)g.out + o);
+        else {
+          const bf16x4 r = *reinterpret_cast<const bf16x4*>((const bf16*)g.out + o);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] += (float)r[e];
+        }
+      }
+  }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int row = m0 + wr * 64 + j * 16 + l15;
@@ -519,26 +558,12 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
     for (int i = 0; i < 4; ++i) {
       const int col = n0 + wc * 64 + i * 16 + q * 4;  // four results of one row
       const int64_t o = (int64_t)row * g.Nn + col;
-      f32x4 v = acc[i][j];
+      const f32x4 v = acc[i][j];
       if (vec) {
         if (col >= g.Nn) continue;
-        if (part) {
-          if (g.add) v += *reinterpret_cast<const f32x4*>(part + o);
-          *reinterpret_cast<f32x4*>(part + o) = v;
-        } else if constexpr (sizeof(T) == 4) {
-          float* out = (float*)g.out + o;
-          v *= f;
-          if (g.add) v += *reinterpret_cast<const f32x4*>(out);
-          *reinterpret_cast<f32x4*>(out) = v;
-        } else {
-          bf16* out = (bf16*)g.out + o;
-          v *= f;
-          bf16x4 r = {0, 0, 0, 0};
-          if (g.add) r = *reinterpret_cast<const bf16x4*>(out);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) r[e] = (bf16)((float)r[e] + v[e]);
-          *reinterpret_cast<bf16x4*>(out) = r;
-        }
+        if (part) *reinterpret_cast<f32x4*>(part + o) = v;
+        else if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4*>((float*)g.out + o) = v;
+        else *reinterpret_cast<bf16x4*>((bf16*)g.out + o) = bf16x4{(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -546,7 +571,7 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
           if (part) part[o + e] = g.add ? part[o + e] + v[e] : v[e];
           else {
             T* out = (T*)g.out + o + e;
-            *out = from_f32<T>(g.add ? to_f32(*out) + v[e] * f : v[e] * f);
+            *out = from_f32<T>(g.add ? to_f32(*out) + v[e] : v[e]);
           }
         }
       }
@@ -665,8 +690,8 @@ void pack_go(const Plan& p, const void* x, const void* w, int N, int V, int K, c
   float* amax = (float*)(ws + p.f_amax);
   const int per = ceil_div(p.ld, 512);
   const int xb = (int)ceil_div64((int64_t)N * per, 4), wb = (int)ceil_div64((int64_t)V * per, 4);
-  auto blocks = [](int64_t elems) {  // of about 8 K elements
-    const int64_t b = ceil_div64(elems, 8192);
+  auto blocks = [](int64_t elems) {  // of one vector per thread where that is enough blocks
+    const int64_t b = ceil_div64(elems, 2048);
     return (int)(b < AMAX_MOST ? b : AMAX_MOST);
   };
   const int xa = blocks((int64_t)N * K), wa = blocks((int64_t)V * K);
@@ -731,7 +756,7 @@ int vc_linear_ce_fwd(int xdtype, int wdtype, const void* x, const void* w, const
   else if (p.pw == 2) hipLaunchKernelGGL((ce_stats_kernel<2, 2, false>), grid, dim3(G_THREADS), 0, stream, a, part, zt);
   else if (more) hipLaunchKernelGGL((ce_stats_kernel<1, 1, true>), grid, dim3(G_THREADS), 0, stream, a, part, zt);
   else hipLaunchKernelGGL((ce_stats_kernel<1, 1, false>), grid, dim3(G_THREADS), 0, stream, a, part, zt);
-  hipLaunchKernelGGL(ce_join_kernel, dim3(ceil_div(N, 32)), dim3(256), 0, stream, part, zt, target, ignore_index, N, V,
+  hipLaunchKernelGGL(ce_join_kernel, dim3(ceil_div(N, 8)), dim3(256), 0, stream, part, zt, target, ignore_index, N, V,
                      a.tiles_v, smoothing, (float*)(sv + p.o_lse), row_loss, pred);
   hipLaunchKernelGGL(ce_total_kernel, dim3(1), dim3(1024), 0, stream, row_loss, target, pred, ignore_index, N, mean, loss,
                      (float*)(sv + p.o_total), correct);

@@ -248,6 +248,25 @@ __device__ __forceinline__ void sym_store(f32x4 (&acc)[4][4], const NsMat& t, co
   const float sb = ldexpf(st.b, st.ep - st.es);
   constexpr int STR = GM + 8;
   f16x4 lo[4][4];
+  if (SQUARE) {  // all of S first: the stores below could alias its loads and would hold them back
+    f16x4 sh[4][4], sl[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = m0 + wm * 64 + i * 16 + q * 4, c = n0 + wn * 64 + j * 16 + l15;
+        const int64_t o = (int64_t)min(c, t.m - 1) * w.ldm + min(r, w.ldm - 4);
+        sh[i][j] = *reinterpret_cast<const f16x4*>(s + o);
+        sl[i][j] = *reinterpret_cast<const f16x4*>(s + o + pl);
+      }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          acc[i][j][k] = fmaf(sb, (float)sh[i][j][k] + (float)sl[i][j][k], acc[i][j][k] * f);
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -255,15 +274,10 @@ __device__ __forceinline__ void sym_store(f32x4 (&acc)[4][4], const NsMat& t, co
       const int r = m0 + wm * 64 + i * 16 + q * 4, c = n0 + wn * 64 + j * 16 + l15;
       const bool in = c < t.m && r < w.ldm;
       const int64_t o = (int64_t)c * w.ldm + r;
-      f16x4 sh = {0, 0, 0, 0}, sl = {0, 0, 0, 0}, h;
-      if (SQUARE && in) {
-        sh = *reinterpret_cast<const f16x4*>(s + o);
-        sl = *reinterpret_cast<const f16x4*>(s + o + pl);
-      }
+      f16x4 h;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        float v = acc[i][j][k] * f;
-        if (SQUARE) v = fmaf(sb, (float)sh[k] + (float)sl[k], v);
+        const float v = SQUARE ? acc[i][j][k] : acc[i][j][k] * f;
         f16 u, e;
         f16_split(v, u, e);
         h[k] = u;
@@ -309,8 +323,8 @@ __global__ __launch_bounds__(G_THREADS, 2) void ns_sym_kernel(NsArgs a, f16* __r
   const NsMat& t = a.mat[i];
   const NsView w(t, parity);
   const int tiles = (t.m + GM - 1) / GM, count = tiles * (tiles + 1) / 2;
-  const int units = t.direct + (count - t.direct) * t.slices;
-  const int id = xcd_run(blockIdx.x - t.t0, units);
+  int id = blockIdx.x - t.t0;  // whole tiles first, then slices; each kind spread over the XCDs by itself
+  id = id < t.direct ? xcd_run(id, t.direct) : t.direct + xcd_run(id - t.direct, (count - t.direct) * t.slices);
   const int ld = SQUARE ? w.ldm : w.ldn;
   int tile = id, k0 = 0, k1 = ld, slot = -1;
   if (id >= t.direct) {
@@ -387,6 +401,25 @@ __global__ __launch_bounds__(G_THREADS, 2) void ns_update_kernel(NsArgs a, f16* 
   const int ey = sc[i].ey;
   T* out = (T*)t.out;
   const bool vec = !t.tall && t.n % 4 == 0 && ((uintptr_t)out & 15) == 0;
+  {
+    f16x4 xh[4][4], xl[4][4];  // all of X's tile first: the stores below could alias its loads and would hold them back
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int ii = 0; ii < 4; ++ii) {
+        const int64_t o = (int64_t)min(m0 + wr * 64 + j * 16 + l15, t.m - 1) * w.ldn +
+                          min(n0 + wc * 64 + ii * 16 + q * 4, w.ldn - 4);
+        xh[ii][j] = *reinterpret_cast<const f16x4*>(x + o);
+        xl[ii][j] = *reinterpret_cast<const f16x4*>(x + o + px);
+      }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int ii = 0; ii < 4; ++ii)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          acc[ii][j][k] = fmaf(st.a, (float)xh[ii][j][k] + (float)xl[ii][j][k], acc[ii][j][k] * f);
+  }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int r = m0 + wr * 64 + j * 16 + l15;
@@ -396,10 +429,7 @@ __global__ __launch_bounds__(G_THREADS, 2) void ns_update_kernel(NsArgs a, f16* 
       const int c = n0 + wc * 64 + ii * 16 + q * 4;
       if (c >= w.ldn) continue;
       const int64_t o = (int64_t)r * w.ldn + c;
-      const f16x4 xh = *reinterpret_cast<const f16x4*>(x + o), xl = *reinterpret_cast<const f16x4*>(x + o + px);
-      float v[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = fmaf(st.a, (float)xh[k] + (float)xl[k], acc[ii][j][k] * f);
+      f32x4 v = acc[ii][j];
       if (!st.last) {
         f16x4 h, l;
 #pragma unroll
@@ -418,7 +448,7 @@ __global__ __launch_bounds__(G_THREADS, 2) void ns_update_kernel(NsArgs a, f16* 
       if (vec) {
         if (c >= t.n) continue;
         T* d = out + (int64_t)r * t.n + c;
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4*>(d) = f32x4{v[0], v[1], v[2], v[3]};
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4*>(d) = v;
         else *reinterpret_cast<bf16x4*>(d) = bf16x4{(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
       } else
 #pragma unroll
@@ -469,14 +499,14 @@ int64_t cut_sym(NsArgs& a, F len, int& joins) {
       const int64_t run = ceil_div64(work, slots) > 8 ? ceil_div64(work, slots) : 8;
       const int64_t s = len(t) / run;
       if (s > 1) {
-        t.slices = (int)(s < 32 ? s : 32);
+        t.slices = (int)(s < 8 ? s : 8);
         t.direct = 0;
       }
     } else if (a.count == 1 && tiles % slots && tiles % slots <= slots / 2) {
       const int tail = (int)(tiles % slots);
       const int s = slots / tail < len(t) / 4 ? slots / tail : len(t) / 4;
       if (s > 1) {
-        t.slices = s < 32 ? s : 32;
+        t.slices = s < 8 ? s : 8;
         t.direct = n - tail;
       }
     }
