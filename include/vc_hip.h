@@ -210,7 +210,8 @@ int vc_layernorm_bwd_add(int dtype, const void* x, const void* dout, const float
  * dresidual: channels-last [N][S][C] in `dtype`; any C with C % G == 0 (16-byte vectors when C is a multiple of 8 and
  * the pointers are 16-byte aligned).  y = act((x - mean) * rstd * gamma + beta + residual) with one mean / rstd
  * [N][G] per sample and group; gamma / beta nullable (1 / 0).  act: 0 none, 1 ReLU, 2 SiLU, 3 GELU (erf).  Backward takes
- * the forward call's mean / rstd, writes dx and dresidual (both nullable) and ACCUMULATES dgamma / dbeta (nullable).
+ * the forward call's mean / rstd and writes dx, dresidual, dgamma and dbeta (each nullable); bit 0 / 1 of `accumulate`
+ * adds to what dgamma / dbeta hold instead.
  * workspace: vc_group_norm_workspace_floats() floats, 8-byte aligned, contents irrelevant before and after; every sum
  * has a fixed order. */
 int64_t vc_group_norm_workspace_floats(int N, int S, int C, int G);
@@ -219,7 +220,8 @@ int vc_group_norm_fwd(int dtype, const void* x, const void* residual, const floa
                       vc_stream_t stream);
 int vc_group_norm_bwd(int dtype, const void* x, const void* dy, const void* residual, const float* gamma,
                       const float* beta, const float* mean, const float* rstd, void* dx, void* dresidual, float* dgamma,
-                      float* dbeta, float* workspace, int N, int S, int C, int G, int act, vc_stream_t stream);
+                      float* dbeta, float* workspace, int N, int S, int C, int G, int act, int accumulate,
+                      vc_stream_t stream);
 
 /* ---- layout, pooling, elementwise ------------------------------------------------------------------ */
 /* x_3d[:, t] slicing + NCHW->channels-last (model_components.py:127, 176, 285, 460; Conv3D input
@@ -357,8 +359,8 @@ int vc_ce_fwd_bwd(int grad_dtype, const float* logits, int ld, const int64_t* ta
  * makes its row's loss and gradients NaN.  mean: divide by the rows that count (by 1 if there are none).
  * fwd: row_loss [N] (0 for ignored rows), loss (nullable, one float), pred [N] (nullable, lowest arg-max) and correct
  *   (nullable).  saved: vc_linear_ce_bytes(0, ..) bytes that backward reads; workspace: vc_linear_ce_bytes(1, ..).
- * bwd: dloss = upstream gradient of the mean or sum, or of every row's loss with per_row; dx (nullable) is written, dw and
- *   db (nullable) are ACCUMULATED into; workspace: vc_linear_ce_bytes(2, ..).  Buffers 256-byte aligned, contents of
+ * bwd: dloss = upstream gradient of the mean or sum, or of every row's loss with per_row; dx, dw and db (each nullable)
+ *   are written, or added to where bit 0 (dw) / bit 1 (db) of `accumulate` is set; workspace: vc_linear_ce_bytes(2, ..).  Buffers 256-byte aligned, contents of
  * the workspaces irrelevant before and after; every sum has a fixed order. */
 int64_t vc_linear_ce_bytes(int what, int xdtype, int wdtype, int N, int V, int K);
 int vc_linear_ce_fwd(int xdtype, int wdtype, const void* x, const void* w, const void* bias, const int64_t* target,
@@ -366,7 +368,7 @@ int vc_linear_ce_fwd(int xdtype, int wdtype, const void* x, const void* w, const
                      int* correct, void* saved, void* workspace, int N, int V, int K, vc_stream_t stream);
 int vc_linear_ce_bwd(int xdtype, int wdtype, const void* bias, const int64_t* target, int64_t ignore_index,
                      float smoothing, int mean, int per_row, const float* dloss, const void* saved, void* dx, void* dw,
-                     void* db, void* workspace, int N, int V, int K, vc_stream_t stream);
+                     void* db, void* workspace, int accumulate, int N, int V, int K, vc_stream_t stream);
 /* optim.Adam (L2-coupled) / AdamW / SGD(momentum) (training_utils.py:324-329) over one flat fp32 buffer.
  * mode 0 Adam, 1 AdamW, 2 SGD (b1 = momentum).  grad_scale folds the 1/world of the all-reduce. */
 int vc_optim_step(int mode, float* p, const float* g, float* m, float* v, int64_t n, float lr, float b1, float b2,

@@ -105,3 +105,27 @@ def f64(v):
 
 def last_error():
     return lib().vc_last_error().decode("utf-8", "replace")
+
+
+# Entry points called with plain Python numbers (pointers as data_ptr() integers or None): ctypes converts by the declared
+# types in C, a third of the time that building one ctypes object per argument takes.  p pointer, i int, l int64, f float,
+# d double; the trailing stream is added by `fast`.
+_SIGNATURES = {
+    "vc_group_norm_fwd": "i" + 8 * "p" + "iiii" + "fi",
+    "vc_group_norm_bwd": "i" + 12 * "p" + "iiii" + "ii",
+    "vc_linear_ce_fwd": "ii" + 4 * "p" + "lfi" + 6 * "p" + "iii",
+    "vc_linear_ce_bwd": "ii" + 2 * "p" + "lfii" + 6 * "p" + "i" + "iii",
+}
+_CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_int64, "f": ctypes.c_float, "d": ctypes.c_double}
+_bound = {}
+
+
+def fast(name, device, *args):
+    """Call entry point `name` on the current stream of `device` (a torch.device with an index)."""
+    fn = _bound.get(name)
+    if fn is None:
+        fn = lib()[name]  # indexing makes a function object of its own, so `call` keeps its untyped one
+        fn.argtypes = [_CTYPES[c] for c in _SIGNATURES[name]] + [ctypes.c_void_p]
+        fn.restype = ctypes.c_int
+        _bound[name] = fn
+    check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)), name)

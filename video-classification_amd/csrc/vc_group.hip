@@ -349,9 +349,10 @@ __global__ __launch_bounds__(64) void gn_bwd_join_kernel(Cover k, const float* _
   }
 }
 
-// dgamma[c] += sum_n B_c, dbeta[c] += sum_n A_c: 64 channels x 4 runs of samples per block, runs joined in order
+// dgamma[c] (+)= sum_n B_c, dbeta[c] (+)= sum_n A_c (added to where bit 0 / bit 1 of `add` is set): 64 channels x 4 runs of
+// samples per block, runs joined in order
 __global__ __launch_bounds__(GT) void gn_bwd_params_kernel(const float* __restrict__ ab, float* __restrict__ dgamma,
-                                                           float* __restrict__ dbeta, int N, int C) {
+                                                           float* __restrict__ dbeta, int N, int C, int add) {
   __shared__ float sa[4][64], sb[4][64];
   const int e = threadIdx.x & 63, run = threadIdx.x >> 6;
   const int c = blockIdx.x * 64 + e;
@@ -366,8 +367,8 @@ __global__ __launch_bounds__(GT) void gn_bwd_params_kernel(const float* __restri
   sb[run][e] = b;
   __syncthreads();
   if (run == 0 && c < C) {
-    if (dbeta) dbeta[c] += (sa[0][e] + sa[1][e]) + (sa[2][e] + sa[3][e]);
-    if (dgamma) dgamma[c] += (sb[0][e] + sb[1][e]) + (sb[2][e] + sb[3][e]);
+    if (dbeta) dbeta[c] = (add & 2 ? dbeta[c] : 0.f) + ((sa[0][e] + sa[1][e]) + (sa[2][e] + sa[3][e]));
+    if (dgamma) dgamma[c] = (add & 1 ? dgamma[c] : 0.f) + ((sb[0][e] + sb[1][e]) + (sb[2][e] + sb[3][e]));
   }
 }
 
@@ -489,7 +490,7 @@ int fwd_go(const Cover& k, int N, const void* x, const void* res, const float* g
 template <typename T, int V>
 int bwd_go(const Cover& k, int N, const void* x, const void* dy, const void* res, const float* gamma, const float* beta,
            const float* mean, const float* rstd, void* dx, void* dres, float* dgamma, float* dbeta, float* ws, int act,
-           hipStream_t st) {
+           int add, hipStream_t st) {
   const dim3 grid(k.chunks, N, ceil_div(k.cv, k.cvb));
   float* ab = ws + (size_t)N * k.chunks * 2 * k.C;
   float2* coef = (float2*)(ab + (size_t)N * 2 * k.C);
@@ -498,7 +499,7 @@ int bwd_go(const Cover& k, int N, const void* x, const void* dy, const void* res
                                 (const T*)dy, (const T*)res, mean, rstd, gamma, beta, ws));
   hipLaunchKernelGGL(gn_bwd_join_kernel, dim3(k.G, N), dim3(64), 0, st, k, ws, gamma, ab, coef);
   if (dgamma || dbeta)
-    hipLaunchKernelGGL(gn_bwd_params_kernel, dim3(ceil_div(k.C, 64)), dim3(GT), 0, st, ab, dgamma, dbeta, N, k.C);
+    hipLaunchKernelGGL(gn_bwd_params_kernel, dim3(ceil_div(k.C, 64)), dim3(GT), 0, st, ab, dgamma, dbeta, N, k.C, add);
   if (dx || dres)
     GN_ACT_RES(act, res,
                hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT, RES>), grid, dim3(GT), 0, st, k, (const T*)x,
@@ -541,7 +542,8 @@ int vc_group_norm_fwd(int dtype, const void* x, const void* residual, const floa
 
 int vc_group_norm_bwd(int dtype, const void* x, const void* dy, const void* residual, const float* gamma,
                       const float* beta, const float* mean, const float* rstd, void* dx, void* dresidual, float* dgamma,
-                      float* dbeta, float* workspace, int N, int S, int C, int G, int act, hipStream_t stream) {
+                      float* dbeta, float* workspace, int N, int S, int C, int G, int act, int accumulate,
+                      hipStream_t stream) {
   const int rc = check_gn("vc_group_norm_bwd", dtype, N, S, C, G, act);
   if (rc != VC_OK) return rc;
   VC_CHECK_ARG(x && dy && mean && rstd && workspace, "vc_group_norm_bwd: null pointer");
@@ -549,10 +551,10 @@ int vc_group_norm_bwd(int dtype, const void* x, const void* dy, const void* resi
   const int V = vec_of(C, {x, dy, residual, dx, dresidual});
   const Cover k = make_cover(N, S, C, G, V);
   if (dtype == VC_BF16)
-    return V == 8 ? bwd_go<bf16, 8>(k, N, x, dy, residual, gamma, beta, mean, rstd, dx, dresidual, dgamma, dbeta, workspace, act, stream)
-                  : bwd_go<bf16, 1>(k, N, x, dy, residual, gamma, beta, mean, rstd, dx, dresidual, dgamma, dbeta, workspace, act, stream);
-  return V == 8 ? bwd_go<float, 8>(k, N, x, dy, residual, gamma, beta, mean, rstd, dx, dresidual, dgamma, dbeta, workspace, act, stream)
-                : bwd_go<float, 1>(k, N, x, dy, residual, gamma, beta, mean, rstd, dx, dresidual, dgamma, dbeta, workspace, act, stream);
+    return V == 8 ? bwd_go<bf16, 8>(k, N, x, dy, residual, gamma, beta, mean, rstd, dx, dresidual, dgamma, dbeta, workspace, act, accumulate, stream)
+                  : bwd_go<bf16, 1>(k, N, x, dy, residual, gamma, beta, mean, rstd, dx, dresidual, dgamma, dbeta, workspace, act, accumulate, stream);
+  return V == 8 ? bwd_go<float, 8>(k, N, x, dy, residual, gamma, beta, mean, rstd, dx, dresidual, dgamma, dbeta, workspace, act, accumulate, stream)
+                : bwd_go<float, 1>(k, N, x, dy, residual, gamma, beta, mean, rstd, dx, dresidual, dgamma, dbeta, workspace, act, accumulate, stream);
 }
 
 }  // extern "C"

@@ -474,16 +474,16 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_grad_kernel(CeArgs a, const f
   }
 }
 
-// db[v] += fac sum over the row tiles of dbpart[tile][v]
+// db[v] (+)= fac sum over the row tiles of dbpart[tile][v]
 template <typename T>
 __global__ __launch_bounds__(256) void ce_bias_kernel(const float* __restrict__ dbpart, int tiles, int V,
-                                                      const float* __restrict__ fac, T* __restrict__ db) {
+                                                      const float* __restrict__ fac, int add, T* __restrict__ db) {
   const int v = blockIdx.x * 256 + threadIdx.x;
   if (v >= V) return;
   float s = 0.f;
 #pragma unroll 4
   for (int t = 0; t < tiles; ++t) s += dbpart[(int64_t)t * V + v];
-  db[v] = from_f32<T>(to_f32(db[v]) + s * (fac[0] / D_SCALE));
+  db[v] = from_f32<T>((add ? to_f32(db[v]) : 0.f) + s * (fac[0] / D_SCALE));
 }
 
 // out[m][c] = factor * sum over the reduction of (row side)[m] (column side)[c]: dx = d W and dW = d^T x
@@ -766,7 +766,7 @@ int vc_linear_ce_fwd(int xdtype, int wdtype, const void* x, const void* w, const
 
 int vc_linear_ce_bwd(int xdtype, int wdtype, const void* bias, const int64_t* target, int64_t ignore_index, float smoothing,
                      int mean, int per_row, const float* dloss, const void* saved, void* dx, void* dw, void* db,
-                     void* workspace, int N, int V, int K, hipStream_t stream) {
+                     void* workspace, int accumulate, int N, int V, int K, hipStream_t stream) {
   const int rc = check_ce("vc_linear_ce_bwd", xdtype, wdtype, N, V, K, smoothing);
   if (rc != VC_OK) return rc;
   VC_CHECK_ARG(target && dloss && saved && workspace, "vc_linear_ce_bwd: null pointer");
@@ -830,21 +830,23 @@ int vc_linear_ce_bwd(int xdtype, int wdtype, const void* bias, const int64_t* ta
       g.splits = p.sw;
       g.kper = p.kw;
       g.part = p.b_pw >= 0 ? (float*)(ws + p.b_pw) : nullptr;
-      g.add = g.part ? 0 : 1;
+      g.add = g.part ? 0 : accumulate & 1;
       g.out = out;
       g.which = 0;
       g.vec = K % 4 == 0 && ((uintptr_t)dw & 15) == 0;
       mm_terms<COL>(p.px, p.pdw, g, wdtype == VC_BF16, stream);
-      if (g.part) reduce_go(g.part, p.sw, (int64_t)rows * K, fac, exps, 0, 1, out, wdtype == VC_BF16, stream);
+      if (g.part) reduce_go(g.part, p.sw, (int64_t)rows * K, fac, exps, 0, accumulate & 1, out, wdtype == VC_BF16, stream);
     }
   }
   if (dx && p.b_px >= 0)
     reduce_go((const float*)(ws + p.b_px), p.sx, (int64_t)N * K, fac, exps, 1, 0, dx, xdtype == VC_BF16, stream);
   if (db) {
     if (wdtype == VC_BF16)
-      hipLaunchKernelGGL((ce_bias_kernel<bf16>), dim3(ceil_div(V, 256)), dim3(256), 0, stream, dbp, tn, V, fac, (bf16*)db);
+      hipLaunchKernelGGL((ce_bias_kernel<bf16>), dim3(ceil_div(V, 256)), dim3(256), 0, stream, dbp, tn, V, fac,
+                         accumulate & 2, (bf16*)db);
     else
-      hipLaunchKernelGGL((ce_bias_kernel<float>), dim3(ceil_div(V, 256)), dim3(256), 0, stream, dbp, tn, V, fac, (float*)db);
+      hipLaunchKernelGGL((ce_bias_kernel<float>), dim3(ceil_div(V, 256)), dim3(256), 0, stream, dbp, tn, V, fac,
+                         accumulate & 2, (float*)db);
   }
   VC_LAUNCH_CHECK("vc_linear_ce_bwd");
   return VC_OK;

@@ -6,6 +6,7 @@ of 8.  PyTorch only owns the memory and the autograd graph; every arithmetic ste
 into libvc_hip.  Parameter gradients are accumulated by the kernels directly into ``param.grad``
 (fp32), so the autograd functions return ``None`` for parameter inputs.
 """
+import contextlib
 import functools
 import os
 
@@ -1371,43 +1372,43 @@ class _LinearCrossEntropy(torch.autograd.Function):
         weight, bias = params  # in a tuple, so that autograd does not see them
         N, K = x.shape
         V = weight.shape[0]
-        xd, wd = L.dtype_code(x.dtype), L.dtype_code(weight.dtype)
+        xd, wd, dev = L.dtype_code(x.dtype), L.dtype_code(weight.dtype), x.device
         w = weight.detach().contiguous()
         b = bias.detach().contiguous() if bias is not None else None
-        dev = x.device
-        saved = torch.empty(L.query("vc_linear_ce_bytes", 0, xd, wd, N, V, K), device=dev, dtype=torch.uint8)
-        ws = torch.empty(L.query("vc_linear_ce_bytes", 1, xd, wd, N, V, K), device=dev, dtype=torch.uint8)
+        saved = torch.empty(_size("vc_linear_ce_bytes", 0, xd, wd, N, V, K), device=dev, dtype=torch.uint8)
+        ws = torch.empty(_size("vc_linear_ce_bytes", 1, xd, wd, N, V, K), device=dev, dtype=torch.uint8)
         rows = torch.empty(N, device=dev, dtype=torch.float32)
         loss = torch.empty((), device=dev, dtype=torch.float32) if reduction != "none" else None
         pred = torch.empty(N, device=dev, dtype=torch.int64) if want_pred else None
         correct = torch.empty(1, device=dev, dtype=torch.int32) if want_pred else None
-        L.call("vc_linear_ce_fwd", xd, wd, L.ptr(x), L.ptr(w), L.ptr(b), L.ptr(target), L.i64(ignore_index),
-               float(smoothing), int(reduction == "mean"), L.ptr(rows), L.ptr(loss), L.ptr(pred), L.ptr(correct),
-               L.ptr(saved), L.ptr(ws), N, V, K, L.stream())
+        L.fast("vc_linear_ce_fwd", dev, xd, wd, x.data_ptr(), w.data_ptr(), _addr(b), target.data_ptr(), ignore_index,
+               smoothing, reduction == "mean", rows.data_ptr(), _addr(loss), _addr(pred), _addr(correct), saved.data_ptr(),
+               ws.data_ptr(), N, V, K)
         ctx.dims, ctx.codes, ctx.opts = (N, V, K), (xd, wd), (ignore_index, smoothing, reduction)
-        ctx.weight, ctx.bias, ctx.xdtype = weight, bias, x.dtype
+        ctx.params, ctx.xdtype = params, x.dtype
         ctx.save_for_backward(saved, target, b)
-        out = rows if loss is None else loss
         if want_pred:
             ctx.mark_non_differentiable(pred, correct)
-        return out, pred, correct
+        return rows if loss is None else loss, pred, correct
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g, _dpred, _dcorrect):
         saved, target, b = ctx.saved_tensors
         (N, V, K), (xd, wd), (ignore_index, smoothing, reduction) = ctx.dims, ctx.codes, ctx.opts
+        weight, bias = ctx.params
+        dev = saved.device
         g = g.contiguous().float()
-        dx = torch.empty(N, K, device=saved.device, dtype=ctx.xdtype) if ctx.needs_input_grad[0] else None
-        dw, db = _grad_target(ctx.weight), _grad_target(ctx.bias)
-        ws = torch.empty(L.query("vc_linear_ce_bytes", 2, xd, wd, N, V, K), device=saved.device, dtype=torch.uint8)
-        L.call("vc_linear_ce_bwd", xd, wd, L.ptr(b), L.ptr(target), L.i64(ignore_index), float(smoothing),
-               int(reduction == "mean"), int(reduction == "none"), L.ptr(g), L.ptr(saved), L.ptr(dx), L.ptr(dw), L.ptr(db),
-               L.ptr(ws), N, V, K, L.stream())
-        for p, t in ((ctx.weight, dw), (ctx.bias, db)):
-            if t is not None:
-                _add_grad(p, t)
-        _ready(ctx.weight, ctx.bias)
+        dx = torch.empty(N, K, device=dev, dtype=ctx.xdtype) if ctx.needs_input_grad[0] else None
+        dw, add_w = _grad_target(weight)
+        db, add_b = _grad_target(bias)
+        ws = torch.empty(_size("vc_linear_ce_bytes", 2, xd, wd, N, V, K), device=dev, dtype=torch.uint8)
+        L.fast("vc_linear_ce_bwd", dev, xd, wd, _addr(b), target.data_ptr(), ignore_index, smoothing, reduction == "mean",
+               reduction == "none", g.data_ptr(), saved.data_ptr(), _addr(dx), _addr(dw), _addr(db), ws.data_ptr(),
+               add_w + 2 * add_b, N, V, K)
+        _put_grad(weight, dw)
+        _put_grad(bias, db)
+        _ready(weight, bias)
         return (dx,) + (None,) * 7
 
 
@@ -1443,9 +1444,9 @@ def linear_cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoot
             stats["pred"] = target.reshape(-1)
             stats["correct"] = torch.zeros(1, device=x.device, dtype=torch.int32)
         return loss
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         _leaf_guard("linear_cross_entropy", x)
-        x2 = x.reshape(-1, x.shape[-1]).contiguous()
+        x2 = (x if x.dim() == 2 else x.reshape(-1, x.shape[-1])).contiguous()
         out, pred, correct = _LinearCrossEntropy.apply(x2, _anchor((x,), (weight, bias)), (weight, bias),
                                                        target.reshape(-1).contiguous(), int(ignore_index),
                                                        float(label_smoothing), reduction, stats is not None)
@@ -1710,12 +1711,30 @@ def _leaf_guard(what, *inputs):
     for t in inputs:
         if t is None or not (t.requires_grad and t.is_leaf):
             continue
-        meta = torch.autograd.graph.get_gradient_edge(t).node.metadata  # lives exactly as long as the node does
+        meta = t.view_as(t).grad_fn.next_functions[0][0].metadata  # lives exactly as long as the gradient node does
         if not _capturing(t):
             meta["vc_eager"] = True
         elif meta.get("vc_eager"):
             raise RuntimeError(f"{what}: a graph capture meets an input whose eager graph is still alive; drop the eager "
                                "result (or its loss) first, or capture on a detached copy of the input")
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(device):
+    """Context in which `device` is the current one."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+@functools.lru_cache(maxsize=1024)
+def _size(name, *ints):
+    """A size query of the library, which depends on its arguments alone."""
+    return L.query(name, *ints)
 
 
 def _same_device(what, first, *rest):
@@ -1739,19 +1758,23 @@ def _f32_param(what, p):
     return p.detach().contiguous()
 
 
-def _add_grad(p, g):
-    """Accumulates g into p.grad unless the kernels wrote p.grad itself."""
-    if g is not p.grad:
-        p.grad.add_(g.view(p.shape))
-
-
 def _grad_target(p):
-    """A dense tensor of p's type the kernels may accumulate p's gradient into: p.grad where it is dense, else a zeroed stand-in
-    that _add_grad folds in.  None where p needs no gradient."""
+    """(tensor, add): where the kernels may put p's gradient -- p.grad itself, to add to, or a new tensor to write.  (None, 0)
+    where p needs no gradient.  _put_grad takes the tensor once it is written."""
     if p is None or not p.requires_grad:
-        return None
-    g = _grad_buf(p)
-    return g if g.is_contiguous() else torch.zeros(p.shape, device=p.device, dtype=p.dtype)
+        return None, 0
+    if p.grad is not None and p.grad.is_contiguous():
+        return p.grad, 1
+    return torch.empty(p.shape, device=p.device, dtype=p.dtype), 0
+
+
+def _put_grad(p, g):
+    if g is None or g is p.grad:
+        return
+    if p.grad is None:
+        p.grad = g
+    else:
+        p.grad.add_(g)
 
 
 class _GroupNorm(torch.autograd.Function):
@@ -1761,13 +1784,16 @@ class _GroupNorm(torch.autograd.Function):
         S = x.numel() // (N * C)
         x = x.contiguous()
         res = residual.contiguous() if residual is not None else None
-        gamma, beta = _f32_param("group_norm", gn.weight), _f32_param("group_norm", gn.bias)
+        weight, bias, dev = gn.weight, gn.bias, x.device
+        gamma, beta = _f32_param("group_norm", weight), _f32_param("group_norm", bias)
+        code, ws_floats = L.dtype_code(x.dtype), _size("vc_group_norm_workspace_floats", N, S, C, G)
         y = torch.empty_like(x)
-        stat = torch.empty(2, N, G, device=x.device, dtype=torch.float32)
-        ws = torch.empty(L.query("vc_group_norm_workspace_floats", N, S, C, G), device=x.device, dtype=torch.float32)
-        L.call("vc_group_norm_fwd", L.dtype_code(x.dtype), L.ptr(x), L.ptr(res), L.ptr(gamma), L.ptr(beta), L.ptr(y),
-               L.ptr(stat[0]), L.ptr(stat[1]), L.ptr(ws), N, S, C, G, float(gn.eps), act, L.stream())
-        ctx.dims, ctx.act, ctx.weight, ctx.bias = (N, S, C, G), act, gn.weight, gn.bias
+        stat = torch.empty(2, N * G, device=dev, dtype=torch.float32)
+        ws = torch.empty(ws_floats, device=dev, dtype=torch.float32)
+        mean = stat.data_ptr()
+        L.fast("vc_group_norm_fwd", dev, code, x.data_ptr(), _addr(res), _addr(gamma), _addr(beta), y.data_ptr(), mean,
+               mean + 4 * N * G, ws.data_ptr(), N, S, C, G, gn.eps, act)
+        ctx.dims, ctx.act, ctx.params, ctx.code, ctx.ws_floats = (N, S, C, G), act, (weight, bias), code, ws_floats
         ctx.save_for_backward(x, res if act else None, stat, gamma, beta)
         return y
 
@@ -1776,21 +1802,24 @@ class _GroupNorm(torch.autograd.Function):
     def backward(ctx, dy):
         x, res, stat, gamma, beta = ctx.saved_tensors
         N, S, C, G = ctx.dims
+        act, dev = ctx.act, x.device
+        weight, bias = ctx.params
         dy = cast(dy.contiguous(), x.dtype)
-        need_dx, need_dres = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        need_dx, need_dres = ctx.needs_input_grad[:2]
         dx = torch.empty_like(x) if need_dx else None
         # without an activation the shortcut's gradient is the incoming one
-        dres = (torch.empty_like(x) if ctx.act else dy) if need_dres else None
-        dw, db = _grad_target(ctx.weight), _grad_target(ctx.bias)
-        if need_dx or dw is not None or db is not None or (need_dres and ctx.act):
-            ws = torch.empty(L.query("vc_group_norm_workspace_floats", N, S, C, G), device=x.device, dtype=torch.float32)
-            L.call("vc_group_norm_bwd", L.dtype_code(x.dtype), L.ptr(x), L.ptr(dy), L.ptr(res), L.ptr(gamma), L.ptr(beta),
-                   L.ptr(stat[0]), L.ptr(stat[1]), L.ptr(dx), L.ptr(dres if ctx.act else None), L.ptr(dw), L.ptr(db),
-                   L.ptr(ws), N, S, C, G, ctx.act, L.stream())
-            for p, g in ((ctx.weight, dw), (ctx.bias, db)):
-                if g is not None:
-                    _add_grad(p, g)
-        _ready(ctx.weight, ctx.bias)
+        dres = (torch.empty_like(x) if act else dy) if need_dres else None
+        dw, add_w = _grad_target(weight)
+        db, add_b = _grad_target(bias)
+        if need_dx or dw is not None or db is not None or (need_dres and act):
+            ws = torch.empty(ctx.ws_floats, device=dev, dtype=torch.float32)
+            mean = stat.data_ptr()
+            L.fast("vc_group_norm_bwd", dev, ctx.code, x.data_ptr(), dy.data_ptr(), _addr(res), _addr(gamma), _addr(beta),
+                   mean, mean + 4 * N * G, _addr(dx), _addr(dres) if act else None, _addr(dw), _addr(db), ws.data_ptr(),
+                   N, S, C, G, act, add_w + 2 * add_b)
+            _put_grad(weight, dw)
+            _put_grad(bias, db)
+        _ready(weight, bias)
         return dx, dres, None, None, None
 
 
@@ -1812,7 +1841,7 @@ def group_norm(x, gn, act="none", residual=None):
     _same_device("group_norm", x, residual, gn.weight, gn.bias)
     if x.numel() == 0:
         return x.clone()
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         _leaf_guard("group_norm", x, residual)
         return _GroupNorm.apply(x, residual, _anchor((x, residual), (gn.weight, gn.bias)), gn, GN_ACTS[act])
 
@@ -1993,7 +2022,7 @@ def newton_schulz(g, steps=5, coeffs=NS_COEFFS, eps=1e-7, inplace=False):
             raise RuntimeError("newton_schulz: in place needs dense tensors outside the autograd graph")
     code = L.dtype_code(first.dtype)
     _same_device("newton_schulz", first, *items)
-    with torch.cuda.device(first.device), torch.no_grad():
+    with _on(first.device), torch.no_grad():
         srcs = [t.detach().contiguous() for t in items]
         outs = items if inplace else [torch.empty_like(t) for t in srcs]
         gp, op, rows, cols = [], [], [], []
