@@ -10,8 +10,9 @@
 // with the transposing ds_read_b64_tr_b16, so no operand is ever copied into the other order).  The second term lies one
 // `plane` behind the first.
 //
-// Four waves in a 2 x 2 grid own 64 x 64 each.  Two LDS stages of (PA + PB) x 128 x BK elements (BK = 64 for single terms,
-// 32 otherwise, so at most 32 KiB a stage and two workgroups per CU).  ROW stages permute the 16-byte chunks of a row so
+// Four waves in a 2 x 2 grid own 64 x 64 each.  NS LDS stages of (PA + PB) x 128 x BK elements (BK = 64 for single terms,
+// 32 otherwise: at most 32 KiB a stage).  Two stages let two workgroups share a CU and hide each other's waits; a launch
+// with at most one workgroup per CU takes four, which keeps three k-steps on their way instead of one.  ROW stages permute the 16-byte chunks of a row so
 // that the 16 rows of a fragment read fall into 16 different slots of the 256-byte bank row; COL stages permute the
 // 32-byte blocks of a row so that the eight rows of a transposing read fall on different groups of banks.  Stages are
 // filled by LDS-DMA requests in opaque assembly (with the builtin the compiler waits for every outstanding request
@@ -65,15 +66,16 @@ __device__ __forceinline__ void f16_split(float v, f16& hi, f16& lo) {
   lo = (f16)(v - (float)hi);
 }
 
-template <int PA, int PB, int KA = ROW, int KB = ROW>
+template <int PA, int PB, int KA = ROW, int KB = ROW, int NS = 2, int BK_ = 0>
 struct G16 {
-  static constexpr int BK = PA + PB == 2 ? 64 : 32;
+  static constexpr int BK = BK_ ? BK_ : PA + PB == 2 ? 64 : 32;
   static constexpr int PLANE = GM * BK;              // elements of one plane of a stage
   static constexpr int STAGE = (PA + PB) * PLANE;
-  static constexpr int LDS = 2 * STAGE;              // elements of shared memory
+  static constexpr int LDS = NS * STAGE;             // elements of shared memory
   static constexpr int CH = BK / 8;                  // 16-byte chunks of a ROW stage's row
   static constexpr int RPI = 64 / CH;                // rows of it that one wave request fills
   static constexpr int REQ = BK / 16;                // requests per wave, plane and stage (1 KiB each)
+  static constexpr int PER = (PA + PB) * REQ;        // requests per wave and stage
 
   __device__ static __forceinline__ int rswz(int row) { return BK == 64 ? (row >> 1) & 7 : (row >> 2) & 3; }
   __device__ static __forceinline__ int cswz(int row) { return (row & 3) | ((row >> 1) & 4); }
@@ -175,13 +177,18 @@ struct G16 {
 #pragma unroll
       for (int p = 0; p < PB; ++p) sb[p].stage(base + (PA + p) * PLANE * 2, vb, k);
     };
-    int s = 0;
-    if (k0 < k1) stage(0, k0);
-    for (int k = k0; k < k1; k += BK, s ^= 1) {
-      // this wave's requests have landed and its reads are done; behind the barrier so are the others', and nobody reads
-      // the other stage any more
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (k + BK < k1) stage(s ^ 1, k + BK);
+    int s = 0;  // the stage that is multiplied; the next NS - 1 k-steps are on their way into the others
+#pragma unroll
+    for (int d = 0; d < NS - 1; ++d)
+      if (k0 + d * BK < k1) stage(d, k0 + d * BK);
+    for (int k = k0; k < k1; k += BK, s = s + 1 == NS ? 0 : s + 1) {
+      // this wave's requests of stage s have landed (the younger ones of NS - 2 stages may be outstanding) and its reads
+      // are done; behind the barrier so are the others', and nobody reads the stage before any more
+      if (NS > 2 && k + (NS - 2) * BK < k1)
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * PER) : "memory");
+      else
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (k + (NS - 1) * BK < k1) stage(s == 0 ? NS - 1 : s - 1, k + (NS - 1) * BK);
       const f16* st = smem + s * STAGE;
 #pragma unroll
       for (int kk = 0; kk < BK / 32; ++kk) {

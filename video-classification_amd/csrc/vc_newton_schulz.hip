@@ -313,11 +313,11 @@ __device__ __forceinline__ void sym_store(f32x4 (&acc)[4][4], const NsMat& t, co
 }
 
 // A tile, or a slice of the reduction of one, of a symmetric product; tiles on and below the diagonal only.
-template <bool SQUARE>
-__global__ __launch_bounds__(G_THREADS, 2) void ns_sym_kernel(NsArgs a, f16* __restrict__ ws,
+template <bool SQUARE, int NS>
+__global__ __launch_bounds__(G_THREADS, NS == 2 ? 2 : 1) void ns_sym_kernel(NsArgs a, f16* __restrict__ ws,
                                                               const NsScale* __restrict__ sc, NsStep st, int parity,
                                                               float* __restrict__ part) {
-  typedef G16<2, 2> G;
+  typedef G16<2, 2, ROW, ROW, NS> G;
   __shared__ __attribute__((aligned(1024))) f16 smem[G::LDS];
   const int i = find_mat(a, blockIdx.x);
   const NsMat& t = a.mat[i];
@@ -377,10 +377,10 @@ __global__ __launch_bounds__(G_THREADS, 2) void ns_sym_join_kernel(NsArgs a, f16
 
 // X <- a X + P X, into the other buffer, or the result in G's orientation after the last step.  The columns of X run along
 // the registers, so X is read and written in groups of four.
-template <typename T>
-__global__ __launch_bounds__(G_THREADS, 2) void ns_update_kernel(NsArgs a, f16* __restrict__ ws,
+template <typename T, int NS>
+__global__ __launch_bounds__(G_THREADS, NS == 2 ? 2 : 1) void ns_update_kernel(NsArgs a, f16* __restrict__ ws,
                                                                  const NsScale* __restrict__ sc, NsStep st, int parity) {
-  typedef G16<2, 2, COL, ROW> G;
+  typedef G16<2, 2, COL, ROW, NS> G;
   __shared__ __attribute__((aligned(1024))) f16 smem[G::LDS];
   const int i = find_mat(a, blockIdx.x);
   const NsMat& t = a.mat[i];
@@ -472,15 +472,14 @@ __global__ __launch_bounds__(256) void ns_copy_kernel(NsArgs a, const NsScale* _
 
 int64_t norm_blocks(int64_t m, int64_t n) { return ceil_div64(m * n, NORM_CHUNK); }
 
-// How the symmetric products of a launch are cut.  `slots` workgroups (two per CU) run at once.
+// How the symmetric products of a launch are cut.  `slots` workgroups (two per CU, or one) run at once.
 //  - Fewer tiles than slots: every reduction is cut into runs of about equal length so that the runs fill the slots.
 //  - One matrix with a little more than whole rounds of tiles: the tiles of the last round are cut instead of leaving
 //    most of the chip idle for it (4096 x 4096: 528 tiles on 512 slots).
 // Returns the partial tiles; fills direct / slices / p0 / f0 of every matrix.  len(t) = its reduction in k-steps of 32.
 template <typename F>
 int64_t cut_sym(NsArgs& a, F len, int& joins) {
-  const int slots = 512;
-  int64_t tiles = 0, work = 0, parts = 0;
+  int64_t slots = 512, tiles = 0, work = 0, parts = 0;
   joins = 0;
   auto count = [](const NsMat& t) {
     const int n = ceil_div(t.m, GM);
@@ -490,6 +489,7 @@ int64_t cut_sym(NsArgs& a, F len, int& joins) {
     tiles += count(a.mat[i]);
     work += (int64_t)count(a.mat[i]) * len(a.mat[i]);
   }
+  if (work < 512 * 16) slots = 256;  // short runs: one workgroup per CU with the deep pipeline
   for (int i = 0; i < a.count; ++i) {
     NsMat& t = a.mat[i];
     const int n = count(t);
@@ -503,8 +503,8 @@ int64_t cut_sym(NsArgs& a, F len, int& joins) {
         t.direct = 0;
       }
     } else if (a.count == 1 && tiles % slots && tiles % slots <= slots / 2) {
-      const int tail = (int)(tiles % slots);
-      const int s = slots / tail < len(t) / 4 ? slots / tail : len(t) / 4;
+      const int tail = (int)(tiles % slots), room = (int)(slots / tail);
+      const int s = room < len(t) / 4 ? room : len(t) / 4;
       if (s > 1) {
         t.slices = s < 8 ? s : 8;
         t.direct = n - tail;
@@ -606,14 +606,18 @@ int vc_newton_schulz(int dtype, int count, const void* const* g, void* const* ou
       a.mat[i].g = g[b + i];
       a.mat[i].out = out[b + i];
     }
-    auto launch = [&](auto blocks_of, auto kernel, int threads, auto... args) {  // blocks in the order of the matrices
+    auto number = [&](auto blocks_of) {  // workgroups in the order of the matrices
       int64_t at = 0;
       for (int i = 0; i < a.count; ++i) {
         a.mat[i].t0 = (int)at;
         at += blocks_of(a.mat[i]);
       }
-      hipLaunchKernelGGL(kernel, dim3((unsigned)at), dim3(threads), 0, stream, a, args...);
+      return at;
     };
+    auto launch = [&](auto blocks_of, auto kernel, int threads, auto... args) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)number(blocks_of)), dim3(threads), 0, stream, a, args...);
+    };
+    auto deep = [&](auto blocks_of) { return number(blocks_of) <= vc_device_cus(); };  // the four-stage pipeline (G16)
     auto by_norm = [](const NsMat& t) { return norm_blocks(t.m, t.n); };
     auto by_init = [](const NsMat& t) { return (int64_t)(up64(t.m) / 64) * (up64(t.n) / 64); };
     auto by_upd = [](const NsMat& t) { return (int64_t)ceil_div(t.m, GM) * ceil_div(t.n, GM); };
@@ -632,14 +636,16 @@ int vc_newton_schulz(int dtype, int count, const void* const* g, void* const* ou
       st.last = k == steps - 1;
       int joins = 0;
       cut_sym(a, [](const NsMat& t) { return up64(t.n) / 32; }, joins);
-      launch(by_sym, ns_sym_kernel<false>, G_THREADS, ws, sc, st, k & 1, part);
+      launch(by_sym, deep(by_sym) ? ns_sym_kernel<false, 4> : ns_sym_kernel<false, 2>, G_THREADS, ws, sc, st, k & 1, part);
       if (joins)
         hipLaunchKernelGGL(ns_sym_join_kernel<false>, dim3(joins), dim3(G_THREADS), 0, stream, a, ws, sc, st, k & 1, part);
       cut_sym(a, [](const NsMat& t) { return up64(t.m) / 32; }, joins);
-      launch(by_sym, ns_sym_kernel<true>, G_THREADS, ws, sc, st, k & 1, part);
+      launch(by_sym, deep(by_sym) ? ns_sym_kernel<true, 4> : ns_sym_kernel<true, 2>, G_THREADS, ws, sc, st, k & 1, part);
       if (joins)
         hipLaunchKernelGGL(ns_sym_join_kernel<true>, dim3(joins), dim3(G_THREADS), 0, stream, a, ws, sc, st, k & 1, part);
-      launch(by_upd, bf ? ns_update_kernel<bf16> : ns_update_kernel<float>, G_THREADS, ws, sc, st, k & 1);
+      if (deep(by_upd))
+        launch(by_upd, bf ? ns_update_kernel<bf16, 4> : ns_update_kernel<float, 4>, G_THREADS, ws, sc, st, k & 1);
+      else launch(by_upd, bf ? ns_update_kernel<bf16, 2> : ns_update_kernel<float, 2>, G_THREADS, ws, sc, st, k & 1);
     }
     VC_LAUNCH_CHECK("vc_newton_schulz");
   }
