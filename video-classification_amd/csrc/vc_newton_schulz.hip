@@ -23,22 +23,38 @@ namespace {
 constexpr int NS_MAX = 64;        // matrices per launch
 constexpr int NORM_CHUNK = 1 << 14;
 
-// One matrix of a launch, in its wide orientation (m <= n).
+// What a launch numbers its workgroups by, matrix after matrix.
+enum { BY_NORM, BY_INIT, BY_UPDATE, BY_S, BY_P, BY_JOIN_S, BY_JOIN_P, KINDS };
+
+// One matrix of a call, in its wide orientation (m <= n).  The table of them lies in the workspace: read from the kernel
+// arguments, which live in host memory, its lookups cost every workgroup microseconds.
 struct NsMat {
   const void* g;
   void* out;
-  int64_t at;  // its buffers in the workspace, in fp16 elements
+  int64_t at;        // its buffers in the workspace, in fp16 elements
   int m, n;
-  int tall;    // G is [n][m]
-  int t0;      // first workgroup of this matrix in the launch
-  // symmetric products: tiles [0, direct) are worked by one workgroup each, the others in `slices` runs of the reduction
-  // whose partial tiles start at p0 and are joined by the workgroups from f0 on of a second launch
-  int direct, slices, p0, f0;
+  int tall;          // G is [n][m]
+  int first[KINDS];  // first workgroup of this matrix
+  // symmetric products S and P: tiles [0, direct) are worked by one workgroup each, the others in `slices` runs of the
+  // reduction whose partial tiles start at p0 and are joined by a second launch
+  struct Cut {
+    int direct, slices, p0;
+  } cut[2];
 };
-struct NsArgs {
-  NsMat mat[NS_MAX];
-  int count;
+constexpr int NS_CHUNK = 32;  // table entries that fit a launch's arguments
+struct NsChunk {
+  NsMat mat[NS_CHUNK];
 };
+__global__ __launch_bounds__(64) void ns_table_kernel(NsChunk c, NsMat* __restrict__ table, int count) {
+  if ((int)threadIdx.x < count) table[threadIdx.x] = c.mat[threadIdx.x];
+}
+
+// the matrix a workgroup belongs to: every lane looks at one entry
+__device__ __forceinline__ int find_mat(const NsMat* __restrict__ table, int count, int kind, int block) {
+  const int lane = threadIdx.x & 63;
+  const int f = lane < count ? table[lane].first[kind] : 0x7fffffff;
+  return __builtin_amdgcn_readfirstlane(63 - __builtin_clzll(__ballot(f <= block)));
+}
 
 // m <- mu m + f g;  u = f g + mu m (nesterov) or m
 __global__ __launch_bounds__(256) void muon_momentum_kernel(const float* __restrict__ g, float* __restrict__ m,
@@ -99,16 +115,6 @@ struct NsScale {
   int ey, pad;
 };
 
-__device__ __forceinline__ int find_mat(const NsArgs& a, int block) {
-  int lo = 0, hi = a.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.mat[mid].t0 <= block) lo = mid;
-    else hi = mid - 1;
-  }
-  return __builtin_amdgcn_readfirstlane(lo);
-}
-
 __device__ __forceinline__ double wave_sum_f64(double v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
@@ -117,11 +123,12 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
 
 // sum of squares of NORM_CHUNK elements, in double: no overflow, no underflow
 template <typename T>
-__global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs a, double* __restrict__ part) {
+__global__ __launch_bounds__(256) void ns_norm_kernel(const NsMat* __restrict__ table, int count,
+                                                    double* __restrict__ part) {
   __shared__ double sm[4];
-  const int i = find_mat(a, blockIdx.x);
-  const NsMat& t = a.mat[i];
-  const int64_t total = (int64_t)t.m * t.n, e0 = (int64_t)(blockIdx.x - t.t0) * NORM_CHUNK;
+  const int i = find_mat(table, count, BY_NORM, blockIdx.x);
+  const NsMat t = table[i];
+  const int64_t total = (int64_t)t.m * t.n, e0 = (int64_t)(blockIdx.x - t.first[BY_NORM]) * NORM_CHUNK;
   const int64_t e1 = e0 + NORM_CHUNK < total ? e0 + NORM_CHUNK : total;
   const T* g = (const T*)t.g;
   double s = 0.0;
@@ -143,10 +150,11 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs a, double* __restri
 }
 
 // one wave per matrix
-__global__ __launch_bounds__(64) void ns_scale_kernel(NsArgs a, int blocks, const double* __restrict__ part, double eps,
-                                                      float cap, float gain, NsScale* __restrict__ sc) {
+__global__ __launch_bounds__(64) void ns_scale_kernel(const NsMat* __restrict__ table, int count, int blocks,
+                                                     const double* __restrict__ part, double eps, float cap, float gain,
+                                                     NsScale* __restrict__ sc) {
   const int i = blockIdx.x;
-  const int b0 = a.mat[i].t0, b1 = i + 1 < a.count ? a.mat[i + 1].t0 : blocks;
+  const int b0 = table[i].first[BY_NORM], b1 = i + 1 < count ? table[i + 1].first[BY_NORM] : blocks;
   double s = 0.0;
   for (int b = b0 + threadIdx.x; b < b1; b += 64) s += part[b];
   s = wave_sum_f64(s);
@@ -165,12 +173,13 @@ __global__ __launch_bounds__(64) void ns_scale_kernel(NsArgs a, int blocks, cons
 
 // Y_0: 64 x 64 tiles of the wide orientation, through LDS where G is tall; zeros in the padding
 template <typename T>
-__global__ __launch_bounds__(256) void ns_init_kernel(NsArgs a, f16* __restrict__ ws, const NsScale* __restrict__ sc) {
+__global__ __launch_bounds__(256) void ns_init_kernel(const NsMat* __restrict__ table, int count, f16* __restrict__ ws,
+                                                    const NsScale* __restrict__ sc) {
   __shared__ float sm[64][65];
-  const int i = find_mat(a, blockIdx.x);
-  const NsMat& t = a.mat[i];
+  const int i = find_mat(table, count, BY_INIT, blockIdx.x);
+  const NsMat t = table[i];
   const NsView w(t, 0);
-  const int id = blockIdx.x - t.t0, tn = w.ldn / 64;
+  const int id = blockIdx.x - t.first[BY_INIT], tn = w.ldn / 64;
   const int r0 = id / tn * 64, c0 = id % tn * 64;  // rows < m, columns < n of X
   const double inv = sc[i].inv;
   const T* g = (const T*)t.g;
@@ -314,23 +323,24 @@ __device__ __forceinline__ void sym_store(f32x4 (&acc)[4][4], const NsMat& t, co
 
 // A tile, or a slice of the reduction of one, of a symmetric product; tiles on and below the diagonal only.
 template <bool SQUARE, int NS>
-__global__ __launch_bounds__(G_THREADS, NS == 2 ? 2 : 1) void ns_sym_kernel(NsArgs a, f16* __restrict__ ws,
+__global__ __launch_bounds__(G_THREADS, NS == 2 ? 2 : 1) void ns_sym_kernel(const NsMat* __restrict__ table, int count, f16* __restrict__ ws,
                                                               const NsScale* __restrict__ sc, NsStep st, int parity,
                                                               float* __restrict__ part) {
   typedef G16<2, 2, ROW, ROW, NS> G;
   __shared__ __attribute__((aligned(1024))) f16 smem[G::LDS];
-  const int i = find_mat(a, blockIdx.x);
-  const NsMat& t = a.mat[i];
+  const int i = find_mat(table, count, SQUARE ? BY_P : BY_S, blockIdx.x);
+  const NsMat t = table[i];
+  const NsMat::Cut cut = t.cut[SQUARE];
   const NsView w(t, parity);
-  const int tiles = (t.m + GM - 1) / GM, count = tiles * (tiles + 1) / 2;
-  int id = blockIdx.x - t.t0;  // whole tiles first, then slices; each kind spread over the XCDs by itself
-  id = id < t.direct ? xcd_run(id, t.direct) : t.direct + xcd_run(id - t.direct, (count - t.direct) * t.slices);
+  const int tiles = (t.m + GM - 1) / GM, all = tiles * (tiles + 1) / 2;
+  int id = blockIdx.x - t.first[SQUARE ? BY_P : BY_S];  // whole tiles first, then slices; each kind spread over the XCDs by itself
+  id = id < cut.direct ? xcd_run(id, cut.direct) : cut.direct + xcd_run(id - cut.direct, (all - cut.direct) * cut.slices);
   const int ld = SQUARE ? w.ldm : w.ldn;
   int tile = id, k0 = 0, k1 = ld, slot = -1;
-  if (id >= t.direct) {
-    slot = id - t.direct;
-    tile = t.direct + slot / t.slices;
-    const int per = (ld / G::BK + t.slices - 1) / t.slices * G::BK, s = slot % t.slices;
+  if (id >= cut.direct) {
+    slot = id - cut.direct;
+    tile = cut.direct + slot / cut.slices;
+    const int per = (ld / G::BK + cut.slices - 1) / cut.slices * G::BK, s = slot % cut.slices;
     k0 = s * per;
     k1 = min(ld, k0 + per);
   }
@@ -344,7 +354,7 @@ __global__ __launch_bounds__(G_THREADS, NS == 2 ? 2 : 1) void ns_sym_kernel(NsAr
   G::run(acc, Op16{src + (int64_t)m0 * ld, plane, ld, t.m - m0, 0}, Op16{src + (int64_t)n0 * ld, plane, ld, t.m - n0, 0}, k0,
          k1, smem);
   if (slot >= 0) {
-    f32x4* o = reinterpret_cast<f32x4*>(part + ((int64_t)t.p0 + slot) * GM * GM) + threadIdx.x;
+    f32x4* o = reinterpret_cast<f32x4*>(part + ((int64_t)cut.p0 + slot) * GM * GM) + threadIdx.x;
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[e * G_THREADS] = acc[e >> 2][e & 3];
     return;
@@ -354,22 +364,21 @@ __global__ __launch_bounds__(G_THREADS, NS == 2 ? 2 : 1) void ns_sym_kernel(NsAr
 
 // joins the slices of a tile in order
 template <bool SQUARE>
-__global__ __launch_bounds__(G_THREADS, 2) void ns_sym_join_kernel(NsArgs a, f16* __restrict__ ws,
+__global__ __launch_bounds__(G_THREADS, 2) void ns_sym_join_kernel(const NsMat* __restrict__ table, int count, f16* __restrict__ ws,
                                                                    const NsScale* __restrict__ sc, NsStep st, int parity,
                                                                    const float* __restrict__ part) {
   __shared__ __attribute__((aligned(1024))) f16 smem[GM * (GM + 8)];
-  int i = 0;
-  while (i + 1 < a.count && a.mat[i + 1].f0 <= (int)blockIdx.x) ++i;
-  i = __builtin_amdgcn_readfirstlane(i);
-  const NsMat& t = a.mat[i];
+  const int i = find_mat(table, count, SQUARE ? BY_JOIN_P : BY_JOIN_S, blockIdx.x);
+  const NsMat t = table[i];
+  const NsMat::Cut cut = t.cut[SQUARE];
   const NsView w(t, parity);
-  const int e0 = blockIdx.x - t.f0;
+  const int e0 = blockIdx.x - t.first[SQUARE ? BY_JOIN_P : BY_JOIN_S];
   int tm, tn;
-  tri_tile(t.direct + e0, (t.m + GM - 1) / GM, tm, tn);
+  tri_tile(cut.direct + e0, (t.m + GM - 1) / GM, tm, tn);
   f32x4 acc[4][4];
   G16<2, 2>::zero(acc);
-  const f32x4* p = reinterpret_cast<const f32x4*>(part + ((int64_t)t.p0 + (int64_t)e0 * t.slices) * GM * GM) + threadIdx.x;
-  for (int s = 0; s < t.slices; ++s, p += GM * GM / 4)
+  const f32x4* p = reinterpret_cast<const f32x4*>(part + ((int64_t)cut.p0 + (int64_t)e0 * cut.slices) * GM * GM) + threadIdx.x;
+  for (int s = 0; s < cut.slices; ++s, p += GM * GM / 4)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[e >> 2][e & 3] += p[e * G_THREADS];
   sym_store<SQUARE>(acc, t, w, ws, sc[i], st, tm * GM, tn * GM, smem);
@@ -378,16 +387,16 @@ __global__ __launch_bounds__(G_THREADS, 2) void ns_sym_join_kernel(NsArgs a, f16
 // X <- a X + P X, into the other buffer, or the result in G's orientation after the last step.  The columns of X run along
 // the registers, so X is read and written in groups of four.
 template <typename T, int NS>
-__global__ __launch_bounds__(G_THREADS, NS == 2 ? 2 : 1) void ns_update_kernel(NsArgs a, f16* __restrict__ ws,
+__global__ __launch_bounds__(G_THREADS, NS == 2 ? 2 : 1) void ns_update_kernel(const NsMat* __restrict__ table, int count, f16* __restrict__ ws,
                                                                  const NsScale* __restrict__ sc, NsStep st, int parity) {
   typedef G16<2, 2, COL, ROW, NS> G;
   __shared__ __attribute__((aligned(1024))) f16 smem[G::LDS];
-  const int i = find_mat(a, blockIdx.x);
-  const NsMat& t = a.mat[i];
+  const int i = find_mat(table, count, BY_UPDATE, blockIdx.x);
+  const NsMat t = table[i];
   const NsView w(t, parity);
   const int tiles_m = (t.m + GM - 1) / GM, tiles_n = (t.n + GM - 1) / GM;
   int tm, tn;
-  g16_tile(blockIdx.x - t.t0, tiles_m * tiles_n, tiles_m, tiles_n, tm, tn);
+  g16_tile(blockIdx.x - t.first[BY_UPDATE], tiles_m * tiles_n, tiles_m, tiles_n, tm, tn);
   const int m0 = tm * GM, n0 = tn * GM;
   const int64_t pp = (int64_t)t.m * w.ldm, px = (int64_t)t.m * w.ldn;
   const f16* x = ws + w.x;
@@ -460,60 +469,58 @@ __global__ __launch_bounds__(G_THREADS, NS == 2 ? 2 : 1) void ns_update_kernel(N
 
 // steps = 0: the normalised matrix itself
 template <typename T>
-__global__ __launch_bounds__(256) void ns_copy_kernel(NsArgs a, const NsScale* __restrict__ sc) {
-  const int i = find_mat(a, blockIdx.x);
-  const NsMat& t = a.mat[i];
-  const int64_t total = (int64_t)t.m * t.n, e0 = (int64_t)(blockIdx.x - t.t0) * NORM_CHUNK;
+__global__ __launch_bounds__(256) void ns_copy_kernel(const NsMat* __restrict__ table, int count,
+                                                    const NsScale* __restrict__ sc) {
+  const int i = find_mat(table, count, BY_NORM, blockIdx.x);
+  const NsMat t = table[i];
+  const int64_t total = (int64_t)t.m * t.n, e0 = (int64_t)(blockIdx.x - t.first[BY_NORM]) * NORM_CHUNK;
   const int64_t e1 = e0 + NORM_CHUNK < total ? e0 + NORM_CHUNK : total;
   const double f = ldexp(sc[i].inv, -sc[i].ey) * (double)sc[i].rho;
   for (int64_t e = e0 + threadIdx.x; e < e1; e += 256)
     ((T*)t.out)[e] = from_f32<T>((float)((double)to_f32(((const T*)t.g)[e]) * f));
 }
 
-int64_t norm_blocks(int64_t m, int64_t n) { return ceil_div64(m * n, NORM_CHUNK); }
+int sym_tiles(const NsMat& t) {
+  const int n = ceil_div(t.m, GM);
+  return n * (n + 1) / 2;
+}
 
 // How the symmetric products of a launch are cut.  `slots` workgroups (two per CU, or one) run at once.
 //  - Fewer tiles than slots: every reduction is cut into runs of about equal length so that the runs fill the slots.
 //  - One matrix with a little more than whole rounds of tiles: the tiles of the last round are cut instead of leaving
 //    most of the chip idle for it (4096 x 4096: 528 tiles on 512 slots).
-// Returns the partial tiles; fills direct / slices / p0 / f0 of every matrix.  len(t) = its reduction in k-steps of 32.
-template <typename F>
-int64_t cut_sym(NsArgs& a, F len, int& joins) {
+// Fills cut[square] of every matrix and returns the partial tiles; the reduction is in k-steps of 32.
+int64_t cut_sym(NsMat* mats, int n, int square) {
   int64_t slots = 512, tiles = 0, work = 0, parts = 0;
-  joins = 0;
-  auto count = [](const NsMat& t) {
-    const int n = ceil_div(t.m, GM);
-    return n * (n + 1) / 2;
-  };
-  for (int i = 0; i < a.count; ++i) {
-    tiles += count(a.mat[i]);
-    work += (int64_t)count(a.mat[i]) * len(a.mat[i]);
+  auto len = [&](const NsMat& t) { return up64(square ? t.m : t.n) / 32; };
+  for (int i = 0; i < n; ++i) {
+    tiles += sym_tiles(mats[i]);
+    work += (int64_t)sym_tiles(mats[i]) * len(mats[i]);
   }
-  if (work < 512 * 16) slots = 256;  // short runs: one workgroup per CU with the deep pipeline
-  for (int i = 0; i < a.count; ++i) {
-    NsMat& t = a.mat[i];
-    const int n = count(t);
-    t.direct = n;
-    t.slices = 1;
+  if (work < 512 * 16) slots = 256;  // short runs: one workgroup per CU
+  for (int i = 0; i < n; ++i) {
+    const NsMat& t = mats[i];
+    NsMat::Cut& c = mats[i].cut[square];
+    const int all = sym_tiles(t);
+    c.direct = all;
+    c.slices = 1;
     if (tiles < slots) {
       const int64_t run = ceil_div64(work, slots) > 8 ? ceil_div64(work, slots) : 8;
       const int64_t s = len(t) / run;
       if (s > 1) {
-        t.slices = (int)(s < 8 ? s : 8);
-        t.direct = 0;
+        c.slices = (int)(s < 8 ? s : 8);
+        c.direct = 0;
       }
-    } else if (a.count == 1 && tiles % slots && tiles % slots <= slots / 2) {
+    } else if (n == 1 && tiles % slots && tiles % slots <= slots / 2) {
       const int tail = (int)(tiles % slots), room = (int)(slots / tail);
       const int s = room < len(t) / 4 ? room : len(t) / 4;
       if (s > 1) {
-        t.slices = s < 8 ? s : 8;
-        t.direct = n - tail;
+        c.slices = s < 8 ? s : 8;
+        c.direct = all - tail;
       }
     }
-    t.p0 = (int)parts;
-    t.f0 = joins;
-    parts += (int64_t)(n - t.direct) * (t.slices > 1 ? t.slices : 0);
-    joins += n - t.direct;
+    c.p0 = (int)parts;
+    parts += (int64_t)(all - c.direct) * c.slices;
   }
   return parts;
 }
@@ -532,33 +539,43 @@ int check_ns(const char* who, int dtype, int count, const int* rows, const int* 
   return VC_OK;
 }
 
-// Sizes of a launch's matrices and where everything lies in the workspace:
-// [NsScale per matrix | partial norms | partial tiles | fp16 buffers]
+// The table of a launch's matrices, the workgroups of every kind of launch, and where everything lies in the workspace:
+// [table | NsScale per matrix | partial norms | partial tiles | fp16 buffers]
 struct NsLayout {
-  int64_t norm_blocks, init_tiles, upd_tiles, part, mats, bytes;
-};
-NsLayout layout(NsArgs& a, const int* rows, const int* cols) {
-  NsLayout l{};
-  int64_t at = 0;
-  for (int i = 0; i < a.count; ++i) {
-    NsMat& t = a.mat[i];
-    t.tall = rows[i] > cols[i];
-    t.m = t.tall ? cols[i] : rows[i];
-    t.n = t.tall ? rows[i] : cols[i];
-    t.at = at;
-    at = NsView(t, 0).end;
-    l.norm_blocks += norm_blocks(t.m, t.n);
-    l.init_tiles += (int64_t)(up64(t.m) / 64) * (up64(t.n) / 64);
-    l.upd_tiles += (int64_t)ceil_div(t.m, GM) * ceil_div(t.n, GM);
+  NsMat mat[NS_MAX];
+  int64_t blocks[KINDS];
+  int64_t norms, part, bufs, bytes;
+  NsLayout(const int* rows, const int* cols, int count) {
+    int64_t at = 0;
+    for (int i = 0; i < count; ++i) {
+      NsMat& t = mat[i];
+      t = NsMat{};
+      t.tall = rows[i] > cols[i];
+      t.m = t.tall ? cols[i] : rows[i];
+      t.n = t.tall ? rows[i] : cols[i];
+      t.at = at;
+      at = NsView(t, 0).end;
+    }
+    const int64_t ps = cut_sym(mat, count, 0), pp = cut_sym(mat, count, 1);
+    for (int k = 0; k < KINDS; ++k) {
+      blocks[k] = 0;
+      for (int i = 0; i < count; ++i) {
+        NsMat& t = mat[i];
+        t.first[k] = (int)blocks[k];
+        const NsMat::Cut& c = t.cut[k == BY_P || k == BY_JOIN_P];
+        blocks[k] += k == BY_NORM     ? ceil_div64((int64_t)t.m * t.n, NORM_CHUNK)
+                     : k == BY_INIT   ? (int64_t)(up64(t.m) / 64) * (up64(t.n) / 64)
+                     : k == BY_UPDATE ? (int64_t)ceil_div(t.m, GM) * ceil_div(t.n, GM)
+                     : k <= BY_P      ? c.direct + (int64_t)(sym_tiles(t) - c.direct) * c.slices
+                                      : sym_tiles(t) - c.direct;
+      }
+    }
+    norms = NS_MAX * (int64_t)(sizeof(NsMat) + sizeof(NsScale));
+    part = norms + up128(blocks[BY_NORM] * 8);
+    bufs = part + (ps > pp ? ps : pp) * GM * GM * 4;
+    bytes = bufs + at * 2;
   }
-  int joins;
-  const int64_t p1 = cut_sym(a, [](const NsMat& t) { return up64(t.n) / 32; }, joins);
-  const int64_t p2 = cut_sym(a, [](const NsMat& t) { return up64(t.m) / 32; }, joins);
-  l.part = NS_MAX * (int64_t)sizeof(NsScale) + up128(l.norm_blocks * 8);
-  l.mats = l.part + (p1 > p2 ? p1 : p2) * GM * GM * 4;
-  l.bytes = l.mats + at * 2;
-  return l;
-}
+};
 
 }  // namespace
 
@@ -568,9 +585,7 @@ int64_t vc_newton_schulz_bytes(int count, const int* rows, const int* cols) {
   if (check_ns("vc_newton_schulz_bytes", VC_F32, count, rows, cols) != VC_OK) return -1;
   int64_t most = 0;
   for (int b = 0; b < count; b += NS_MAX) {
-    NsArgs a{};
-    a.count = count - b < NS_MAX ? count - b : NS_MAX;
-    const int64_t bytes = layout(a, rows + b, cols + b).bytes;
+    const int64_t bytes = NsLayout(rows + b, cols + b, count - b < NS_MAX ? count - b : NS_MAX).bytes;
     if (bytes > most) most = bytes;
   }
   return most;
@@ -588,64 +603,49 @@ int vc_newton_schulz(int dtype, int count, const void* const* g, void* const* ou
                "vc_newton_schulz: bounds cap %g, gain %g, pmax %g outside [1, 16], [1, 8192], (0, 8192]", (double)cap,
                (double)gain, (double)pmax);
   for (int i = 0; i < count; ++i) VC_CHECK_ARG(g[i] && out[i], "vc_newton_schulz: null matrix %d", i);
-  NsScale* sc = (NsScale*)workspace;
-  double* norms = (double*)((char*)workspace + NS_MAX * sizeof(NsScale));
   NsStep st;
   st.es = (int)floorf(log2f(60000.f / (cap * cap)));
   st.ep = (int)floorf(log2f(60000.f / pmax));
   const bool bf = dtype == VC_BF16;
+  NsMat* table = (NsMat*)workspace;
+  NsScale* sc = (NsScale*)(table + NS_MAX);
   for (int b = 0; b < count; b += NS_MAX) {
-    NsArgs a{};
-    a.count = count - b < NS_MAX ? count - b : NS_MAX;
-    const NsLayout l = layout(a, rows + b, cols + b);
-    VC_CHECK_SHAPE(l.norm_blocks < (1ll << 31) && l.init_tiles < (1ll << 31) && l.upd_tiles < (1ll << 31),
-                   "vc_newton_schulz: too many tiles");
+    const int n = count - b < NS_MAX ? count - b : NS_MAX;
+    NsLayout l(rows + b, cols + b, n);
+    for (int k = 0; k < KINDS; ++k) VC_CHECK_SHAPE(l.blocks[k] < (1ll << 31), "vc_newton_schulz: too many tiles");
+    double* norms = (double*)((char*)workspace + l.norms);
     float* part = (float*)((char*)workspace + l.part);
-    f16* ws = (f16*)((char*)workspace + l.mats);
-    for (int i = 0; i < a.count; ++i) {
-      a.mat[i].g = g[b + i];
-      a.mat[i].out = out[b + i];
+    f16* ws = (f16*)((char*)workspace + l.bufs);
+    for (int i = 0; i < n; ++i) {
+      l.mat[i].g = g[b + i];
+      l.mat[i].out = out[b + i];
     }
-    auto number = [&](auto blocks_of) {  // workgroups in the order of the matrices
-      int64_t at = 0;
-      for (int i = 0; i < a.count; ++i) {
-        a.mat[i].t0 = (int)at;
-        at += blocks_of(a.mat[i]);
-      }
-      return at;
+    for (int i = 0; i < n; i += NS_CHUNK) {
+      NsChunk c;
+      const int k = n - i < NS_CHUNK ? n - i : NS_CHUNK;
+      memcpy(c.mat, l.mat + i, k * sizeof(NsMat));
+      hipLaunchKernelGGL(ns_table_kernel, dim3(1), dim3(64), 0, stream, c, table + i, k);
+    }
+    auto launch = [&](int kind, auto kernel, int threads, auto... args) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)l.blocks[kind]), dim3(threads), 0, stream, table, n, args...);
     };
-    auto launch = [&](auto blocks_of, auto kernel, int threads, auto... args) {
-      hipLaunchKernelGGL(kernel, dim3((unsigned)number(blocks_of)), dim3(threads), 0, stream, a, args...);
-    };
-    auto deep = [&](auto blocks_of) { return number(blocks_of) <= vc_device_cus(); };  // the four-stage pipeline (G16)
-    auto by_norm = [](const NsMat& t) { return norm_blocks(t.m, t.n); };
-    auto by_init = [](const NsMat& t) { return (int64_t)(up64(t.m) / 64) * (up64(t.n) / 64); };
-    auto by_upd = [](const NsMat& t) { return (int64_t)ceil_div(t.m, GM) * ceil_div(t.n, GM); };
-    auto by_sym = [](const NsMat& t) {
-      const int64_t n = ceil_div(t.m, GM);
-      return t.direct + (n * (n + 1) / 2 - t.direct) * t.slices;
-    };
-    launch(by_norm, bf ? ns_norm_kernel<bf16> : ns_norm_kernel<float>, 256, norms);
-    hipLaunchKernelGGL(ns_scale_kernel, dim3(a.count), dim3(64), 0, stream, a, (int)l.norm_blocks, norms, eps, cap, gain, sc);
-    if (steps == 0) launch(by_norm, bf ? ns_copy_kernel<bf16> : ns_copy_kernel<float>, 256, sc);
-    else launch(by_init, bf ? ns_init_kernel<bf16> : ns_init_kernel<float>, 256, ws, sc);
+    auto deep = [&](int kind) { return l.blocks[kind] <= vc_device_cus(); };  // the four-stage pipeline (G16)
+    launch(BY_NORM, bf ? ns_norm_kernel<bf16> : ns_norm_kernel<float>, 256, norms);
+    hipLaunchKernelGGL(ns_scale_kernel, dim3(n), dim3(64), 0, stream, table, n, (int)l.blocks[BY_NORM], norms, eps, cap, gain, sc);
+    if (steps == 0) launch(BY_NORM, bf ? ns_copy_kernel<bf16> : ns_copy_kernel<float>, 256, sc);
+    else launch(BY_INIT, bf ? ns_init_kernel<bf16> : ns_init_kernel<float>, 256, ws, sc);
     for (int k = 0; k < steps; ++k) {
       st.a = coeffs[3 * k];
       st.b = coeffs[3 * k + 1];
       st.c = coeffs[3 * k + 2];
       st.last = k == steps - 1;
-      int joins = 0;
-      cut_sym(a, [](const NsMat& t) { return up64(t.n) / 32; }, joins);
-      launch(by_sym, deep(by_sym) ? ns_sym_kernel<false, 4> : ns_sym_kernel<false, 2>, G_THREADS, ws, sc, st, k & 1, part);
-      if (joins)
-        hipLaunchKernelGGL(ns_sym_join_kernel<false>, dim3(joins), dim3(G_THREADS), 0, stream, a, ws, sc, st, k & 1, part);
-      cut_sym(a, [](const NsMat& t) { return up64(t.m) / 32; }, joins);
-      launch(by_sym, deep(by_sym) ? ns_sym_kernel<true, 4> : ns_sym_kernel<true, 2>, G_THREADS, ws, sc, st, k & 1, part);
-      if (joins)
-        hipLaunchKernelGGL(ns_sym_join_kernel<true>, dim3(joins), dim3(G_THREADS), 0, stream, a, ws, sc, st, k & 1, part);
-      if (deep(by_upd))
-        launch(by_upd, bf ? ns_update_kernel<bf16, 4> : ns_update_kernel<float, 4>, G_THREADS, ws, sc, st, k & 1);
-      else launch(by_upd, bf ? ns_update_kernel<bf16, 2> : ns_update_kernel<float, 2>, G_THREADS, ws, sc, st, k & 1);
+      launch(BY_S, deep(BY_S) ? ns_sym_kernel<false, 4> : ns_sym_kernel<false, 2>, G_THREADS, ws, sc, st, k & 1, part);
+      if (l.blocks[BY_JOIN_S]) launch(BY_JOIN_S, ns_sym_join_kernel<false>, G_THREADS, ws, sc, st, k & 1, part);
+      launch(BY_P, deep(BY_P) ? ns_sym_kernel<true, 4> : ns_sym_kernel<true, 2>, G_THREADS, ws, sc, st, k & 1, part);
+      if (l.blocks[BY_JOIN_P]) launch(BY_JOIN_P, ns_sym_join_kernel<true>, G_THREADS, ws, sc, st, k & 1, part);
+      if (deep(BY_UPDATE))
+        launch(BY_UPDATE, bf ? ns_update_kernel<bf16, 4> : ns_update_kernel<float, 4>, G_THREADS, ws, sc, st, k & 1);
+      else launch(BY_UPDATE, bf ? ns_update_kernel<bf16, 2> : ns_update_kernel<float, 2>, G_THREADS, ws, sc, st, k & 1);
     }
     VC_LAUNCH_CHECK("vc_newton_schulz");
   }
