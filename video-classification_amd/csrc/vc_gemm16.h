@@ -223,6 +223,44 @@ struct G16 {
   }
 };
 
+// An accumulated tile through LDS, so that global memory sees whole rows: T[B row][A row] in fp32, 64 B rows (those of the
+// waves with wn == half) at a time.  Rows of 132 floats; the groups of four of a row are permuted by the row, so that
+// reading it along its rows, in 16-byte pieces, or across them meets few bank conflicts.
+constexpr int G_ROW = GM + 4;
+constexpr int G_TILE = 64 * G_ROW;  // floats
+__device__ __forceinline__ int g16_at(int row, int col) {
+  return row * G_ROW + ((((col >> 2) ^ (row >> 3)) << 2) | (col & 3));
+}
+__device__ __forceinline__ void g16_put(const f32x4 (&acc)[4][4], int half, float* t) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, l15 = lane & 15;
+  if ((wave & 1) != half) return;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      *reinterpret_cast<f32x4*>(t + g16_at(j * 16 + l15, (wave >> 1) * 64 + i * 16 + q * 4)) = acc[i][j];
+}
+// eight consecutive values of a row (col a multiple of 8)
+__device__ __forceinline__ F8 g16_get(const float* t, int row, int col) {
+  F8 r;
+  const f32x4 a = *reinterpret_cast<const f32x4*>(t + g16_at(row, col)), b = *reinterpret_cast<const f32x4*>(t + g16_at(row, col + 4));
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    r.v[e] = a[e];
+    r.v[4 + e] = b[e];
+  }
+  return r;
+}
+__device__ __forceinline__ void f16_split8(const F8& v, f16x8& hi, f16x8& lo) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    f16 h, l;
+    f16_split(v.v[e], h, l);
+    hi[e] = h;
+    lo[e] = l;
+  }
+}
+
 // Workgroup -> tile: consecutive workgroups of one XCD (every eighth) walk bands of eight tile rows, so that the rows of A
 // and B they share stay in that XCD's L2.
 __device__ __forceinline__ void g16_tile(int id, int total, int tm, int tn, int& m, int& n) {

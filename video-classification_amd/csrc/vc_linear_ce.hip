@@ -441,24 +441,31 @@ __global__ __launch_bounds__(G_THREADS, NS == 2 ? 2 : 1) void ce_grad_kernel(CeA
       for (int e = 0; e < 16; ++e)
         if (e == hit) acc[e >> 2][j][e & 3] -= (1.f - smooth) * D_SCALE;
     const bool live = w != 0.f;  // rows that do not count vanish whatever they hold
-    f16* o = dn + (int64_t)n * vcols + (v0 - vbeg + wm * 64 + q * 4);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f16x4 hi, lo;
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float d = live ? acc[i][j][r] * w : 0.f;
-        col[i][r] += d;
-        f16 h, e;
-        f16_split(d, h, e);
-        hi[r] = h;
-        lo[r] = e;
+        acc[i][j][r] = live ? acc[i][j][r] * w : 0.f;
+        col[i][r] += acc[i][j][r];
       }
+  }
+  float* tile = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    g16_put(acc, half, tile);
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int e = threadIdx.x + u * G_THREADS, n = n0 + half * 64 + (e >> 4);
+      f16x8 hi, lo;
+      f16_split8(g16_get(tile, e >> 4, (e & 15) * 8), hi, lo);
       if (n < a.N) {
-        *reinterpret_cast<f16x4*>(o + i * 16) = hi;
-        if (PD == 2) *reinterpret_cast<f16x4*>(o + plane + i * 16) = lo;
+        f16* o = dn + (int64_t)n * vcols + (v0 - vbeg + (e & 15) * 8);
+        *reinterpret_cast<f16x8*>(o) = hi;
+        if (PD == 2) *reinterpret_cast<f16x8*>(o + plane) = lo;
       }
     }
+    __syncthreads();
   }
   if (dbpart) {
 #pragma unroll

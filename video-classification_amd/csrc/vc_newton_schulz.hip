@@ -243,81 +243,70 @@ __device__ __forceinline__ int xcd_run(int id, int total) {
 }
 
 // What becomes of an accumulated tile (rows m0 + .. in registers, columns n0 + .. across lanes) of a symmetric product:
-// S = rho^2 Y Y^T, or P = b S + c S S (SQUARE), stored at (column, row) straight from the registers and, off the
-// diagonal, at (row, column) through LDS.
+// S = rho^2 Y Y^T, or P = b S + c S S (SQUARE).  It is stored at (column, row) and, off the diagonal, at (row, column), both
+// in whole 16-byte pieces.
 template <bool SQUARE>
-__device__ __forceinline__ void sym_store(f32x4 (&acc)[4][4], const NsMat& t, const NsView& w, f16* ws, const NsScale& sc,
-                                          const NsStep& st, int m0, int n0, f16* smem) {
-  const int lane = threadIdx.x & 63, q = lane >> 4, l15 = lane & 15;
-  const int wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
+__device__ __forceinline__ void sym_store(const f32x4 (&acc)[4][4], const NsMat& t, const NsView& w, f16* ws,
+                                          const NsScale& sc, const NsStep& st, int m0, int n0, float* tile) {
   const f16* s = ws + w.s;
   f16* dst = ws + (SQUARE ? w.p : w.s);
   const int64_t pl = (int64_t)t.m * w.ldm;
   const float f = SQUARE ? ldexpf(st.c, st.ep - 2 * st.es) : ldexpf(sc.rho2, st.es - 2 * sc.ey);
   const float sb = ldexpf(st.b, st.ep - st.es);
-  constexpr int STR = GM + 8;
-  f16x4 lo[4][4];
-  if (SQUARE) {  // all of S first: the stores below could alias its loads and would hold them back
-    f16x4 sh[4][4], sl[4][4];
+  const bool mirror = m0 != n0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+  for (int half = 0; half < 2; ++half) {
+    const int c0 = n0 + half * 64;
+    f16x8 sh[4], sl[4];  // S where it is needed, on its way while the tile passes through LDS
+    if (SQUARE)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int r = m0 + wm * 64 + i * 16 + q * 4, c = n0 + wn * 64 + j * 16 + l15;
-        const int64_t o = (int64_t)min(c, t.m - 1) * w.ldm + min(r, w.ldm - 4);
-        sh[i][j] = *reinterpret_cast<const f16x4*>(s + o);
-        sl[i][j] = *reinterpret_cast<const f16x4*>(s + o + pl);
+      for (int u = 0; u < 4; ++u) {
+        const int e = threadIdx.x + u * G_THREADS;
+        const int64_t o = (int64_t)min(c0 + (e >> 4), t.m - 1) * w.ldm + min(m0 + (e & 15) * 8, w.ldm - 8);
+        sh[u] = *reinterpret_cast<const f16x8*>(s + o);
+        sl[u] = *reinterpret_cast<const f16x8*>(s + o + pl);
       }
+    g16_put(acc, half, tile);
+    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int u = 0; u < 4; ++u) {
+      const int e = threadIdx.x + u * G_THREADS, cl = e >> 4, rl = (e & 15) * 8;
+      F8 v = g16_get(tile, cl, rl);
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          acc[i][j][k] = fmaf(sb, (float)sh[i][j][k] + (float)sl[i][j][k], acc[i][j][k] * f);
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int r = m0 + wm * 64 + i * 16 + q * 4, c = n0 + wn * 64 + j * 16 + l15;
-      const bool in = c < t.m && r < w.ldm;
-      const int64_t o = (int64_t)c * w.ldm + r;
-      f16x4 h;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float v = SQUARE ? acc[i][j][k] : acc[i][j][k] * f;
-        f16 u, e;
-        f16_split(v, u, e);
-        h[k] = u;
-        lo[i][j][k] = e;
-        if (m0 != n0) smem[(r - m0 + k) * STR + c - n0] = u;
+      for (int k = 0; k < 8; ++k) {
+        v.v[k] *= f;
+        if (SQUARE) v.v[k] = fmaf(sb, (float)sh[u][k] + (float)sl[u][k], v.v[k]);
       }
-      if (in) {
-        *reinterpret_cast<f16x4*>(dst + o) = h;
-        *reinterpret_cast<f16x4*>(dst + o + pl) = lo[i][j];
+      if (mirror) {
+        *reinterpret_cast<f32x4*>(tile + g16_at(cl, rl)) = f32x4{v.v[0], v.v[1], v.v[2], v.v[3]};
+        *reinterpret_cast<f32x4*>(tile + g16_at(cl, rl + 4)) = f32x4{v.v[4], v.v[5], v.v[6], v.v[7]};
       }
-    }
-  if (m0 == n0) return;
-#pragma unroll
-  for (int p = 0; p < 2; ++p) {
-    if (p) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            smem[(wm * 64 + i * 16 + q * 4 + k) * STR + wn * 64 + j * 16 + l15] = lo[i][j][k];
+      if (c0 + cl < t.m && m0 + rl < w.ldm) {
+        f16x8 h, l;
+        f16_split8(v, h, l);
+        f16* d = dst + (int64_t)(c0 + cl) * w.ldm + m0 + rl;
+        *reinterpret_cast<f16x8*>(d) = h;
+        *reinterpret_cast<f16x8*>(d + pl) = l;
+      }
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < GM * 16; e += G_THREADS) {
-      const int r = e >> 4, c = (e & 15) * 8;  // below the diagonal every column of the tile is inside
-      if (m0 + r < t.m)
-        *reinterpret_cast<f16x8*>(dst + p * pl + (int64_t)(m0 + r) * w.ldm + n0 + c) =
-            *reinterpret_cast<const f16x8*>(smem + r * STR + c);
+    if (mirror) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int e = threadIdx.x + u * G_THREADS, rl = e >> 3, cl = (e & 7) * 8;
+        F8 v;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v.v[k] = tile[g16_at(cl + k, rl)];
+        if (m0 + rl < t.m) {  // below the diagonal every column of the tile is inside
+          f16x8 h, l;
+          f16_split8(v, h, l);
+          f16* d = dst + (int64_t)(m0 + rl) * w.ldm + c0 + cl;
+          *reinterpret_cast<f16x8*>(d) = h;
+          *reinterpret_cast<f16x8*>(d + pl) = l;
+        }
+      }
+      __syncthreads();
     }
-    __syncthreads();
   }
 }
 
@@ -359,7 +348,7 @@ __global__ __launch_bounds__(G_THREADS, NS == 2 ? 2 : 1) void ns_sym_kernel(cons
     for (int e = 0; e < 16; ++e) o[e * G_THREADS] = acc[e >> 2][e & 3];
     return;
   }
-  sym_store<SQUARE>(acc, t, w, ws, sc[i], st, m0, n0, smem);
+  sym_store<SQUARE>(acc, t, w, ws, sc[i], st, m0, n0, reinterpret_cast<float*>(smem));
 }
 
 // joins the slices of a tile in order
@@ -367,7 +356,7 @@ template <bool SQUARE>
 __global__ __launch_bounds__(G_THREADS, 2) void ns_sym_join_kernel(const NsMat* __restrict__ table, int count, f16* __restrict__ ws,
                                                                    const NsScale* __restrict__ sc, NsStep st, int parity,
                                                                    const float* __restrict__ part) {
-  __shared__ __attribute__((aligned(1024))) f16 smem[GM * (GM + 8)];
+  __shared__ __attribute__((aligned(1024))) float smem[G_TILE];
   const int i = find_mat(table, count, SQUARE ? BY_JOIN_P : BY_JOIN_S, blockIdx.x);
   const NsMat t = table[i];
   const NsMat::Cut cut = t.cut[SQUARE];
@@ -378,6 +367,7 @@ __global__ __launch_bounds__(G_THREADS, 2) void ns_sym_join_kernel(const NsMat* 
   f32x4 acc[4][4];
   G16<2, 2>::zero(acc);
   const f32x4* p = reinterpret_cast<const f32x4*>(part + ((int64_t)cut.p0 + (int64_t)e0 * cut.slices) * GM * GM) + threadIdx.x;
+#pragma unroll 2
   for (int s = 0; s < cut.slices; ++s, p += GM * GM / 4)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[e >> 2][e & 3] += p[e * G_THREADS];
@@ -403,66 +393,62 @@ __global__ __launch_bounds__(G_THREADS, NS == 2 ? 2 : 1) void ns_update_kernel(c
   f32x4 acc[4][4];
   G::zero(acc);
   G::run(acc, Op16{x, px, w.ldn, t.m, n0}, Op16{ws + w.p + (int64_t)m0 * w.ldm, pp, w.ldm, t.m - m0, 0}, 0, w.ldm, smem);
-  const int lane = threadIdx.x & 63, q = lane >> 4, l15 = lane & 15;
-  const int wave = threadIdx.x >> 6, wc = wave >> 1, wr = wave & 1;
   f16* xo = ws + w.xo;
   const float f = ldexpf(1.f, -st.ep), fo = sc[i].rho;
   const int ey = sc[i].ey;
   T* out = (T*)t.out;
-  const bool vec = !t.tall && t.n % 4 == 0 && ((uintptr_t)out & 15) == 0;
-  {
-    f16x4 xh[4][4], xl[4][4];  // all of X's tile first: the stores below could alias its loads and would hold them back
+  const bool vec = !t.tall && t.n % 8 == 0 && ((uintptr_t)out & 15) == 0;
+  float* tile = reinterpret_cast<float*>(smem);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+  for (int half = 0; half < 2; ++half) {
+    const int r0 = m0 + half * 64;
+    f16x8 xh[4], xl[4];  // X's tile, on its way while P X passes through LDS
 #pragma unroll
-      for (int ii = 0; ii < 4; ++ii) {
-        const int64_t o = (int64_t)min(m0 + wr * 64 + j * 16 + l15, t.m - 1) * w.ldn +
-                          min(n0 + wc * 64 + ii * 16 + q * 4, w.ldn - 4);
-        xh[ii][j] = *reinterpret_cast<const f16x4*>(x + o);
-        xl[ii][j] = *reinterpret_cast<const f16x4*>(x + o + px);
+    for (int u = 0; u < 4; ++u) {
+      const int e = threadIdx.x + u * G_THREADS;
+      const int64_t o = (int64_t)min(r0 + (e >> 4), t.m - 1) * w.ldn + min(n0 + (e & 15) * 8, w.ldn - 8);
+      xh[u] = *reinterpret_cast<const f16x8*>(x + o);
+      xl[u] = *reinterpret_cast<const f16x8*>(x + o + px);
+    }
+    g16_put(acc, half, tile);
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int e = threadIdx.x + u * G_THREADS, r = r0 + (e >> 4), c = n0 + (e & 15) * 8;
+      F8 v = g16_get(tile, e >> 4, (e & 15) * 8);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v.v[k] = fmaf(st.a, (float)xh[u][k] + (float)xl[u][k], v.v[k] * f);
+      if (st.last) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v.v[k] = fo * ldexpf(v.v[k], -ey);
       }
+      if (st.last && t.tall) {  // the result is transposed: through LDS once more
+        *reinterpret_cast<f32x4*>(tile + g16_at(e >> 4, (e & 15) * 8)) = f32x4{v.v[0], v.v[1], v.v[2], v.v[3]};
+        *reinterpret_cast<f32x4*>(tile + g16_at(e >> 4, (e & 15) * 8 + 4)) = f32x4{v.v[4], v.v[5], v.v[6], v.v[7]};
+      } else if (st.last) {
+        if (r < t.m && c < t.n) {
+          T* d = out + (int64_t)r * t.n + c;
+          if (vec) store8(d, v);
+          else
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int ii = 0; ii < 4; ++ii)
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          acc[ii][j][k] = fmaf(st.a, (float)xh[ii][j][k] + (float)xl[ii][j][k], acc[ii][j][k] * f);
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int r = m0 + wr * 64 + j * 16 + l15;
-    if (r >= t.m) continue;
-#pragma unroll
-    for (int ii = 0; ii < 4; ++ii) {
-      const int c = n0 + wc * 64 + ii * 16 + q * 4;
-      if (c >= w.ldn) continue;
-      const int64_t o = (int64_t)r * w.ldn + c;
-      f32x4 v = acc[ii][j];
-      if (!st.last) {
-        f16x4 h, l;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          f16 u, e;
-          f16_split(v[k], u, e);
-          h[k] = u;
-          l[k] = e;
+            for (int k = 0; k < 8; ++k)
+              if (c + k < t.n) d[k] = from_f32<T>(v.v[k]);
         }
-        *reinterpret_cast<f16x4*>(xo + o) = h;
-        *reinterpret_cast<f16x4*>(xo + o + px) = l;
-        continue;
+      } else if (r < t.m && c < w.ldn) {
+        f16x8 h, l;
+        f16_split8(v, h, l);
+        const int64_t o = (int64_t)r * w.ldn + c;
+        *reinterpret_cast<f16x8*>(xo + o) = h;
+        *reinterpret_cast<f16x8*>(xo + o + px) = l;
       }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = fo * ldexpf(v[k], -ey);
-      if (vec) {
-        if (c >= t.n) continue;
-        T* d = out + (int64_t)r * t.n + c;
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4*>(d) = v;
-        else *reinterpret_cast<bf16x4*>(d) = bf16x4{(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
-      } else
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (c + k < t.n) out[t.tall ? (int64_t)(c + k) * t.m + r : (int64_t)r * t.n + c + k] = from_f32<T>(v[k]);
+    }
+    __syncthreads();
+    if (st.last && t.tall) {
+      for (int e = threadIdx.x; e < GM * 64; e += G_THREADS) {
+        const int cl = e >> 6, rl = e & 63;
+        if (n0 + cl < t.n && r0 + rl < t.m) out[(int64_t)(n0 + cl) * t.m + r0 + rl] = from_f32<T>(tile[g16_at(rl, cl)]);
+      }
+      __syncthreads();
     }
   }
 }
