@@ -15,31 +15,11 @@
 // joined by the exact identity for the union of two samples (means and second moments about the means).
 #include <initializer_list>
 
-#include "vc_common.h"
+#include "vc_group.h"
 
 namespace {
 
 constexpr int GT = 256;  // threads per block
-
-enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3 };
-
-template <int ACT>
-__device__ __forceinline__ float act_fwd(float z) {
-  if (ACT == ACT_RELU) return z < 0.f ? 0.f : z;  // NaN stays NaN
-  if (ACT == ACT_SILU) return z * __builtin_amdgcn_rcpf(1.f + __expf(-z));
-  if (ACT == ACT_GELU) return vc_gelu(z);
-  return z;
-}
-template <int ACT>
-__device__ __forceinline__ float act_slope(float z) {
-  if (ACT == ACT_RELU) return z > 0.f ? 1.f : 0.f;
-  if (ACT == ACT_SILU) {
-    const float s = __builtin_amdgcn_rcpf(1.f + __expf(-z));
-    return s * fmaf(z, 1.f - s, 1.f);
-  }
-  if (ACT == ACT_GELU) return vc_gelu_grad(z);
-  return 1.f;
-}
 
 template <typename T, int V>
 __device__ __forceinline__ void loadv(const T* p, float (&v)[V]) {
@@ -412,8 +392,8 @@ __global__ __launch_bounds__(GT) void gn_bwd_apply_kernel(Cover k, const T* __re
   }
 }
 
-// `rows` is chosen so that a launch has about eight blocks per CU where the data allows it, and so that a thread
-// still sums a few rows: the partial statistics of a block are 8 bytes per channel
+// `rows` is chosen so that a launch has the five blocks per CU that are resident at once where the data allows it, and so
+// that a thread still sums a few rows: the partial statistics of a block are 8 bytes per channel
 Cover make_cover(int N, int S, int C, int G, int V) {
   Cover k;
   k.S = S;
@@ -424,7 +404,7 @@ Cover make_cover(int N, int S, int C, int G, int V) {
   k.cvb = k.cv < GT ? k.cv : GT;
   k.ry = GT / k.cvb;
   const int64_t slabs = ceil_div(k.cv, k.cvb);
-  const int64_t want = ceil_div64(8 * 256, (int64_t)N * slabs);  // chunks per sample
+  const int64_t want = ceil_div64(5 * 256, (int64_t)N * slabs);  // chunks per sample
   int64_t rows = ceil_div64(S, want);
   const int64_t least = (int64_t)k.ry * 8;
   if (rows < least) rows = least;
@@ -532,6 +512,10 @@ int vc_group_norm_fwd(int dtype, const void* x, const void* residual, const floa
   if (rc != VC_OK) return rc;
   VC_CHECK_ARG(x && y && mean && rstd && workspace, "vc_group_norm_fwd: null pointer");
   const int V = vec_of(C, {x, residual, y});
+  if (V == 8 && vc_gn_slab_fwd(dtype, x, residual, gamma, beta, y, mean, rstd, N, S, C, G, eps, act, stream)) {
+    VC_LAUNCH_CHECK("vc_group_norm_fwd");
+    return VC_OK;
+  }
   const Cover k = make_cover(N, S, C, G, V);
   if (dtype == VC_BF16)
     return V == 8 ? fwd_go<bf16, 8>(k, N, x, residual, gamma, beta, y, mean, rstd, workspace, eps, act, stream)
@@ -549,6 +533,14 @@ int vc_group_norm_bwd(int dtype, const void* x, const void* dy, const void* resi
   VC_CHECK_ARG(x && dy && mean && rstd && workspace, "vc_group_norm_bwd: null pointer");
   VC_CHECK_ARG(((uintptr_t)workspace & 7) == 0, "vc_group_norm_bwd: workspace must be 8-byte aligned");
   const int V = vec_of(C, {x, dy, residual, dx, dresidual});
+  if (V == 8 && vc_gn_slab_bwd(dtype, x, dy, residual, gamma, beta, mean, rstd, dx, dresidual, workspace, N, S, C, G, act,
+                               stream)) {
+    if (dgamma || dbeta)
+      hipLaunchKernelGGL(gn_bwd_params_kernel, dim3(ceil_div(C, 64)), dim3(GT), 0, stream, workspace, dgamma, dbeta, N, C,
+                         accumulate);
+    VC_LAUNCH_CHECK("vc_group_norm_bwd");
+    return VC_OK;
+  }
   const Cover k = make_cover(N, S, C, G, V);
   if (dtype == VC_BF16)
     return V == 8 ? bwd_go<bf16, 8>(k, N, x, dy, residual, gamma, beta, mean, rstd, dx, dresidual, dgamma, dbeta, workspace, act, accumulate, stream)
