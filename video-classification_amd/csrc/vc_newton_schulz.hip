@@ -466,6 +466,112 @@ __global__ __launch_bounds__(256) void ns_copy_kernel(const NsMat* __restrict__ 
     ((T*)t.out)[e] = from_f32<T>((float)((double)to_f32(((const T*)t.g)[e]) * f));
 }
 
+// Matrices of at most 16 rows (columns, if tall): all steps in one workgroup, X in LDS, in fp64 where it fits twice and
+// fp32 otherwise.  A 128 x 128 product tile would be nine tenths padding, and a matrix this small has nothing to average
+// the two-term rounding over: its result was off by up to five times fp32's error.  One workgroup's time grows with
+// m^2 n (12 x 199 in 49 us, 16 x 2200 in 230, against about 110 for the launches of the tiled form), hence the third bound.
+constexpr int SMALL_ROWS = 16, SMALL_ELEMS = 36000, SMALL_THREADS = 512, SMALL_MAX = 96;
+struct NsSmall {
+  const void* g;
+  void* out;
+  int m, n, tall;
+};
+struct NsSmallArgs {
+  NsSmall mat[SMALL_MAX];
+};
+bool is_small(int rows, int cols) {
+  const int64_t m = rows < cols ? rows : cols, total = (int64_t)rows * cols;
+  return m <= SMALL_ROWS && total <= SMALL_ELEMS && m * total <= 200000;
+}
+
+template <typename F>
+__device__ __forceinline__ F wave_sum_of(F v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+struct NsCoeffs {
+  float v[3 * 64];
+};
+
+template <typename T, typename F>
+__device__ __forceinline__ void small_steps(const NsSmall& t, const NsCoeffs& c, int steps, double eps, F* x,
+                                            F (&s)[SMALL_ROWS][SMALL_ROWS + 1], F (&p)[SMALL_ROWS][SMALL_ROWS],
+                                            double (&sums)[SMALL_THREADS / 64]) {
+  constexpr int R = SMALL_ROWS;
+  const int m = t.m, n = t.n, total = m * n;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const T* g = (const T*)t.g;
+  double sq = 0.0;
+  for (int e = threadIdx.x; e < total; e += SMALL_THREADS) {
+    const float v = to_f32(g[e]);
+    x[t.tall ? e % m * n + e / m : e] = v;
+    sq += (double)v * (double)v;
+  }
+  sq = wave_sum_f64(sq);
+  if (lane == 0) sums[wave] = sq;
+  for (int e = threadIdx.x; e < R * R; e += SMALL_THREADS) p[e / R][e % R] = 0;
+  __syncthreads();
+  double norm = 0.0;
+#pragma unroll
+  for (int w = 0; w < SMALL_THREADS / 64; ++w) norm += sums[w];
+  norm = sqrt(norm) + eps;
+  const double inv = norm == 0.0 ? 0.0 : 1.0 / norm;
+  for (int e = threadIdx.x; e < total; e += SMALL_THREADS) x[e] = (F)((double)x[e] * inv);
+  for (int k = 0; k < steps; ++k) {
+    __syncthreads();
+    // S: a wave per pair of rows
+    for (int pr = wave; pr < m * (m + 1) / 2; pr += SMALL_THREADS / 64) {
+      int i = (int)((sqrtf(8.f * pr + 1.f) - 1.f) * 0.5f);
+      while ((i + 1) * (i + 2) / 2 <= pr) ++i;
+      while (i * (i + 1) / 2 > pr) --i;
+      const int j = pr - i * (i + 1) / 2;
+      F d = 0;
+      for (int e = lane; e < n; e += 64) d = fma(x[i * n + e], x[j * n + e], d);
+      d = wave_sum_of(d);
+      if (lane == 0) s[i][j] = s[j][i] = d;
+    }
+    __syncthreads();
+    // P = b S + c S S
+    const F ca = c.v[3 * k], cb = c.v[3 * k + 1], cc = c.v[3 * k + 2];
+    for (int e = threadIdx.x; e < m * m; e += SMALL_THREADS) {
+      const int i = e / m, j = e - i * m;
+      F d = 0;
+      for (int q = 0; q < m; ++q) d = fma(s[i][q], s[q][j], d);
+      p[i][j] = fma(cb, s[i][j], cc * d);
+    }
+    __syncthreads();
+    // X <- a X + P X: a thread owns whole columns
+    for (int e = threadIdx.x; e < n; e += SMALL_THREADS) {
+      F v[R];
+#pragma unroll
+      for (int i = 0; i < R; ++i) v[i] = i < m ? x[i * n + e] : (F)0;
+      for (int i = 0; i < m; ++i) {
+        F d = 0;
+#pragma unroll
+        for (int q = 0; q < R; ++q) d = fma(p[i][q], v[q], d);
+        x[i * n + e] = fma(ca, x[i * n + e], d);
+      }
+    }
+  }
+  __syncthreads();
+  T* o = (T*)t.out;
+  for (int e = threadIdx.x; e < total; e += SMALL_THREADS) o[e] = from_f32<T>((float)x[t.tall ? e % m * n + e / m : e]);
+}
+
+template <typename T>
+__global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(NsSmallArgs a, NsCoeffs c, int steps, double eps) {
+  constexpr int R = SMALL_ROWS;
+  __shared__ __attribute__((aligned(16))) float x[SMALL_ELEMS];  // [m][n]
+  __shared__ double s[R][R + 1], p[R][R], sums[SMALL_THREADS / 64];
+  const NsSmall t = a.mat[blockIdx.x];
+  if (t.m * t.n <= SMALL_ELEMS / 2) small_steps<T, double>(t, c, steps, eps, (double*)x, s, p, sums);
+  else
+    small_steps<T, float>(t, c, steps, eps, x, reinterpret_cast<float(&)[R][R + 1]>(s), reinterpret_cast<float(&)[R][R]>(p),
+                          sums);
+}
+
 int sym_tiles(const NsMat& t) {
   const int n = ceil_div(t.m, GM);
   return n * (n + 1) / 2;
@@ -569,9 +675,15 @@ extern "C" {
 
 int64_t vc_newton_schulz_bytes(int count, const int* rows, const int* cols) {
   if (check_ns("vc_newton_schulz_bytes", VC_F32, count, rows, cols) != VC_OK) return -1;
-  int64_t most = 0;
-  for (int b = 0; b < count; b += NS_MAX) {
-    const int64_t bytes = NsLayout(rows + b, cols + b, count - b < NS_MAX ? count - b : NS_MAX).bytes;
+  int64_t most = 256;
+  for (int b = 0; b < count;) {
+    int r[NS_MAX], c[NS_MAX], n = 0;
+    for (; b < count && n < NS_MAX; ++b)
+      if (!is_small(rows[b], cols[b])) {
+        r[n] = rows[b];
+        c[n++] = cols[b];
+      }
+    const int64_t bytes = n ? NsLayout(r, c, n).bytes : 0;
     if (bytes > most) most = bytes;
   }
   return most;
@@ -595,22 +707,42 @@ int vc_newton_schulz(int dtype, int count, const void* const* g, void* const* ou
   const bool bf = dtype == VC_BF16;
   NsMat* table = (NsMat*)workspace;
   NsScale* sc = (NsScale*)(table + NS_MAX);
-  for (int b = 0; b < count; b += NS_MAX) {
-    const int n = count - b < NS_MAX ? count - b : NS_MAX;
-    NsLayout l(rows + b, cols + b, n);
+  NsSmallArgs small;
+  int ns = 0;
+  auto flush = [&]() {
+    NsCoeffs c{};
+    for (int k = 0; k < 3 * steps; ++k) c.v[k] = coeffs[k];
+    if (ns) hipLaunchKernelGGL((bf ? ns_small_kernel<bf16> : ns_small_kernel<float>), dim3(ns), dim3(SMALL_THREADS), 0, stream, small, c, steps, eps);
+    ns = 0;
+  };
+  for (int b = 0; b < count;) {
+    int r[NS_MAX], c[NS_MAX], src[NS_MAX], n = 0;
+    for (; b < count && n < NS_MAX; ++b) {
+      if (is_small(rows[b], cols[b])) {
+        const bool tall = rows[b] > cols[b];
+        small.mat[ns++] = NsSmall{g[b], out[b], tall ? cols[b] : rows[b], tall ? rows[b] : cols[b], tall};
+        if (ns == SMALL_MAX) flush();
+      } else {
+        r[n] = rows[b];
+        c[n] = cols[b];
+        src[n++] = b;
+      }
+    }
+    if (!n) break;  // the rest was small
+    NsLayout l(r, c, n);
     for (int k = 0; k < KINDS; ++k) VC_CHECK_SHAPE(l.blocks[k] < (1ll << 31), "vc_newton_schulz: too many tiles");
     double* norms = (double*)((char*)workspace + l.norms);
     float* part = (float*)((char*)workspace + l.part);
     f16* ws = (f16*)((char*)workspace + l.bufs);
     for (int i = 0; i < n; ++i) {
-      l.mat[i].g = g[b + i];
-      l.mat[i].out = out[b + i];
+      l.mat[i].g = g[src[i]];
+      l.mat[i].out = out[src[i]];
     }
     for (int i = 0; i < n; i += NS_CHUNK) {
-      NsChunk c;
+      NsChunk e;
       const int k = n - i < NS_CHUNK ? n - i : NS_CHUNK;
-      memcpy(c.mat, l.mat + i, k * sizeof(NsMat));
-      hipLaunchKernelGGL(ns_table_kernel, dim3(1), dim3(64), 0, stream, c, table + i, k);
+      memcpy(e.mat, l.mat + i, k * sizeof(NsMat));
+      hipLaunchKernelGGL(ns_table_kernel, dim3(1), dim3(64), 0, stream, e, table + i, k);
     }
     auto launch = [&](int kind, auto kernel, int threads, auto... args) {
       hipLaunchKernelGGL(kernel, dim3((unsigned)l.blocks[kind]), dim3(threads), 0, stream, table, n, args...);
@@ -633,8 +765,9 @@ int vc_newton_schulz(int dtype, int count, const void* const* g, void* const* ou
         launch(BY_UPDATE, bf ? ns_update_kernel<bf16, 4> : ns_update_kernel<float, 4>, G_THREADS, ws, sc, st, k & 1);
       else launch(BY_UPDATE, bf ? ns_update_kernel<bf16, 2> : ns_update_kernel<float, 2>, G_THREADS, ws, sc, st, k & 1);
     }
-    VC_LAUNCH_CHECK("vc_newton_schulz");
   }
+  flush();
+  VC_LAUNCH_CHECK("vc_newton_schulz");
   return VC_OK;
 }
 
