@@ -352,7 +352,13 @@ __global__ __launch_bounds__(GT) void gn_bwd_params_kernel(const float* __restri
   }
 }
 
-// dx = rstd * (gamma * dz - c1 - xhat * c2), dres = dz
+// dx = rstd * (gamma * dz - c1 - xhat * c2), dres = dz.  With few samples (fold) the first workgroups of sample 0 also
+// write the parameters' gradients, which saves the launch of gn_bwd_params_kernel.
+struct Fold {
+  const float* ab;
+  float *dgamma, *dbeta;
+  int N, add;
+};
 template <typename T, int V, int ACT, bool RES>
 __global__ __launch_bounds__(GT) void gn_bwd_apply_kernel(Cover k, const T* __restrict__ x, const T* __restrict__ dy,
                                                           const T* __restrict__ res, const float* __restrict__ mean,
@@ -360,9 +366,20 @@ __global__ __launch_bounds__(GT) void gn_bwd_apply_kernel(Cover k, const T* __re
                                                           const float* __restrict__ gamma,
                                                           const float* __restrict__ beta,
                                                           const float2* __restrict__ coef, T* __restrict__ dx,
-                                                          T* __restrict__ dres) {
+                                                          T* __restrict__ dres, Fold f) {
   const Slot<V> t(k);
   if (!t.on) return;
+  if (f.N && t.n == 0 && blockIdx.x == 0 && t.ty == 0)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      float a = 0.f, b = 0.f;
+      for (int n = 0; n < f.N; ++n) {
+        a += f.ab[(size_t)n * 2 * k.C + t.c + i];
+        b += f.ab[(size_t)n * 2 * k.C + k.C + t.c + i];
+      }
+      if (f.dbeta) f.dbeta[t.c + i] = (f.add & 2 ? f.dbeta[t.c + i] : 0.f) + a;
+      if (f.dgamma) f.dgamma[t.c + i] = (f.add & 1 ? f.dgamma[t.c + i] : 0.f) + b;
+    }
   const Chan<V> h(k, t.n, t.c, mean, rstd, gamma, beta);
   float c1[V], c2[V];
 #pragma unroll
@@ -478,12 +495,14 @@ int bwd_go(const Cover& k, int N, const void* x, const void* dy, const void* res
              hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, V, ACT, RES>), grid, dim3(GT), 0, st, k, (const T*)x,
                                 (const T*)dy, (const T*)res, mean, rstd, gamma, beta, ws));
   hipLaunchKernelGGL(gn_bwd_join_kernel, dim3(k.G, N), dim3(64), 0, st, k, ws, gamma, ab, coef);
-  if (dgamma || dbeta)
+  const bool params = dgamma || dbeta, fold = params && (dx || dres) && N <= 8;
+  if (params && !fold)
     hipLaunchKernelGGL(gn_bwd_params_kernel, dim3(ceil_div(k.C, 64)), dim3(GT), 0, st, ab, dgamma, dbeta, N, k.C, add);
+  const Fold f{ab, dgamma, dbeta, fold ? N : 0, add};
   if (dx || dres)
     GN_ACT_RES(act, res,
                hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT, RES>), grid, dim3(GT), 0, st, k, (const T*)x,
-                                  (const T*)dy, (const T*)res, mean, rstd, gamma, beta, coef, (T*)dx, (T*)dres));
+                                  (const T*)dy, (const T*)res, mean, rstd, gamma, beta, coef, (T*)dx, (T*)dres, f));
   VC_LAUNCH_CHECK("vc_group_norm_bwd");
   return VC_OK;
 }

@@ -144,6 +144,7 @@ struct CeArgs {
   const f16* x;      // [px][N][ld]
   const void* bias;  // nullable, float or bf16
   const int64_t* target;
+  int64_t ignore;
   const int* exps;
   int N, V, ld, bias_bf16;
   int tiles_v, tiles_n;
@@ -272,23 +273,50 @@ __global__ __launch_bounds__(G_THREADS, NS == 2 ? 2 : 1) void ce_stats_kernel(Ce
     }
 }
 
-// Per row: lse (in units of log2), loss (0 for ignored rows, NaN for a target outside [0, V)), arg-max.  8 rows x 32 runs of tiles per block.
-__global__ __launch_bounds__(256) void ce_join_kernel(const float4* __restrict__ part, const float* __restrict__ zt,
-                                                      const int64_t* __restrict__ target, int64_t ignore, int N, int V,
-                                                      int tiles_v, float smooth, float* __restrict__ lse,
-                                                      float* __restrict__ rowloss, int64_t* __restrict__ pred) {
-  __shared__ Stat sm[32][8];
-  const int e = threadIdx.x & 7, run = threadIdx.x >> 3;
-  const int n = blockIdx.x * 8 + e;
-  Stat s{-INFINITY, 0.f, 0.f, V};
-  if (n < N) {
-    const int per = (tiles_v + 31) / 32, t1 = min(tiles_v, (run + 1) * per);
-#pragma unroll 4
-    for (int t = run * per; t < t1; ++t) {
-      const float4 o = part[(int64_t)t * N + n];
-      stat_join(s, Stat{o.x, o.y, o.z, __float_as_int(o.w)});
+// Per row, from its joined statistics: lse (in units of log2), loss (0 for ignored rows, NaN for a target outside [0, V)),
+// arg-max.
+struct CeRows {
+  const float* zt;
+  const int64_t* target;
+  int64_t ignore;
+  int N, V, tiles_v;
+  float smooth;
+  float *lse, *rowloss;
+  int64_t* pred;
+};
+__device__ __forceinline__ float row_out(const CeRows& k, int n, const Stat& s) {
+  const float l = (s.m == -INFINITY ? 0.f : s.m) + log2f(s.s);
+  k.lse[n] = l;
+  const int64_t t = k.target[n];
+  float loss = 0.f;
+  if (t != k.ignore) {
+    if (t < 0 || t >= k.V) loss = NAN;
+    else {
+      const float d = l - k.zt[n];
+      loss = LN2 * (k.smooth > 0.f ? (1.f - k.smooth) * d + k.smooth * (l - s.z / (float)k.V) : d);
     }
   }
+  k.rowloss[n] = loss;
+  if (k.pred) k.pred[n] = s.arg < k.V ? s.arg : 0;
+  return loss;
+}
+__device__ __forceinline__ Stat row_join(const CeRows& k, const float4* part, int n, int t0, int t1) {
+  Stat s{-INFINITY, 0.f, 0.f, k.V};
+#pragma unroll 4
+  for (int t = t0; t < t1; ++t) {
+    const float4 o = part[(int64_t)t * k.N + n];
+    stat_join(s, Stat{o.x, o.y, o.z, __float_as_int(o.w)});
+  }
+  return s;
+}
+
+// 8 rows x 32 runs of tiles per block
+__global__ __launch_bounds__(256) void ce_join_kernel(CeRows k, const float4* __restrict__ part) {
+  __shared__ Stat sm[32][8];
+  const int e = threadIdx.x & 7, run = threadIdx.x >> 3;
+  const int n = blockIdx.x * 8 + e, per = (k.tiles_v + 31) / 32;
+  Stat s{-INFINITY, 0.f, 0.f, k.V};
+  if (n < k.N) s = row_join(k, part, n, run * per, min(k.tiles_v, (run + 1) * per));
   sm[run][e] = s;
   __syncthreads();
 #pragma unroll
@@ -299,91 +327,85 @@ __global__ __launch_bounds__(256) void ce_join_kernel(const float4* __restrict__
     }
     __syncthreads();
   }
-  if (run == 0 && n < N) {
+  if (run == 0 && n < k.N) {
     stat_join(s, sm[1][e]);
-    const float l = (s.m == -INFINITY ? 0.f : s.m) + log2f(s.s);
-    lse[n] = l;
-    const int64_t t = target[n];
-    float loss = 0.f;
-    if (t != ignore) {
-      if (t < 0 || t >= V) loss = NAN;
-      else {
-        const float d = l - zt[n];
-        loss = LN2 * (smooth > 0.f ? (1.f - smooth) * d + smooth * (l - s.z / (float)V) : d);
-      }
-    }
-    rowloss[n] = loss;
-    if (pred) pred[n] = s.arg < V ? s.arg : 0;
+    row_out(k, n, s);
   }
 }
 
 // loss (nullable) = sum of the row losses (mean: divided by the counted rows, or by 1 if there are none), total[0] = that
 // count; correct (nullable) = counted rows whose arg-max is the target.  One block.
-__global__ __launch_bounds__(1024) void ce_total_kernel(const float* __restrict__ rowloss, const int64_t* __restrict__ target,
-                                                        const int64_t* __restrict__ pred, int64_t ignore, int N, int mean,
+// JOIN: the rows' statistics have not been joined yet (few rows and tiles: one launch instead of two).
+template <bool JOIN>
+__global__ __launch_bounds__(1024) void ce_total_kernel(CeRows k, const float4* __restrict__ part, int mean,
                                                         float* __restrict__ loss, float* __restrict__ total,
                                                         int* __restrict__ correct) {
   __shared__ double sd[16];
   __shared__ int sc[16], sk[16];
   double a = 0.0;
-  int c = 0, k = 0;
-  for (int n = threadIdx.x; n < N; n += 1024) {
-    const int64_t t = target[n];
-    if (t != ignore) {
-      a += (double)rowloss[n];
+  int c = 0, hits = 0;
+  for (int n = threadIdx.x; n < k.N; n += 1024) {
+    const float l = JOIN ? row_out(k, n, row_join(k, part, n, 0, k.tiles_v)) : k.rowloss[n];
+    const int64_t t = k.target[n];
+    if (t != k.ignore) {
+      a += (double)l;
       ++c;
-      if (pred && pred[n] == t) ++k;
+      if (k.pred && k.pred[n] == t) ++hits;
     }
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     a += __shfl_xor(a, o, 64);
     c += __shfl_xor(c, o, 64);
-    k += __shfl_xor(k, o, 64);
+    hits += __shfl_xor(hits, o, 64);
   }
   if ((threadIdx.x & 63) == 0) {
     sd[threadIdx.x >> 6] = a;
     sc[threadIdx.x >> 6] = c;
-    sk[threadIdx.x >> 6] = k;
+    sk[threadIdx.x >> 6] = hits;
   }
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int i = 1; i < 16; ++i) {
       a += sd[i];
       c += sc[i];
-      k += sk[i];
+      hits += sk[i];
     }
     if (loss) *loss = (float)(mean ? a / (double)max(c, 1) : a);
     total[0] = (float)c;
-    if (correct) *correct = k;
+    if (correct) *correct = hits;
   }
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------------
-// rs[n] = weight of row n relative to the largest one (0 for ignored rows), fac[0] = that largest weight.
-// per_row: g[N], else g[0] (divided by the counted rows for the mean).
-__global__ __launch_bounds__(1024) void ce_weights_kernel(const float* __restrict__ g, const float* __restrict__ total,
-                                                          const int64_t* __restrict__ target, int64_t ignore, int N,
-                                                          int mean, int per_row, float* __restrict__ rs,
+// Per-row upstream gradients: rs[n] = weight of row n relative to the largest one (0 for ignored rows), fac[0] = that largest
+// weight.
+__global__ __launch_bounds__(1024) void ce_weights_kernel(const float* __restrict__ g, const int64_t* __restrict__ target,
+                                                          int64_t ignore, int N, float* __restrict__ rs,
                                                           float* __restrict__ fac) {
   __shared__ float sm[16];
-  float big = 1.f;
-  if (per_row) {
-    big = 0.f;
-    for (int n = threadIdx.x; n < N; n += 1024)
-      if (target[n] != ignore) big = fmaxf(big, finite_mag(g[n]));
-    big = wave_max(big);
-    if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = big;
-    __syncthreads();
-    big = sm[0];
-    for (int i = 1; i < 16; ++i) big = fmaxf(big, sm[i]);
-    if (!(big > 0.f)) big = 1.f;
-  }
-  for (int n = threadIdx.x; n < N; n += 1024) rs[n] = target[n] == ignore ? 0.f : per_row ? g[n] / big : 1.f;
-  if (threadIdx.x == 0) fac[0] = per_row ? big : mean ? g[0] / fmaxf(total[0], 1.f) : g[0];
+  float big = 0.f;
+  for (int n = threadIdx.x; n < N; n += 1024)
+    if (target[n] != ignore) big = fmaxf(big, finite_mag(g[n]));
+  big = wave_max(big);
+  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = big;
+  __syncthreads();
+  big = sm[0];
+  for (int i = 1; i < 16; ++i) big = fmaxf(big, sm[i]);
+  if (!(big > 0.f)) big = 1.f;
+  for (int n = threadIdx.x; n < N; n += 1024) rs[n] = target[n] == ignore ? 0.f : g[n] / big;
+  if (threadIdx.x == 0) fac[0] = big;
 }
 
 constexpr float D_SCALE = 32768.f;  // of d's fp16 terms, and of dbpart
+
+// The largest row weight: what ce_weights_kernel found, or for a mean or sum the upstream gradient itself.
+struct CeFac {
+  const float* fac;    // per-row weights
+  const float* g;      // else the one gradient,
+  const float* total;  // of a mean (the counted rows) or, null, of a sum
+  __device__ __forceinline__ float get() const { return fac ? fac[0] : total ? g[0] / fmaxf(total[0], 1.f) : g[0]; }
+};
 
 __device__ __forceinline__ float row16_sum(float v) {  // over the 16 lanes of a DPP row
   v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, true));
@@ -393,13 +415,18 @@ __device__ __forceinline__ float row16_sum(float v) {  // over the 16 lanes of a
   return v;
 }
 
+template <typename T>
+__device__ __forceinline__ void bias_out(T* db, float s, const CeFac& fac, int add) {
+  *db = from_f32<T>((add ? to_f32(*db) : 0.f) + s * (fac.get() / D_SCALE));
+}
+
 // One 128 x 128 tile of d for the classes [vbeg, vbeg + vcols), as dn[n][vcols] in PD terms scaled by 2^15, and its column
-// sums dbpart[tile n][v].
+// sums dbpart[tile n][v] (db itself where there is one row tile).
 template <int PW, int PX, int PD, int NS>
 __global__ __launch_bounds__(G_THREADS, NS == 2 ? 2 : 1) void ce_grad_kernel(CeArgs a, const float* __restrict__ lse,
                                                                const float* __restrict__ rs, float smooth, int vbeg,
                                                                int vcols, f16* __restrict__ dn,
-                                                               float* __restrict__ dbpart) {
+                                                               float* __restrict__ dbpart, CeFac fac, void* db, int add) {
   __shared__ __attribute__((aligned(1024))) f16 smem[G16<PW, PX, ROW, ROW, NS>::LDS];
   __shared__ float sb[2][GM];
   int tv, tn;
@@ -420,7 +447,7 @@ __global__ __launch_bounds__(G_THREADS, NS == 2 ? 2 : 1) void ce_grad_kernel(CeA
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int n = n0 + wn * 64 + j * 16 + l15;
-    const float w = n < a.N ? rs[n] : 0.f;
+    const float w = n >= a.N ? 0.f : rs ? rs[n] : a.target[n] == a.ignore ? 0.f : 1.f;
     const int t = row_target(a, n);
     float l = w != 0.f ? lse[n] - 15.f : 0.f;  // 2^(z - l) is the scaled probability
     if (w != 0.f && (t < 0 || t >= a.V)) l = NAN;
@@ -476,21 +503,26 @@ __global__ __launch_bounds__(G_THREADS, NS == 2 ? 2 : 1) void ce_grad_kernel(CeA
         if (l15 == 0) sb[wn][wm * 64 + i * 16 + q * 4 + r] = s;
       }
     __syncthreads();
-    if (threadIdx.x < GM && v0 + (int)threadIdx.x < a.V)
-      dbpart[(int64_t)tn * a.V + v0 + threadIdx.x] = sb[0][threadIdx.x] + sb[1][threadIdx.x];
+    const int v = v0 + threadIdx.x;
+    if (threadIdx.x < GM && v < a.V) {
+      const float s = sb[0][threadIdx.x] + sb[1][threadIdx.x];
+      if (a.tiles_n > 1) dbpart[(int64_t)tn * a.V + v] = s;
+      else if (a.bias_bf16) bias_out((bf16*)db + v, s, fac, add);  // the only row tile
+      else bias_out((float*)db + v, s, fac, add);
+    }
   }
 }
 
 // db[v] (+)= fac sum over the row tiles of dbpart[tile][v]
 template <typename T>
 __global__ __launch_bounds__(256) void ce_bias_kernel(const float* __restrict__ dbpart, int tiles, int V,
-                                                      const float* __restrict__ fac, int add, T* __restrict__ db) {
+                                                      CeFac fac, int add, T* __restrict__ db) {
   const int v = blockIdx.x * 256 + threadIdx.x;
   if (v >= V) return;
   float s = 0.f;
 #pragma unroll 4
   for (int t = 0; t < tiles; ++t) s += dbpart[(int64_t)t * V + v];
-  db[v] = from_f32<T>((add ? to_f32(db[v]) : 0.f) + s * (fac[0] / D_SCALE));
+  bias_out(db + v, s, fac, add);
 }
 
 // out[m][c] = factor * sum over the reduction of (row side)[m] (column side)[c]: dx = d W and dW = d^T x
@@ -501,14 +533,14 @@ struct MmArgs {
   float* part;                 // [splits][M][Nn], or null: write out
   int add;                     // add to what part / out hold
   void* out;                   // [M][Nn]
-  const float* fac;
+  CeFac fac;
   const int* exps;
   int which;                   // whose scale exponent the column side carries
   int vec;                     // rows of the result start on 16-byte (fp32) / 8-byte (bf16) boundaries
 };
 
-__device__ __forceinline__ float mm_factor(const float* fac, const int* exps, int which) {
-  return ldexpf(fac[0], -15 - exps[which]);
+__device__ __forceinline__ float mm_factor(const CeFac& fac, const int* exps, int which) {
+  return ldexpf(fac.get(), -15 - exps[which]);
 }
 
 template <int PC, int PM, int KM, int NS, typename T>
@@ -589,8 +621,7 @@ __global__ __launch_bounds__(G_THREADS, NS == 2 ? 2 : 1) void ce_mm_kernel(MmArg
 // out (+)= factor * sum over the slices, in order
 template <typename T>
 __global__ __launch_bounds__(256) void ce_reduce_kernel(const float* __restrict__ part, int slices, int64_t n,
-                                                        const float* __restrict__ fac, const int* __restrict__ exps,
-                                                        int which, int add, T* __restrict__ out) {
+                                                        CeFac fac, const int* __restrict__ exps, int which, int add, T* __restrict__ out) {
   const float f = mm_factor(fac, exps, which);
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
     float s = 0.f;
@@ -739,11 +770,13 @@ void stats_go(const CeArgs& a, bool more, float4* part, float* zt, hipStream_t s
 }
 template <int PW, int PX, int PD>
 void grad_go(const CeArgs& a, const float* lse, const float* rs, float smooth, int vbeg, int vcols, f16* dn, float* dbp,
-             hipStream_t st) {
+             const CeFac& fac, void* db, int add, hipStream_t st) {
   const dim3 grid(a.tiles_v * a.tiles_n), blk(G_THREADS);
   if (deep(grid.x))
-    hipLaunchKernelGGL((ce_grad_kernel<PW, PX, PD, 4>), grid, blk, 0, st, a, lse, rs, smooth, vbeg, vcols, dn, dbp);
-  else hipLaunchKernelGGL((ce_grad_kernel<PW, PX, PD, 2>), grid, blk, 0, st, a, lse, rs, smooth, vbeg, vcols, dn, dbp);
+    hipLaunchKernelGGL((ce_grad_kernel<PW, PX, PD, 4>), grid, blk, 0, st, a, lse, rs, smooth, vbeg, vcols, dn, dbp,
+                       fac, db, add);
+  else hipLaunchKernelGGL((ce_grad_kernel<PW, PX, PD, 2>), grid, blk, 0, st, a, lse, rs, smooth, vbeg, vcols, dn, dbp,
+                       fac, db, add);
 }
 template <int KM>
 void mm_terms(int pc, int pm, const MmArgs& g, int out_bf16, hipStream_t st) {
@@ -751,7 +784,7 @@ void mm_terms(int pc, int pm, const MmArgs& g, int out_bf16, hipStream_t st) {
   else if (pc == 1) mm_go<1, 2, KM>(g, out_bf16, st);
   else mm_go<2, 2, KM>(g, out_bf16, st);
 }
-void reduce_go(const float* part, int slices, int64_t n, const float* fac, const int* exps, int which, int add, void* out,
+void reduce_go(const float* part, int slices, int64_t n, const CeFac& fac, const int* exps, int which, int add, void* out,
                int out_bf16, hipStream_t st) {
   const int grid = (int)(ceil_div64(n, 256) < 4096 ? ceil_div64(n, 256) : 4096);
   if (out_bf16)
@@ -783,17 +816,21 @@ int vc_linear_ce_fwd(int xdtype, int wdtype, const void* x, const void* w, const
   if (xdtype == VC_F32) pack_go<float, float>(p, x, w, N, V, K, target, ignore_index, sv, ws, stream);
   else if (wdtype == VC_F32) pack_go<bf16, float>(p, x, w, N, V, K, target, ignore_index, sv, ws, stream);
   else pack_go<bf16, bf16>(p, x, w, N, V, K, target, ignore_index, sv, ws, stream);
-  CeArgs a{(const f16*)(sv + p.o_wp), (const f16*)(sv + p.o_xp), bias, target, (const int*)(sv + p.o_exps), N, V, p.ld,
+  CeArgs a{(const f16*)(sv + p.o_wp), (const f16*)(sv + p.o_xp), bias, target, ignore_index, (const int*)(sv + p.o_exps), N, V, p.ld,
            wdtype == VC_BF16, ceil_div(V, GM), ceil_div(N, GM)};
   float4* part = (float4*)(ws + p.f_part);
   float* zt = (float*)(ws + p.f_zt);
   const bool more = smoothing > 0.f || pred;
   if (p.pw == 2) stats_go<2, 2>(a, more, part, zt, stream);
   else stats_go<1, 1>(a, more, part, zt, stream);
-  hipLaunchKernelGGL(ce_join_kernel, dim3(ceil_div(N, 8)), dim3(256), 0, stream, part, zt, target, ignore_index, N, V,
-                     a.tiles_v, smoothing, (float*)(sv + p.o_lse), row_loss, pred);
-  hipLaunchKernelGGL(ce_total_kernel, dim3(1), dim3(1024), 0, stream, row_loss, target, pred, ignore_index, N, mean, loss,
-                     (float*)(sv + p.o_total), correct);
+  const CeRows rows{zt, target, ignore_index, N, V, a.tiles_v, smoothing, (float*)(sv + p.o_lse), row_loss, pred};
+  float* total = (float*)(sv + p.o_total);
+  if (N <= 1024 && a.tiles_v <= 16) {
+    hipLaunchKernelGGL(ce_total_kernel<true>, dim3(1), dim3(1024), 0, stream, rows, part, mean, loss, total, correct);
+  } else {
+    hipLaunchKernelGGL(ce_join_kernel, dim3(ceil_div(N, 8)), dim3(256), 0, stream, rows, part);
+    hipLaunchKernelGGL(ce_total_kernel<false>, dim3(1), dim3(1024), 0, stream, rows, part, mean, loss, total, correct);
+  }
   VC_LAUNCH_CHECK("vc_linear_ce_fwd");
   return VC_OK;
 }
@@ -814,18 +851,19 @@ int vc_linear_ce_bwd(int xdtype, int wdtype, const void* bias, const int64_t* ta
   f16* dn = (f16*)(ws + p.b_dn);
   const int* exps = (const int*)(sv + p.o_exps);
   const float* lse = (const float*)(sv + p.o_lse);
-  float *rs = (float*)(ws + p.b_rs), *fac = (float*)(ws + p.b_fac), *dbp = (float*)(ws + p.b_db);
+  float *rs = (float*)(ws + p.b_rs), *big = (float*)(ws + p.b_fac), *dbp = (float*)(ws + p.b_db);
+  const CeFac fac{per_row ? big : nullptr, dloss, mean ? (const float*)(sv + p.o_total) : nullptr};
   const int tn = ceil_div(N, GM), tk = ceil_div(K, GM);
-  hipLaunchKernelGGL(ce_weights_kernel, dim3(1), dim3(1024), 0, stream, dloss, (const float*)(sv + p.o_total), target,
-                     ignore_index, N, mean, per_row, rs, fac);
+  if (per_row) hipLaunchKernelGGL(ce_weights_kernel, dim3(1), dim3(1024), 0, stream, dloss, target, ignore_index, N, rs, big);
+  else rs = nullptr;
   for (int c = 0; c < p.pieces; ++c) {
     const int vbeg = c * p.piece;
     const int vcols = p.piece < ceil_div(V - vbeg, GM) * GM ? p.piece : ceil_div(V - vbeg, GM) * GM;
-    CeArgs a{wp, xp, bias, target, exps, N, V, p.ld, wdtype == VC_BF16, vcols / GM, tn};
+    CeArgs a{wp, xp, bias, target, ignore_index, exps, N, V, p.ld, wdtype == VC_BF16, vcols / GM, tn};
     float* dbq = db ? dbp : nullptr;
-    if (p.pw == 2) grad_go<2, 2, 2>(a, lse, rs, smoothing, vbeg, vcols, dn, dbq, stream);
-    else if (p.pd == 2) grad_go<1, 1, 2>(a, lse, rs, smoothing, vbeg, vcols, dn, dbq, stream);
-    else grad_go<1, 1, 1>(a, lse, rs, smoothing, vbeg, vcols, dn, dbq, stream);
+    if (p.pw == 2) grad_go<2, 2, 2>(a, lse, rs, smoothing, vbeg, vcols, dn, dbq, fac, db, accumulate & 2, stream);
+    else if (p.pd == 2) grad_go<1, 1, 2>(a, lse, rs, smoothing, vbeg, vcols, dn, dbq, fac, db, accumulate & 2, stream);
+    else grad_go<1, 1, 1>(a, lse, rs, smoothing, vbeg, vcols, dn, dbq, fac, db, accumulate & 2, stream);
     const int rows = vcols < V - vbeg ? vcols : V - vbeg;
     MmArgs g{};
     g.Nn = K;
@@ -867,7 +905,7 @@ int vc_linear_ce_bwd(int xdtype, int wdtype, const void* bias, const int64_t* ta
   }
   if (dx && p.b_px >= 0)
     reduce_go((const float*)(ws + p.b_px), p.sx, (int64_t)N * K, fac, exps, 1, 0, dx, xdtype == VC_BF16, stream);
-  if (db) {
+  if (db && tn > 1) {
     if (wdtype == VC_BF16)
       hipLaunchKernelGGL((ce_bias_kernel<bf16>), dim3(ceil_div(V, 256)), dim3(256), 0, stream, dbp, tn, V, fac,
                          accumulate & 2, (bf16*)db);

@@ -469,7 +469,7 @@ __global__ __launch_bounds__(256) void ns_copy_kernel(const NsMat* __restrict__ 
 // Matrices of at most 16 rows (columns, if tall): all steps in one workgroup, X in LDS, in fp64 where it fits twice and
 // fp32 otherwise.  A 128 x 128 product tile would be nine tenths padding, and a matrix this small has nothing to average
 // the two-term rounding over: its result was off by up to five times fp32's error.  One workgroup's time grows with
-// m^2 n (12 x 199 in 49 us, 16 x 2200 in 230, against about 110 for the launches of the tiled form), hence the third bound.
+// m^2 n (12 x 199 in 49 us; 16 x 2200 in 230 against 173 for the launches of the tiled form), hence the third bound.
 constexpr int SMALL_ROWS = 16, SMALL_ELEMS = 36000, SMALL_THREADS = 512, SMALL_MAX = 96;
 struct NsSmall {
   const void* g;

@@ -1779,12 +1779,13 @@ def _put_grad(p, g):
 
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, residual, anchor, gn, act):
-        N, C, G = x.shape[0], x.shape[-1], gn.num_groups
+    def forward(ctx, x, residual, anchor, params, G, eps, act):
+        weight, bias = params  # in a tuple, so that autograd does not see them
+        N, C = x.shape[0], x.shape[-1]
         S = x.numel() // (N * C)
         x = x.contiguous()
         res = residual.contiguous() if residual is not None else None
-        weight, bias, dev = gn.weight, gn.bias, x.device
+        dev = x.device
         gamma, beta = _f32_param("group_norm", weight), _f32_param("group_norm", bias)
         code, ws_floats = L.dtype_code(x.dtype), _size("vc_group_norm_workspace_floats", N, S, C, G)
         y = torch.empty_like(x)
@@ -1792,8 +1793,8 @@ class _GroupNorm(torch.autograd.Function):
         ws = torch.empty(ws_floats, device=dev, dtype=torch.float32)
         mean = stat.data_ptr()
         L.fast("vc_group_norm_fwd", dev, code, x.data_ptr(), _addr(res), _addr(gamma), _addr(beta), y.data_ptr(), mean,
-               mean + 4 * N * G, ws.data_ptr(), N, S, C, G, gn.eps, act)
-        ctx.dims, ctx.act, ctx.params, ctx.code, ctx.ws_floats = (N, S, C, G), act, (weight, bias), code, ws_floats
+               mean + 4 * N * G, ws.data_ptr(), N, S, C, G, eps, act)
+        ctx.dims, ctx.act, ctx.params, ctx.code, ctx.ws_floats = (N, S, C, G), act, params, code, ws_floats
         ctx.save_for_backward(x, res if act else None, stat, gamma, beta)
         return y
 
@@ -1820,7 +1821,7 @@ class _GroupNorm(torch.autograd.Function):
             _put_grad(weight, dw)
             _put_grad(bias, db)
         _ready(weight, bias)
-        return dx, dres, None, None, None
+        return dx, dres, None, None, None, None, None
 
 
 def group_norm(x, gn, act="none", residual=None):
@@ -1838,12 +1839,14 @@ def group_norm(x, gn, act="none", residual=None):
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise RuntimeError(f"group_norm: residual {tuple(residual.shape)} {residual.dtype} does not match the input "
                            f"{tuple(x.shape)} {x.dtype}")
-    _same_device("group_norm", x, residual, gn.weight, gn.bias)
+    weight, bias = gn.weight, gn.bias
+    _same_device("group_norm", x, residual, weight, bias)
     if x.numel() == 0:
         return x.clone()
     with _on(x.device):
         _leaf_guard("group_norm", x, residual)
-        return _GroupNorm.apply(x, residual, _anchor((x, residual), (gn.weight, gn.bias)), gn, GN_ACTS[act])
+        return _GroupNorm.apply(x, residual, _anchor((x, residual), (weight, bias)), (weight, bias), gn.num_groups, gn.eps,
+                                GN_ACTS[act])
 
 
 class _LayerNormFork(torch.autograd.Function):
