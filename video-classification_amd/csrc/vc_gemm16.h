@@ -10,12 +10,11 @@
 // with the transposing ds_read_b64_tr_b16, so no operand is ever copied into the other order).  The second term lies one
 // `plane` behind the first.
 //
-// Four waves in a 2 x 2 grid own 64 x 64 each.  NS LDS stages of (PA + PB) x 128 x BK elements (BK = 64 for single terms,
-// 32 otherwise: at most 32 KiB a stage).  Two stages let two workgroups share a CU and hide each other's waits; a launch
-// with at most one workgroup per CU takes four, which keeps three k-steps on their way instead of one.  ROW stages permute the 16-byte chunks of a row so
-// that the 16 rows of a fragment read fall into 16 different slots of the 256-byte bank row; COL stages permute the
-// 32-byte blocks of a row so that the eight rows of a transposing read fall on different groups of banks.  Stages are
-// filled by LDS-DMA requests in opaque assembly (with the builtin the compiler waits for every outstanding request
+// Four waves in a 2 x 2 grid own 64 x 64 each.  Two LDS stages of (PA + PB) x 128 x BK elements (BK = 64 for single terms,
+// 32 otherwise: at most 32 KiB a stage), so that two workgroups share a CU.  ROW stages permute the 16-byte chunks of a
+// row so that the 16 rows of a fragment read fall into 16 different slots of the 256-byte bank row; COL stages permute
+// the 32-byte blocks of a row so that the eight rows of a transposing read fall on different groups of banks.  Stages
+// are filled by LDS-DMA requests in opaque assembly (with the builtin the compiler waits for every outstanding request
 // before each LDS read); what lies behind the operand's last row falls outside its buffer descriptor and reads as zero.
 #pragma once
 #include "vc_common.h"
@@ -66,18 +65,23 @@ __device__ __forceinline__ void f16_split(float v, f16& hi, f16& lo) {
   lo = (f16)(v - (float)hi);
 }
 
-template <int PA, int PB, int KA = ROW, int KB = ROW, int NS = 2, int BK_ = 0>
+template <int PA, int PB, int KA = ROW, int KB = ROW>
 struct G16 {
-  static constexpr int BK = BK_ ? BK_ : PA + PB == 2 ? 64 : 32;
+  static constexpr int BK = PA + PB == 2 ? 64 : 32;
   static constexpr int PLANE = GM * BK;              // elements of one plane of a stage
   static constexpr int STAGE = (PA + PB) * PLANE;
-  static constexpr int LDS = NS * STAGE;             // elements of shared memory
+  static constexpr int LDS = 2 * STAGE;              // elements of shared memory
   static constexpr int CH = BK / 8;                  // 16-byte chunks of a ROW stage's row
   static constexpr int RPI = 64 / CH;                // rows of it that one wave request fills
   static constexpr int REQ = BK / 16;                // requests per wave, plane and stage (1 KiB each)
   static constexpr int PER = (PA + PB) * REQ;        // requests per wave and stage
 
-  __device__ static __forceinline__ int rswz(int row) { return BK == 64 ? (row >> 1) & 7 : (row >> 2) & 3; }
+  // A 16-byte read is served 16 lanes at a time, lanes 0-3, 12-15, 20-27 and 4-11, 16-19, 28-31 of each half of the wave: with
+  // 64-byte rows (BK = 32) the four groups of four rows need 0, 2, 3, 1 for both sets to meet 16 different slots (0, 1, 2, 3
+  // left a third to a half of the LDS cycles to conflicts).
+  __device__ static __forceinline__ int rswz(int row) {
+    return BK == 64 ? (row >> 1) & 7 : (((row >> 2) & 1) << 1) ^ (((row >> 3) & 1) * 3);
+  }
   __device__ static __forceinline__ int cswz(int row) { return (row & 3) | ((row >> 1) & 4); }
 
   // byte offset of this lane's 16 bytes of request t, relative to the tile's corner of the k-step
@@ -129,14 +133,13 @@ struct G16 {
     }
   };
 
-  // fragment of the 16 tile rows (ROW) or columns (COL) of block `blk` (0..7), 32 reduction elements from kk * 32
+  // Fragment of the 16 tile rows (ROW) or columns (COL) of block `blk` (0..7), 32 reduction elements from kk * 32.  The swizzles
+  // are those of the row within its block: adding a block does not change them.
   template <int KIND>
   __device__ static __forceinline__ f16x8 frag(const f16* st, int blk, int kk, int lane) {
     const int l15 = lane & 15, q = lane >> 4;
-    if (KIND == ROW) {
-      const int row = blk * 16 + l15;
-      return *reinterpret_cast<const f16x8*>(st + row * BK + (((kk * 4 + q) ^ rswz(row)) << 3));
-    }
+    if (KIND == ROW)
+      return *reinterpret_cast<const f16x8*>(st + (blk * 16 + l15) * BK + (((kk * 4 + q) ^ rswz(l15)) << 3));
     typedef short s16x4_t __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) s16x4_t lds4;
     const int r0 = 8 * q + ((lane >> 2) & 3);  // this lane supplies row r0, columns 4 (lane & 3) .. + 3, then row r0 + 4
@@ -152,6 +155,11 @@ struct G16 {
 
   // acc[i][j][r] += sum over k in [k0, k1) of A's tile row wm*64 + i*16 + (lane>>4)*4 + r and B's tile row wn*64 + j*16 +
   // (lane&15).  k0, k1 multiples of BK.  The LDS is free again for the caller when the function returns.
+  //
+  // A k-step is two phases: single terms its two 32-deep halves, two terms the product of the first terms and then the mixed
+  // ones.  While a phase multiplies out of registers the next phase's fragments are read, one read behind every second
+  // product, so no product waits for LDS.  The barrier lies between the phases: by then every wave has read all of the
+  // stage, which takes the k-step after next, and has waited for its own requests of the next one.
   __device__ static __forceinline__ void run(f32x4 (&acc)[4][4], const Op16& a, const Op16& b, int k0, int k1, f16* smem) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -164,6 +172,7 @@ struct G16 {
     }
     k0 = __builtin_amdgcn_readfirstlane(k0);
     k1 = __builtin_amdgcn_readfirstlane(k1);
+    if (k0 >= k1) return;
     Stream<KA> sa[PA];
     Stream<KB> sb[PB];
 #pragma unroll
@@ -177,39 +186,58 @@ struct G16 {
 #pragma unroll
       for (int p = 0; p < PB; ++p) sb[p].stage(base + (PA + p) * PLANE * 2, vb, k);
     };
-    int s = 0;  // the stage that is multiplied; the next NS - 1 k-steps are on their way into the others
+    constexpr bool ONE = PA + PB == 2;  // phase 2: the second half, or the second terms
+    f16x8 a1[4], b1[4], a2[4], b2[4];
+    // fragment r of a phase: 0..3 A's (where the phase has its own), 4..7 B's
+    auto read1 = [&](const f16* st, int r, f16x8(&fa)[4], f16x8(&fb)[4]) __attribute__((always_inline)) {
+      if (r < 4) fa[r] = frag<KA>(st, wm * 4 + r, 0, lane);
+      else fb[r - 4] = frag<KB>(st + PA * PLANE, wn * 4 + r - 4, 0, lane);
+    };
+    auto read2 = [&](const f16* st, int r) __attribute__((always_inline)) {
+      if (r < 4) {
+        if (ONE) a2[r] = frag<KA>(st, wm * 4 + r, 1, lane);
+        else if (PA == 2) a2[r] = frag<KA>(st + PLANE, wm * 4 + r, 0, lane);
+      } else if (ONE) b2[r - 4] = frag<KB>(st + PA * PLANE, wn * 4 + r - 4, 1, lane);
+      else if (PB == 2) b2[r - 4] = frag<KB>(st + (PA + 1) * PLANE, wn * 4 + r - 4, 0, lane);
+    };
+    stage(0, k0);
+    if (k0 + BK < k1) {
+      stage(1, k0 + BK);
+      asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(PER) : "memory");
+    } else
+      asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
-    for (int d = 0; d < NS - 1; ++d)
-      if (k0 + d * BK < k1) stage(d, k0 + d * BK);
-    for (int k = k0; k < k1; k += BK, s = s + 1 == NS ? 0 : s + 1) {
-      // this wave's requests of stage s have landed (the younger ones of NS - 2 stages may be outstanding) and its reads
-      // are done; behind the barrier so are the others', and nobody reads the stage before any more
-      if (NS > 2 && k + (NS - 2) * BK < k1)
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * PER) : "memory");
-      else
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (k + (NS - 1) * BK < k1) stage(s == 0 ? NS - 1 : s - 1, k + (NS - 1) * BK);
-      const f16* st = smem + s * STAGE;
+    for (int r = 0; r < 8; ++r) read1(smem, r, a1, b1);
+    int s = 0;
+    for (int k = k0; k < k1; k += BK, s ^= 1) {
+      const f16 *st = smem + s * STAGE, *sn = smem + (s ^ 1) * STAGE;
 #pragma unroll
-      for (int kk = 0; kk < BK / 32; ++kk) {
-        f16x8 fa[PA][4], fb[PB][4];
+      for (int n = 0; n < 16; ++n) {
+        const int i = n >> 2, j = n & 3;
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1[i], b1[j], acc[i][j], 0, 0, 0);
+        if ((n & 1) == 0) read2(st, n >> 1);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (k + 2 * BK < k1) stage(s, k + 2 * BK);
+      // behind the last k-step the reads below meet stale LDS, which is never multiplied
+      f16x8 an[4], bn[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+      for (int n = 0; n < 16; ++n) {
+        const int i = n >> 2, j = n & 3;
+        if (ONE) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a2[i], b2[j], acc[i][j], 0, 0, 0);
+        else if (PB == 2) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1[i], b2[j], acc[i][j], 0, 0, 0);
+        if ((n & 1) == 0) read1(sn, n >> 1, an, bn);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (!ONE && PA == 2)
 #pragma unroll
-          for (int p = 0; p < PA; ++p) fa[p][i] = frag<KA>(st + p * PLANE, wm * 4 + i, kk, lane);
+        for (int n = 0; n < 16; ++n)
+          acc[n >> 2][n & 3] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a2[n >> 2], b1[n & 3], acc[n >> 2][n & 3], 0, 0, 0);
 #pragma unroll
-          for (int p = 0; p < PB; ++p) fb[p][i] = frag<KB>(st + (PA + p) * PLANE, wn * 4 + i, kk, lane);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[0][i], fb[0][j], acc[i][j], 0, 0, 0);
-            if constexpr (PB == 2)
-              acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[0][i], fb[1][j], acc[i][j], 0, 0, 0);
-            if constexpr (PA == 2)
-              acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[1][i], fb[0][j], acc[i][j], 0, 0, 0);
-          }
+      for (int r = 0; r < 4; ++r) {
+        a1[r] = an[r];
+        b1[r] = bn[r];
       }
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");

@@ -151,10 +151,10 @@ struct CeArgs {
 };
 
 // acc = z log2(e) without the bias, which follows in `bias` (-inf behind the last class): rows v0 + .., columns n0 + ..
-template <int PW, int PX, int NS>
+template <int PW, int PX>
 __device__ __forceinline__ void logit_tile(const CeArgs& a, int v0, int n0, f16* smem, f32x4 (&acc)[4][4],
                                            float (&bias)[4][4], float& scale) {
-  typedef G16<PW, PX, ROW, ROW, NS> G;
+  typedef G16<PW, PX> G;
   G::zero(acc);
   G::run(acc, Op16{a.w + (int64_t)v0 * a.ld, (int64_t)a.V * a.ld, a.ld, a.V - v0, 0},
          Op16{a.x + (int64_t)n0 * a.ld, (int64_t)a.N * a.ld, a.ld, a.N - n0, 0}, 0, a.ld, smem);
@@ -209,16 +209,16 @@ __device__ __forceinline__ Stat stat_shfl(const Stat& a, int o) {
 
 // part[vt][n] = (max, sum, sum z, arg) of the tile, zt[n] = the target's logit.  MORE: also sum z and arg (label smoothing,
 // predictions), which cost four operations more per logit.
-template <int PW, int PX, bool MORE, int NS>
-__global__ __launch_bounds__(G_THREADS, NS == 2 ? 2 : 1) void ce_stats_kernel(CeArgs a, float4* __restrict__ part,
+template <int PW, int PX, bool MORE>
+__global__ __launch_bounds__(G_THREADS, 2) void ce_stats_kernel(CeArgs a, float4* __restrict__ part,
                                                                 float* __restrict__ zt) {
-  __shared__ __attribute__((aligned(1024))) f16 smem[G16<PW, PX, ROW, ROW, NS>::LDS];
+  __shared__ __attribute__((aligned(1024))) f16 smem[G16<PW, PX>::LDS];
   int tv, tn;
   g16_tile(blockIdx.x, gridDim.x, a.tiles_v, a.tiles_n, tv, tn);
   const int v0 = tv * GM, n0 = tn * GM;
   f32x4 acc[4][4];
   float bias[4][4], scale;
-  logit_tile<PW, PX, NS>(a, v0, n0, smem, acc, bias, scale);
+  logit_tile<PW, PX>(a, v0, n0, smem, acc, bias, scale);
   const int lane = threadIdx.x & 63, q = lane >> 4, l15 = lane & 15;
   const int wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
   float4* xch = reinterpret_cast<float4*>(smem);
@@ -422,19 +422,19 @@ __device__ __forceinline__ void bias_out(T* db, float s, const CeFac& fac, int a
 
 // One 128 x 128 tile of d for the classes [vbeg, vbeg + vcols), as dn[n][vcols] in PD terms scaled by 2^15, and its column
 // sums dbpart[tile n][v] (db itself where there is one row tile).
-template <int PW, int PX, int PD, int NS>
-__global__ __launch_bounds__(G_THREADS, NS == 2 ? 2 : 1) void ce_grad_kernel(CeArgs a, const float* __restrict__ lse,
+template <int PW, int PX, int PD>
+__global__ __launch_bounds__(G_THREADS, 2) void ce_grad_kernel(CeArgs a, const float* __restrict__ lse,
                                                                const float* __restrict__ rs, float smooth, int vbeg,
                                                                int vcols, f16* __restrict__ dn,
                                                                float* __restrict__ dbpart, CeFac fac, void* db, int add) {
-  __shared__ __attribute__((aligned(1024))) f16 smem[G16<PW, PX, ROW, ROW, NS>::LDS];
+  __shared__ __attribute__((aligned(1024))) f16 smem[G16<PW, PX>::LDS];
   __shared__ float sb[2][GM];
   int tv, tn;
   g16_tile(blockIdx.x, gridDim.x, a.tiles_v, a.tiles_n, tv, tn);
   const int v0 = vbeg + tv * GM, n0 = tn * GM;
   f32x4 acc[4][4];
   float bias[4][4], scale;
-  logit_tile<PW, PX, NS>(a, v0, n0, smem, acc, bias, scale);
+  logit_tile<PW, PX>(a, v0, n0, smem, acc, bias, scale);
   const int lane = threadIdx.x & 63, q = lane >> 4, l15 = lane & 15;
   const int wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
   const float each = smooth / (float)a.V * D_SCALE;
@@ -543,9 +543,9 @@ __device__ __forceinline__ float mm_factor(const CeFac& fac, const int* exps, in
   return ldexpf(fac.get(), -15 - exps[which]);
 }
 
-template <int PC, int PM, int KM, int NS, typename T>
-__global__ __launch_bounds__(G_THREADS, NS == 2 ? 2 : 1) void ce_mm_kernel(MmArgs g) {
-  typedef G16<PC, PM, COL, KM, NS> G;
+template <int PC, int PM, int KM, typename T>
+__global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
+  typedef G16<PC, PM, COL, KM> G;
   __shared__ __attribute__((aligned(1024))) f16 smem[G::LDS];
   const int tiles = g.tiles_m * g.tiles_n;
   const int split = blockIdx.x / tiles;
@@ -742,41 +742,23 @@ void pack_go(const Plan& p, const void* x, const void* w, int N, int V, int K, c
                      (int*)(saved + p.o_exps), xb, xa, wa);
 }
 
-// Launches of at most one workgroup per CU take the four-stage pipeline (G16): 32 rows against 101 classes run in
-// 8 instead of 9 us per product, 1003 x 327 against 10007 in fp32 in 29 instead of 37 us.
-bool deep(int64_t blocks) { return blocks <= vc_device_cus(); }
-
 template <int PC, int PM, int KM>
 void mm_go(const MmArgs& g, int out_bf16, hipStream_t st) {
   const dim3 grid(g.tiles_m * g.tiles_n * g.splits), blk(G_THREADS);
-  if (deep(grid.x)) {
-    if (out_bf16) hipLaunchKernelGGL((ce_mm_kernel<PC, PM, KM, 4, bf16>), grid, blk, 0, st, g);
-    else hipLaunchKernelGGL((ce_mm_kernel<PC, PM, KM, 4, float>), grid, blk, 0, st, g);
-  } else {
-    if (out_bf16) hipLaunchKernelGGL((ce_mm_kernel<PC, PM, KM, 2, bf16>), grid, blk, 0, st, g);
-    else hipLaunchKernelGGL((ce_mm_kernel<PC, PM, KM, 2, float>), grid, blk, 0, st, g);
-  }
+  if (out_bf16) hipLaunchKernelGGL((ce_mm_kernel<PC, PM, KM, bf16>), grid, blk, 0, st, g);
+  else hipLaunchKernelGGL((ce_mm_kernel<PC, PM, KM, float>), grid, blk, 0, st, g);
 }
 template <int PW, int PX>
 void stats_go(const CeArgs& a, bool more, float4* part, float* zt, hipStream_t st) {
   const dim3 grid(a.tiles_v * a.tiles_n), blk(G_THREADS);
-  if (deep(grid.x)) {
-    if (more) hipLaunchKernelGGL((ce_stats_kernel<PW, PX, true, 4>), grid, blk, 0, st, a, part, zt);
-    else hipLaunchKernelGGL((ce_stats_kernel<PW, PX, false, 4>), grid, blk, 0, st, a, part, zt);
-  } else {
-    if (more) hipLaunchKernelGGL((ce_stats_kernel<PW, PX, true, 2>), grid, blk, 0, st, a, part, zt);
-    else hipLaunchKernelGGL((ce_stats_kernel<PW, PX, false, 2>), grid, blk, 0, st, a, part, zt);
-  }
+  if (more) hipLaunchKernelGGL((ce_stats_kernel<PW, PX, true>), grid, blk, 0, st, a, part, zt);
+  else hipLaunchKernelGGL((ce_stats_kernel<PW, PX, false>), grid, blk, 0, st, a, part, zt);
 }
 template <int PW, int PX, int PD>
 void grad_go(const CeArgs& a, const float* lse, const float* rs, float smooth, int vbeg, int vcols, f16* dn, float* dbp,
              const CeFac& fac, void* db, int add, hipStream_t st) {
-  const dim3 grid(a.tiles_v * a.tiles_n), blk(G_THREADS);
-  if (deep(grid.x))
-    hipLaunchKernelGGL((ce_grad_kernel<PW, PX, PD, 4>), grid, blk, 0, st, a, lse, rs, smooth, vbeg, vcols, dn, dbp,
-                       fac, db, add);
-  else hipLaunchKernelGGL((ce_grad_kernel<PW, PX, PD, 2>), grid, blk, 0, st, a, lse, rs, smooth, vbeg, vcols, dn, dbp,
-                       fac, db, add);
+  hipLaunchKernelGGL((ce_grad_kernel<PW, PX, PD>), dim3(a.tiles_v * a.tiles_n), dim3(G_THREADS), 0, st, a, lse, rs, smooth,
+                     vbeg, vcols, dn, dbp, fac, db, add);
 }
 template <int KM>
 void mm_terms(int pc, int pm, const MmArgs& g, int out_bf16, hipStream_t st) {

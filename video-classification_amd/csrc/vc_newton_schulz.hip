@@ -311,11 +311,11 @@ __device__ __forceinline__ void sym_store(const f32x4 (&acc)[4][4], const NsMat&
 }
 
 // A tile, or a slice of the reduction of one, of a symmetric product; tiles on and below the diagonal only.
-template <bool SQUARE, int NS>
-__global__ __launch_bounds__(G_THREADS, NS == 2 ? 2 : 1) void ns_sym_kernel(const NsMat* __restrict__ table, int count, f16* __restrict__ ws,
+template <bool SQUARE>
+__global__ __launch_bounds__(G_THREADS, 2) void ns_sym_kernel(const NsMat* __restrict__ table, int count, f16* __restrict__ ws,
                                                               const NsScale* __restrict__ sc, NsStep st, int parity,
                                                               float* __restrict__ part) {
-  typedef G16<2, 2, ROW, ROW, NS> G;
+  typedef G16<2, 2> G;
   __shared__ __attribute__((aligned(1024))) f16 smem[G::LDS];
   const int i = find_mat(table, count, SQUARE ? BY_P : BY_S, blockIdx.x);
   const NsMat t = table[i];
@@ -376,10 +376,10 @@ __global__ __launch_bounds__(G_THREADS, 2) void ns_sym_join_kernel(const NsMat* 
 
 // X <- a X + P X, into the other buffer, or the result in G's orientation after the last step.  The columns of X run along
 // the registers, so X is read and written in groups of four.
-template <typename T, int NS>
-__global__ __launch_bounds__(G_THREADS, NS == 2 ? 2 : 1) void ns_update_kernel(const NsMat* __restrict__ table, int count, f16* __restrict__ ws,
+template <typename T>
+__global__ __launch_bounds__(G_THREADS, 2) void ns_update_kernel(const NsMat* __restrict__ table, int count, f16* __restrict__ ws,
                                                                  const NsScale* __restrict__ sc, NsStep st, int parity) {
-  typedef G16<2, 2, COL, ROW, NS> G;
+  typedef G16<2, 2, COL, ROW> G;
   __shared__ __attribute__((aligned(1024))) f16 smem[G::LDS];
   const int i = find_mat(table, count, BY_UPDATE, blockIdx.x);
   const NsMat t = table[i];
@@ -747,7 +747,6 @@ int vc_newton_schulz(int dtype, int count, const void* const* g, void* const* ou
     auto launch = [&](int kind, auto kernel, int threads, auto... args) {
       hipLaunchKernelGGL(kernel, dim3((unsigned)l.blocks[kind]), dim3(threads), 0, stream, table, n, args...);
     };
-    auto deep = [&](int kind) { return l.blocks[kind] <= vc_device_cus(); };  // the four-stage pipeline (G16)
     launch(BY_NORM, bf ? ns_norm_kernel<bf16> : ns_norm_kernel<float>, 256, norms);
     hipLaunchKernelGGL(ns_scale_kernel, dim3(n), dim3(64), 0, stream, table, n, (int)l.blocks[BY_NORM], norms, eps, cap, gain, sc);
     if (steps == 0) launch(BY_NORM, bf ? ns_copy_kernel<bf16> : ns_copy_kernel<float>, 256, sc);
@@ -757,13 +756,11 @@ int vc_newton_schulz(int dtype, int count, const void* const* g, void* const* ou
       st.b = coeffs[3 * k + 1];
       st.c = coeffs[3 * k + 2];
       st.last = k == steps - 1;
-      launch(BY_S, deep(BY_S) ? ns_sym_kernel<false, 4> : ns_sym_kernel<false, 2>, G_THREADS, ws, sc, st, k & 1, part);
+      launch(BY_S, ns_sym_kernel<false>, G_THREADS, ws, sc, st, k & 1, part);
       if (l.blocks[BY_JOIN_S]) launch(BY_JOIN_S, ns_sym_join_kernel<false>, G_THREADS, ws, sc, st, k & 1, part);
-      launch(BY_P, deep(BY_P) ? ns_sym_kernel<true, 4> : ns_sym_kernel<true, 2>, G_THREADS, ws, sc, st, k & 1, part);
+      launch(BY_P, ns_sym_kernel<true>, G_THREADS, ws, sc, st, k & 1, part);
       if (l.blocks[BY_JOIN_P]) launch(BY_JOIN_P, ns_sym_join_kernel<true>, G_THREADS, ws, sc, st, k & 1, part);
-      if (deep(BY_UPDATE))
-        launch(BY_UPDATE, bf ? ns_update_kernel<bf16, 4> : ns_update_kernel<float, 4>, G_THREADS, ws, sc, st, k & 1);
-      else launch(BY_UPDATE, bf ? ns_update_kernel<bf16, 2> : ns_update_kernel<float, 2>, G_THREADS, ws, sc, st, k & 1);
+      launch(BY_UPDATE, bf ? ns_update_kernel<bf16> : ns_update_kernel<float>, G_THREADS, ws, sc, st, k & 1);
     }
   }
   flush();
