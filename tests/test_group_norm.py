@@ -279,3 +279,71 @@ def test_anchor_only_for_parameters_alone():
     assert ops._anchor((torch.zeros(2),), (types.SimpleNamespace(requires_grad=False),)) is None
     with torch.no_grad():
         assert ops._anchor((torch.zeros(2),), (p,)) is None
+
+
+@pytest.mark.gpu
+def test_more_samples_than_one_launch_takes(cuda):
+    """65535 samples go into one call of the library; more of them are the same as two calls that add up."""
+    from video_classification_amd import ops
+    N, cut = 70001, 65535
+    x, gn, res, dy = (t.to(cuda) for t in make((N, 3, 16), 4, torch.float32))
+    got = []
+    for parts in (((0, N),), ((0, cut), (cut, N))):
+        gn.zero_grad()
+        row = []
+        for a, b in parts:
+            xs, rs = x[a:b].clone().requires_grad_(True), res[a:b].clone().requires_grad_(True)
+            y = ops.group_norm(xs, gn, "silu", rs)
+            y.backward(dy[a:b])
+            row.append((y.detach(), xs.grad, rs.grad))
+        got.append([torch.cat(c) for c in zip(*row)] + [gn.weight.grad.clone(), gn.bias.grad.clone()])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    assert (got[0][0][cut:].double() - act64(ref64(x[cut:].double(), gn, "none", res[cut:].double())[3], "silu")).abs().max() < 1e-4
+
+
+@pytest.mark.gpu
+def test_backward_passes_of_two_streams_follow_each_other(cuda):
+    """Forward calls on two streams write the same parameter gradients: the second pass waits for the first."""
+    from video_classification_amd import ops
+    x, gn, _, dy = (t.to(cuda) for t in make((64, 1, 56, 56, 64), 8, torch.bfloat16))
+    ops.group_norm(x, gn, "relu").backward(dy)
+    once = [p.grad.clone() for p in gn.parameters()]
+    gn.zero_grad()
+    main, streams, ys = torch.cuda.current_stream(), [torch.cuda.Stream() for _ in range(2)], []
+    for s in streams:
+        s.wait_stream(main)
+        with torch.cuda.stream(s):
+            ys.append(ops.group_norm(x, gn, "relu"))
+    torch.autograd.backward(ys, [dy, dy])
+    for p, a in zip(gn.parameters(), once):
+        assert torch.equal(p.grad, 2 * a)
+    ops.group_norm(x, gn, "relu").backward(dy)  # and the default stream after them
+    for p, a in zip(gn.parameters(), once):
+        assert torch.equal(p.grad, 2 * a + a)
+
+
+@pytest.mark.gpu
+def test_refuses_computed_parameters_and_sizes(cuda):
+    from video_classification_amd import ops
+    x = torch.zeros(2, 3, 32, device=cuda)
+    w = torch.ones(32, device=cuda, requires_grad=True)
+    gn = types.SimpleNamespace(num_groups=4, num_channels=32, eps=1e-5, weight=w * 2, bias=None)
+    with pytest.raises(RuntimeError, match="must be leaves"):
+        ops.group_norm(x, gn)
+    with torch.no_grad():
+        assert ops.group_norm(x, gn).shape == x.shape
+    wide = types.SimpleNamespace(num_groups=1, num_channels=(1 << 20) + 8, eps=1e-5, weight=None, bias=None)
+    with pytest.raises(RuntimeError, match="exceed"):
+        ops.group_norm(torch.zeros(1, 1, device=cuda).expand(1, (1 << 20) + 8), wide)
+    gn.weight, gn.num_groups, gn.num_channels = None, 1, 1
+    with pytest.raises(RuntimeError, match="exceed"):
+        ops.group_norm(torch.zeros(1, 1, 1, device=cuda).expand(1, (1 << 32) + 1, 1), gn)
+
+
+def test_runs_of_samples_cover_them_once():
+    from video_classification_amd import ops
+    for n in (1, 65535, 65536, 131070, 200000):
+        runs = list(ops._gn_runs(n, 24))
+        assert sum(k for _, k, _ in runs) == n and all(0 < k <= 65535 and o == 24 * a for a, k, o in runs)
+        assert [a for a, _, _ in runs] == [sum(k for _, k, _ in runs[:i]) for i in range(len(runs))]

@@ -379,3 +379,46 @@ def test_plan_covers_every_size():
         assert sizes[0] >= 2 * (n + v) * k
     small = L.query("vc_linear_ce_bytes", 2, 1, 1, 8192, 65536, 64)
     assert small < (8192 + 65536) * 64 * 2 + (400 << 20)
+
+
+@pytest.mark.gpu
+def test_backward_passes_of_two_streams_follow_each_other(cuda):
+    """Forward calls on two streams write the same parameter gradients: the second pass waits for the first."""
+    from video_classification_amd import ops
+    x, w, b, t = make(1000, 256, 5000, "mixed")
+    ops.linear_cross_entropy(x, w, b, t).backward()
+    once = [p.grad.clone() for p in (w, b)]
+    w.grad = b.grad = None
+    main, streams, losses = torch.cuda.current_stream(), [torch.cuda.Stream() for _ in range(2)], []
+    for s in streams:
+        s.wait_stream(main)
+        with torch.cuda.stream(s):
+            losses.append(ops.linear_cross_entropy(x, w, b, t))
+    torch.autograd.backward(losses)
+    for p, a in zip((w, b), once):
+        assert torch.equal(p.grad, 2 * a)
+
+
+@pytest.mark.gpu
+def test_computed_weights_sizes_and_empty_batches(cuda):
+    from video_classification_amd import ops
+    x, w, b, t = make(6, 16, 20, "f32")
+    ce = ops.linear_cross_entropy
+    with pytest.raises(RuntimeError, match="must be leaves"):
+        ce(x, w * 2, b, t)
+    with pytest.raises(RuntimeError, match="must be leaves"):
+        ce(x, w, b + 1, t)
+    with torch.no_grad():
+        ce(x, w * 2, b + 1, t)
+    n = (1 << 22) + 1
+    with pytest.raises(RuntimeError, match="exceed"):
+        ce(x[:1].expand(n, 16), w, b, t[:1].expand(n))
+    with pytest.raises(RuntimeError, match="exceed"):
+        ce(x[:, :1].expand(6, (1 << 20) + 1), w[:, :1].detach().expand(20, (1 << 20) + 1), b, t)
+    with pytest.raises(ValueError, match="int64"):
+        ce(x, w, b, t, ignore_index=1 << 64)
+    for reduction in ("mean", "sum", "none"):  # nothing but the parameters needs gradients, and there are no rows
+        loss = ce(x[:0], w, b, t[:0], reduction=reduction)
+        assert loss.shape == ((0,) if reduction == "none" else ())
+        loss.sum().backward()
+        assert w.grad is None

@@ -207,3 +207,28 @@ def test_bounds_of_the_coefficients():
     assert 1.202 < cap < 1.24 and 484 < gain < 496 and 2.80 < pmax < 2.95
     cap, gain, _ = ops._ns_bounds(((1.5, -0.5, 0.0),) * 5)
     assert cap == pytest.approx(1.02) and 7.5 < gain < 7.8
+
+
+@pytest.mark.gpu
+def test_refuses_shared_memory_in_place(cuda):
+    from video_classification_amd import ops
+    buf = torch.randn(3 * 20, 30, generator=torch.Generator().manual_seed(0)).to(cuda)
+    a, b = buf[:20], buf[20:40]
+    for pair in ([a, a], [a, buf[19:39]], [buf, b]):
+        with pytest.raises(RuntimeError, match="share no memory"):
+            ops.newton_schulz(pair, inplace=True)
+    want = ops.newton_schulz([a, a, b])  # out of place the same matrix may come twice
+    assert torch.equal(want[0], want[1])
+    ops.newton_schulz([b, a], inplace=True)  # neighbours share nothing
+    assert torch.equal(a, want[0]) and torch.equal(b, want[2])
+    with pytest.raises(RuntimeError, match="exceed"):
+        ops.newton_schulz(buf[:1, :1].expand(2, (1 << 20) + 1))
+
+
+def test_disjoint():
+    from video_classification_amd import ops
+    buf = torch.zeros(4, 6)
+    ops._disjoint("op", [buf[2:], buf[:2], buf[:0]])
+    for pair in ([buf, buf], [buf[:3], buf[2:]], [buf, buf[1:2]]):
+        with pytest.raises(RuntimeError, match="share no memory"):
+            ops._disjoint("op", pair)

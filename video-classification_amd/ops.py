@@ -1403,11 +1403,13 @@ class _LinearCrossEntropy(torch.autograd.Function):
         dw, add_w = _grad_target(weight)
         db, add_b = _grad_target(bias)
         ws = torch.empty(_size("vc_linear_ce_bytes", 2, xd, wd, N, V, K), device=dev, dtype=torch.uint8)
+        _before_grads(dw, db)
         L.fast("vc_linear_ce_bwd", dev, xd, wd, _addr(b), target.data_ptr(), ignore_index, smoothing, reduction == "mean",
                reduction == "none", g.data_ptr(), saved.data_ptr(), _addr(dx), _addr(dw), _addr(db), ws.data_ptr(),
                add_w + 2 * add_b, N, V, K)
         _put_grad(weight, dw)
         _put_grad(bias, db)
+        _after_grads(dw, db)
         _ready(weight, bias)
         return (dx,) + (None,) * 7
 
@@ -1419,8 +1421,9 @@ def linear_cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoot
     x [..., K] float32 or bfloat16, weight [V, K] and bias [V] (or None) float32, or bfloat16 next to bfloat16 x, target
     int64 of x's leading shape.  Rows whose target is `ignore_index` count for nothing; any other target outside [0, V)
     makes the loss NaN.  reduction: "mean" over the rows that count (0 if there are none), "sum", or "none" (a loss per row,
-    0 where ignored).  The loss is float32; gradients of weight and bias are accumulated into .grad.  stats: a dict that
-    receives "pred" (arg-max per row) and "correct" (rows that count and are right)."""
+    0 where ignored).  The loss is float32; gradients of weight and bias, which have to be leaves, are accumulated into
+    .grad.  With "none", a row's gradient is resolved to 2^-39 of the largest row's weight.  stats: a dict that receives
+    "pred" (arg-max per row) and "correct" (rows that count and are right).  At most 2^22 rows, 2^22 classes and K = 2^20."""
     _require_cuda(x, "linear_cross_entropy")
     xd, wd = L.dtype_code(x.dtype), L.dtype_code(weight.dtype)
     if xd == L.VC_F32 and wd != L.VC_F32:
@@ -1437,9 +1440,16 @@ def linear_cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoot
         raise ValueError(f"linear_cross_entropy: label_smoothing {label_smoothing} outside [0, 1]")
     if reduction not in CE_REDUCTIONS:
         raise ValueError(f"linear_cross_entropy: reduction must be one of {CE_REDUCTIONS}, not {reduction!r}")
+    _leaf_params("linear_cross_entropy", weight, bias)
     _same_device("linear_cross_entropy", x, weight, bias, target)
+    _fits("linear_cross_entropy", (1 << 22, 1 << 22, 1 << 20), (target.numel(), *weight.shape))
+    if not -(1 << 63) <= ignore_index < 1 << 63:
+        raise ValueError(f"linear_cross_entropy: ignore_index {ignore_index} is not an int64")
     if target.numel() == 0:
         loss = x.float().sum(-1) if reduction == "none" else x.float().sum()
+        anchor = _anchor((x,), (weight, bias))
+        if anchor is not None:
+            loss = loss + anchor.float().sum()
         if stats is not None:
             stats["pred"] = target.reshape(-1)
             stats["correct"] = torch.zeros(1, device=x.device, dtype=torch.int32)
@@ -1727,8 +1737,8 @@ def _on(device):
     return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
-def _addr(t):
-    return None if t is None else t.data_ptr()
+def _addr(t, offset=0):
+    return None if t is None else t.data_ptr() + offset
 
 
 @functools.lru_cache(maxsize=1024)
@@ -1743,10 +1753,40 @@ def _same_device(what, first, *rest):
             raise RuntimeError(f"{what}: tensors on {first.device} and {t.device}")
 
 
+def _leaf_params(what, *params):
+    """Refuses a parameter that is itself computed from others: its gradient would end in its own .grad."""
+    for p in params:
+        if p is not None and p.requires_grad and not p.is_leaf and torch.is_grad_enabled():
+            raise RuntimeError(f"{what}: parameters must be leaves, gradients are written into their .grad; this one was "
+                               "computed (detach it, or pass the leaf)")
+
+
+def _disjoint(what, dense):
+    """Refuses dense tensors that share memory: each is read and written without regard to the others."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in dense if t.numel())
+    for (_, end), (start, _) in zip(spans, spans[1:]):
+        if start < end:
+            raise RuntimeError(f"{what}: in place needs tensors that share no memory")
+
+
+def _fits(what, limits, sizes):
+    for limit, size in zip(limits, sizes):
+        if size > limit:
+            raise RuntimeError(f"{what}: sizes {tuple(sizes)} exceed {tuple(limits)}")
+
+
 # ----------------------------------------------------------------------------------------------
 # group normalisation
 # ----------------------------------------------------------------------------------------------
 GN_ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
+GN_SAMPLES = 65535  # of one call of the library
+
+
+def _gn_runs(N, sample_bytes):
+    """(first sample, samples, byte offset) of the calls that cover N samples."""
+    if N <= GN_SAMPLES:
+        return ((0, N, 0),)
+    return [(n, min(GN_SAMPLES, N - n), n * sample_bytes) for n in range(0, N, GN_SAMPLES)]
 
 
 def _f32_param(what, p):
@@ -1756,6 +1796,38 @@ def _f32_param(what, p):
     if p.dtype != torch.float32:
         raise TypeError(f"{what}: parameters must be float32, not {p.dtype}")
     return p.detach().contiguous()
+
+
+# Autograd orders the backward passes of forward calls on different streams at a parameter's gradient node; the parameters
+# of these operators have none, so passes that write gradients follow each other here.  Per device: the stream of the last
+# such pass and, unless it is the default one, an event behind it.
+_last_writer = {}
+
+
+def _before_grads(*grads):
+    """Called before the kernels that write these gradients (None entries are skipped)."""
+    dev = next((g.device.index for g in grads if g is not None), None)
+    if dev is None or dev not in _last_writer:
+        return
+    stream, event = _last_writer[dev]
+    if stream == torch._C._cuda_getCurrentRawStream(dev) or torch.cuda.is_current_stream_capturing():
+        return  # a capture starts behind everything that was enqueued before it
+    here = torch.cuda.current_stream(dev)
+    here.wait_event(event) if event is not None else here.wait_stream(torch.cuda.default_stream(dev))
+    for g in grads:
+        if g is not None:
+            g.record_stream(here)
+
+
+def _after_grads(*grads):
+    dev = next((g.device.index for g in grads if g is not None), None)
+    if dev is None or torch.cuda.is_current_stream_capturing():
+        return
+    stream, event = torch._C._cuda_getCurrentRawStream(dev), None
+    if stream:
+        event = torch.cuda.Event()
+        event.record(torch.cuda.current_stream(dev))
+    _last_writer[dev] = stream, event
 
 
 def _grad_target(p):
@@ -1787,13 +1859,14 @@ class _GroupNorm(torch.autograd.Function):
         res = residual.contiguous() if residual is not None else None
         dev = x.device
         gamma, beta = _f32_param("group_norm", weight), _f32_param("group_norm", bias)
-        code, ws_floats = L.dtype_code(x.dtype), _size("vc_group_norm_workspace_floats", N, S, C, G)
+        code, ws_floats = L.dtype_code(x.dtype), _size("vc_group_norm_workspace_floats", min(N, GN_SAMPLES), S, C, G)
         y = torch.empty_like(x)
         stat = torch.empty(2, N * G, device=dev, dtype=torch.float32)
         ws = torch.empty(ws_floats, device=dev, dtype=torch.float32)
         mean = stat.data_ptr()
-        L.fast("vc_group_norm_fwd", dev, code, x.data_ptr(), _addr(res), _addr(gamma), _addr(beta), y.data_ptr(), mean,
-               mean + 4 * N * G, ws.data_ptr(), N, S, C, G, eps, act)
+        for n, k, o in _gn_runs(N, S * C * x.element_size()):
+            L.fast("vc_group_norm_fwd", dev, code, x.data_ptr() + o, _addr(res, o), _addr(gamma), _addr(beta),
+                   y.data_ptr() + o, mean + 4 * n * G, mean + 4 * (N + n) * G, ws.data_ptr(), k, S, C, G, eps, act)
         ctx.dims, ctx.act, ctx.params, ctx.code, ctx.ws_floats = (N, S, C, G), act, params, code, ws_floats
         ctx.save_for_backward(x, res if act else None, stat, gamma, beta)
         return y
@@ -1815,11 +1888,14 @@ class _GroupNorm(torch.autograd.Function):
         if need_dx or dw is not None or db is not None or (need_dres and act):
             ws = torch.empty(ctx.ws_floats, device=dev, dtype=torch.float32)
             mean = stat.data_ptr()
-            L.fast("vc_group_norm_bwd", dev, ctx.code, x.data_ptr(), dy.data_ptr(), _addr(res), _addr(gamma), _addr(beta),
-                   mean, mean + 4 * N * G, _addr(dx), _addr(dres) if act else None, _addr(dw), _addr(db), ws.data_ptr(),
-                   N, S, C, G, act, add_w + 2 * add_b)
+            _before_grads(dw, db)
+            for n, k, o in _gn_runs(N, S * C * x.element_size()):
+                L.fast("vc_group_norm_bwd", dev, ctx.code, x.data_ptr() + o, dy.data_ptr() + o, _addr(res, o), _addr(gamma),
+                       _addr(beta), mean + 4 * n * G, mean + 4 * (N + n) * G, _addr(dx, o), _addr(dres, o) if act else None,
+                       _addr(dw), _addr(db), ws.data_ptr(), k, S, C, G, act, 3 if n else add_w + 2 * add_b)
             _put_grad(weight, dw)
             _put_grad(bias, db)
+            _after_grads(dw, db)
         _ready(weight, bias)
         return dx, dres, None, None, None, None, None
 
@@ -1829,11 +1905,12 @@ def group_norm(x, gn, act="none", residual=None):
     ``gn.num_groups`` groups over all its positions (a frame of [F,1,H,W,C], a whole clip of [B,D,H,W,C], a row of [M,C]).
     gn: an nn.GroupNorm holding num_groups / eps / weight / bias (its own forward is not used); act: "none", "relu",
     "silu" or "gelu"; residual: same shape and type as x.  x is float32 or bfloat16; statistics, sums and the parameters'
-    gradients (accumulated into .grad) are float32."""
+    gradients (accumulated into .grad of the parameters, which have to be leaves) are float32."""
     _require_cuda(x, "group_norm")
     if act not in GN_ACTS:
         raise ValueError(f"group_norm: act must be one of {sorted(GN_ACTS)}, not {act!r}")
     L.dtype_code(x.dtype)
+    _leaf_params("group_norm", gn.weight, gn.bias)
     if x.dim() < 2 or x.shape[-1] != gn.num_channels:
         raise RuntimeError(f"group_norm: input of shape {tuple(x.shape)} does not end in {gn.num_channels} channels")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
@@ -1843,6 +1920,7 @@ def group_norm(x, gn, act="none", residual=None):
     _same_device("group_norm", x, residual, weight, bias)
     if x.numel() == 0:
         return x.clone()
+    _fits("group_norm", (1 << 30, 1 << 20), (x.numel() // (x.shape[0] * x.shape[-1]), x.shape[-1]))
     with _on(x.device):
         _leaf_guard("group_norm", x, residual)
         return _GroupNorm.apply(x, residual, _anchor((x, residual), (weight, bias)), (weight, bias), gn.num_groups, gn.eps,
@@ -1995,8 +2073,8 @@ def newton_schulz(g, steps=5, coeffs=NS_COEFFS, eps=1e-7, inplace=False):
 
     g: a tensor [..., m, n], or a list or tuple of such tensors of any shapes (all of one type, float32 or bfloat16, on one
     device); all their matrices go through the same launches.  coeffs: (a, b, c), or `steps` such triples.  Returns new
-    tensors of g's structure, shapes and type, or with `inplace` the (dense) tensors of g themselves; products are carried
-    at float32 accuracy whatever the type.  Not differentiable: gradients are its input."""
+    tensors of g's structure, shapes and type, or with `inplace` the tensors of g themselves (dense, sharing no memory);
+    products are carried at float32 accuracy whatever the type.  Not differentiable: gradients are its input."""
     single = isinstance(g, torch.Tensor)
     items = [g] if single else list(g)
     if not items:
@@ -2025,6 +2103,10 @@ def newton_schulz(g, steps=5, coeffs=NS_COEFFS, eps=1e-7, inplace=False):
             raise RuntimeError("newton_schulz: in place needs dense tensors outside the autograd graph")
     code = L.dtype_code(first.dtype)
     _same_device("newton_schulz", first, *items)
+    for t in items:
+        _fits("newton_schulz", (1 << 20, 1 << 20, 1 << 31), (*t.shape[-2:], t.shape[-2] * t.shape[-1]))
+    if inplace:
+        _disjoint("newton_schulz", items)
     with _on(first.device), torch.no_grad():
         srcs = [t.detach().contiguous() for t in items]
         outs = items if inplace else [torch.empty_like(t) for t in srcs]
