@@ -207,8 +207,8 @@ int vc_layernorm_bwd_add(int dtype, const void* x, const void* dout, const float
 
 /* ---- group normalisation with its activation -----------------------------------------------------------
  * No counterpart in the reference, whose encoders normalise over the batch.  x, residual (nullable), y, dy, dx,
- * dresidual: channels-last [N][S][C] in `dtype`; N up to 65535, S to 2^30, C to 2^20 with C % G == 0 (16-byte vectors when C is a multiple of 8 and
- * the pointers are 16-byte aligned).  y = act((x - mean) * rstd * gamma + beta + residual) with one mean / rstd
+ * dresidual: channels-last [N][S][C] in `dtype`; N up to 65535, S to 2^30, C to 2^20 with C % G == 0 (16-byte vectors when C
+ * is a multiple of 8 and the pointers are 16-byte aligned).  y = act((x - mean) * rstd * gamma + beta + residual) with one mean / rstd
  * [N][G] per sample and group; gamma / beta nullable (1 / 0).  act: 0 none, 1 ReLU, 2 SiLU, 3 GELU (erf).  Backward takes
  * the forward call's mean / rstd and writes dx, dresidual, dgamma and dbeta (each nullable); bit 0 / 1 of `accumulate`
  * adds to what dgamma / dbeta hold instead.
@@ -355,8 +355,9 @@ int vc_ce_fwd_bwd(int grad_dtype, const float* logits, int ld, const int64_t* ta
 /* Softmax cross entropy of a linear classifier z = x W^T + b without the logit matrix (the last nn.Linear of a decoder
  * and nn.CrossEntropyLoss in one, for label sets whose logits should not be kept; no counterpart in the reference).
  * x [N][K] (xdtype), w [V][K], bias [V] nullable, db [V], dw [V][K] (wdtype), dx [N][K] (xdtype); fp32 x needs fp32 w;
- * any N, V, K.  Rows with target == ignore_index count for nothing, whatever x holds there; a target outside [0, V)
- * makes its row's loss and gradients NaN.  mean: divide by the rows that count (by 1 if there are none).
+ * N and V up to 2^22, K up to 2^20.  Values of x and of w are resolved to 2^-39 of the largest finite one.  Rows with
+ * target == ignore_index count for nothing, whatever x holds there; a target outside [0, V) makes its row's loss and
+ * gradients NaN.  mean: divide by the rows that count (by 1 if there are none).
  * fwd: row_loss [N] (0 for ignored rows), loss (nullable, one float), pred [N] (nullable, lowest arg-max) and correct
  *   (nullable).  saved: vc_linear_ce_bytes(0, ..) bytes that backward reads; workspace: vc_linear_ce_bytes(1, ..).
  * bwd: dloss = upstream gradient of the mean or sum, or with per_row of every row's loss (each resolved to 2^-39 of the
@@ -381,7 +382,8 @@ int vc_optim_step(int mode, float* p, const float* g, float* m, float* v, int64_
  * be g[i].  The caller bounds the iterates over singular values in [0, 1]: cap = the largest |value| any iterate takes,
  * gain = the largest ratio of an iterate to its start, pmax = the largest |b l + c l^2| for l in [0, cap^2].
  * workspace: vc_newton_schulz_bytes() bytes, 256-byte aligned, contents irrelevant; all matrices share each launch (64 at a
- * time; small ones of up to 16 rows run apart, all steps in one launch).  Different matrices share no memory.  Products are as accurate as fp32's; a zero matrix stays zero. */
+ * time; small ones of up to 16 rows run apart, all steps in one launch).  Different matrices share no memory.  Products are
+ * as accurate as fp32's; a zero matrix stays zero. */
 int64_t vc_newton_schulz_bytes(int count, const int* rows, const int* cols);
 int vc_newton_schulz(int dtype, int count, const void* const* g, void* const* out, const int* rows, const int* cols,
                      int steps, const float* coeffs, double eps, float cap, float gain, float pmax, void* workspace,

@@ -1422,8 +1422,9 @@ def linear_cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoot
     int64 of x's leading shape.  Rows whose target is `ignore_index` count for nothing; any other target outside [0, V)
     makes the loss NaN.  reduction: "mean" over the rows that count (0 if there are none), "sum", or "none" (a loss per row,
     0 where ignored).  The loss is float32; gradients of weight and bias, which have to be leaves, are accumulated into
-    .grad.  With "none", a row's gradient is resolved to 2^-39 of the largest row's weight.  stats: a dict that receives
-    "pred" (arg-max per row) and "correct" (rows that count and are right).  At most 2^22 rows, 2^22 classes and K = 2^20."""
+    .grad.  Values of x and of the weight are resolved to 2^-39 of the largest finite one of each, and with "none" a row's
+    gradient to 2^-39 of the largest upstream gradient.  stats: a dict that receives "pred" (arg-max per row) and "correct"
+    (rows that count and are right).  At most 2^22 rows, 2^22 classes and K = 2^20."""
     _require_cuda(x, "linear_cross_entropy")
     xd, wd = L.dtype_code(x.dtype), L.dtype_code(weight.dtype)
     if xd == L.VC_F32 and wd != L.VC_F32:
