@@ -368,9 +368,9 @@ int64_t vc_linear_ce_bytes(int what, int xdtype, int wdtype, int N, int V, int K
 int vc_linear_ce_fwd(int xdtype, int wdtype, const void* x, const void* w, const void* bias, const int64_t* target,
                      int64_t ignore_index, float smoothing, int mean, float* row_loss, float* loss, int64_t* pred,
                      int* correct, void* saved, void* workspace, int N, int V, int K, vc_stream_t stream);
-int vc_linear_ce_bwd(int xdtype, int wdtype, const void* bias, const int64_t* target, int64_t ignore_index,
-                     float smoothing, int mean, int per_row, const float* dloss, const void* saved, void* dx, void* dw,
-                     void* db, void* workspace, int accumulate, int N, int V, int K, vc_stream_t stream);
+int vc_linear_ce_bwd(int xdtype, int wdtype, const int64_t* target, int64_t ignore_index, float smoothing, int mean,
+                     int per_row, const float* dloss, const void* saved, void* dx, void* dw, void* db, void* workspace,
+                     int accumulate, int N, int V, int K, vc_stream_t stream);
 /* optim.Adam (L2-coupled) / AdamW / SGD(momentum) (training_utils.py:324-329) over one flat fp32 buffer.
  * mode 0 Adam, 1 AdamW, 2 SGD (b1 = momentum).  grad_scale folds the 1/world of the all-reduce. */
 int vc_optim_step(int mode, float* p, const float* g, float* m, float* v, int64_t n, float lr, float b1, float b2,

@@ -119,56 +119,54 @@ __device__ __forceinline__ void pack_rows(const T* __restrict__ src, f16* __rest
   if (planes == 2) *reinterpret_cast<f16x8*>(dst + plane + row * ld + c0) = lo;
 }
 
-// exps[0] / [1] = scale exponents of x / W; the first `xblocks` workgroups pack x, the others W
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+// exps[0] / [1] = scale exponents of x / W; the first `xblocks` workgroups pack x, the others W and the bias: bl = bias
+// log2(e) over whole tiles of classes, -inf behind the last one, which leaves the epilogues of the products four plain
+// vector loads (clamped and converted there, these cost a fifth of a tile's time).
 template <typename TX, typename TW>
 __global__ __launch_bounds__(256) void ce_pack_kernel(const TX* __restrict__ x, const TW* __restrict__ w, int N, int V,
                                                       int K, int ld, int px, int pw, const int64_t* __restrict__ target,
                                                       int64_t ignore, const float* __restrict__ amax, f16* __restrict__ xp,
                                                       f16* __restrict__ wp, int* __restrict__ exps, int xblocks, int xb,
-                                                      int wb) {
+                                                      int wb, const TW* __restrict__ bias, float* __restrict__ bl) {
   __shared__ float sm[4];
   const bool isx = (int)blockIdx.x < xblocks;
   const int e = scale_exp(isx ? amax : amax + AMAX_MOST, isx ? xb : wb, sm);
   if (threadIdx.x == 0 && ((int)blockIdx.x == 0 || (int)blockIdx.x == xblocks)) exps[isx ? 0 : 1] = e;
   const int64_t unit = (int64_t)(isx ? blockIdx.x : blockIdx.x - xblocks) * 4 + (threadIdx.x >> 6);
   if (isx) pack_rows(x, xp, (int64_t)N * ld, N, K, ld, px, e, target, ignore, unit);
-  else pack_rows(w, wp, (int64_t)V * ld, V, K, ld, pw, e, (const int64_t*)nullptr, 0, unit);
+  else {
+    pack_rows(w, wp, (int64_t)V * ld, V, K, ld, pw, e, (const int64_t*)nullptr, 0, unit);
+    const int64_t v = (int64_t)(blockIdx.x - xblocks) * 256 + threadIdx.x;  // four rows or more per workgroup: all classes
+    if (v < (V + GM - 1) / GM * GM) bl[v] = v >= V ? -INFINITY : bias ? to_f32(bias[v]) * LOG2E : 0.f;
+  }
 }
 
 // ---- logits of a 128-class x 128-row tile ---------------------------------------------------------------------------
 // Everything behind the products works on z log2(e): the exponentials are then one subtraction and one v_exp_f32.
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-
 struct CeArgs {
   const f16* w;      // [pw][V][ld]
   const f16* x;      // [px][N][ld]
-  const void* bias;  // nullable, float or bf16
+  const float* bl;   // bias log2(e), -inf behind the last class
   const int64_t* target;
   int64_t ignore;
   const int* exps;
-  int N, V, ld, bias_bf16;
+  int N, V, ld, db_bf16;
   int tiles_v, tiles_n;
 };
 
 // acc = z log2(e) without the bias, which follows in `bias` (-inf behind the last class): rows v0 + .., columns n0 + ..
 template <int PW, int PX>
 __device__ __forceinline__ void logit_tile(const CeArgs& a, int v0, int n0, f16* smem, f32x4 (&acc)[4][4],
-                                           float (&bias)[4][4], float& scale) {
+                                           f32x4 (&bias)[4], float& scale) {
   typedef G16<PW, PX> G;
   G::zero(acc);
   G::run(acc, Op16{a.w + (int64_t)v0 * a.ld, (int64_t)a.V * a.ld, a.ld, a.V - v0, 0},
          Op16{a.x + (int64_t)n0 * a.ld, (int64_t)a.N * a.ld, a.ld, a.N - n0, 0}, 0, a.ld, smem);
-  const int lane = threadIdx.x & 63, q = lane >> 4, wm = threadIdx.x >> 7;
+  const float* bl = a.bl + v0 + (threadIdx.x >> 7) * 64 + ((threadIdx.x & 63) >> 4) * 4;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int v = v0 + wm * 64 + i * 16 + q * 4 + r;
-      float b = 0.f;
-      if (v >= a.V) b = -INFINITY;
-      else if (a.bias) b = (a.bias_bf16 ? (float)((const bf16*)a.bias)[v] : ((const float*)a.bias)[v]) * LOG2E;
-      bias[i][r] = b;
-    }
+  for (int i = 0; i < 4; ++i) bias[i] = *reinterpret_cast<const f32x4*>(bl + i * 16);
   int es = -(a.exps[0] + a.exps[1]);
   if (es < -120 || es > 120) {  // operands of extreme magnitude: two factors
     const float f = ldexpf(1.f, es / 2);
@@ -187,7 +185,8 @@ __device__ __forceinline__ int lane_class(int t, int v0) {
   return (unsigned)d < 64u && (d & 12) == 0 ? (d >> 4) * 4 + (d & 3) : -1;
 }
 __device__ __forceinline__ int row_target(const CeArgs& a, int n) {
-  return n < a.N ? (int)min(max(a.target[n], (int64_t)-1), (int64_t)a.V) : -1;
+  const int t = (int)min(max(a.target[min(n, a.N - 1)], (int64_t)-1), (int64_t)a.V);
+  return n < a.N ? t : -1;
 }
 
 // ---- forward: statistics of a tile -----------------------------------------------------------------------------------
@@ -217,12 +216,16 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_stats_kernel(CeArgs a, float4
   g16_tile(blockIdx.x, gridDim.x, a.tiles_v, a.tiles_n, tv, tn);
   const int v0 = tv * GM, n0 = tn * GM;
   f32x4 acc[4][4];
-  float bias[4][4], scale;
+  f32x4 bias[4];
+  float scale;
   logit_tile<PW, PX>(a, v0, n0, smem, acc, bias, scale);
   const int lane = threadIdx.x & 63, q = lane >> 4, l15 = lane & 15;
   const int wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
   float4* xch = reinterpret_cast<float4*>(smem);
   Stat st[4];
+  int target[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) target[j] = row_target(a, n0 + wn * 64 + j * 16 + l15);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int n = n0 + wn * 64 + j * 16 + l15;
@@ -243,7 +246,7 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_stats_kernel(CeArgs a, float4
         if (v < a.V) s.z += z;
       }
     }
-    const int hit = lane_class(row_target(a, n), v0);
+    const int hit = lane_class(target[j], v0);
     if (hit >= 0) {
       float z = 0.f;
 #pragma unroll
@@ -433,7 +436,8 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_grad_kernel(CeArgs a, const f
   g16_tile(blockIdx.x, gridDim.x, a.tiles_v, a.tiles_n, tv, tn);
   const int v0 = vbeg + tv * GM, n0 = tn * GM;
   f32x4 acc[4][4];
-  float bias[4][4], scale;
+  f32x4 bias[4];
+  float scale;
   logit_tile<PW, PX>(a, v0, n0, smem, acc, bias, scale);
   const int lane = threadIdx.x & 63, q = lane >> 4, l15 = lane & 15;
   const int wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
@@ -444,14 +448,21 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_grad_kernel(CeArgs a, const f
 #pragma unroll
     for (int r = 0; r < 4; ++r) col[i][r] = 0.f;
   const int64_t plane = (int64_t)a.N * vcols;
+  int target[4];
+  float weight[4], low[4];  // 2^(z - low) is the scaled probability
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int n = n0 + wn * 64 + j * 16 + l15;
-    const float w = n >= a.N ? 0.f : rs ? rs[n] : a.target[n] == a.ignore ? 0.f : 1.f;
-    const int t = row_target(a, n);
-    float l = w != 0.f ? lse[n] - 15.f : 0.f;  // 2^(z - l) is the scaled probability
-    if (w != 0.f && (t < 0 || t >= a.V)) l = NAN;
-    const int hit = lane_class(t, v0);
+    const int n = n0 + wn * 64 + j * 16 + l15, at = min(n, a.N - 1);
+    target[j] = row_target(a, n);
+    low[j] = lse[at] - 15.f;
+    weight[j] = rs ? rs[at] : a.target[at] == a.ignore ? 0.f : 1.f;
+    if (n >= a.N) weight[j] = 0.f;
+    if (target[j] < 0 || target[j] >= a.V) low[j] = NAN;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float w = weight[j], l = low[j];
+    const int hit = lane_class(target[j], v0);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -507,7 +518,7 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_grad_kernel(CeArgs a, const f
     if (threadIdx.x < GM && v < a.V) {
       const float s = sb[0][threadIdx.x] + sb[1][threadIdx.x];
       if (a.tiles_n > 1) dbpart[(int64_t)tn * a.V + v] = s;
-      else if (a.bias_bf16) bias_out((bf16*)db + v, s, fac, add);  // the only row tile
+      else if (a.db_bf16) bias_out((bf16*)db + v, s, fac, add);  // the only row tile
       else bias_out((float*)db + v, s, fac, add);
     }
   }
@@ -641,8 +652,8 @@ struct Plan {
   int pdx, pdw, pd;            // terms of d for dx and dW, and the larger of the two
   int piece, pieces;           // classes of a piece
   int sx, kx, sw, kw;          // slices of the reductions of dx (per piece) and dW, and their lengths
-  // forward workspace (saved for backward): packed x, packed W, exponents, lse, total
-  int64_t o_xp, o_wp, o_exps, o_lse, o_total, saved;
+  // forward workspace (saved for backward): packed x, packed W, exponents, bias, lse, total
+  int64_t o_xp, o_wp, o_exps, o_bl, o_lse, o_total, saved;
   // forward scratch
   int64_t f_amax, f_part, f_zt, fwd;
   // backward scratch
@@ -689,6 +700,7 @@ Plan make_plan(int xf32, int wf32, int N, int V, int K) {
   p.o_xp = take((int64_t)p.px * N * p.ld * 2);
   p.o_wp = take((int64_t)p.pw * V * p.ld * 2);
   p.o_exps = take(16);
+  p.o_bl = take((int64_t)all * 4);
   p.o_lse = take((int64_t)N * 4);
   p.o_total = take(16);
   p.saved = o;
@@ -726,7 +738,7 @@ int check_ce(const char* who, int xdtype, int wdtype, int N, int V, int K, float
 }
 
 template <typename TX, typename TW>
-void pack_go(const Plan& p, const void* x, const void* w, int N, int V, int K, const int64_t* target, int64_t ignore,
+void pack_go(const Plan& p, const void* x, const void* w, const void* bias, int N, int V, int K, const int64_t* target, int64_t ignore,
              char* saved, char* ws, hipStream_t st) {
   float* amax = (float*)(ws + p.f_amax);
   const int per = ceil_div(p.ld, 512);
@@ -740,7 +752,7 @@ void pack_go(const Plan& p, const void* x, const void* w, int N, int V, int K, c
                      ignore, amax, xa);
   hipLaunchKernelGGL((ce_pack_kernel<TX, TW>), dim3(xb + wb), dim3(256), 0, st, (const TX*)x, (const TW*)w, N, V, K, p.ld,
                      p.px, p.pw, target, ignore, amax, (f16*)(saved + p.o_xp), (f16*)(saved + p.o_wp),
-                     (int*)(saved + p.o_exps), xb, xa, wa);
+                     (int*)(saved + p.o_exps), xb, xa, wa, (const TW*)bias, (float*)(saved + p.o_bl));
 }
 
 template <int PC, int PM, int KM>
@@ -796,10 +808,10 @@ int vc_linear_ce_fwd(int xdtype, int wdtype, const void* x, const void* w, const
   VC_CHECK_ARG((((uintptr_t)saved | (uintptr_t)workspace) & 255) == 0, "vc_linear_ce_fwd: buffers must be 256-byte aligned");
   const Plan p = make_plan(xdtype == VC_F32, wdtype == VC_F32, N, V, K);
   char *sv = (char*)saved, *ws = (char*)workspace;
-  if (xdtype == VC_F32) pack_go<float, float>(p, x, w, N, V, K, target, ignore_index, sv, ws, stream);
-  else if (wdtype == VC_F32) pack_go<bf16, float>(p, x, w, N, V, K, target, ignore_index, sv, ws, stream);
-  else pack_go<bf16, bf16>(p, x, w, N, V, K, target, ignore_index, sv, ws, stream);
-  CeArgs a{(const f16*)(sv + p.o_wp), (const f16*)(sv + p.o_xp), bias, target, ignore_index, (const int*)(sv + p.o_exps), N, V, p.ld,
+  if (xdtype == VC_F32) pack_go<float, float>(p, x, w, bias, N, V, K, target, ignore_index, sv, ws, stream);
+  else if (wdtype == VC_F32) pack_go<bf16, float>(p, x, w, bias, N, V, K, target, ignore_index, sv, ws, stream);
+  else pack_go<bf16, bf16>(p, x, w, bias, N, V, K, target, ignore_index, sv, ws, stream);
+  CeArgs a{(const f16*)(sv + p.o_wp), (const f16*)(sv + p.o_xp), (const float*)(sv + p.o_bl), target, ignore_index, (const int*)(sv + p.o_exps), N, V, p.ld,
            wdtype == VC_BF16, ceil_div(V, GM), ceil_div(N, GM)};
   float4* part = (float4*)(ws + p.f_part);
   float* zt = (float*)(ws + p.f_zt);
@@ -818,8 +830,8 @@ int vc_linear_ce_fwd(int xdtype, int wdtype, const void* x, const void* w, const
   return VC_OK;
 }
 
-int vc_linear_ce_bwd(int xdtype, int wdtype, const void* bias, const int64_t* target, int64_t ignore_index, float smoothing,
-                     int mean, int per_row, const float* dloss, const void* saved, void* dx, void* dw, void* db,
+int vc_linear_ce_bwd(int xdtype, int wdtype, const int64_t* target, int64_t ignore_index, float smoothing, int mean,
+                     int per_row, const float* dloss, const void* saved, void* dx, void* dw, void* db,
                      void* workspace, int accumulate, int N, int V, int K, hipStream_t stream) {
   const int rc = check_ce("vc_linear_ce_bwd", xdtype, wdtype, N, V, K, smoothing);
   if (rc != VC_OK) return rc;
@@ -842,7 +854,7 @@ int vc_linear_ce_bwd(int xdtype, int wdtype, const void* bias, const int64_t* ta
   for (int c = 0; c < p.pieces; ++c) {
     const int vbeg = c * p.piece;
     const int vcols = p.piece < ceil_div(V - vbeg, GM) * GM ? p.piece : ceil_div(V - vbeg, GM) * GM;
-    CeArgs a{wp, xp, bias, target, ignore_index, exps, N, V, p.ld, wdtype == VC_BF16, vcols / GM, tn};
+    CeArgs a{wp, xp, (const float*)(sv + p.o_bl), target, ignore_index, exps, N, V, p.ld, wdtype == VC_BF16, vcols / GM, tn};
     float* dbq = db ? dbp : nullptr;
     if (p.pw == 2) grad_go<2, 2, 2>(a, lse, rs, smoothing, vbeg, vcols, dn, dbq, fac, db, accumulate & 2, stream);
     else if (p.pd == 2) grad_go<1, 1, 2>(a, lse, rs, smoothing, vbeg, vcols, dn, dbq, fac, db, accumulate & 2, stream);

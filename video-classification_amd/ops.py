@@ -1386,7 +1386,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
                ws.data_ptr(), N, V, K)
         ctx.dims, ctx.codes, ctx.opts = (N, V, K), (xd, wd), (ignore_index, smoothing, reduction)
         ctx.params, ctx.xdtype = params, x.dtype
-        ctx.save_for_backward(saved, target, b)
+        ctx.save_for_backward(saved, target)
         if want_pred:
             ctx.mark_non_differentiable(pred, correct)
         return rows if loss is None else loss, pred, correct
@@ -1394,7 +1394,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g, _dpred, _dcorrect):
-        saved, target, b = ctx.saved_tensors
+        saved, target = ctx.saved_tensors
         (N, V, K), (xd, wd), (ignore_index, smoothing, reduction) = ctx.dims, ctx.codes, ctx.opts
         weight, bias = ctx.params
         dev = saved.device
@@ -1404,7 +1404,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         db, add_b = _grad_target(bias)
         ws = torch.empty(_size("vc_linear_ce_bytes", 2, xd, wd, N, V, K), device=dev, dtype=torch.uint8)
         _before_grads(dw, db)
-        L.fast("vc_linear_ce_bwd", dev, xd, wd, _addr(b), target.data_ptr(), ignore_index, smoothing, reduction == "mean",
+        L.fast("vc_linear_ce_bwd", dev, xd, wd, target.data_ptr(), ignore_index, smoothing, reduction == "mean",
                reduction == "none", g.data_ptr(), saved.data_ptr(), _addr(dx), _addr(dw), _addr(db), ws.data_ptr(),
                add_w + 2 * add_b, N, V, K)
         _put_grad(weight, dw)
