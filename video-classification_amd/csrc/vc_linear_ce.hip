@@ -202,10 +202,6 @@ __device__ __forceinline__ void stat_join(Stat& a, const Stat& b) {
   a.m = m;
   a.z += b.z;
 }
-__device__ __forceinline__ Stat stat_shfl(const Stat& a, int o) {
-  return Stat{__shfl_xor(a.m, o, 64), __shfl_xor(a.s, o, 64), __shfl_xor(a.z, o, 64), __shfl_xor(a.arg, o, 64)};
-}
-
 // part[vt][n] = (max, sum, sum z, arg) of the tile, zt[n] = the target's logit.  MORE: also sum z and arg (label smoothing,
 // predictions), which cost four operations more per logit.
 template <int PW, int PX, bool MORE>
@@ -226,24 +222,32 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_stats_kernel(CeArgs a, float4
   int target[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) target[j] = row_target(a, n0 + wn * 64 + j * 16 + l15);
+  // the maximum over the wave's 64 classes first, so that no lane's sum needs rescaling when they are joined
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int n = n0 + wn * 64 + j * 16 + l15;
-    Stat s{-INFINITY, 0.f, 0.f, a.V};
+    st[j] = Stat{-INFINITY, 0.f, 0.f, a.V};
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         acc[i][j][r] = fmaf(acc[i][j][r], scale, bias[i][r]);
-        s.m = fmaxf(s.m, acc[i][j][r]);
+        st[j].m = fmaxf(st[j].m, acc[i][j][r]);
       }
+  }
+#pragma unroll
+  for (int o = 16; o < 64; o <<= 1)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) st[j].m = fmaxf(st[j].m, __shfl_xor(st[j].m, o, 64));
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int n = n0 + wn * 64 + j * 16 + l15;
     if (MORE) {
 #pragma unroll
       for (int e = 15; e >= 0; --e) {
         const int v = v0 + wm * 64 + (e >> 2) * 16 + q * 4 + (e & 3);
         const float z = acc[e >> 2][j][e & 3];
-        if (z == s.m) s.arg = v;
-        if (v < a.V) s.z += z;
+        if (z == st[j].m) st[j].arg = v;
+        if (v < a.V) st[j].z += z;
       }
     }
     const int hit = lane_class(target[j], v0);
@@ -254,16 +258,26 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_stats_kernel(CeArgs a, float4
         if (e == hit) z = acc[e >> 2][j][e & 3];
       if (n < a.N && v0 + wm * 64 + (hit >> 2) * 16 + q * 4 + (hit & 3) < a.V) zt[n] = z;
     }
-    const float ref = s.m == -INFINITY ? 0.f : s.m;
+    const float ref = st[j].m == -INFINITY ? 0.f : st[j].m;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) s.s += __builtin_amdgcn_exp2f(acc[i][j][r] - ref);
-    stat_join(s, stat_shfl(s, 16));
-    stat_join(s, stat_shfl(s, 32));
-    st[j] = s;
-    if (wm == 1 && q == 0) xch[wn * 64 + j * 16 + l15] = make_float4(s.m, s.s, s.z, __int_as_float(s.arg));
+      for (int r = 0; r < 4; ++r) st[j].s += __builtin_amdgcn_exp2f(acc[i][j][r] - ref);
   }
+#pragma unroll
+  for (int o = 16; o < 64; o <<= 1)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      st[j].s += __shfl_xor(st[j].s, o, 64);
+      if (MORE) {
+        st[j].z += __shfl_xor(st[j].z, o, 64);
+        st[j].arg = min(st[j].arg, __shfl_xor(st[j].arg, o, 64));
+      }
+    }
+  if (wm == 1 && q == 0)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      xch[wn * 64 + j * 16 + l15] = make_float4(st[j].m, st[j].s, st[j].z, __int_as_float(st[j].arg));
   __syncthreads();
   if (wm == 0 && q == 0)
 #pragma unroll
