@@ -469,10 +469,12 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_grad_kernel(CeArgs a, const f
     const int n = n0 + wn * 64 + j * 16 + l15, at = min(n, a.N - 1);
     target[j] = row_target(a, n);
     low[j] = lse[at] - 15.f;
-    weight[j] = rs ? rs[at] : a.target[at] == a.ignore ? 0.f : 1.f;
-    if (n >= a.N) weight[j] = 0.f;
+    weight[j] = a.target[at] == a.ignore || n >= a.N ? 0.f : 1.f;
     if (target[j] < 0 || target[j] >= a.V) low[j] = NAN;
   }
+  if (rs)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) weight[j] *= rs[min(n0 + wn * 64 + j * 16 + l15, a.N - 1)];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const float w = weight[j], l = low[j];
@@ -506,11 +508,14 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_grad_kernel(CeArgs a, const f
   for (int half = 0; half < 2; ++half) {
     g16_put(acc, half, tile);
     __syncthreads();
+    F8 d[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) d[u] = g16_get(tile, (threadIdx.x >> 4) + u * 16, (threadIdx.x & 15) * 8);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int e = threadIdx.x + u * G_THREADS, n = n0 + half * 64 + (e >> 4);
       f16x8 hi, lo;
-      f16_split8(g16_get(tile, e >> 4, (e & 15) * 8), hi, lo);
+      f16_split8(d[u], hi, lo);
       if (n < a.N) {
         f16* o = dn + (int64_t)n * vcols + (v0 - vbeg + (e & 15) * 8);
         *reinterpret_cast<f16x8*>(o) = hi;
