@@ -356,10 +356,10 @@ int vc_ce_fwd_bwd(int grad_dtype, const float* logits, int ld, const int64_t* ta
  * and nn.CrossEntropyLoss in one, for label sets whose logits should not be kept; no counterpart in the reference).
  * x [N][K] (xdtype), w [V][K], bias [V] nullable, db [V], dw [V][K] (wdtype), dx [N][K] (xdtype); fp32 x needs fp32 w;
  * N and V up to 2^22, K up to 2^20.  Values of x and of w are resolved to 2^-39 of the largest finite one.  Rows with
- * target == ignore_index count for nothing, whatever x holds there; a target outside [0, V) makes its row's loss and
+ * target == ignore_index count for nothing, are not read, and cost no products; a target outside [0, V) makes its row's loss and
  * gradients NaN.  mean: divide by the rows that count (by 1 if there are none).
- * fwd: row_loss [N] (0 for ignored rows), loss (nullable, one float), pred [N] (nullable, lowest arg-max) and correct
- *   (nullable).  saved: vc_linear_ce_bytes(0, ..) bytes that backward reads; workspace: vc_linear_ce_bytes(1, ..).
+ * fwd: row_loss [N] (0 for ignored rows), loss (nullable, one float), pred [N] (nullable, lowest arg-max, 0 for ignored
+ *   rows) and correct (nullable).  saved: vc_linear_ce_bytes(0, ..) bytes that backward reads; workspace: vc_linear_ce_bytes(1, ..).
  * bwd: dloss = upstream gradient of the mean or sum, or with per_row of every row's loss (each resolved to 2^-39 of the
  *   largest); dx, dw and db (each nullable) are written, or added to where bit 0 (dw) / bit 1 (db) of `accumulate` is
  *   set; workspace: vc_linear_ce_bytes(2, ..).
@@ -368,9 +368,9 @@ int64_t vc_linear_ce_bytes(int what, int xdtype, int wdtype, int N, int V, int K
 int vc_linear_ce_fwd(int xdtype, int wdtype, const void* x, const void* w, const void* bias, const int64_t* target,
                      int64_t ignore_index, float smoothing, int mean, float* row_loss, float* loss, int64_t* pred,
                      int* correct, void* saved, void* workspace, int N, int V, int K, vc_stream_t stream);
-int vc_linear_ce_bwd(int xdtype, int wdtype, const int64_t* target, int64_t ignore_index, float smoothing, int mean,
-                     int per_row, const float* dloss, const void* saved, void* dx, void* dw, void* db, void* workspace,
-                     int accumulate, int N, int V, int K, vc_stream_t stream);
+int vc_linear_ce_bwd(int xdtype, int wdtype, float smoothing, int mean, int per_row, const float* dloss, const void* saved,
+                     void* dx, void* dw, void* db, void* workspace, int accumulate, int N, int V, int K,
+                     vc_stream_t stream);
 /* optim.Adam (L2-coupled) / AdamW / SGD(momentum) (training_utils.py:324-329) over one flat fp32 buffer.
  * mode 0 Adam, 1 AdamW, 2 SGD (b1 = momentum).  grad_scale folds the 1/world of the all-reduce. */
 int vc_optim_step(int mode, float* p, const float* g, float* m, float* v, int64_t n, float lr, float b1, float b2,

@@ -114,7 +114,7 @@ _SIGNATURES = {
     "vc_group_norm_fwd": "i" + 8 * "p" + "iiii" + "fi",
     "vc_group_norm_bwd": "i" + 12 * "p" + "iiii" + "ii",
     "vc_linear_ce_fwd": "ii" + 4 * "p" + "lfi" + 6 * "p" + "iii",
-    "vc_linear_ce_bwd": "ii" + "p" + "lfii" + 6 * "p" + "i" + "iii",
+    "vc_linear_ce_bwd": "iifii" + 6 * "p" + "i" + "iii",
 }
 _CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_int64, "f": ctypes.c_float, "d": ctypes.c_double}
 _bound = {}

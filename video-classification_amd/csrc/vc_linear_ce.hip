@@ -4,7 +4,9 @@
 //   lse_n = log sum_v exp(z_nv),  loss_n = lse_n - (1 - eps) z_{n,t_n} - eps / V sum_v z_nv
 //   d_nv = (exp(z_nv - lse_n) - (1 - eps) [v = t_n] - eps / V) r_n          (r_n the row's weight in the loss)
 //   dx = d W,  dW += d^T x,  db += sum_n d
-// Rows whose target is ignore_index have r_n = 0 and are read as zeros, whatever they hold.
+// Rows whose target is ignore_index have r_n = 0 and are never read: the rows that count are packed one behind the other, and
+// every kernel behind the packing works on those alone, their number read from the device.  (Masked-token losses and padded
+// batches leave out most of their rows; a quarter of them ignored takes a quarter off every product.)
 //
 // 2 N V K operations forward, 6 N V K backward (the logits once more, dx, dW): bound by the matrix pipes for the sizes where
 // time matters, which is why the logits are recomputed rather than kept: N x V fp32 logits written and read cost as much
@@ -13,7 +15,7 @@
 // All products run on fp16 terms (vc_gemm16.h).  x and W are scaled by one power of two each (from their largest finite
 // magnitude): bf16 values are exact in one term over 29 binades and within 2^-40 of the largest magnitude below that, fp32
 // values take two terms (22 bits).  An fp32 master weight next to bf16 activations takes one term (11 bits, against the
-// 8 of a bf16 copy).  d is at most 1 in magnitude and is scaled by 2^15: one term (2^-12 of the value) where the gradient
+// 8 of a bf16 copy).  d is at most 1 in magnitude and is scaled by 2^15: one term (2^-11 of the value) where the gradient
 // it makes is bf16, two where it is fp32.
 #include "vc_gemm16.h"
 
@@ -60,15 +62,71 @@ __device__ __forceinline__ float amax_part(const T* p, int64_t rows, int K, cons
   return m;
 }
 
-// amax[0 .. xb) / [AMAX_MOST ..] = largest finite magnitudes met by the xb blocks of x / the others' of W
+// The rows of a call in the order they are packed: order[0 .. count) = the rows that count, in order, then the others;
+// target[k] = class of the k-th of them, -1 if there is no such class.
+struct RowList {
+  int *order, *target, *count;
+};
+
+// One workgroup, 4096 rows at a time.  Rows that do not count get their loss (0) and prediction (0) here.
+__device__ __forceinline__ void list_rows(const int64_t* __restrict__ target, int64_t ignore, int N, int V, const RowList& l,
+                                          float* __restrict__ rowloss, int64_t* __restrict__ pred) {
+  constexpr int U = 16;
+  __shared__ int counts[2][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int base = 0;
+  for (int n0 = 0, par = 0; n0 < N; n0 += U * 256, par ^= 1) {
+    int64_t t[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) t[u] = target[min(n0 + u * 256 + (int)threadIdx.x, N - 1)];
+    uint64_t keep[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      keep[u] = __ballot(n0 + u * 256 + (int)threadIdx.x < N && t[u] != ignore);
+      if (lane == 0) counts[par][u * 4 + wave] = __popcll(keep[u]);
+    }
+    __syncthreads();
+    const int mine = counts[par][lane];
+    int upto = mine;  // inclusive sum over the 64 runs of 64 rows
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(upto, o, 64);
+      if (lane >= o) upto += v;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int n = n0 + u * 256 + threadIdx.x;
+      const int before = base + __shfl(upto - mine, u * 4 + wave, 64) + __popcll(keep[u] & ((1ull << lane) - 1));
+      if (n >= N) continue;
+      if (keep[u] >> lane & 1) {
+        l.order[before] = n;
+        l.target[before] = t[u] >= 0 && t[u] < V ? (int)t[u] : -1;
+      } else {
+        l.order[N - 1 - (n - before)] = n;
+        rowloss[n] = 0.f;
+        if (pred) pred[n] = 0;
+      }
+    }
+    base += __shfl(upto, 63, 64);
+  }
+  if (threadIdx.x == 0) *l.count = base;
+}
+
+// amax[0 .. xb) / [AMAX_MOST ..] = largest finite magnitudes met by the xb blocks of x / the next ones' of W; the last block
+// lists the rows
 template <typename TX, typename TW>
 __global__ __launch_bounds__(256) void ce_amax_kernel(const TX* __restrict__ x, const TW* __restrict__ w, int N, int V,
                                                       int K, const int64_t* __restrict__ target, int64_t ignore,
-                                                      float* __restrict__ amax, int xb) {
+                                                      float* __restrict__ amax, int xb, RowList rows,
+                                                      float* __restrict__ rowloss, int64_t* __restrict__ pred) {
   __shared__ float sm[4];
-  const int b = blockIdx.x;
+  const int b = blockIdx.x, wb = (int)gridDim.x - 1 - xb;
+  if (b == xb + wb) {
+    list_rows(target, ignore, N, V, rows, rowloss, pred);
+    return;
+  }
   float m = b < xb ? amax_part(x, N, K, target, ignore, b, xb)
-                   : amax_part(w, V, K, (const int64_t*)nullptr, 0, b - xb, (int)gridDim.x - xb);
+                   : amax_part(w, V, K, (const int64_t*)nullptr, 0, b - xb, wb);
   m = wave_max(m);
   if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
   __syncthreads();
@@ -87,25 +145,24 @@ __device__ __forceinline__ int scale_exp(const float* amax, int parts, float* sm
 }
 
 // ---- packing -----------------------------------------------------------------------------------------------------
-// dst[plane][row][ld] = terms of src[row][k] 2^e, zeros behind K; ignored rows are zeros.  A wave per row and 512 columns.
+// dst[plane][row][ld] = terms of src[order[row]][k] 2^e (order null: row), zeros behind K.  A wave per row and 512 columns.
 template <typename T>
 __device__ __forceinline__ void pack_rows(const T* __restrict__ src, f16* __restrict__ dst, int64_t plane, int rows, int K,
-                                          int ld, int planes, int e, const int64_t* target, int64_t ignore, int64_t unit) {
+                                          int ld, int planes, int e, const int* order, int64_t unit) {
   const int per = (ld + 511) / 512;
   const int64_t row = unit / per;
   if (row >= rows) return;
   const int c0 = (int)(unit - row * per) * 512 + (threadIdx.x & 63) * 8;
   if (c0 >= ld) return;
-  const bool drop = target && target[row] == ignore;
-  const T* s = src + row * K;
+  const T* s = src + (order ? order[row] : row) * (int64_t)K;
   float v[8];
-  if (!drop && c0 + 8 <= K && ((uintptr_t)(s + c0) & 15) == 0) {
+  if (c0 + 8 <= K && ((uintptr_t)(s + c0) & 15) == 0) {
     const F8 t = load8(s + c0);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = t.v[i];
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = !drop && c0 + i < K ? to_f32(s[c0 + i]) : 0.f;
+    for (int i = 0; i < 8; ++i) v[i] = c0 + i < K ? to_f32(s[c0 + i]) : 0.f;
   }
   f16x8 hi, lo;
 #pragma unroll
@@ -121,13 +178,13 @@ __device__ __forceinline__ void pack_rows(const T* __restrict__ src, f16* __rest
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
-// exps[0] / [1] = scale exponents of x / W; the first `xblocks` workgroups pack x, the others W and the bias: bl = bias
+// exps[0] / [1] = scale exponents of x / W, [2] = rows that count; the first `xblocks` workgroups pack x, the others W and the bias: bl = bias
 // log2(e) over whole tiles of classes, -inf behind the last one, which leaves the epilogues of the products four plain
 // vector loads (clamped and converted there, these cost a fifth of a tile's time).
 template <typename TX, typename TW>
 __global__ __launch_bounds__(256) void ce_pack_kernel(const TX* __restrict__ x, const TW* __restrict__ w, int N, int V,
-                                                      int K, int ld, int px, int pw, const int64_t* __restrict__ target,
-                                                      int64_t ignore, const float* __restrict__ amax, f16* __restrict__ xp,
+                                                      int K, int ld, int px, int pw, const int* __restrict__ order,
+                                                      const float* __restrict__ amax, f16* __restrict__ xp,
                                                       f16* __restrict__ wp, int* __restrict__ exps, int xblocks, int xb,
                                                       int wb, const TW* __restrict__ bias, float* __restrict__ bl) {
   __shared__ float sm[4];
@@ -135,9 +192,9 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(const TX* __restrict__ x, 
   const int e = scale_exp(isx ? amax : amax + AMAX_MOST, isx ? xb : wb, sm);
   if (threadIdx.x == 0 && ((int)blockIdx.x == 0 || (int)blockIdx.x == xblocks)) exps[isx ? 0 : 1] = e;
   const int64_t unit = (int64_t)(isx ? blockIdx.x : blockIdx.x - xblocks) * 4 + (threadIdx.x >> 6);
-  if (isx) pack_rows(x, xp, (int64_t)N * ld, N, K, ld, px, e, target, ignore, unit);
+  if (isx) pack_rows(x, xp, (int64_t)N * ld, exps[2], K, ld, px, e, order, unit);
   else {
-    pack_rows(w, wp, (int64_t)V * ld, V, K, ld, pw, e, (const int64_t*)nullptr, 0, unit);
+    pack_rows(w, wp, (int64_t)V * ld, V, K, ld, pw, e, (const int*)nullptr, unit);
     const int64_t v = (int64_t)(blockIdx.x - xblocks) * 256 + threadIdx.x;  // four rows or more per workgroup: all classes
     if (v < (V + GM - 1) / GM * GM) bl[v] = v >= V ? -INFINITY : bias ? to_f32(bias[v]) * LOG2E : 0.f;
   }
@@ -149,11 +206,19 @@ struct CeArgs {
   const f16* w;      // [pw][V][ld]
   const f16* x;      // [px][N][ld]
   const float* bl;   // bias log2(e), -inf behind the last class
-  const int64_t* target;
-  int64_t ignore;
+  const int* target; // of the packed rows
   const int* exps;
   int N, V, ld, db_bf16;
-  int tiles_v, tiles_n;
+  int tiles_v;
+
+  __device__ __forceinline__ int rows() const { return exps[2]; }
+  // this workgroup's tile; false behind the rows that count (one row tile is worked even if there are none)
+  __device__ __forceinline__ bool tile(int& tv, int& tn) const {
+    const int tiles_n = max(1, (rows() + GM - 1) / GM), total = tiles_v * tiles_n;
+    if ((int)blockIdx.x >= total) return false;
+    g16_tile(blockIdx.x, total, tiles_v, tiles_n, tv, tn);
+    return true;
+  }
 };
 
 // acc = z log2(e) without the bias, which follows in `bias` (-inf behind the last class): rows v0 + .., columns n0 + ..
@@ -163,7 +228,7 @@ __device__ __forceinline__ void logit_tile(const CeArgs& a, int v0, int n0, f16*
   typedef G16<PW, PX> G;
   G::zero(acc);
   G::run(acc, Op16{a.w + (int64_t)v0 * a.ld, (int64_t)a.V * a.ld, a.ld, a.V - v0, 0},
-         Op16{a.x + (int64_t)n0 * a.ld, (int64_t)a.N * a.ld, a.ld, a.N - n0, 0}, 0, a.ld, smem);
+         Op16{a.x + (int64_t)n0 * a.ld, (int64_t)a.N * a.ld, a.ld, a.rows() - n0, 0}, 0, a.ld, smem);
   const float* bl = a.bl + v0 + (threadIdx.x >> 7) * 64 + ((threadIdx.x & 63) >> 4) * 4;
 #pragma unroll
   for (int i = 0; i < 4; ++i) bias[i] = *reinterpret_cast<const f32x4*>(bl + i * 16);
@@ -185,8 +250,8 @@ __device__ __forceinline__ int lane_class(int t, int v0) {
   return (unsigned)d < 64u && (d & 12) == 0 ? (d >> 4) * 4 + (d & 3) : -1;
 }
 __device__ __forceinline__ int row_target(const CeArgs& a, int n) {
-  const int t = (int)min(max(a.target[min(n, a.N - 1)], (int64_t)-1), (int64_t)a.V);
-  return n < a.N ? t : -1;
+  const int t = a.target[max(min(n, a.rows() - 1), 0)];
+  return n < a.rows() ? t : -1;
 }
 
 // ---- forward: statistics of a tile -----------------------------------------------------------------------------------
@@ -209,7 +274,7 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_stats_kernel(CeArgs a, float4
                                                                 float* __restrict__ zt) {
   __shared__ __attribute__((aligned(1024))) f16 smem[G16<PW, PX>::LDS];
   int tv, tn;
-  g16_tile(blockIdx.x, gridDim.x, a.tiles_v, a.tiles_n, tv, tn);
+  if (!a.tile(tv, tn)) return;
   const int v0 = tv * GM, n0 = tn * GM;
   f32x4 acc[4][4];
   f32x4 bias[4];
@@ -256,7 +321,7 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_stats_kernel(CeArgs a, float4
 #pragma unroll
       for (int e = 0; e < 16; ++e)
         if (e == hit) z = acc[e >> 2][j][e & 3];
-      if (n < a.N && v0 + wm * 64 + (hit >> 2) * 16 + q * 4 + (hit & 3) < a.V) zt[n] = z;
+      zt[n] = z;  // a target lies in [0, V), its row counts
     }
     const float ref = st[j].m == -INFINITY ? 0.f : st[j].m;
 #pragma unroll
@@ -285,17 +350,16 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_stats_kernel(CeArgs a, float4
       const int c = wn * 64 + j * 16 + l15;
       const float4 o = xch[c];
       stat_join(st[j], Stat{o.x, o.y, o.z, __float_as_int(o.w)});
-      if (n0 + c < a.N)
+      if (n0 + c < a.rows())
         part[(int64_t)tv * a.N + n0 + c] = make_float4(st[j].m, st[j].s, st[j].z, __int_as_float(st[j].arg));
     }
 }
 
-// Per row, from its joined statistics: lse (in units of log2), loss (0 for ignored rows, NaN for a target outside [0, V)),
-// arg-max.
+// Per packed row, from its joined statistics: lse (in units of log2); at its place in the call: loss (NaN for a target outside
+// [0, V)) and arg-max.
 struct CeRows {
   const float* zt;
-  const int64_t* target;
-  int64_t ignore;
+  const int *target, *order, *exps;
   int N, V, tiles_v;
   float smooth;
   float *lse, *rowloss;
@@ -304,17 +368,14 @@ struct CeRows {
 __device__ __forceinline__ float row_out(const CeRows& k, int n, const Stat& s) {
   const float l = (s.m == -INFINITY ? 0.f : s.m) + log2f(s.s);
   k.lse[n] = l;
-  const int64_t t = k.target[n];
-  float loss = 0.f;
-  if (t != k.ignore) {
-    if (t < 0 || t >= k.V) loss = NAN;
-    else {
-      const float d = l - k.zt[n];
-      loss = LN2 * (k.smooth > 0.f ? (1.f - k.smooth) * d + k.smooth * (l - s.z / (float)k.V) : d);
-    }
+  float loss = NAN;
+  if (k.target[n] >= 0) {
+    const float d = l - k.zt[n];
+    loss = LN2 * (k.smooth > 0.f ? (1.f - k.smooth) * d + k.smooth * (l - s.z / (float)k.V) : d);
   }
-  k.rowloss[n] = loss;
-  if (k.pred) k.pred[n] = s.arg < k.V ? s.arg : 0;
+  const int at = k.order[n];
+  k.rowloss[at] = loss;
+  if (k.pred) k.pred[at] = s.arg < k.V ? s.arg : 0;
   return loss;
 }
 __device__ __forceinline__ Stat row_join(const CeRows& k, const float4* part, int n, int t0, int t1) {
@@ -331,9 +392,10 @@ __device__ __forceinline__ Stat row_join(const CeRows& k, const float4* part, in
 __global__ __launch_bounds__(256) void ce_join_kernel(CeRows k, const float4* __restrict__ part) {
   __shared__ Stat sm[32][8];
   const int e = threadIdx.x & 7, run = threadIdx.x >> 3;
-  const int n = blockIdx.x * 8 + e, per = (k.tiles_v + 31) / 32;
+  const int n = blockIdx.x * 8 + e, per = (k.tiles_v + 31) / 32, rows = k.exps[2];
+  if (blockIdx.x * 8 >= rows) return;
   Stat s{-INFINITY, 0.f, 0.f, k.V};
-  if (n < k.N) s = row_join(k, part, n, run * per, min(k.tiles_v, (run + 1) * per));
+  if (n < rows) s = row_join(k, part, n, run * per, min(k.tiles_v, (run + 1) * per));
   sm[run][e] = s;
   __syncthreads();
 #pragma unroll
@@ -344,7 +406,7 @@ __global__ __launch_bounds__(256) void ce_join_kernel(CeRows k, const float4* __
     }
     __syncthreads();
   }
-  if (run == 0 && n < k.N) {
+  if (run == 0 && n < rows) {
     stat_join(s, sm[1][e]);
     row_out(k, n, s);
   }
@@ -358,59 +420,52 @@ __global__ __launch_bounds__(1024) void ce_total_kernel(CeRows k, const float4* 
                                                         float* __restrict__ loss, float* __restrict__ total,
                                                         int* __restrict__ correct) {
   __shared__ double sd[16];
-  __shared__ int sc[16], sk[16];
+  __shared__ int sk[16];
   double a = 0.0;
-  int c = 0, hits = 0;
-  for (int n = threadIdx.x; n < k.N; n += 1024) {
-    const float l = JOIN ? row_out(k, n, row_join(k, part, n, 0, k.tiles_v)) : k.rowloss[n];
-    const int64_t t = k.target[n];
-    if (t != k.ignore) {
-      a += (double)l;
-      ++c;
-      if (k.pred && k.pred[n] == t) ++hits;
-    }
+  int hits = 0;
+  const int rows = k.exps[2];
+  for (int n = threadIdx.x; n < rows; n += 1024) {
+    const int at = k.order[n];
+    a += (double)(JOIN ? row_out(k, n, row_join(k, part, n, 0, k.tiles_v)) : k.rowloss[at]);
+    if (k.pred && k.pred[at] == k.target[n]) ++hits;
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     a += __shfl_xor(a, o, 64);
-    c += __shfl_xor(c, o, 64);
     hits += __shfl_xor(hits, o, 64);
   }
   if ((threadIdx.x & 63) == 0) {
     sd[threadIdx.x >> 6] = a;
-    sc[threadIdx.x >> 6] = c;
     sk[threadIdx.x >> 6] = hits;
   }
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int i = 1; i < 16; ++i) {
       a += sd[i];
-      c += sc[i];
       hits += sk[i];
     }
-    if (loss) *loss = (float)(mean ? a / (double)max(c, 1) : a);
-    total[0] = (float)c;
+    if (loss) *loss = (float)(mean ? a / (double)max(rows, 1) : a);
+    total[0] = (float)rows;
     if (correct) *correct = hits;
   }
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------------
-// Per-row upstream gradients: rs[n] = weight of row n relative to the largest one (0 for ignored rows), fac[0] = that largest
-// weight.
-__global__ __launch_bounds__(1024) void ce_weights_kernel(const float* __restrict__ g, const int64_t* __restrict__ target,
-                                                          int64_t ignore, int N, float* __restrict__ rs,
+// Per-row upstream gradients: rs[k] = weight of packed row k relative to the largest one, fac[0] = that largest weight.
+__global__ __launch_bounds__(1024) void ce_weights_kernel(const float* __restrict__ g, const int* __restrict__ order,
+                                                          const int* __restrict__ exps, float* __restrict__ rs,
                                                           float* __restrict__ fac) {
   __shared__ float sm[16];
+  const int rows = exps[2];
   float big = 0.f;
-  for (int n = threadIdx.x; n < N; n += 1024)
-    if (target[n] != ignore) big = fmaxf(big, finite_mag(g[n]));
+  for (int k = threadIdx.x; k < rows; k += 1024) big = fmaxf(big, finite_mag(g[order[k]]));
   big = wave_max(big);
   if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = big;
   __syncthreads();
   big = sm[0];
   for (int i = 1; i < 16; ++i) big = fmaxf(big, sm[i]);
   if (!(big > 0.f)) big = 1.f;
-  for (int n = threadIdx.x; n < N; n += 1024) rs[n] = target[n] == ignore ? 0.f : g[n] / big;
+  for (int k = threadIdx.x; k < rows; k += 1024) rs[k] = g[order[k]] / big;
   if (threadIdx.x == 0) fac[0] = big;
 }
 
@@ -447,7 +502,7 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_grad_kernel(CeArgs a, const f
   __shared__ __attribute__((aligned(1024))) f16 smem[G16<PW, PX>::LDS];
   __shared__ float sb[2][GM];
   int tv, tn;
-  g16_tile(blockIdx.x, gridDim.x, a.tiles_v, a.tiles_n, tv, tn);
+  if (!a.tile(tv, tn)) return;
   const int v0 = vbeg + tv * GM, n0 = tn * GM;
   f32x4 acc[4][4];
   f32x4 bias[4];
@@ -462,19 +517,23 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_grad_kernel(CeArgs a, const f
 #pragma unroll
     for (int r = 0; r < 4; ++r) col[i][r] = 0.f;
   const int64_t plane = (int64_t)a.N * vcols;
+  const int rows = a.rows();
   int target[4];
   float weight[4], low[4];  // 2^(z - low) is the scaled probability
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int n = n0 + wn * 64 + j * 16 + l15, at = min(n, a.N - 1);
+    const int n = n0 + wn * 64 + j * 16 + l15;
     target[j] = row_target(a, n);
-    low[j] = lse[at] - 15.f;
-    weight[j] = a.target[at] == a.ignore || n >= a.N ? 0.f : 1.f;
-    if (target[j] < 0 || target[j] >= a.V) low[j] = NAN;
+    low[j] = lse[max(min(n, rows - 1), 0)] - 15.f;
+    weight[j] = n < rows ? 1.f : 0.f;
+    if (target[j] < 0) low[j] = NAN;
   }
   if (rs)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) weight[j] *= rs[min(n0 + wn * 64 + j * 16 + l15, a.N - 1)];
+    for (int j = 0; j < 4; ++j) {
+      const int n = n0 + wn * 64 + j * 16 + l15;
+      if (n < rows) weight[j] = rs[n];
+    }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const float w = weight[j], l = low[j];
@@ -494,7 +553,7 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_grad_kernel(CeArgs a, const f
 #pragma unroll
       for (int e = 0; e < 16; ++e)
         if (e == hit) acc[e >> 2][j][e & 3] -= (1.f - smooth) * D_SCALE;
-    const bool live = w != 0.f;  // rows that do not count vanish whatever they hold
+    const bool live = w != 0.f;  // a row without weight vanishes whatever it holds
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -516,7 +575,7 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_grad_kernel(CeArgs a, const f
       const int e = threadIdx.x + u * G_THREADS, n = n0 + half * 64 + (e >> 4);
       f16x8 hi, lo;
       f16_split8(d[u], hi, lo);
-      if (n < a.N) {
+      if (n < rows) {
         f16* o = dn + (int64_t)n * vcols + (v0 - vbeg + (e & 15) * 8);
         *reinterpret_cast<f16x8*>(o) = hi;
         if (PD == 2) *reinterpret_cast<f16x8*>(o + plane) = lo;
@@ -536,7 +595,7 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_grad_kernel(CeArgs a, const f
     const int v = v0 + threadIdx.x;
     if (threadIdx.x < GM && v < a.V) {
       const float s = sb[0][threadIdx.x] + sb[1][threadIdx.x];
-      if (a.tiles_n > 1) dbpart[(int64_t)tn * a.V + v] = s;
+      if (a.N > GM) dbpart[(int64_t)tn * a.V + v] = s;
       else if (a.db_bf16) bias_out((bf16*)db + v, s, fac, add);  // the only row tile
       else bias_out((float*)db + v, s, fac, add);
     }
@@ -545,8 +604,9 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_grad_kernel(CeArgs a, const f
 
 // db[v] (+)= fac sum over the row tiles of dbpart[tile][v]
 template <typename T>
-__global__ __launch_bounds__(256) void ce_bias_kernel(const float* __restrict__ dbpart, int tiles, int V,
+__global__ __launch_bounds__(256) void ce_bias_kernel(const float* __restrict__ dbpart, const int* __restrict__ exps, int V,
                                                       CeFac fac, int add, T* __restrict__ db) {
+  const int tiles = max(1, (exps[2] + GM - 1) / GM);
   const int v = blockIdx.x * 256 + threadIdx.x;
   if (v >= V) return;
   float s = 0.f;
@@ -558,13 +618,14 @@ __global__ __launch_bounds__(256) void ce_bias_kernel(const float* __restrict__ 
 // out[m][c] = factor * sum over the reduction of (row side)[m] (column side)[c]: dx = d W and dW = d^T x
 struct MmArgs {
   Op16 c, m;                   // column side (W or x, COL) and row side (d: ROW for dx, COL for dW), at their corners
-  int M, Nn, k;                // rows and columns of the result, reduction length (a multiple of 64)
+  int M, Nn, k;                // rows and columns of the result, reduction length of dx (a multiple of 64)
   int tiles_m, tiles_n, splits, kper;
+  const int* order;            // dx: where its packed rows go
   float* part;                 // [splits][M][Nn], or null: write out
   int add;                     // add to what part / out hold
   void* out;                   // [M][Nn]
   CeFac fac;
-  const int* exps;
+  const int* exps;             // exps[2] = rows that count: rows of dx that are worked, reduction length of dW
   int which;                   // whose scale exponent the column side carries
   int vec;                     // rows of the result start on 16-byte (fp32) / 8-byte (bf16) boundaries
 };
@@ -577,22 +638,34 @@ template <int PC, int PM, int KM, typename T>
 __global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
   typedef G16<PC, PM, COL, KM> G;
   __shared__ __attribute__((aligned(1024))) f16 smem[G::LDS];
-  const int tiles = g.tiles_m * g.tiles_n;
-  const int split = blockIdx.x / tiles;
-  int tm, tn;
-  g16_tile(blockIdx.x - split * tiles, tiles, g.tiles_m, g.tiles_n, tm, tn);
+  const int rows = g.exps[2];
+  const int tiles_m = KM == ROW ? max(1, (rows + GM - 1) / GM) : g.tiles_m, tiles = tiles_m * g.tiles_n;
+  int split = blockIdx.x / tiles, tm, tn;
+  const bool idle = split >= g.splits;  // dx: behind the rows that count
+  if (idle) {
+    if (g.part) return;  // ce_dx_kernel writes their zeros
+    const int id = blockIdx.x - tiles * g.splits;
+    tm = tiles_m + id / g.tiles_n;
+    tn = id % g.tiles_n;
+    split = 0;
+  } else
+    g16_tile(blockIdx.x - split * tiles, tiles, tiles_m, g.tiles_n, tm, tn);
   const int m0 = tm * GM, n0 = tn * GM;
   f32x4 acc[4][4];
   G::zero(acc);
-  const int k0 = split * g.kper, k1 = min(g.k, k0 + g.kper);
+  const int klen = KM == ROW ? g.k : (rows + 63) / 64 * 64;
+  const int per = KM == ROW ? g.kper : ((klen + g.splits - 1) / g.splits + 63) / 64 * 64;
+  const int k0 = split * per, k1 = min(klen, k0 + per);
   Op16 c = g.c, m = g.m;
   c.side = n0;
   if (KM == ROW) {
     m.p += (int64_t)m0 * m.ld;
-    m.n = g.M - m0;
-  } else
+    m.n = rows - m0;
+  } else {
     m.side = m0;
-  G::run(acc, c, m, k0, k1, smem);
+    m.n = c.n = rows;
+  }
+  if (!idle) G::run(acc, c, m, k0, k1, smem);
   const int lane = threadIdx.x & 63, q = lane >> 4, l15 = lane & 15;
   const int wave = threadIdx.x >> 6, wc = wave >> 1, wr = wave & 1;
   const float f = g.part ? 1.f : mm_factor(g.fac, g.exps, g.which);
@@ -603,13 +676,24 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[i][j] *= f;
+  // dx: packed rows go to their places, those that do not count as zeros
+  const int live = KM == ROW ? rows : g.M, end = KM == ROW && part ? rows : g.M;
+  int64_t at[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int row = m0 + wr * 64 + j * 16 + l15, r = min(row, g.M - 1);
+    at[j] = (int64_t)(KM == ROW && !part ? g.order[r] : r) * g.Nn;
+    if (row >= live)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
   // what is added to comes first: the stores could alias these loads and would hold them back
   if (vec && g.add) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int64_t o = (int64_t)min(m0 + wr * 64 + j * 16 + l15, g.M - 1) * g.Nn + min(n0 + wc * 64 + i * 16 + q * 4, g.Nn - 4);
+        const int64_t o = at[j] + min(n0 + wc * 64 + i * 16 + q * 4, g.Nn - 4);
         if (part) acc[i][j] += *reinterpret_cast<const f32x4*>(part + o);
         else if constexpr (sizeof(T) == 4) acc[i][j] += *reinterpret_cast<const f32x4*>((const float*)g.out + o);
         else {
@@ -621,12 +705,11 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int row = m0 + wr * 64 + j * 16 + l15;
-    if (row >= g.M) continue;
+    if (m0 + wr * 64 + j * 16 + l15 >= end) continue;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int col = n0 + wc * 64 + i * 16 + q * 4;  // four results of one row
-      const int64_t o = (int64_t)row * g.Nn + col;
+      const int64_t o = at[j] + col;
       const f32x4 v = acc[i][j];
       if (vec) {
         if (col >= g.Nn) continue;
@@ -644,6 +727,49 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
           }
         }
       }
+    }
+  }
+}
+
+// dx[order[r]] = factor * sum over the slices, in order, of packed row r; zeros for rows that do not count.  A wave per row and
+// 512 columns.
+template <typename T>
+__global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ part, int slices, int N, int K, CeFac fac,
+                                                    const int* __restrict__ exps, const int* __restrict__ order, int vec,
+                                                    T* __restrict__ out) {
+  const int per = (K + 511) / 512;
+  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), n = (int64_t)N * K;
+  const int r = (int)(unit / per), c0 = (int)(unit - (int64_t)r * per) * 512 + (threadIdx.x & 63) * (vec ? 8 : 1);
+  if (r >= N) return;
+  const bool live = r < exps[2];
+  const float f = mm_factor(fac, exps, 1);
+  const float* p = part + (int64_t)r * K;
+  T* o = out + (int64_t)order[r] * K;
+  if (vec) {
+    if (c0 >= K) return;
+    F8 s;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s.v[e] = 0.f;
+    if (live)
+#pragma unroll 4
+      for (int k = 0; k < slices; ++k) {
+        const F8 v = load8(p + k * n + c0);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s.v[e] += v.v[e];
+      }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s.v[e] *= f;
+    if (!live)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s.v[e] = 0.f;
+    store8(o + c0, s);
+  } else {
+    for (int c = c0; c < c0 + 512 && c < K; c += 64) {
+      float s = 0.f;
+      if (live)
+#pragma unroll 4
+        for (int k = 0; k < slices; ++k) s += p[k * n + c];
+      o[c] = from_f32<T>(live ? s * f : 0.f);
     }
   }
 }
@@ -671,8 +797,8 @@ struct Plan {
   int pdx, pdw, pd;            // terms of d for dx and dW, and the larger of the two
   int piece, pieces;           // classes of a piece
   int sx, kx, sw, kw;          // slices of the reductions of dx (per piece) and dW, and their lengths
-  // forward workspace (saved for backward): packed x, packed W, exponents, bias, lse, total
-  int64_t o_xp, o_wp, o_exps, o_bl, o_lse, o_total, saved;
+  // forward workspace (saved for backward): packed x, packed W, exponents and count, bias, row list, lse, total
+  int64_t o_xp, o_wp, o_exps, o_bl, o_order, o_target, o_lse, o_total, saved;
   // forward scratch
   int64_t f_amax, f_part, f_zt, fwd;
   // backward scratch
@@ -720,6 +846,8 @@ Plan make_plan(int xf32, int wf32, int N, int V, int K) {
   p.o_wp = take((int64_t)p.pw * V * p.ld * 2);
   p.o_exps = take(16);
   p.o_bl = take((int64_t)all * 4);
+  p.o_order = take((int64_t)N * 4);
+  p.o_target = take((int64_t)N * 4);
   p.o_lse = take((int64_t)N * 4);
   p.o_total = take(16);
   p.saved = o;
@@ -758,7 +886,7 @@ int check_ce(const char* who, int xdtype, int wdtype, int N, int V, int K, float
 
 template <typename TX, typename TW>
 void pack_go(const Plan& p, const void* x, const void* w, const void* bias, int N, int V, int K, const int64_t* target, int64_t ignore,
-             char* saved, char* ws, hipStream_t st) {
+             float* rowloss, int64_t* pred, char* saved, char* ws, hipStream_t st) {
   float* amax = (float*)(ws + p.f_amax);
   const int per = ceil_div(p.ld, 512);
   const int xb = (int)ceil_div64((int64_t)N * per, 4), wb = (int)ceil_div64((int64_t)V * per, 4);
@@ -767,10 +895,11 @@ void pack_go(const Plan& p, const void* x, const void* w, const void* bias, int 
     return (int)(b < AMAX_MOST ? b : AMAX_MOST);
   };
   const int xa = blocks((int64_t)N * K), wa = blocks((int64_t)V * K);
-  hipLaunchKernelGGL((ce_amax_kernel<TX, TW>), dim3(xa + wa), dim3(256), 0, st, (const TX*)x, (const TW*)w, N, V, K, target,
-                     ignore, amax, xa);
+  hipLaunchKernelGGL((ce_amax_kernel<TX, TW>), dim3(xa + wa + 1), dim3(256), 0, st, (const TX*)x, (const TW*)w, N, V, K,
+                     target, ignore, amax, xa, RowList{(int*)(saved + p.o_order), (int*)(saved + p.o_target), (int*)(saved + p.o_exps) + 2},
+                     rowloss, pred);
   hipLaunchKernelGGL((ce_pack_kernel<TX, TW>), dim3(xb + wb), dim3(256), 0, st, (const TX*)x, (const TW*)w, N, V, K, p.ld,
-                     p.px, p.pw, target, ignore, amax, (f16*)(saved + p.o_xp), (f16*)(saved + p.o_wp),
+                     p.px, p.pw, (const int*)(saved + p.o_order), amax, (f16*)(saved + p.o_xp), (f16*)(saved + p.o_wp),
                      (int*)(saved + p.o_exps), xb, xa, wa, (const TW*)bias, (float*)(saved + p.o_bl));
 }
 
@@ -782,14 +911,14 @@ void mm_go(const MmArgs& g, int out_bf16, hipStream_t st) {
 }
 template <int PW, int PX>
 void stats_go(const CeArgs& a, bool more, float4* part, float* zt, hipStream_t st) {
-  const dim3 grid(a.tiles_v * a.tiles_n), blk(G_THREADS);
+  const dim3 grid(a.tiles_v * ceil_div(a.N, GM)), blk(G_THREADS);
   if (more) hipLaunchKernelGGL((ce_stats_kernel<PW, PX, true>), grid, blk, 0, st, a, part, zt);
   else hipLaunchKernelGGL((ce_stats_kernel<PW, PX, false>), grid, blk, 0, st, a, part, zt);
 }
 template <int PW, int PX, int PD>
 void grad_go(const CeArgs& a, const float* lse, const float* rs, float smooth, int vbeg, int vcols, f16* dn, float* dbp,
              const CeFac& fac, void* db, int add, hipStream_t st) {
-  hipLaunchKernelGGL((ce_grad_kernel<PW, PX, PD>), dim3(a.tiles_v * a.tiles_n), dim3(G_THREADS), 0, st, a, lse, rs, smooth,
+  hipLaunchKernelGGL((ce_grad_kernel<PW, PX, PD>), dim3(a.tiles_v * ceil_div(a.N, GM)), dim3(G_THREADS), 0, st, a, lse, rs, smooth,
                      vbeg, vcols, dn, dbp, fac, db, add);
 }
 template <int KM>
@@ -797,6 +926,13 @@ void mm_terms(int pc, int pm, const MmArgs& g, int out_bf16, hipStream_t st) {
   if (pm == 1) mm_go<1, 1, KM>(g, out_bf16, st);
   else if (pc == 1) mm_go<1, 2, KM>(g, out_bf16, st);
   else mm_go<2, 2, KM>(g, out_bf16, st);
+}
+void dx_go(const float* part, int slices, int N, int K, const CeFac& fac, const int* exps, const int* order, void* dx,
+           int out_bf16, hipStream_t st) {
+  const dim3 grid((unsigned)ceil_div64((int64_t)N * ceil_div(K, 512), 4));
+  const int vec = K % 8 == 0 && ((uintptr_t)dx & 15) == 0;
+  if (out_bf16) hipLaunchKernelGGL((ce_dx_kernel<bf16>), grid, dim3(256), 0, st, part, slices, N, K, fac, exps, order, vec, (bf16*)dx);
+  else hipLaunchKernelGGL((ce_dx_kernel<float>), grid, dim3(256), 0, st, part, slices, N, K, fac, exps, order, vec, (float*)dx);
 }
 void reduce_go(const float* part, int slices, int64_t n, const CeFac& fac, const int* exps, int which, int add, void* out,
                int out_bf16, hipStream_t st) {
@@ -827,17 +963,17 @@ int vc_linear_ce_fwd(int xdtype, int wdtype, const void* x, const void* w, const
   VC_CHECK_ARG((((uintptr_t)saved | (uintptr_t)workspace) & 255) == 0, "vc_linear_ce_fwd: buffers must be 256-byte aligned");
   const Plan p = make_plan(xdtype == VC_F32, wdtype == VC_F32, N, V, K);
   char *sv = (char*)saved, *ws = (char*)workspace;
-  if (xdtype == VC_F32) pack_go<float, float>(p, x, w, bias, N, V, K, target, ignore_index, sv, ws, stream);
-  else if (wdtype == VC_F32) pack_go<bf16, float>(p, x, w, bias, N, V, K, target, ignore_index, sv, ws, stream);
-  else pack_go<bf16, bf16>(p, x, w, bias, N, V, K, target, ignore_index, sv, ws, stream);
-  CeArgs a{(const f16*)(sv + p.o_wp), (const f16*)(sv + p.o_xp), (const float*)(sv + p.o_bl), target, ignore_index, (const int*)(sv + p.o_exps), N, V, p.ld,
-           wdtype == VC_BF16, ceil_div(V, GM), ceil_div(N, GM)};
+  if (xdtype == VC_F32) pack_go<float, float>(p, x, w, bias, N, V, K, target, ignore_index, row_loss, pred, sv, ws, stream);
+  else if (wdtype == VC_F32) pack_go<bf16, float>(p, x, w, bias, N, V, K, target, ignore_index, row_loss, pred, sv, ws, stream);
+  else pack_go<bf16, bf16>(p, x, w, bias, N, V, K, target, ignore_index, row_loss, pred, sv, ws, stream);
+  CeArgs a{(const f16*)(sv + p.o_wp), (const f16*)(sv + p.o_xp), (const float*)(sv + p.o_bl), (const int*)(sv + p.o_target), (const int*)(sv + p.o_exps), N, V, p.ld,
+           wdtype == VC_BF16, ceil_div(V, GM)};
   float4* part = (float4*)(ws + p.f_part);
   float* zt = (float*)(ws + p.f_zt);
   const bool more = smoothing > 0.f || pred;
   if (p.pw == 2) stats_go<2, 2>(a, more, part, zt, stream);
   else stats_go<1, 1>(a, more, part, zt, stream);
-  const CeRows rows{zt, target, ignore_index, N, V, a.tiles_v, smoothing, (float*)(sv + p.o_lse), row_loss, pred};
+  const CeRows rows{zt, a.target, (const int*)(sv + p.o_order), a.exps, N, V, a.tiles_v, smoothing, (float*)(sv + p.o_lse), row_loss, pred};
   float* total = (float*)(sv + p.o_total);
   if (N <= 1024 && a.tiles_v <= 16) {
     hipLaunchKernelGGL(ce_total_kernel<true>, dim3(1), dim3(1024), 0, stream, rows, part, mean, loss, total, correct);
@@ -849,12 +985,12 @@ int vc_linear_ce_fwd(int xdtype, int wdtype, const void* x, const void* w, const
   return VC_OK;
 }
 
-int vc_linear_ce_bwd(int xdtype, int wdtype, const int64_t* target, int64_t ignore_index, float smoothing, int mean,
+int vc_linear_ce_bwd(int xdtype, int wdtype, float smoothing, int mean,
                      int per_row, const float* dloss, const void* saved, void* dx, void* dw, void* db,
                      void* workspace, int accumulate, int N, int V, int K, hipStream_t stream) {
   const int rc = check_ce("vc_linear_ce_bwd", xdtype, wdtype, N, V, K, smoothing);
   if (rc != VC_OK) return rc;
-  VC_CHECK_ARG(target && dloss && saved && workspace, "vc_linear_ce_bwd: null pointer");
+  VC_CHECK_ARG(dloss && saved && workspace, "vc_linear_ce_bwd: null pointer");
   VC_CHECK_ARG(!(mean && per_row), "vc_linear_ce_bwd: a mean has one upstream gradient");
   VC_CHECK_ARG((((uintptr_t)saved | (uintptr_t)workspace) & 255) == 0, "vc_linear_ce_bwd: buffers must be 256-byte aligned");
   if (!dx && !dw && !db) return VC_OK;
@@ -864,16 +1000,17 @@ int vc_linear_ce_bwd(int xdtype, int wdtype, const int64_t* target, int64_t igno
   const f16 *xp = (const f16*)(sv + p.o_xp), *wp = (const f16*)(sv + p.o_wp);
   f16* dn = (f16*)(ws + p.b_dn);
   const int* exps = (const int*)(sv + p.o_exps);
+  const int* order = (const int*)(sv + p.o_order);
   const float* lse = (const float*)(sv + p.o_lse);
   float *rs = (float*)(ws + p.b_rs), *big = (float*)(ws + p.b_fac), *dbp = (float*)(ws + p.b_db);
   const CeFac fac{per_row ? big : nullptr, dloss, mean ? (const float*)(sv + p.o_total) : nullptr};
   const int tn = ceil_div(N, GM), tk = ceil_div(K, GM);
-  if (per_row) hipLaunchKernelGGL(ce_weights_kernel, dim3(1), dim3(1024), 0, stream, dloss, target, ignore_index, N, rs, big);
+  if (per_row) hipLaunchKernelGGL(ce_weights_kernel, dim3(1), dim3(1024), 0, stream, dloss, order, exps, rs, big);
   else rs = nullptr;
   for (int c = 0; c < p.pieces; ++c) {
     const int vbeg = c * p.piece;
     const int vcols = p.piece < ceil_div(V - vbeg, GM) * GM ? p.piece : ceil_div(V - vbeg, GM) * GM;
-    CeArgs a{wp, xp, (const float*)(sv + p.o_bl), target, ignore_index, exps, N, V, p.ld, wdtype == VC_BF16, vcols / GM, tn};
+    CeArgs a{wp, xp, (const float*)(sv + p.o_bl), (const int*)(sv + p.o_target), exps, N, V, p.ld, wdtype == VC_BF16, vcols / GM};
     float* dbq = db ? dbp : nullptr;
     if (p.pw == 2) grad_go<2, 2, 2>(a, lse, rs, smoothing, vbeg, vcols, dn, dbq, fac, db, accumulate & 2, stream);
     else if (p.pd == 2) grad_go<1, 1, 2>(a, lse, rs, smoothing, vbeg, vcols, dn, dbq, fac, db, accumulate & 2, stream);
@@ -888,6 +1025,7 @@ int vc_linear_ce_bwd(int xdtype, int wdtype, const int64_t* target, int64_t igno
       g.c = Op16{wp + (int64_t)vbeg * p.ld, (int64_t)V * p.ld, p.ld, rows, 0};
       g.m = Op16{dn, (int64_t)N * vcols, vcols, N, 0};
       g.M = N;
+      g.order = order;
       g.k = pad64(rows);
       g.tiles_m = tn;
       g.splits = p.sx;
@@ -918,13 +1056,13 @@ int vc_linear_ce_bwd(int xdtype, int wdtype, const int64_t* target, int64_t igno
     }
   }
   if (dx && p.b_px >= 0)
-    reduce_go((const float*)(ws + p.b_px), p.sx, (int64_t)N * K, fac, exps, 1, 0, dx, xdtype == VC_BF16, stream);
+    dx_go((const float*)(ws + p.b_px), p.sx, N, K, fac, exps, order, dx, xdtype == VC_BF16, stream);
   if (db && tn > 1) {
     if (wdtype == VC_BF16)
-      hipLaunchKernelGGL((ce_bias_kernel<bf16>), dim3(ceil_div(V, 256)), dim3(256), 0, stream, dbp, tn, V, fac,
+      hipLaunchKernelGGL((ce_bias_kernel<bf16>), dim3(ceil_div(V, 256)), dim3(256), 0, stream, dbp, exps, V, fac,
                          accumulate & 2, (bf16*)db);
     else
-      hipLaunchKernelGGL((ce_bias_kernel<float>), dim3(ceil_div(V, 256)), dim3(256), 0, stream, dbp, tn, V, fac,
+      hipLaunchKernelGGL((ce_bias_kernel<float>), dim3(ceil_div(V, 256)), dim3(256), 0, stream, dbp, exps, V, fac,
                          accumulate & 2, (float*)db);
   }
   VC_LAUNCH_CHECK("vc_linear_ce_bwd");

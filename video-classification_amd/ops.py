@@ -1384,9 +1384,9 @@ class _LinearCrossEntropy(torch.autograd.Function):
         L.fast("vc_linear_ce_fwd", dev, xd, wd, x.data_ptr(), w.data_ptr(), _addr(b), target.data_ptr(), ignore_index,
                smoothing, reduction == "mean", rows.data_ptr(), _addr(loss), _addr(pred), _addr(correct), saved.data_ptr(),
                ws.data_ptr(), N, V, K)
-        ctx.dims, ctx.codes, ctx.opts = (N, V, K), (xd, wd), (ignore_index, smoothing, reduction)
+        ctx.dims, ctx.codes, ctx.opts = (N, V, K), (xd, wd), (smoothing, reduction)
         ctx.params, ctx.xdtype = params, x.dtype
-        ctx.save_for_backward(saved, target)
+        ctx.save_for_backward(saved)
         if want_pred:
             ctx.mark_non_differentiable(pred, correct)
         return rows if loss is None else loss, pred, correct
@@ -1394,8 +1394,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g, _dpred, _dcorrect):
-        saved, target = ctx.saved_tensors
-        (N, V, K), (xd, wd), (ignore_index, smoothing, reduction) = ctx.dims, ctx.codes, ctx.opts
+        saved, = ctx.saved_tensors
+        (N, V, K), (xd, wd), (smoothing, reduction) = ctx.dims, ctx.codes, ctx.opts
         weight, bias = ctx.params
         dev = saved.device
         g = g.contiguous().float()
@@ -1404,9 +1404,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
         db, add_b = _grad_target(bias)
         ws = torch.empty(_size("vc_linear_ce_bytes", 2, xd, wd, N, V, K), device=dev, dtype=torch.uint8)
         _before_grads(dw, db)
-        L.fast("vc_linear_ce_bwd", dev, xd, wd, target.data_ptr(), ignore_index, smoothing, reduction == "mean",
-               reduction == "none", g.data_ptr(), saved.data_ptr(), _addr(dx), _addr(dw), _addr(db), ws.data_ptr(),
-               add_w + 2 * add_b, N, V, K)
+        L.fast("vc_linear_ce_bwd", dev, xd, wd, smoothing, reduction == "mean", reduction == "none", g.data_ptr(),
+               saved.data_ptr(), _addr(dx), _addr(dw), _addr(db), ws.data_ptr(), add_w + 2 * add_b, N, V, K)
         _put_grad(weight, dw)
         _put_grad(bias, db)
         _after_grads(dw, db)
@@ -1419,12 +1418,13 @@ def linear_cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoot
     ``cross_entropy(linear(x, weight, bias, out_f32=True), target)`` computes, in pieces of the classes.
 
     x [..., K] float32 or bfloat16, weight [V, K] and bias [V] (or None) float32, or bfloat16 next to bfloat16 x, target
-    int64 of x's leading shape.  Rows whose target is `ignore_index` count for nothing; any other target outside [0, V)
-    makes the loss NaN.  reduction: "mean" over the rows that count (0 if there are none), "sum", or "none" (a loss per row,
-    0 where ignored).  The loss is float32; gradients of weight and bias, which have to be leaves, are accumulated into
-    .grad.  Values of x and of the weight are resolved to 2^-39 of the largest finite one of each, and with "none" a row's
-    gradient to 2^-39 of the largest upstream gradient.  stats: a dict that receives "pred" (arg-max per row) and "correct"
-    (rows that count and are right).  At most 2^22 rows, 2^22 classes and K = 2^20."""
+    int64 of x's leading shape.  Rows whose target is `ignore_index` count for nothing, are not read and cost no products;
+    any other target outside [0, V) makes the loss NaN.  reduction: "mean" over the rows that count (0 if there are none),
+    "sum", or "none" (a loss per row, 0 where ignored).  The loss is float32; gradients of weight and bias, which have to be
+    leaves, are accumulated into .grad.  Values of x and of the weight are resolved to 2^-39 of the largest finite one of
+    each, and with "none" a row's gradient to 2^-39 of the largest upstream gradient.  stats: a dict that receives "pred"
+    (arg-max per row, 0 where ignored) and "correct" (rows that count and are right).  At most 2^22 rows, 2^22 classes and
+    K = 2^20."""
     _require_cuda(x, "linear_cross_entropy")
     xd, wd = L.dtype_code(x.dtype), L.dtype_code(weight.dtype)
     if xd == L.VC_F32 and wd != L.VC_F32:
