@@ -1403,12 +1403,12 @@ class _LinearCrossEntropy(torch.autograd.Function):
         dw, add_w = _grad_target(weight)
         db, add_b = _grad_target(bias)
         ws = torch.empty(_size("vc_linear_ce_bytes", 2, xd, wd, N, V, K), device=dev, dtype=torch.uint8)
-        _before_grads(dw, db)
+        _before_grads(dev, dw, db)
         L.fast("vc_linear_ce_bwd", dev, xd, wd, smoothing, reduction == "mean", reduction == "none", g.data_ptr(),
                saved.data_ptr(), _addr(dx), _addr(dw), _addr(db), ws.data_ptr(), add_w + 2 * add_b, N, V, K)
         _put_grad(weight, dw)
         _put_grad(bias, db)
-        _after_grads(dw, db)
+        _after_grads(dev)
         _ready(weight, bias)
         return (dx,) + (None,) * 7
 
@@ -1443,7 +1443,9 @@ def linear_cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoot
         raise ValueError(f"linear_cross_entropy: reduction must be one of {CE_REDUCTIONS}, not {reduction!r}")
     _leaf_params("linear_cross_entropy", weight, bias)
     _same_device("linear_cross_entropy", x, weight, bias, target)
-    _fits("linear_cross_entropy", (1 << 22, 1 << 22, 1 << 20), (target.numel(), *weight.shape))
+    if target.numel() > 1 << 22 or weight.shape[0] > 1 << 22 or weight.shape[1] > 1 << 20:
+        raise RuntimeError(f"linear_cross_entropy: {target.numel()} rows and a weight {tuple(weight.shape)} exceed 2^22 rows, "
+                           "2^22 classes or K = 2^20")
     if not -(1 << 63) <= ignore_index < 1 << 63:
         raise ValueError(f"linear_cross_entropy: ignore_index {ignore_index} is not an int64")
     if target.numel() == 0:
@@ -1757,7 +1759,7 @@ def _same_device(what, first, *rest):
 def _leaf_params(what, *params):
     """Refuses a parameter that is itself computed from others: its gradient would end in its own .grad."""
     for p in params:
-        if p is not None and p.requires_grad and not p.is_leaf and torch.is_grad_enabled():
+        if p is not None and not p.is_leaf and torch.is_grad_enabled():
             raise RuntimeError(f"{what}: parameters must be leaves, gradients are written into their .grad; this one was "
                                "computed (detach it, or pass the leaf)")
 
@@ -1768,12 +1770,6 @@ def _disjoint(what, dense):
     for (_, end), (start, _) in zip(spans, spans[1:]):
         if start < end:
             raise RuntimeError(f"{what}: in place needs tensors that share no memory")
-
-
-def _fits(what, limits, sizes):
-    for limit, size in zip(limits, sizes):
-        if size > limit:
-            raise RuntimeError(f"{what}: sizes {tuple(sizes)} exceed {tuple(limits)}")
 
 
 # ----------------------------------------------------------------------------------------------
@@ -1800,35 +1796,31 @@ def _f32_param(what, p):
 
 
 # Autograd orders the backward passes of forward calls on different streams at a parameter's gradient node; the parameters
-# of these operators have none, so passes that write gradients follow each other here.  Per device: the stream of the last
-# such pass and, unless it is the default one, an event behind it.
+# of these operators have none, so passes that write gradients follow each other here.  Per device: handle and stream of the
+# last such pass, and for a stream that is not torch's own, which may be gone by the next one, an event behind it.
 _last_writer = {}
 
 
-def _before_grads(*grads):
+def _before_grads(dev, *grads):
     """Called before the kernels that write these gradients (None entries are skipped)."""
-    dev = next((g.device.index for g in grads if g is not None), None)
-    if dev is None or dev not in _last_writer:
+    last = _last_writer.get(dev.index)
+    if last is None or last[0] == torch._C._cuda_getCurrentRawStream(dev.index) or \
+            torch.cuda.is_current_stream_capturing():  # a capture starts behind everything that was enqueued before it
         return
-    stream, event = _last_writer[dev]
-    if stream == torch._C._cuda_getCurrentRawStream(dev) or torch.cuda.is_current_stream_capturing():
-        return  # a capture starts behind everything that was enqueued before it
     here = torch.cuda.current_stream(dev)
-    here.wait_event(event) if event is not None else here.wait_stream(torch.cuda.default_stream(dev))
+    here.wait_stream(last[1]) if last[2] is None else here.wait_event(last[2])
     for g in grads:
         if g is not None:
             g.record_stream(here)
 
 
-def _after_grads(*grads):
-    dev = next((g.device.index for g in grads if g is not None), None)
-    if dev is None or torch.cuda.is_current_stream_capturing():
+def _after_grads(dev):
+    handle, last = torch._C._cuda_getCurrentRawStream(dev.index), _last_writer.get(dev.index)
+    if (last is not None and last[0] == handle and last[2] is None) or torch.cuda.is_current_stream_capturing():
         return
-    stream, event = torch._C._cuda_getCurrentRawStream(dev), None
-    if stream:
-        event = torch.cuda.Event()
-        event.record(torch.cuda.current_stream(dev))
-    _last_writer[dev] = stream, event
+    stream = torch.cuda.current_stream(dev)
+    foreign = stream.stream_id != 0 and stream.stream_id == stream.cuda_stream
+    _last_writer[dev.index] = handle, stream, stream.record_event() if foreign else None
 
 
 def _grad_target(p):
@@ -1889,14 +1881,14 @@ class _GroupNorm(torch.autograd.Function):
         if need_dx or dw is not None or db is not None or (need_dres and act):
             ws = torch.empty(ctx.ws_floats, device=dev, dtype=torch.float32)
             mean = stat.data_ptr()
-            _before_grads(dw, db)
+            _before_grads(dev, dw, db)
             for n, k, o in _gn_runs(N, S * C * x.element_size()):
                 L.fast("vc_group_norm_bwd", dev, ctx.code, x.data_ptr() + o, dy.data_ptr() + o, _addr(res, o), _addr(gamma),
                        _addr(beta), mean + 4 * n * G, mean + 4 * (N + n) * G, _addr(dx, o), _addr(dres, o) if act else None,
                        _addr(dw), _addr(db), ws.data_ptr(), k, S, C, G, act, 3 if n else add_w + 2 * add_b)
             _put_grad(weight, dw)
             _put_grad(bias, db)
-            _after_grads(dw, db)
+            _after_grads(dev)
         _ready(weight, bias)
         return dx, dres, None, None, None, None, None
 
@@ -1921,7 +1913,8 @@ def group_norm(x, gn, act="none", residual=None):
     _same_device("group_norm", x, residual, weight, bias)
     if x.numel() == 0:
         return x.clone()
-    _fits("group_norm", (1 << 30, 1 << 20), (x.numel() // (x.shape[0] * x.shape[-1]), x.shape[-1]))
+    if x.shape[-1] > 1 << 20 or x.numel() // (x.shape[0] * x.shape[-1]) > 1 << 30:
+        raise RuntimeError(f"group_norm: sizes {tuple(x.shape)} exceed 2^30 positions of a sample or 2^20 channels")
     with _on(x.device):
         _leaf_guard("group_norm", x, residual)
         return _GroupNorm.apply(x, residual, _anchor((x, residual), (weight, bias)), (weight, bias), gn.num_groups, gn.eps,
@@ -2105,7 +2098,8 @@ def newton_schulz(g, steps=5, coeffs=NS_COEFFS, eps=1e-7, inplace=False):
     code = L.dtype_code(first.dtype)
     _same_device("newton_schulz", first, *items)
     for t in items:
-        _fits("newton_schulz", (1 << 20, 1 << 20, 1 << 31), (*t.shape[-2:], t.shape[-2] * t.shape[-1]))
+        if max(t.shape[-2:]) > 1 << 20 or t.shape[-2] * t.shape[-1] > 1 << 31:
+            raise RuntimeError(f"newton_schulz: matrices of {tuple(t.shape)} exceed sides of 2^20 or 2^31 elements")
     if inplace:
         _disjoint("newton_schulz", items)
     with _on(first.device), torch.no_grad():
