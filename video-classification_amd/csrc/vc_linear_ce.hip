@@ -764,13 +764,16 @@ __global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ pa
       for (int e = 0; e < 8; ++e) s.v[e] = 0.f;
     store8(o + c0, s);
   } else {
-    for (int c = c0; c < c0 + 512 && c < K; c += 64) {
-      float s = 0.f;
-      if (live)
-#pragma unroll 4
-        for (int k = 0; k < slices; ++k) s += p[k * n + c];
-      o[c] = from_f32<T>(live ? s * f : 0.f);
-    }
+    float s[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[e] = 0.f;
+    if (live)
+      for (int k = 0; k < slices; ++k)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] += p[k * n + min(c0 + e * 64, K - 1)];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c0 + e * 64 < K) o[c0 + e * 64] = from_f32<T>(live ? s[e] * f : 0.f);
   }
 }
 
