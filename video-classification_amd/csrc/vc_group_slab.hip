@@ -4,8 +4,11 @@
 //
 // Covered: groups of 1, 2, 4, 8, .. 64 channels whose slab fits the register file, up to 512 threads x 28 (bf16) or 16
 // (fp32) vectors of eight values forward and 8 backward, which holds the input and the gradient.  (512 threads with 256
-// registers each hold as much as 1024 with 128 and spend half as many on what every thread needs besides the data.)  The slabs of a sample lie
-// next to each other on one XCD, so the parts of a 128-byte line that different slabs read meet in its L2.
+// registers each hold as much as 1024 with 128 and spend half as many on what every thread needs besides the data.)  The slabs
+// of a sample lie next to each other on one XCD, so the parts of a 128-byte line that different slabs read meet in its L2.
+//
+// Bound by memory: 128 x 56 x 56 x 256 bf16 forward 105 us (3.9 TB/s; two passes take 45 us more), 64 x 28 x
+// 28 x 512 with a shortcut 28 us (5.4 TB/s, partly from the last-level cache), 2 x 7 x 7 x 512 in one launch of 5 us.
 #include "vc_group.h"
 
 namespace {

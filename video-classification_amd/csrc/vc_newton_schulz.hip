@@ -3,9 +3,13 @@
 //   X_0 = G / (|G|_F + e);   S = X X^T,  X <- a X + (b S + c S S) X,  `steps` times;   with X the wide orientation of G
 // (m <= n; a tall matrix is transposed on the way in and out).  The polynomial drives every singular value towards 1.
 //
-// 2 m^2 n + 2 m^3 + 2 m^2 n operations a step (S and S S are symmetric: only tiles on and below the diagonal are computed
-// and stored twice), bound by the matrix pipes for large matrices and by launches for small ones, so all matrices of a
-// call share three launches a step.
+// m^2 n + m^3 + 2 m^2 n operations a step (S and S S are symmetric: only tiles on and below the diagonal are computed
+// and stored twice), bound by the matrix pipes for large matrices and by the chain of launches for small ones, so all
+// matrices of a call share each launch, three a step and a join where a reduction is cut.
+//   4096 x 4096: S 210 + 14 us, P 212 + 15, update 389 (1.06 PFLOP/s of fp16 products); 5 steps 3.9 ms
+//   52 matrices of a ResNet-50 (64 to 2048 rows): 200 us a step, 1.01 ms in all
+//   4 matrices of up to 256 x 1152: 45 us a step -- ten microseconds a launch, most of them latency of eight to
+//   thirty-six dependent k-steps
 //
 // Precision: a gradient's small singular values are amplified by a^steps (485 for the usual coefficients) and with them the
 // rounding of X, so bf16 products leave errors of 1 % of the largest entry for random matrices and 50 % for matrices of
