@@ -232,3 +232,19 @@ def test_disjoint():
     for pair in ([buf, buf], [buf[:3], buf[2:]], [buf, buf[1:2]]):
         with pytest.raises(RuntimeError, match="share no memory"):
             ops._disjoint("op", pair)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", list(DT))
+def test_large_tiles(cuda, dt):
+    """A call with enough work for the large tiles: odd shapes, tall and wide, whole and cut reductions beside a big matrix."""
+    from video_classification_amd import ops
+    shapes = [(2053, 2100), (130, 257), (257, 130), (129, 127), (300, 1000), (700, 64), (40, 2050), (64, 576), (384, 384)]
+    mats = [gaussian(m, n, i).to(DT[dt]).to(cuda) for i, (m, n) in enumerate(shapes)]
+    outs = ops.newton_schulz(mats)
+    for o, g in zip(outs[1:], mats[1:]):
+        close(o, g)
+    want, norms = reference(mats[0])
+    unit = (4 + 3 * 2100 ** 0.5 / 16) * 2.0 ** -22
+    tol = sum(C[0] ** (5 - k) * unit * float(n) for k, n in enumerate(norms)) + torch.finfo(DT[dt]).eps / 2 * float(want.norm())
+    assert float((outs[0].double() - want).norm()) <= tol

@@ -574,11 +574,11 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_grad_kernel(CeArgs a, const f
   float* tile = reinterpret_cast<float*>(smem);
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
-    g16_put(acc, half, tile);
+    Tile16<4>::put(acc, half, tile);
     __syncthreads();
     F8 d[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) d[u] = g16_get(tile, (threadIdx.x >> 4) + u * 16, (threadIdx.x & 15) * 8);
+    for (int u = 0; u < 4; ++u) d[u] = Tile16<4>::get(tile, (threadIdx.x >> 4) + u * 16, (threadIdx.x & 15) * 8);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int e = threadIdx.x + u * G_THREADS, n = n0 + half * 64 + (e >> 4);

@@ -8,8 +8,7 @@
 // matrices of a call share each launch, three a step and a join where a reduction is cut.
 //   4096 x 4096: S 210 + 14 us, P 212 + 15, update 389 (1.06 PFLOP/s of fp16 products); 5 steps 3.9 ms
 //   52 matrices of a ResNet-50 (64 to 2048 rows): 200 us a step, 1.01 ms in all
-//   4 matrices of up to 256 x 1152: 45 us a step -- ten microseconds a launch, most of them latency of eight to
-//   thirty-six dependent k-steps
+//   4 matrices of up to 256 x 1152, on 64 x 64 tiles: 24 us a step -- six microseconds a launch, most of them latency
 //
 // Precision: a gradient's small singular values are amplified by a^steps (485 for the usual coefficients) and with them the
 // rounding of X, so bf16 products leave errors of 1 % of the largest entry for random matrices and 50 % for matrices of
@@ -20,12 +19,19 @@
 // follow X exactly.  With `cap` the largest value any iterate takes on [0, 1] and `gain` the largest ratio of an iterate
 // to its start, |Y| <= min(cap / rho, gain), which fixes the power of two that scales Y into fp16; S and the polynomial
 // of S are scaled by powers of two from cap alone.
+#include <type_traits>
+
 #include "vc_gemm16.h"
 
 namespace {
 
 constexpr int NS_MAX = 64;        // matrices per launch
 constexpr int NORM_CHUNK = 1 << 14;
+// Launches with up to this many operations a step work on 64 x 64 tiles, which are four times as many and a quarter as long,
+// the others on 128 x 128, which load half as much per product.  64 against 128, us: four matrices up to 256 x 1152 (0.3 G)
+// 132 / 238, 1024^2 (4 G) 215 / 385, two of them 324 / 419, 1024 x 4096 (14 G) 444 / 481, 1536^2 (14 G) 509 / 516, 2048^2
+// (34 G) 878 / 781.
+constexpr double NS_SMALL_WORK = 15e9;
 
 // What a launch numbers its workgroups by, matrix after matrix.
 enum { BY_NORM, BY_INIT, BY_UPDATE, BY_S, BY_P, BY_JOIN_S, BY_JOIN_P, KINDS };
@@ -249,8 +255,8 @@ __device__ __forceinline__ int xcd_run(int id, int total) {
 // What becomes of an accumulated tile (rows m0 + .. in registers, columns n0 + .. across lanes) of a symmetric product:
 // S = rho^2 Y Y^T, or P = b S + c S S (SQUARE).  It is stored at (column, row) and, off the diagonal, at (row, column), both
 // in whole 16-byte pieces.
-template <bool SQUARE>
-__device__ __forceinline__ void sym_store(const f32x4 (&acc)[4][4], const NsMat& t, const NsView& w, f16* ws,
+template <bool SQUARE, int TB>
+__device__ __forceinline__ void sym_store(const f32x4 (&acc)[TB][TB], const NsMat& t, const NsView& w, f16* ws,
                                           const NsScale& sc, const NsStep& st, int m0, int n0, float* tile) {
   const f16* s = ws + w.s;
   f16* dst = ws + (SQUARE ? w.p : w.s);
@@ -258,33 +264,31 @@ __device__ __forceinline__ void sym_store(const f32x4 (&acc)[4][4], const NsMat&
   const float f = SQUARE ? ldexpf(st.c, st.ep - 2 * st.es) : ldexpf(sc.rho2, st.es - 2 * sc.ey);
   const float sb = ldexpf(st.b, st.ep - st.es);
   const bool mirror = m0 != n0;
+  typedef Tile16<TB> L;
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
+  for (int half = 0; half < L::HALVES; ++half) {
     const int c0 = n0 + half * 64;
-    f16x8 sh[4], sl[4];  // S where it is needed, on its way while the tile passes through LDS
+    f16x8 sh[L::UNITS], sl[L::UNITS];  // S where it is needed, on its way while the tile passes through LDS
     if (SQUARE)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < L::UNITS; ++u) {
         const int e = threadIdx.x + u * G_THREADS;
-        const int64_t o = (int64_t)min(c0 + (e >> 4), t.m - 1) * w.ldm + min(m0 + (e & 15) * 8, w.ldm - 8);
+        const int64_t o = (int64_t)min(c0 + e / L::VPR, t.m - 1) * w.ldm + min(m0 + e % L::VPR * 8, w.ldm - 8);
         sh[u] = *reinterpret_cast<const f16x8*>(s + o);
         sl[u] = *reinterpret_cast<const f16x8*>(s + o + pl);
       }
-    g16_put(acc, half, tile);
+    L::put(acc, half, tile);
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int e = threadIdx.x + u * G_THREADS, cl = e >> 4, rl = (e & 15) * 8;
-      F8 v = g16_get(tile, cl, rl);
+    for (int u = 0; u < L::UNITS; ++u) {
+      const int e = threadIdx.x + u * G_THREADS, cl = e / L::VPR, rl = e % L::VPR * 8;
+      F8 v = L::get(tile, cl, rl);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         v.v[k] *= f;
         if (SQUARE) v.v[k] = fmaf(sb, (float)sh[u][k] + (float)sl[u][k], v.v[k]);
       }
-      if (mirror) {
-        *reinterpret_cast<f32x4*>(tile + g16_at(cl, rl)) = f32x4{v.v[0], v.v[1], v.v[2], v.v[3]};
-        *reinterpret_cast<f32x4*>(tile + g16_at(cl, rl + 4)) = f32x4{v.v[4], v.v[5], v.v[6], v.v[7]};
-      }
+      if (mirror) L::set(tile, cl, rl, v);
       if (c0 + cl < t.m && m0 + rl < w.ldm) {
         f16x8 h, l;
         f16_split8(v, h, l);
@@ -296,11 +300,11 @@ __device__ __forceinline__ void sym_store(const f32x4 (&acc)[4][4], const NsMat&
     __syncthreads();
     if (mirror) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < L::UNITS; ++u) {
         const int e = threadIdx.x + u * G_THREADS, rl = e >> 3, cl = (e & 7) * 8;
         F8 v;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v.v[k] = tile[g16_at(cl + k, rl)];
+        for (int k = 0; k < 8; ++k) v.v[k] = tile[L::at(cl + k, rl)];
         if (m0 + rl < t.m) {  // below the diagonal every column of the tile is inside
           f16x8 h, l;
           f16_split8(v, h, l);
@@ -315,17 +319,17 @@ __device__ __forceinline__ void sym_store(const f32x4 (&acc)[4][4], const NsMat&
 }
 
 // A tile, or a slice of the reduction of one, of a symmetric product; tiles on and below the diagonal only.
-template <bool SQUARE>
+template <bool SQUARE, int TB>
 __global__ __launch_bounds__(G_THREADS, 2) void ns_sym_kernel(const NsMat* __restrict__ table, int count, f16* __restrict__ ws,
                                                               const NsScale* __restrict__ sc, NsStep st, int parity,
                                                               float* __restrict__ part) {
-  typedef G16<2, 2> G;
+  typedef G16<2, 2, ROW, ROW, TB> G;
   __shared__ __attribute__((aligned(1024))) f16 smem[G::LDS];
   const int i = find_mat(table, count, SQUARE ? BY_P : BY_S, blockIdx.x);
   const NsMat t = table[i];
   const NsMat::Cut cut = t.cut[SQUARE];
   const NsView w(t, parity);
-  const int tiles = (t.m + GM - 1) / GM, all = tiles * (tiles + 1) / 2;
+  const int tiles = (t.m + G::T - 1) / G::T, all = tiles * (tiles + 1) / 2;
   int id = blockIdx.x - t.first[SQUARE ? BY_P : BY_S];  // whole tiles first, then slices; each kind spread over the XCDs by itself
   id = id < cut.direct ? xcd_run(id, cut.direct) : cut.direct + xcd_run(id - cut.direct, (all - cut.direct) * cut.slices);
   const int ld = SQUARE ? w.ldm : w.ldn;
@@ -339,62 +343,64 @@ __global__ __launch_bounds__(G_THREADS, 2) void ns_sym_kernel(const NsMat* __res
   }
   int tm, tn;
   tri_tile(tile, tiles, tm, tn);
-  const int m0 = tm * GM, n0 = tn * GM;
+  const int m0 = tm * G::T, n0 = tn * G::T;
   const f16* src = ws + (SQUARE ? w.s : w.x);
   const int64_t plane = (int64_t)t.m * ld;
-  f32x4 acc[4][4];
+  f32x4 acc[TB][TB];
   G::zero(acc);
   G::run(acc, Op16{src + (int64_t)m0 * ld, plane, ld, t.m - m0, 0}, Op16{src + (int64_t)n0 * ld, plane, ld, t.m - n0, 0}, k0,
          k1, smem);
   if (slot >= 0) {
-    f32x4* o = reinterpret_cast<f32x4*>(part + ((int64_t)cut.p0 + slot) * GM * GM) + threadIdx.x;
+    f32x4* o = reinterpret_cast<f32x4*>(part + ((int64_t)cut.p0 + slot) * G::T * G::T) + threadIdx.x;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) o[e * G_THREADS] = acc[e >> 2][e & 3];
+    for (int e = 0; e < TB * TB; ++e) o[e * G_THREADS] = acc[e / TB][e % TB];
     return;
   }
-  sym_store<SQUARE>(acc, t, w, ws, sc[i], st, m0, n0, reinterpret_cast<float*>(smem));
+  sym_store<SQUARE, TB>(acc, t, w, ws, sc[i], st, m0, n0, reinterpret_cast<float*>(smem));
 }
 
 // joins the slices of a tile in order
-template <bool SQUARE>
+template <bool SQUARE, int TB>
 __global__ __launch_bounds__(G_THREADS, 2) void ns_sym_join_kernel(const NsMat* __restrict__ table, int count, f16* __restrict__ ws,
                                                                    const NsScale* __restrict__ sc, NsStep st, int parity,
                                                                    const float* __restrict__ part) {
-  __shared__ __attribute__((aligned(1024))) float smem[G_TILE];
+  constexpr int T = 32 * TB;
+  __shared__ __attribute__((aligned(1024))) float smem[Tile16<TB>::FLOATS];
   const int i = find_mat(table, count, SQUARE ? BY_JOIN_P : BY_JOIN_S, blockIdx.x);
   const NsMat t = table[i];
   const NsMat::Cut cut = t.cut[SQUARE];
   const NsView w(t, parity);
   const int e0 = blockIdx.x - t.first[SQUARE ? BY_JOIN_P : BY_JOIN_S];
   int tm, tn;
-  tri_tile(cut.direct + e0, (t.m + GM - 1) / GM, tm, tn);
-  f32x4 acc[4][4];
-  G16<2, 2>::zero(acc);
-  const f32x4* p = reinterpret_cast<const f32x4*>(part + ((int64_t)cut.p0 + (int64_t)e0 * cut.slices) * GM * GM) + threadIdx.x;
+  tri_tile(cut.direct + e0, (t.m + T - 1) / T, tm, tn);
+  f32x4 acc[TB][TB];
+  G16<2, 2, ROW, ROW, TB>::zero(acc);
+  const f32x4* p = reinterpret_cast<const f32x4*>(part + ((int64_t)cut.p0 + (int64_t)e0 * cut.slices) * T * T) + threadIdx.x;
 #pragma unroll 2
-  for (int s = 0; s < cut.slices; ++s, p += GM * GM / 4)
+  for (int s = 0; s < cut.slices; ++s, p += T * T / 4)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) acc[e >> 2][e & 3] += p[e * G_THREADS];
-  sym_store<SQUARE>(acc, t, w, ws, sc[i], st, tm * GM, tn * GM, smem);
+    for (int e = 0; e < TB * TB; ++e) acc[e / TB][e % TB] += p[e * G_THREADS];
+  sym_store<SQUARE, TB>(acc, t, w, ws, sc[i], st, tm * T, tn * T, smem);
 }
 
 // X <- a X + P X, into the other buffer, or the result in G's orientation after the last step.  The columns of X run along
 // the registers, so X is read and written in groups of four.
-template <typename T>
+template <typename T, int TB>
 __global__ __launch_bounds__(G_THREADS, 2) void ns_update_kernel(const NsMat* __restrict__ table, int count, f16* __restrict__ ws,
                                                                  const NsScale* __restrict__ sc, NsStep st, int parity) {
-  typedef G16<2, 2, COL, ROW> G;
+  typedef G16<2, 2, COL, ROW, TB> G;
+  typedef Tile16<TB> L;
   __shared__ __attribute__((aligned(1024))) f16 smem[G::LDS];
   const int i = find_mat(table, count, BY_UPDATE, blockIdx.x);
   const NsMat t = table[i];
   const NsView w(t, parity);
-  const int tiles_m = (t.m + GM - 1) / GM, tiles_n = (t.n + GM - 1) / GM;
+  const int tiles_m = (t.m + G::T - 1) / G::T, tiles_n = (t.n + G::T - 1) / G::T;
   int tm, tn;
   g16_tile(blockIdx.x - t.first[BY_UPDATE], tiles_m * tiles_n, tiles_m, tiles_n, tm, tn);
-  const int m0 = tm * GM, n0 = tn * GM;
+  const int m0 = tm * G::T, n0 = tn * G::T;
   const int64_t pp = (int64_t)t.m * w.ldm, px = (int64_t)t.m * w.ldn;
   const f16* x = ws + w.x;
-  f32x4 acc[4][4];
+  f32x4 acc[TB][TB];
   G::zero(acc);
   G::run(acc, Op16{x, px, w.ldn, t.m, n0}, Op16{ws + w.p + (int64_t)m0 * w.ldm, pp, w.ldm, t.m - m0, 0}, 0, w.ldm, smem);
   f16* xo = ws + w.xo;
@@ -404,22 +410,22 @@ __global__ __launch_bounds__(G_THREADS, 2) void ns_update_kernel(const NsMat* __
   const bool vec = !t.tall && t.n % 8 == 0 && ((uintptr_t)out & 15) == 0;
   float* tile = reinterpret_cast<float*>(smem);
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
+  for (int half = 0; half < L::HALVES; ++half) {
     const int r0 = m0 + half * 64;
-    f16x8 xh[4], xl[4];  // X's tile, on its way while P X passes through LDS
+    f16x8 xh[L::UNITS], xl[L::UNITS];  // X's tile, on its way while P X passes through LDS
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < L::UNITS; ++u) {
       const int e = threadIdx.x + u * G_THREADS;
-      const int64_t o = (int64_t)min(r0 + (e >> 4), t.m - 1) * w.ldn + min(n0 + (e & 15) * 8, w.ldn - 8);
+      const int64_t o = (int64_t)min(r0 + e / L::VPR, t.m - 1) * w.ldn + min(n0 + e % L::VPR * 8, w.ldn - 8);
       xh[u] = *reinterpret_cast<const f16x8*>(x + o);
       xl[u] = *reinterpret_cast<const f16x8*>(x + o + px);
     }
-    g16_put(acc, half, tile);
+    L::put(acc, half, tile);
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int e = threadIdx.x + u * G_THREADS, r = r0 + (e >> 4), c = n0 + (e & 15) * 8;
-      F8 v = g16_get(tile, e >> 4, (e & 15) * 8);
+    for (int u = 0; u < L::UNITS; ++u) {
+      const int e = threadIdx.x + u * G_THREADS, rl = e / L::VPR, cl = e % L::VPR * 8, r = r0 + rl, c = n0 + cl;
+      F8 v = L::get(tile, rl, cl);
 #pragma unroll
       for (int k = 0; k < 8; ++k) v.v[k] = fmaf(st.a, (float)xh[u][k] + (float)xl[u][k], v.v[k] * f);
       if (st.last) {
@@ -427,8 +433,7 @@ __global__ __launch_bounds__(G_THREADS, 2) void ns_update_kernel(const NsMat* __
         for (int k = 0; k < 8; ++k) v.v[k] = fo * ldexpf(v.v[k], -ey);
       }
       if (st.last && t.tall) {  // the result is transposed: through LDS once more
-        *reinterpret_cast<f32x4*>(tile + g16_at(e >> 4, (e & 15) * 8)) = f32x4{v.v[0], v.v[1], v.v[2], v.v[3]};
-        *reinterpret_cast<f32x4*>(tile + g16_at(e >> 4, (e & 15) * 8 + 4)) = f32x4{v.v[4], v.v[5], v.v[6], v.v[7]};
+        L::set(tile, rl, cl, v);
       } else if (st.last) {
         if (r < t.m && c < t.n) {
           T* d = out + (int64_t)r * t.n + c;
@@ -448,9 +453,9 @@ __global__ __launch_bounds__(G_THREADS, 2) void ns_update_kernel(const NsMat* __
     }
     __syncthreads();
     if (st.last && t.tall) {
-      for (int e = threadIdx.x; e < GM * 64; e += G_THREADS) {
+      for (int e = threadIdx.x; e < G::T * 64; e += G_THREADS) {
         const int cl = e >> 6, rl = e & 63;
-        if (n0 + cl < t.n && r0 + rl < t.m) out[(int64_t)(n0 + cl) * t.m + r0 + rl] = from_f32<T>(tile[g16_at(rl, cl)]);
+        if (n0 + cl < t.n && r0 + rl < t.m) out[(int64_t)(n0 + cl) * t.m + r0 + rl] = from_f32<T>(tile[L::at(rl, cl)]);
       }
       __syncthreads();
     }
@@ -576,8 +581,8 @@ __global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(NsSmallArgs a, 
                           sums);
 }
 
-int sym_tiles(const NsMat& t) {
-  const int n = ceil_div(t.m, GM);
+int sym_tiles(const NsMat& t, int tile) {
+  const int n = ceil_div(t.m, tile);
   return n * (n + 1) / 2;
 }
 
@@ -586,18 +591,18 @@ int sym_tiles(const NsMat& t) {
 //  - One matrix with a little more than whole rounds of tiles: the tiles of the last round are cut instead of leaving
 //    most of the chip idle for it (4096 x 4096: 528 tiles on 512 slots).
 // Fills cut[square] of every matrix and returns the partial tiles; the reduction is in k-steps of 32.
-int64_t cut_sym(NsMat* mats, int n, int square) {
+int64_t cut_sym(NsMat* mats, int n, int square, int tile) {
   int64_t slots = 512, tiles = 0, work = 0, parts = 0;
   auto len = [&](const NsMat& t) { return up64(square ? t.m : t.n) / 32; };
   for (int i = 0; i < n; ++i) {
-    tiles += sym_tiles(mats[i]);
-    work += (int64_t)sym_tiles(mats[i]) * len(mats[i]);
+    tiles += sym_tiles(mats[i], tile);
+    work += (int64_t)sym_tiles(mats[i], tile) * len(mats[i]);
   }
   if (work < 512 * 16) slots = 256;  // short runs: one workgroup per CU
   for (int i = 0; i < n; ++i) {
     const NsMat& t = mats[i];
     NsMat::Cut& c = mats[i].cut[square];
-    const int all = sym_tiles(t);
+    const int all = sym_tiles(t, tile);
     c.direct = all;
     c.slices = 1;
     if (tiles < slots) {
@@ -641,8 +646,10 @@ struct NsLayout {
   NsMat mat[NS_MAX];
   int64_t blocks[KINDS];
   int64_t norms, part, bufs, bytes;
+  int tile;  // 128, or 64
   NsLayout(const int* rows, const int* cols, int count) {
     int64_t at = 0;
+    double work = 0;
     for (int i = 0; i < count; ++i) {
       NsMat& t = mat[i];
       t = NsMat{};
@@ -651,8 +658,10 @@ struct NsLayout {
       t.n = t.tall ? rows[i] : cols[i];
       t.at = at;
       at = NsView(t, 0).end;
+      work += (double)t.m * t.m * (3.0 * t.n + t.m);
     }
-    const int64_t ps = cut_sym(mat, count, 0), pp = cut_sym(mat, count, 1);
+    tile = work <= NS_SMALL_WORK ? 64 : 128;
+    const int64_t ps = cut_sym(mat, count, 0, tile), pp = cut_sym(mat, count, 1, tile);
     for (int k = 0; k < KINDS; ++k) {
       blocks[k] = 0;
       for (int i = 0; i < count; ++i) {
@@ -661,14 +670,14 @@ struct NsLayout {
         const NsMat::Cut& c = t.cut[k == BY_P || k == BY_JOIN_P];
         blocks[k] += k == BY_NORM     ? ceil_div64((int64_t)t.m * t.n, NORM_CHUNK)
                      : k == BY_INIT   ? (int64_t)(up64(t.m) / 64) * (up64(t.n) / 64)
-                     : k == BY_UPDATE ? (int64_t)ceil_div(t.m, GM) * ceil_div(t.n, GM)
-                     : k <= BY_P      ? c.direct + (int64_t)(sym_tiles(t) - c.direct) * c.slices
-                                      : sym_tiles(t) - c.direct;
+                     : k == BY_UPDATE ? (int64_t)ceil_div(t.m, tile) * ceil_div(t.n, tile)
+                     : k <= BY_P      ? c.direct + (int64_t)(sym_tiles(t, tile) - c.direct) * c.slices
+                                      : sym_tiles(t, tile) - c.direct;
       }
     }
     norms = NS_MAX * (int64_t)(sizeof(NsMat) + sizeof(NsScale));
     part = norms + up128(blocks[BY_NORM] * 8);
-    bufs = part + (ps > pp ? ps : pp) * GM * GM * 4;
+    bufs = part + (ps > pp ? ps : pp) * tile * tile * 4;
     bytes = bufs + at * 2;
   }
 };
@@ -760,11 +769,16 @@ int vc_newton_schulz(int dtype, int count, const void* const* g, void* const* ou
       st.b = coeffs[3 * k + 1];
       st.c = coeffs[3 * k + 2];
       st.last = k == steps - 1;
-      launch(BY_S, ns_sym_kernel<false>, G_THREADS, ws, sc, st, k & 1, part);
-      if (l.blocks[BY_JOIN_S]) launch(BY_JOIN_S, ns_sym_join_kernel<false>, G_THREADS, ws, sc, st, k & 1, part);
-      launch(BY_P, ns_sym_kernel<true>, G_THREADS, ws, sc, st, k & 1, part);
-      if (l.blocks[BY_JOIN_P]) launch(BY_JOIN_P, ns_sym_join_kernel<true>, G_THREADS, ws, sc, st, k & 1, part);
-      launch(BY_UPDATE, bf ? ns_update_kernel<bf16> : ns_update_kernel<float>, G_THREADS, ws, sc, st, k & 1);
+      auto step = [&](auto tb) {
+        constexpr int TB = decltype(tb)::value;
+        launch(BY_S, ns_sym_kernel<false, TB>, G_THREADS, ws, sc, st, k & 1, part);
+        if (l.blocks[BY_JOIN_S]) launch(BY_JOIN_S, ns_sym_join_kernel<false, TB>, G_THREADS, ws, sc, st, k & 1, part);
+        launch(BY_P, ns_sym_kernel<true, TB>, G_THREADS, ws, sc, st, k & 1, part);
+        if (l.blocks[BY_JOIN_P]) launch(BY_JOIN_P, ns_sym_join_kernel<true, TB>, G_THREADS, ws, sc, st, k & 1, part);
+        launch(BY_UPDATE, bf ? ns_update_kernel<bf16, TB> : ns_update_kernel<float, TB>, G_THREADS, ws, sc, st, k & 1);
+      };
+      if (l.tile == 64) step(std::integral_constant<int, 2>());
+      else step(std::integral_constant<int, 4>());
     }
   }
   flush();
