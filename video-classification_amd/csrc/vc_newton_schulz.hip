@@ -6,8 +6,8 @@
 // m^2 n + m^3 + 2 m^2 n operations a step (S and S S are symmetric: only tiles on and below the diagonal are computed
 // and stored twice), bound by the matrix pipes for large matrices and by the chain of launches for small ones, so all
 // matrices of a call share each launch, three a step and a join where a reduction is cut.
-//   4096 x 4096: S 210 + 14 us, P 212 + 15, update 389 (1.06 PFLOP/s of fp16 products); 5 steps 3.9 ms
-//   52 matrices of a ResNet-50 (64 to 2048 rows): 200 us a step, 1.01 ms in all
+//   4096 x 4096: S 210 + 9 us, P 212 + 10, update 389 (1.06 PFLOP/s of fp16 products); 5 steps 3.9 ms
+//   52 matrices of a ResNet-50 (64 to 2048 rows): 195 us a step, 0.97 ms in all
 //   4 matrices of up to 256 x 1152, on 64 x 64 tiles: 24 us a step -- six microseconds a launch, most of them latency
 //
 // Precision: a gradient's small singular values are amplified by a^steps (485 for the usual coefficients) and with them the
@@ -27,11 +27,11 @@ namespace {
 
 constexpr int NS_MAX = 64;        // matrices per launch
 constexpr int NORM_CHUNK = 1 << 14;
-// Launches with up to this many operations a step work on 64 x 64 tiles, which are four times as many and a quarter as long,
+// Calls with up to this many operations a step work on 64 x 64 tiles, which are four times as many and a quarter as long,
 // the others on 128 x 128, which load half as much per product.  64 against 128, us: four matrices up to 256 x 1152 (0.3 G)
-// 132 / 238, 1024^2 (4 G) 215 / 385, two of them 324 / 419, 1024 x 4096 (14 G) 444 / 481, 1536^2 (14 G) 509 / 516, 2048^2
-// (34 G) 878 / 781.
-constexpr double NS_SMALL_WORK = 15e9;
+// 131 / 214, 1024^2 (4 G) 215 / 335, two of them 323 / 381, 1024 x 4096 (14 G) 446 / 429, 1536^2 (14 G) 511 / 480, 2048^2
+// (34 G) 880 / 753.
+constexpr double NS_SMALL_WORK = 10e9;
 
 // What a launch numbers its workgroups by, matrix after matrix.
 enum { BY_NORM, BY_INIT, BY_UPDATE, BY_S, BY_P, BY_JOIN_S, BY_JOIN_P, KINDS };
@@ -359,28 +359,34 @@ __global__ __launch_bounds__(G_THREADS, 2) void ns_sym_kernel(const NsMat* __res
   sym_store<SQUARE, TB>(acc, t, w, ws, sc[i], st, m0, n0, reinterpret_cast<float*>(smem));
 }
 
-// joins the slices of a tile in order
+// Joins the slices of a tile in order.  A workgroup takes 64 x 64 of it, of a 128 x 128 tile the part of one wave: reading
+// its slices is what a join spends its time on (eight of 128 x 128 are 512 KiB: 13 us in one workgroup, 5 in four).
 template <bool SQUARE, int TB>
 __global__ __launch_bounds__(G_THREADS, 2) void ns_sym_join_kernel(const NsMat* __restrict__ table, int count, f16* __restrict__ ws,
                                                                    const NsScale* __restrict__ sc, NsStep st, int parity,
                                                                    const float* __restrict__ part) {
-  constexpr int T = 32 * TB;
-  __shared__ __attribute__((aligned(1024))) float smem[Tile16<TB>::FLOATS];
+  constexpr int T = 32 * TB, PARTS = TB * TB / 4;
+  __shared__ __attribute__((aligned(1024))) float smem[Tile16<2>::FLOATS];
   const int i = find_mat(table, count, SQUARE ? BY_JOIN_P : BY_JOIN_S, blockIdx.x);
   const NsMat t = table[i];
   const NsMat::Cut cut = t.cut[SQUARE];
   const NsView w(t, parity);
-  const int e0 = blockIdx.x - t.first[SQUARE ? BY_JOIN_P : BY_JOIN_S];
+  const int id = blockIdx.x - t.first[SQUARE ? BY_JOIN_P : BY_JOIN_S], e0 = id / PARTS, wave = id % PARTS;
   int tm, tn;
   tri_tile(cut.direct + e0, (t.m + T - 1) / T, tm, tn);
-  f32x4 acc[TB][TB];
-  G16<2, 2, ROW, ROW, TB>::zero(acc);
-  const f32x4* p = reinterpret_cast<const f32x4*>(part + ((int64_t)cut.p0 + (int64_t)e0 * cut.slices) * T * T) + threadIdx.x;
-#pragma unroll 2
+  const int m0 = tm * T + (wave >> 1) * 64, n0 = tn * T + (wave & 1) * 64;
+  if (m0 < n0 || m0 >= t.m) return;  // the mirror image of another part, or nothing
+  const int lane = threadIdx.x & 63, wm = threadIdx.x >> 7, wn = (threadIdx.x >> 6) & 1;
+  // where this thread's blocks (2 wm + i, 2 wn + j) of the part lie in a slice
+  const int at = TB == 4 ? wave * 64 + lane + (wm * 8 + wn * 2) * G_THREADS : threadIdx.x;
+  f32x4 acc[2][2];
+  G16<2, 2, ROW, ROW, 2>::zero(acc);
+  const f32x4* p = reinterpret_cast<const f32x4*>(part + ((int64_t)cut.p0 + (int64_t)e0 * cut.slices) * T * T) + at;
+#pragma unroll 4
   for (int s = 0; s < cut.slices; ++s, p += T * T / 4)
 #pragma unroll
-    for (int e = 0; e < TB * TB; ++e) acc[e / TB][e % TB] += p[e * G_THREADS];
-  sym_store<SQUARE, TB>(acc, t, w, ws, sc[i], st, tm * T, tn * T, smem);
+    for (int e = 0; e < 4; ++e) acc[e >> 1][e & 1] += p[((e >> 1) * TB + (e & 1)) * G_THREADS];
+  sym_store<SQUARE, 2>(acc, t, w, ws, sc[i], st, m0, n0, smem);
 }
 
 // X <- a X + P X, into the other buffer, or the result in G's orientation after the last step.  The columns of X run along
@@ -672,7 +678,7 @@ struct NsLayout {
                      : k == BY_INIT   ? (int64_t)(up64(t.m) / 64) * (up64(t.n) / 64)
                      : k == BY_UPDATE ? (int64_t)ceil_div(t.m, tile) * ceil_div(t.n, tile)
                      : k <= BY_P      ? c.direct + (int64_t)(sym_tiles(t, tile) - c.direct) * c.slices
-                                      : sym_tiles(t, tile) - c.direct;
+                                      : (int64_t)(sym_tiles(t, tile) - c.direct) * (tile * tile / 4096);
       }
     }
     norms = NS_MAX * (int64_t)(sizeof(NsMat) + sizeof(NsScale));
