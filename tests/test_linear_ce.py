@@ -458,3 +458,17 @@ def test_many_ignored_rows(cuda, types, N, K, V, share):
     check(ref, types, None, xg.grad, w.grad, b.grad, one_term=FEW_ROWS)
     if not count:
         assert not w.grad.any() and not b.grad.any()
+
+
+@pytest.mark.gpu
+def test_slices_of_few_rows(cuda):
+    """dx is summed over more slices of the classes the fewer rows count; from all rows to one, in one buffer."""
+    from video_classification_amd import ops
+    x, w, b, t = make(1500, 130, 16500, "bf16", seed=9)
+    for count in (1500, 1100, 700, 300, 129, 128, 1):
+        tt = t.clone()
+        tt[torch.randperm(1500, generator=torch.Generator().manual_seed(count))[count:].to(cuda)] = -100
+        xg = x.clone().requires_grad_(True)
+        ops.linear_cross_entropy(xg, w.detach(), b.detach(), tt, reduction="sum").backward()
+        check(reference(x, w, b, tt, 0.0, torch.ones(1500, device=cuda)), "bf16", dx=xg.grad, one_term=FEW_ROWS)
+        assert (xg.grad[tt == -100] == 0).all()

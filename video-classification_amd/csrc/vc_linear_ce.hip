@@ -624,6 +624,19 @@ __global__ __launch_bounds__(256) void ce_bias_kernel(const float* __restrict__ 
   bias_out(db + v, s, fac, add);
 }
 
+// slices of a reduction of length k (a multiple of 64) over `tiles` output tiles: two workgroups per CU where the slices
+// are at least 1024 long, else one, down to 256 elements; at most 16
+__host__ __device__ inline void slices(int tiles, int k, int& s, int& per) {
+  if (tiles < 1) tiles = 1;
+  int want = 512 / tiles;
+  if (want > 1 && k / want < 1024) want = 256 / tiles;
+  const int most = k / 256 < 16 ? k / 256 : 16;
+  if (want > most) want = most;
+  if (want < 1) want = 1;
+  per = ((k + want - 1) / want + 63) / 64 * 64;
+  s = (k + per - 1) / per;
+}
+
 // out[m][c] = factor * sum over the reduction of (row side)[m] (column side)[c]: dx = d W and dW = d^T x.  Operands that lie
 // along the reduction the wrong way are read from LDS with transposing reads, so nothing is stored twice.  139 and 132 us
 // for a piece of 8192 classes of 8192 x 1024 (1.0 PFLOP/s); fp32 dW of bf16 rows, d in two terms: 94 us per piece of
@@ -631,9 +644,10 @@ __global__ __launch_bounds__(256) void ce_bias_kernel(const float* __restrict__ 
 struct MmArgs {
   Op16 c, m;                   // column side (W or x, COL) and row side (d: ROW for dx, COL for dW), at their corners
   int M, Nn, k;                // rows and columns of the result, reduction length of dx (a multiple of 64)
-  int tiles_m, tiles_n, splits, kper;
+  int tiles_m, tiles_n, splits;
+  int piece;                   // dx: classes of a whole piece, whose slices every piece takes
   const int* order;            // dx: where its packed rows go
-  float* part;                 // [splits][M][Nn], or null: write out
+  float* part;                 // [splits][M, of dx: rows that count][Nn], or null: write out
   int add;                     // add to what part / out hold
   void* out;                   // [M][Nn]
   CeFac fac;
@@ -652,11 +666,13 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
   __shared__ __attribute__((aligned(1024))) f16 smem[G::LDS];
   const int rows = g.exps[2];
   const int tiles_m = KM == ROW ? max(1, (rows + GM - 1) / GM) : g.tiles_m, tiles = tiles_m * g.tiles_n;
+  int splits = g.splits, per = 0;
+  if (KM == ROW && g.part) slices(tiles, g.piece, splits, per);  // by the rows that count
   int split = blockIdx.x / tiles, tm, tn;
-  const bool idle = split >= g.splits;  // dx: behind the rows that count
+  const bool idle = split >= splits;  // dx: behind the rows that count
   if (idle) {
     if (g.part) return;  // ce_dx_kernel writes their zeros
-    const int id = blockIdx.x - tiles * g.splits;
+    const int id = blockIdx.x - tiles;
     tm = tiles_m + id / g.tiles_n;
     tn = id % g.tiles_n;
     split = 0;
@@ -666,7 +682,8 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
   f32x4 acc[4][4];
   G::zero(acc);
   const int klen = KM == ROW ? g.k : (rows + 63) / 64 * 64;
-  const int per = KM == ROW ? g.kper : ((klen + g.splits - 1) / g.splits + 63) / 64 * 64;
+  if (KM == COL) per = ((klen + splits - 1) / splits + 63) / 64 * 64;
+  else if (!g.part) per = klen;
   const int k0 = split * per, k1 = min(klen, k0 + per);
   Op16 c = g.c, m = g.m;
   c.side = n0;
@@ -681,7 +698,7 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
   const int lane = threadIdx.x & 63, q = lane >> 4, l15 = lane & 15;
   const int wave = threadIdx.x >> 6, wc = wave >> 1, wr = wave & 1;
   const float f = g.part ? 1.f : mm_factor(g.fac, g.exps, g.which);
-  float* part = g.part ? g.part + (int64_t)split * g.M * g.Nn : nullptr;
+  float* part = g.part ? g.part + (int64_t)split * (KM == ROW ? rows : g.M) * g.Nn : nullptr;
   const bool vec = g.vec;
   if (!part)
 #pragma unroll
@@ -746,14 +763,17 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
 // dx[order[r]] = factor * sum over the slices, in order, of packed row r; zeros for rows that do not count.  A wave per row and
 // 512 columns.
 template <typename T>
-__global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ part, int slices, int N, int K, CeFac fac,
+__global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ part, int piece, int N, int K, CeFac fac,
                                                     const int* __restrict__ exps, const int* __restrict__ order, int vec,
                                                     T* __restrict__ out) {
   const int per = (K + 511) / 512;
-  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), n = (int64_t)N * K;
+  const int rows = exps[2];
+  int splits, len;
+  slices(max(1, (rows + GM - 1) / GM) * ((K + GM - 1) / GM), piece, splits, len);
+  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), n = (int64_t)rows * K;
   const int r = (int)(unit / per), c0 = (int)(unit - (int64_t)r * per) * 512 + (threadIdx.x & 63) * (vec ? 8 : 1);
   if (r >= N) return;
-  const bool live = r < exps[2];
+  const bool live = r < rows;
   const float f = mm_factor(fac, exps, 1);
   const float* p = part + (int64_t)r * K;
   T* o = out + (int64_t)order[r] * K;
@@ -764,7 +784,7 @@ __global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ pa
     for (int e = 0; e < 8; ++e) s.v[e] = 0.f;
     if (live)
 #pragma unroll 4
-      for (int k = 0; k < slices; ++k) {
+      for (int k = 0; k < splits; ++k) {
         const F8 v = load8(p + k * n + c0);
 #pragma unroll
         for (int e = 0; e < 8; ++e) s.v[e] += v.v[e];
@@ -780,7 +800,7 @@ __global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ pa
 #pragma unroll
     for (int e = 0; e < 8; ++e) s[e] = 0.f;
     if (live)
-      for (int k = 0; k < slices; ++k)
+      for (int k = 0; k < splits; ++k)
 #pragma unroll
         for (int e = 0; e < 8; ++e) s[e] += p[k * n + min(c0 + e * 64, K - 1)];
 #pragma unroll
@@ -811,7 +831,7 @@ struct Plan {
   int ld, px, pw;              // row length and terms of the packed operands
   int pdx, pdw, pd;            // terms of d for dx and dW, and the larger of the two
   int piece, pieces;           // classes of a piece
-  int sx, kx, sw, kw;          // slices of the reductions of dx (per piece) and dW, and their lengths
+  int sx, sw;                  // slices of the reductions of dx (per piece, if all rows count) and dW
   // forward workspace (saved for backward): packed x, packed W, exponents and count, bias, row list, lse, total
   int64_t o_xp, o_wp, o_exps, o_bl, o_order, o_target, o_lse, o_total, saved;
   // forward scratch
@@ -819,19 +839,6 @@ struct Plan {
   // backward scratch
   int64_t b_rs, b_fac, b_dn, b_db, b_px, b_pw, bwd;
 };
-
-// slices of a reduction of length k (a multiple of 64) over `tiles` output tiles: two workgroups per CU where the slices
-// are at least 1024 long, else one, down to 256 elements; at most 16
-void slices(int tiles, int k, int& s, int& per) {
-  if (tiles < 1) tiles = 1;
-  int want = 512 / tiles;
-  if (want > 1 && k / want < 1024) want = 256 / tiles;
-  const int most = k / 256 < 16 ? k / 256 : 16;
-  if (want > most) want = most;
-  if (want < 1) want = 1;
-  per = pad64((k + want - 1) / want);
-  s = (k + per - 1) / per;
-}
 
 Plan make_plan(int xf32, int wf32, int N, int V, int K) {
   Plan p;
@@ -849,8 +856,9 @@ Plan make_plan(int xf32, int wf32, int N, int V, int K) {
   p.piece = (int)(((all / GM + p.pieces - 1) / p.pieces) * GM);
   p.pieces = (all + p.piece - 1) / p.piece;
   const int tn = ceil_div(N, GM), tk = ceil_div(K, GM);
-  slices(tn * tk, p.piece, p.sx, p.kx);
-  slices((p.piece / GM) * tk, pad64(N), p.sw, p.kw);
+  int per;
+  slices(tn * tk, p.piece, p.sx, per);
+  slices((p.piece / GM) * tk, pad64(N), p.sw, per);
   int64_t o = 0;
   auto take = [&](int64_t bytes) {
     const int64_t at = o;
@@ -876,7 +884,9 @@ Plan make_plan(int xf32, int wf32, int N, int V, int K) {
   p.b_fac = take(16);
   p.b_dn = take((int64_t)p.pd * N * p.piece * 2);
   p.b_db = take((int64_t)tn * V * 4);
-  p.b_px = (p.pieces > 1 || p.sx > 1) ? take((int64_t)p.sx * N * K * 4) : -1;
+  // dx in slices: fewer rows that count take more of them, s <= 512 / (row tiles x tk), so s x rows stays below this
+  const int64_t most = 512 * GM / tk > N ? 512 * GM / tk : N;
+  p.b_px = (p.pieces > 1 || p.sx > 1) ? take((most < 16ll * N ? most : 16ll * N) * K * 4) : -1;
   p.b_pw = p.sw > 1 ? take((int64_t)p.sw * p.piece * K * 4) : -1;
   p.bwd = o;
   return p;
@@ -920,7 +930,9 @@ void pack_go(const Plan& p, const void* x, const void* w, const void* bias, int 
 
 template <int PC, int PM, int KM>
 void mm_go(const MmArgs& g, int out_bf16, hipStream_t st) {
-  const dim3 grid(g.tiles_m * g.tiles_n * g.splits), blk(G_THREADS);
+  int blocks = g.tiles_m * g.tiles_n * g.splits;
+  if (KM == ROW && g.part) blocks = max(g.tiles_m * g.tiles_n, 512);  // more than one slice only up to 512 workgroups
+  const dim3 grid(blocks), blk(G_THREADS);
   if (out_bf16) hipLaunchKernelGGL((ce_mm_kernel<PC, PM, KM, bf16>), grid, blk, 0, st, g);
   else hipLaunchKernelGGL((ce_mm_kernel<PC, PM, KM, float>), grid, blk, 0, st, g);
 }
@@ -942,12 +954,12 @@ void mm_terms(int pc, int pm, const MmArgs& g, int out_bf16, hipStream_t st) {
   else if (pc == 1) mm_go<1, 2, KM>(g, out_bf16, st);
   else mm_go<2, 2, KM>(g, out_bf16, st);
 }
-void dx_go(const float* part, int slices, int N, int K, const CeFac& fac, const int* exps, const int* order, void* dx,
+void dx_go(const float* part, int piece, int N, int K, const CeFac& fac, const int* exps, const int* order, void* dx,
            int out_bf16, hipStream_t st) {
   const dim3 grid((unsigned)ceil_div64((int64_t)N * ceil_div(K, 512), 4));
   const int vec = K % 8 == 0 && ((uintptr_t)dx & 15) == 0;
-  if (out_bf16) hipLaunchKernelGGL((ce_dx_kernel<bf16>), grid, dim3(256), 0, st, part, slices, N, K, fac, exps, order, vec, (bf16*)dx);
-  else hipLaunchKernelGGL((ce_dx_kernel<float>), grid, dim3(256), 0, st, part, slices, N, K, fac, exps, order, vec, (float*)dx);
+  if (out_bf16) hipLaunchKernelGGL((ce_dx_kernel<bf16>), grid, dim3(256), 0, st, part, piece, N, K, fac, exps, order, vec, (bf16*)dx);
+  else hipLaunchKernelGGL((ce_dx_kernel<float>), grid, dim3(256), 0, st, part, piece, N, K, fac, exps, order, vec, (float*)dx);
 }
 void reduce_go(const float* part, int slices, int64_t n, const CeFac& fac, const int* exps, int which, int add, void* out,
                int out_bf16, hipStream_t st) {
@@ -1044,7 +1056,7 @@ int vc_linear_ce_bwd(int xdtype, int wdtype, float smoothing, int mean,
       g.k = pad64(rows);
       g.tiles_m = tn;
       g.splits = p.sx;
-      g.kper = p.kx;
+      g.piece = p.piece;
       g.part = p.b_px >= 0 ? (float*)(ws + p.b_px) : nullptr;
       g.add = c > 0;
       g.out = dx;
@@ -1060,7 +1072,6 @@ int vc_linear_ce_bwd(int xdtype, int wdtype, float smoothing, int mean,
       g.k = pad64(N);
       g.tiles_m = ceil_div(rows, GM);
       g.splits = p.sw;
-      g.kper = p.kw;
       g.part = p.b_pw >= 0 ? (float*)(ws + p.b_pw) : nullptr;
       g.add = g.part ? 0 : accumulate & 1;
       g.out = out;
@@ -1071,7 +1082,7 @@ int vc_linear_ce_bwd(int xdtype, int wdtype, float smoothing, int mean,
     }
   }
   if (dx && p.b_px >= 0)
-    dx_go((const float*)(ws + p.b_px), p.sx, N, K, fac, exps, order, dx, xdtype == VC_BF16, stream);
+    dx_go((const float*)(ws + p.b_px), p.piece, N, K, fac, exps, order, dx, xdtype == VC_BF16, stream);
   if (db && tn > 1) {
     if (wdtype == VC_BF16)
       hipLaunchKernelGGL((ce_bias_kernel<bf16>), dim3(ceil_div(V, 256)), dim3(256), 0, stream, dbp, exps, V, fac,
