@@ -1366,36 +1366,41 @@ def cross_entropy(logits, target, stats=None):
 CE_REDUCTIONS = ("mean", "sum", "none")
 
 
+def _lce_forward(x, weight, bias, target, ignore_index, smoothing, reduction, want_pred):
+    """((loss or the rows' losses, predictions, correct rows), what the backward pass reads, sizes)."""
+    N, K = x.shape
+    V = weight.shape[0]
+    xd, wd, dev = L.dtype_code(x.dtype), L.dtype_code(weight.dtype), x.device
+    w = weight.detach().contiguous()
+    b = bias.detach().contiguous() if bias is not None else None
+    saved = torch.empty(_size("vc_linear_ce_bytes", 0, xd, wd, N, V, K), device=dev, dtype=torch.uint8)
+    ws = torch.empty(_size("vc_linear_ce_bytes", 1, xd, wd, N, V, K), device=dev, dtype=torch.uint8)
+    rows = torch.empty(N, device=dev, dtype=torch.float32)
+    loss = torch.empty((), device=dev, dtype=torch.float32) if reduction != "none" else None
+    pred = torch.empty(N, device=dev, dtype=torch.int64) if want_pred else None
+    correct = torch.empty(1, device=dev, dtype=torch.int32) if want_pred else None
+    L.fast("vc_linear_ce_fwd", dev, xd, wd, x.data_ptr(), w.data_ptr(), _addr(b), target.data_ptr(), ignore_index,
+           smoothing, reduction == "mean", rows.data_ptr(), _addr(loss), _addr(pred), _addr(correct), saved.data_ptr(),
+           ws.data_ptr(), N, V, K)
+    return (rows if loss is None else loss, pred, correct), saved, (N, V, K, xd, wd)
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, anchor, params, target, ignore_index, smoothing, reduction, want_pred):
-        weight, bias = params  # in a tuple, so that autograd does not see them
-        N, K = x.shape
-        V = weight.shape[0]
-        xd, wd, dev = L.dtype_code(x.dtype), L.dtype_code(weight.dtype), x.device
-        w = weight.detach().contiguous()
-        b = bias.detach().contiguous() if bias is not None else None
-        saved = torch.empty(_size("vc_linear_ce_bytes", 0, xd, wd, N, V, K), device=dev, dtype=torch.uint8)
-        ws = torch.empty(_size("vc_linear_ce_bytes", 1, xd, wd, N, V, K), device=dev, dtype=torch.uint8)
-        rows = torch.empty(N, device=dev, dtype=torch.float32)
-        loss = torch.empty((), device=dev, dtype=torch.float32) if reduction != "none" else None
-        pred = torch.empty(N, device=dev, dtype=torch.int64) if want_pred else None
-        correct = torch.empty(1, device=dev, dtype=torch.int32) if want_pred else None
-        L.fast("vc_linear_ce_fwd", dev, xd, wd, x.data_ptr(), w.data_ptr(), _addr(b), target.data_ptr(), ignore_index,
-               smoothing, reduction == "mean", rows.data_ptr(), _addr(loss), _addr(pred), _addr(correct), saved.data_ptr(),
-               ws.data_ptr(), N, V, K)
-        ctx.dims, ctx.codes, ctx.opts = (N, V, K), (xd, wd), (smoothing, reduction)
-        ctx.params, ctx.xdtype = params, x.dtype
+        # the parameters come in a tuple, so that autograd does not see them
+        out, saved, ctx.dims = _lce_forward(x, *params, target, ignore_index, smoothing, reduction, want_pred)
+        ctx.opts, ctx.params, ctx.xdtype = (smoothing, reduction), params, x.dtype
         ctx.save_for_backward(saved)
         if want_pred:
-            ctx.mark_non_differentiable(pred, correct)
-        return rows if loss is None else loss, pred, correct
+            ctx.mark_non_differentiable(*out[1:])
+        return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g, _dpred, _dcorrect):
         saved, = ctx.saved_tensors
-        (N, V, K), (xd, wd), (smoothing, reduction) = ctx.dims, ctx.codes, ctx.opts
+        (N, V, K, xd, wd), (smoothing, reduction) = ctx.dims, ctx.opts
         weight, bias = ctx.params
         dev = saved.device
         g = g.contiguous().float()
@@ -1458,11 +1463,13 @@ def linear_cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoot
             stats["correct"] = torch.zeros(1, device=x.device, dtype=torch.int32)
         return loss
     with _on(x.device):
-        _leaf_guard("linear_cross_entropy", x)
         x2 = (x if x.dim() == 2 else x.reshape(-1, x.shape[-1])).contiguous()
-        out, pred, correct = _LinearCrossEntropy.apply(x2, _anchor((x,), (weight, bias)), (weight, bias),
-                                                       target.reshape(-1).contiguous(), int(ignore_index),
-                                                       float(label_smoothing), reduction, stats is not None)
+        args = (target.reshape(-1).contiguous(), int(ignore_index), float(label_smoothing), reduction, stats is not None)
+        if not _wants_grad(x, weight, bias):
+            out, pred, correct = _lce_forward(x2, weight, bias, *args)[0]
+        else:
+            _leaf_guard("linear_cross_entropy", x)
+            out, pred, correct = _LinearCrossEntropy.apply(x2, _anchor((x,), (weight, bias)), (weight, bias), *args)
     if stats is not None:
         stats["pred"], stats["correct"] = pred, correct
     return out.view(target.shape) if reduction == "none" else out
@@ -1712,6 +1719,14 @@ def _anchor(inputs, params):
     return None
 
 
+def _wants_grad(*tensors):
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
 def _capturing(t):
     return t.is_cuda and torch.cuda.is_current_stream_capturing()
 
@@ -1842,33 +1857,39 @@ def _put_grad(p, g):
         p.grad.add_(g)
 
 
+def _gn_forward(x, residual, weight, bias, G, eps, act):
+    """(y, what the backward pass reads, sizes)."""
+    N, C = x.shape[0], x.shape[-1]
+    S = x.numel() // (N * C)
+    x = x.contiguous()
+    res = residual.contiguous() if residual is not None else None
+    dev = x.device
+    gamma, beta = _f32_param("group_norm", weight), _f32_param("group_norm", bias)
+    code, ws_floats = L.dtype_code(x.dtype), _size("vc_group_norm_workspace_floats", min(N, GN_SAMPLES), S, C, G)
+    y = torch.empty_like(x)
+    stat = torch.empty(2, N * G, device=dev, dtype=torch.float32)
+    ws = torch.empty(ws_floats, device=dev, dtype=torch.float32)
+    mean = stat.data_ptr()
+    for n, k, o in _gn_runs(N, S * C * x.element_size()):
+        L.fast("vc_group_norm_fwd", dev, code, x.data_ptr() + o, _addr(res, o), _addr(gamma), _addr(beta),
+               y.data_ptr() + o, mean + 4 * n * G, mean + 4 * (N + n) * G, ws.data_ptr(), k, S, C, G, eps, act)
+    return y, (x, res if act else None, stat, gamma, beta), (N, S, C, G, code, ws_floats)
+
+
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, anchor, params, G, eps, act):
-        weight, bias = params  # in a tuple, so that autograd does not see them
-        N, C = x.shape[0], x.shape[-1]
-        S = x.numel() // (N * C)
-        x = x.contiguous()
-        res = residual.contiguous() if residual is not None else None
-        dev = x.device
-        gamma, beta = _f32_param("group_norm", weight), _f32_param("group_norm", bias)
-        code, ws_floats = L.dtype_code(x.dtype), _size("vc_group_norm_workspace_floats", min(N, GN_SAMPLES), S, C, G)
-        y = torch.empty_like(x)
-        stat = torch.empty(2, N * G, device=dev, dtype=torch.float32)
-        ws = torch.empty(ws_floats, device=dev, dtype=torch.float32)
-        mean = stat.data_ptr()
-        for n, k, o in _gn_runs(N, S * C * x.element_size()):
-            L.fast("vc_group_norm_fwd", dev, code, x.data_ptr() + o, _addr(res, o), _addr(gamma), _addr(beta),
-                   y.data_ptr() + o, mean + 4 * n * G, mean + 4 * (N + n) * G, ws.data_ptr(), k, S, C, G, eps, act)
-        ctx.dims, ctx.act, ctx.params, ctx.code, ctx.ws_floats = (N, S, C, G), act, params, code, ws_floats
-        ctx.save_for_backward(x, res if act else None, stat, gamma, beta)
+        # the parameters come in a tuple, so that autograd does not see them
+        y, saved, ctx.dims = _gn_forward(x, residual, *params, G, eps, act)
+        ctx.act, ctx.params = act, params
+        ctx.save_for_backward(*saved)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         x, res, stat, gamma, beta = ctx.saved_tensors
-        N, S, C, G = ctx.dims
+        N, S, C, G, code, ws_floats = ctx.dims
         act, dev = ctx.act, x.device
         weight, bias = ctx.params
         dy = cast(dy.contiguous(), x.dtype)
@@ -1879,11 +1900,11 @@ class _GroupNorm(torch.autograd.Function):
         dw, add_w = _grad_target(weight)
         db, add_b = _grad_target(bias)
         if need_dx or dw is not None or db is not None or (need_dres and act):
-            ws = torch.empty(ctx.ws_floats, device=dev, dtype=torch.float32)
+            ws = torch.empty(ws_floats, device=dev, dtype=torch.float32)
             mean = stat.data_ptr()
             _before_grads(dev, dw, db)
             for n, k, o in _gn_runs(N, S * C * x.element_size()):
-                L.fast("vc_group_norm_bwd", dev, ctx.code, x.data_ptr() + o, dy.data_ptr() + o, _addr(res, o), _addr(gamma),
+                L.fast("vc_group_norm_bwd", dev, code, x.data_ptr() + o, dy.data_ptr() + o, _addr(res, o), _addr(gamma),
                        _addr(beta), mean + 4 * n * G, mean + 4 * (N + n) * G, _addr(dx, o), _addr(dres, o) if act else None,
                        _addr(dw), _addr(db), ws.data_ptr(), k, S, C, G, act, 3 if n else add_w + 2 * add_b)
             _put_grad(weight, dw)
@@ -1903,19 +1924,21 @@ def group_norm(x, gn, act="none", residual=None):
     if act not in GN_ACTS:
         raise ValueError(f"group_norm: act must be one of {sorted(GN_ACTS)}, not {act!r}")
     L.dtype_code(x.dtype)
-    _leaf_params("group_norm", gn.weight, gn.bias)
+    weight, bias = gn.weight, gn.bias
+    _leaf_params("group_norm", weight, bias)
     if x.dim() < 2 or x.shape[-1] != gn.num_channels:
         raise RuntimeError(f"group_norm: input of shape {tuple(x.shape)} does not end in {gn.num_channels} channels")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise RuntimeError(f"group_norm: residual {tuple(residual.shape)} {residual.dtype} does not match the input "
                            f"{tuple(x.shape)} {x.dtype}")
-    weight, bias = gn.weight, gn.bias
     _same_device("group_norm", x, residual, weight, bias)
     if x.numel() == 0:
         return x.clone()
     if x.shape[-1] > 1 << 20 or x.numel() // (x.shape[0] * x.shape[-1]) > 1 << 30:
         raise RuntimeError(f"group_norm: sizes {tuple(x.shape)} exceed 2^30 positions of a sample or 2^20 channels")
     with _on(x.device):
+        if not _wants_grad(x, residual, weight, bias):
+            return _gn_forward(x, residual, weight, bias, gn.num_groups, gn.eps, GN_ACTS[act])[0]
         _leaf_guard("group_norm", x, residual)
         return _GroupNorm.apply(x, residual, _anchor((x, residual), (weight, bias)), (weight, bias), gn.num_groups, gn.eps,
                                 GN_ACTS[act])
