@@ -359,7 +359,8 @@ int vc_ce_fwd_bwd(int grad_dtype, const float* logits, int ld, const int64_t* ta
  * target == ignore_index count for nothing, are not read, and cost no products; a target outside [0, V) makes its row's loss and
  * gradients NaN.  mean: divide by the rows that count (by 1 if there are none).
  * fwd: row_loss [N] (0 for ignored rows), loss (nullable, one float), pred [N] (nullable, lowest arg-max, 0 for ignored
- *   rows) and correct (nullable).  saved: vc_linear_ce_bytes(0, ..) bytes that backward reads; workspace: vc_linear_ce_bytes(1, ..).
+ *   rows) and correct (nullable).  saved: vc_linear_ce_bytes(0, ..) bytes that backward reads; workspace: vc_linear_ce_bytes(1, ..),
+ *   or with saved = null, for a call without a backward pass, vc_linear_ce_bytes(4, ..).
  * bwd: dloss = upstream gradient of the mean or sum, or with per_row of every row's loss (each resolved to 2^-39 of the
  *   largest); dx, dw and db (each nullable) are written, or added to where bit 0 (dw) / bit 1 (db) of `accumulate` is
  *   set; workspace: vc_linear_ce_bytes(2, ..).

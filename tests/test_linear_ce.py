@@ -472,3 +472,52 @@ def test_slices_of_few_rows(cuda):
         ops.linear_cross_entropy(xg, w.detach(), b.detach(), tt, reduction="sum").backward()
         check(reference(x, w, b, tt, 0.0, torch.ones(1500, device=cuda)), "bf16", dx=xg.grad, one_term=FEW_ROWS)
         assert (xg.grad[tt == -100] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("types,N,K,V,eps", [("bf16", 300, 64, 257, 0.0), ("bf16", 1, 128, 1, 0.0), ("bf16", 777, 192, 2100, 0.2),
+                                             ("bf16", 300, 72, 257, 0.1), ("mixed", 300, 64, 257, 0.0), ("f32", 90, 64, 300, 0.1)])
+def test_without_gradients(cuda, types, N, K, V, eps):
+    """A call that keeps nothing for a backward pass: bf16 operands with K a multiple of 64 are multiplied as they are."""
+    from video_classification_amd import ops
+    x, w, b, t = make(N, K, V, types, seed=12, ignored=0.4 if N > 1 else 0.0)
+    x[t == -100] = float("inf")
+    ref = reference(x, w, b, t, eps, torch.ones(N, device=cuda))
+    count = max(1, int((t != -100).sum()))
+    with torch.no_grad():
+        stats = {}
+        rows = ops.linear_cross_entropy(x, w, b, t, label_smoothing=eps, reduction="none", stats=stats)
+        mean = ops.linear_cross_entropy(x, w, b, t, label_smoothing=eps)
+        off = torch.empty(V * K + 1, device=cuda, dtype=w.dtype)[1:].view(V, K)  # a weight and rows off the 16-byte grid
+        off.copy_(w)
+        offx = torch.empty(N * K + 1, device=cuda, dtype=x.dtype)[1:].view(N, K)
+        offx.copy_(x)
+        shifted = ops.linear_cross_entropy(offx, off, b, t, label_smoothing=eps, reduction="none")
+        moved, still = (ops.linear_cross_entropy(v, w, b, t, label_smoothing=eps, reduction="none") for v in (offx, x))
+        bare = ops.linear_cross_entropy(x, w, None, t, reduction="sum")
+    check(ref, types, rows)
+    check(ref, types, shifted)
+    assert torch.equal(moved, still)
+    assert abs(mean.item() - float(ref["rows"].sum() / count)) <= 4 * ref["dz"] + 2.0 ** -20 * (1 + float(ref["lse"].abs().max()))
+    live = t != -100
+    top, picked = ref["z"].max(1).values, ref["z"].gather(1, stats["pred"][:, None])[:, 0]
+    assert (top - picked <= 2 * ref["dz"])[live].all() and (stats["pred"][~live] == 0).all()
+    assert int(stats["correct"]) == int(((stats["pred"] == t) & live).sum())
+    plain = reference(x, w, None, t, 0.0, torch.ones(N, device=cuda))
+    assert abs(bare.item() - float(plain["rows"].sum())) <= N * (4 * plain["dz"] + 2.0 ** -20 * (1 + float(plain["lse"].abs().max())))
+
+
+@pytest.mark.gpu
+def test_bf16_without_gradients_keeps_the_whole_range(cuda):
+    """Rows of very different magnitude do not take precision from each other where bf16 operands are used as they are."""
+    from video_classification_amd import ops
+    x, w, b, t = make(200, 64, 300, "bf16", seed=13)
+    want = torch.nn.functional.cross_entropy(x.double() @ w.detach().double().t() + b.detach().double(), t, reduction="none")
+    big = x.clone()
+    big[7] = 3e38
+    with torch.no_grad():
+        got = ops.linear_cross_entropy(big, w, b, t, reduction="none")
+        alone = ops.linear_cross_entropy(x, w, b, t, reduction="none")
+    keep = torch.arange(200, device=cuda) != 7
+    assert torch.equal(got[keep], alone[keep])
+    assert float((got.double() - want)[keep].abs().max()) < 1e-4

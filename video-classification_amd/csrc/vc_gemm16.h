@@ -74,9 +74,15 @@ __device__ __forceinline__ void f16_split(float v, f16& hi, f16& lo) {
   lo = (f16)(v - (float)hi);
 }
 
-// TB: blocks of 16 on either side of a wave's part of the tile, 4 (tiles of 128 x 128) or 2 (64 x 64)
-template <int PA, int PB, int KA = ROW, int KB = ROW, int TB = 4>
+// TB: blocks of 16 on either side of a wave's part of the tile, 4 (tiles of 128 x 128) or 2 (64 x 64).  BF: the operands are
+// bf16 as they came (one term each).
+template <int PA, int PB, int KA = ROW, int KB = ROW, int TB = 4, bool BF = false>
 struct G16 {
+  __device__ static __forceinline__ f32x4 mma(const f16x8& a, const f16x8& b, const f32x4& c) {
+    if constexpr (BF) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+
   static constexpr int T = 32 * TB;                  // rows of A and of B per tile
   static constexpr int BK = PA + PB == 2 ? 64 : 32;
   static constexpr int PLANE = T * BK;               // elements of one plane of a stage
@@ -232,7 +238,7 @@ struct G16 {
 #pragma unroll
       for (int n = 0; n < TB * TB; ++n) {
         const int i = n / TB, j = n % TB;
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1[i], b1[j], acc[i][j], 0, 0, 0);
+        acc[i][j] = mma(a1[i], b1[j], acc[i][j]);
         if (n % SP == 0) read2(st, n / SP);
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -247,15 +253,15 @@ struct G16 {
 #pragma unroll
       for (int n = 0; n < TB * TB; ++n) {
         const int i = n / TB, j = n % TB;
-        if (ONE) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a2[i], b2[j], acc[i][j], 0, 0, 0);
-        else if (PB == 2) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1[i], b2[j], acc[i][j], 0, 0, 0);
+        if (ONE) acc[i][j] = mma(a2[i], b2[j], acc[i][j]);
+        else if (PB == 2) acc[i][j] = mma(a1[i], b2[j], acc[i][j]);
         if (n % SP == 0) read1(sn, n / SP, an, bn);
         __builtin_amdgcn_sched_barrier(0);
       }
       if (!ONE && PA == 2)
 #pragma unroll
         for (int n = 0; n < TB * TB; ++n)
-          acc[n / TB][n % TB] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a2[n / TB], b1[n % TB], acc[n / TB][n % TB], 0, 0, 0);
+          acc[n / TB][n % TB] = mma(a2[n / TB], b1[n % TB], acc[n / TB][n % TB]);
 #pragma unroll
       for (int r = 0; r < TB; ++r) {
         a1[r] = an[r];

@@ -204,6 +204,34 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(const TX* __restrict__ x, 
   }
 }
 
+// A forward call whose operands are bf16 with K a multiple of 64 and that keeps nothing for a backward pass multiplies them as
+// they are: no scales, no copy of W (20011 x 512: 12 us of 75), the rows that count copied one behind the other.
+__global__ __launch_bounds__(256) void ce_list_kernel(const int64_t* __restrict__ target, int64_t ignore, int N, int V, RowList rows,
+                                                      float* __restrict__ rowloss, int64_t* __restrict__ pred) {
+  list_rows(target, ignore, N, V, rows, rowloss, pred);
+}
+__global__ __launch_bounds__(256) void ce_copy_kernel(const bf16* __restrict__ x, int V, int K, const int* __restrict__ order,
+                                                      bf16* __restrict__ xp, int* __restrict__ exps,
+                                                      const bf16* __restrict__ bias, float* __restrict__ bl) {
+  if (blockIdx.x == 0 && threadIdx.x < 2) exps[threadIdx.x] = 0;
+  const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
+  for (int64_t v = first; v < (V + GM - 1) / GM * GM; v += step) bl[v] = v >= V ? -INFINITY : bias ? to_f32(bias[v]) * LOG2E : 0.f;
+  const int per = K / 8;
+  const int64_t total = (int64_t)exps[2] * per;
+  const bool vec = ((uintptr_t)x & 15) == 0;
+  for (int64_t u = first; u < total; u += step) {
+    const int64_t row = u / per;
+    const int c = (int)(u - row * per) * 8;
+    const bf16* s = x + (int64_t)order[row] * K + c;
+    bf16x8 v;
+    if (vec) v = *reinterpret_cast<const bf16x8*>(s);
+    else
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = s[e];
+    *reinterpret_cast<bf16x8*>(xp + row * K + c) = v;
+  }
+}
+
 // ---- logits of a 128-class x 128-row tile ---------------------------------------------------------------------------
 // Everything behind the products works on z log2(e): the exponentials are then one subtraction and one v_exp_f32.
 struct CeArgs {
@@ -226,10 +254,10 @@ struct CeArgs {
 };
 
 // acc = z log2(e) without the bias, which follows in `bias` (-inf behind the last class): rows v0 + .., columns n0 + ..
-template <int PW, int PX>
+template <int PW, int PX, bool BF = false>
 __device__ __forceinline__ void logit_tile(const CeArgs& a, int v0, int n0, f16* smem, f32x4 (&acc)[4][4],
                                            f32x4 (&bias)[4], float& scale) {
-  typedef G16<PW, PX> G;
+  typedef G16<PW, PX, ROW, ROW, 4, BF> G;
   G::zero(acc);
   G::run(acc, Op16{a.w + (int64_t)v0 * a.ld, (int64_t)a.V * a.ld, a.ld, a.V - v0, 0},
          Op16{a.x + (int64_t)n0 * a.ld, (int64_t)a.N * a.ld, a.ld, a.rows() - n0, 0}, 0, a.ld, smem);
@@ -276,7 +304,7 @@ __device__ __forceinline__ void stat_join(Stat& a, const Stat& b) {
 //
 // part[vt][n] = (max, sum, sum z, arg) of the tile, zt[n] = the target's logit.  MORE: also sum z and arg (label smoothing,
 // predictions), which cost four operations more per logit.
-template <int PW, int PX, bool MORE>
+template <int PW, int PX, bool MORE, bool BF>
 __global__ __launch_bounds__(G_THREADS, 2) void ce_stats_kernel(CeArgs a, float4* __restrict__ part,
                                                                 float* __restrict__ zt) {
   __shared__ __attribute__((aligned(1024))) f16 smem[G16<PW, PX>::LDS];
@@ -286,7 +314,7 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_stats_kernel(CeArgs a, float4
   f32x4 acc[4][4];
   f32x4 bias[4];
   float scale;
-  logit_tile<PW, PX>(a, v0, n0, smem, acc, bias, scale);
+  logit_tile<PW, PX, BF>(a, v0, n0, smem, acc, bias, scale);
   const int lane = threadIdx.x & 63, q = lane >> 4, l15 = lane & 15;
   const int wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
   float4* xch = reinterpret_cast<float4*>(smem);
@@ -936,11 +964,11 @@ void mm_go(const MmArgs& g, int out_bf16, hipStream_t st) {
   if (out_bf16) hipLaunchKernelGGL((ce_mm_kernel<PC, PM, KM, bf16>), grid, blk, 0, st, g);
   else hipLaunchKernelGGL((ce_mm_kernel<PC, PM, KM, float>), grid, blk, 0, st, g);
 }
-template <int PW, int PX>
+template <int PW, int PX, bool BF = false>
 void stats_go(const CeArgs& a, bool more, float4* part, float* zt, hipStream_t st) {
   const dim3 grid(a.tiles_v * ceil_div(a.N, GM)), blk(G_THREADS);
-  if (more) hipLaunchKernelGGL((ce_stats_kernel<PW, PX, true>), grid, blk, 0, st, a, part, zt);
-  else hipLaunchKernelGGL((ce_stats_kernel<PW, PX, false>), grid, blk, 0, st, a, part, zt);
+  if (more) hipLaunchKernelGGL((ce_stats_kernel<PW, PX, true, BF>), grid, blk, 0, st, a, part, zt);
+  else hipLaunchKernelGGL((ce_stats_kernel<PW, PX, false, BF>), grid, blk, 0, st, a, part, zt);
 }
 template <int PW, int PX, int PD>
 void grad_go(const CeArgs& a, const float* lse, const float* rs, float smooth, int vbeg, int vcols, f16* dn, float* dbp,
@@ -977,7 +1005,7 @@ extern "C" {
 int64_t vc_linear_ce_bytes(int what, int xdtype, int wdtype, int N, int V, int K) {
   if (check_ce("vc_linear_ce_bytes", xdtype, wdtype, N, V, K, 0.f) != VC_OK) return -1;
   const Plan p = make_plan(xdtype == VC_F32, wdtype == VC_F32, N, V, K);
-  return what == 0 ? p.saved : what == 1 ? p.fwd : what == 2 ? p.bwd : -1;
+  return what == 0 ? p.saved : what == 1 ? p.fwd : what == 2 ? p.bwd : what == 4 ? p.fwd + p.saved : -1;
 }
 
 int vc_linear_ce_fwd(int xdtype, int wdtype, const void* x, const void* w, const void* bias, const int64_t* target,
@@ -985,28 +1013,41 @@ int vc_linear_ce_fwd(int xdtype, int wdtype, const void* x, const void* w, const
                      int* correct, void* saved, void* workspace, int N, int V, int K, hipStream_t stream) {
   const int rc = check_ce("vc_linear_ce_fwd", xdtype, wdtype, N, V, K, smoothing);
   if (rc != VC_OK) return rc;
-  VC_CHECK_ARG(x && w && target && row_loss && saved && workspace, "vc_linear_ce_fwd: null pointer");
+  VC_CHECK_ARG(x && w && target && row_loss && workspace, "vc_linear_ce_fwd: null pointer");
+  VC_CHECK_ARG(loss || !mean, "vc_linear_ce_fwd: a mean without its place");
   VC_CHECK_ARG(!correct || pred, "vc_linear_ce_fwd: the count of correct rows needs pred");
   VC_CHECK_ARG((((uintptr_t)saved | (uintptr_t)workspace) & 255) == 0, "vc_linear_ce_fwd: buffers must be 256-byte aligned");
   const Plan p = make_plan(xdtype == VC_F32, wdtype == VC_F32, N, V, K);
-  char *sv = (char*)saved, *ws = (char*)workspace;
-  if (xdtype == VC_F32) pack_go<float, float>(p, x, w, bias, N, V, K, target, ignore_index, row_loss, pred, sv, ws, stream);
+  char *ws = (char*)workspace, *sv = saved ? (char*)saved : ws + p.fwd;
+  const bool raw = !saved && xdtype == VC_BF16 && wdtype == VC_BF16 && K % 64 == 0 && ((uintptr_t)w & 15) == 0;
+  const RowList list{(int*)(sv + p.o_order), (int*)(sv + p.o_target), (int*)(sv + p.o_exps) + 2};
+  if (raw) {
+    hipLaunchKernelGGL(ce_list_kernel, dim3(1), dim3(256), 0, stream, target, ignore_index, N, V, list, row_loss, pred);
+    const int64_t units = (int64_t)N * (K / 8), most = units > V ? units : V;
+    hipLaunchKernelGGL(ce_copy_kernel, dim3((unsigned)(ceil_div64(most, 256) < 2048 ? ceil_div64(most, 256) : 2048)), dim3(256), 0,
+                       stream, (const bf16*)x, V, K, list.order, (bf16*)(sv + p.o_xp), (int*)(sv + p.o_exps), (const bf16*)bias,
+                       (float*)(sv + p.o_bl));
+  } else if (xdtype == VC_F32) pack_go<float, float>(p, x, w, bias, N, V, K, target, ignore_index, row_loss, pred, sv, ws, stream);
   else if (wdtype == VC_F32) pack_go<bf16, float>(p, x, w, bias, N, V, K, target, ignore_index, row_loss, pred, sv, ws, stream);
   else pack_go<bf16, bf16>(p, x, w, bias, N, V, K, target, ignore_index, row_loss, pred, sv, ws, stream);
-  CeArgs a{(const f16*)(sv + p.o_wp), (const f16*)(sv + p.o_xp), (const float*)(sv + p.o_bl), (const int*)(sv + p.o_target), (const int*)(sv + p.o_exps), N, V, p.ld,
+  CeArgs a{raw ? (const f16*)w : (const f16*)(sv + p.o_wp), (const f16*)(sv + p.o_xp), (const float*)(sv + p.o_bl),
+           list.target, (const int*)(sv + p.o_exps), N, V, p.ld,
            wdtype == VC_BF16, ceil_div(V, GM)};
   float4* part = (float4*)(ws + p.f_part);
   float* zt = (float*)(ws + p.f_zt);
   const bool more = smoothing > 0.f || pred;
-  if (p.pw == 2) stats_go<2, 2>(a, more, part, zt, stream);
+  if (raw) stats_go<1, 1, true>(a, more, part, zt, stream);
+  else if (p.pw == 2) stats_go<2, 2>(a, more, part, zt, stream);
   else stats_go<1, 1>(a, more, part, zt, stream);
   const CeRows rows{zt, a.target, (const int*)(sv + p.o_order), a.exps, N, V, a.tiles_v, smoothing, (float*)(sv + p.o_lse), row_loss, pred};
   float* total = (float*)(sv + p.o_total);
-  if (N <= 1024 && a.tiles_v <= 16) {
+  const bool sums = loss || correct;
+  if (sums && N <= 1024 && a.tiles_v <= 16) {
     hipLaunchKernelGGL(ce_total_kernel<true>, dim3(1), dim3(1024), 0, stream, rows, part, mean, loss, total, correct);
   } else {
     hipLaunchKernelGGL(ce_join_kernel, dim3(ceil_div(N, 8)), dim3(256), 0, stream, rows, part);
-    hipLaunchKernelGGL(ce_total_kernel<false>, dim3(1), dim3(1024), 0, stream, rows, part, mean, loss, total, correct);
+    if (sums)
+      hipLaunchKernelGGL(ce_total_kernel<false>, dim3(1), dim3(1024), 0, stream, rows, part, mean, loss, total, correct);
   }
   VC_LAUNCH_CHECK("vc_linear_ce_fwd");
   return VC_OK;

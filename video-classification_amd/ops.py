@@ -1366,21 +1366,21 @@ def cross_entropy(logits, target, stats=None):
 CE_REDUCTIONS = ("mean", "sum", "none")
 
 
-def _lce_forward(x, weight, bias, target, ignore_index, smoothing, reduction, want_pred):
+def _lce_forward(x, weight, bias, target, ignore_index, smoothing, reduction, want_pred, keep=True):
     """((loss or the rows' losses, predictions, correct rows), what the backward pass reads, sizes)."""
     N, K = x.shape
     V = weight.shape[0]
     xd, wd, dev = L.dtype_code(x.dtype), L.dtype_code(weight.dtype), x.device
     w = weight.detach().contiguous()
     b = bias.detach().contiguous() if bias is not None else None
-    saved = torch.empty(_size("vc_linear_ce_bytes", 0, xd, wd, N, V, K), device=dev, dtype=torch.uint8)
-    ws = torch.empty(_size("vc_linear_ce_bytes", 1, xd, wd, N, V, K), device=dev, dtype=torch.uint8)
+    saved = torch.empty(_size("vc_linear_ce_bytes", 0, xd, wd, N, V, K), device=dev, dtype=torch.uint8) if keep else None
+    ws = torch.empty(_size("vc_linear_ce_bytes", 1 if keep else 4, xd, wd, N, V, K), device=dev, dtype=torch.uint8)
     rows = torch.empty(N, device=dev, dtype=torch.float32)
     loss = torch.empty((), device=dev, dtype=torch.float32) if reduction != "none" else None
     pred = torch.empty(N, device=dev, dtype=torch.int64) if want_pred else None
     correct = torch.empty(1, device=dev, dtype=torch.int32) if want_pred else None
     L.fast("vc_linear_ce_fwd", dev, xd, wd, x.data_ptr(), w.data_ptr(), _addr(b), target.data_ptr(), ignore_index,
-           smoothing, reduction == "mean", rows.data_ptr(), _addr(loss), _addr(pred), _addr(correct), saved.data_ptr(),
+           smoothing, reduction == "mean", rows.data_ptr(), _addr(loss), _addr(pred), _addr(correct), _addr(saved),
            ws.data_ptr(), N, V, K)
     return (rows if loss is None else loss, pred, correct), saved, (N, V, K, xd, wd)
 
@@ -1466,7 +1466,7 @@ def linear_cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoot
         x2 = (x if x.dim() == 2 else x.reshape(-1, x.shape[-1])).contiguous()
         args = (target.reshape(-1).contiguous(), int(ignore_index), float(label_smoothing), reduction, stats is not None)
         if not _wants_grad(x, weight, bias):
-            out, pred, correct = _lce_forward(x2, weight, bias, *args)[0]
+            out, pred, correct = _lce_forward(x2, weight, bias, *args, keep=False)[0]
         else:
             _leaf_guard("linear_cross_entropy", x)
             out, pred, correct = _LinearCrossEntropy.apply(x2, _anchor((x,), (weight, bias)), (weight, bias), *args)
