@@ -11,7 +11,7 @@
 // 2 N V K operations forward, 6 N V K backward (the logits once more, dx, dW): bound by the matrix pipes for the sizes where
 // time matters, which is why the logits are recomputed rather than kept: N x V fp32 logits written and read cost as much
 // as the product at K = 1024 and gigabytes of memory.  8192 x 1024 x 65536 in bf16: 4.39 ms forward and backward, 1.0 PFLOP/s
-// over its four products; 2048 x 512 x 20011 forward: 75 us, 53 of them the statistics (0.8 PFLOP/s).
+// over its four products; 2048 x 512 x 20011 forward: 64 us, 54 of them the statistics (0.8 PFLOP/s).
 //
 // All products run on fp16 terms (vc_gemm16.h).  x and W are scaled by one power of two each (from their largest finite
 // magnitude): bf16 values are exact in one term over 29 binades and within 2^-40 of the largest magnitude below that, fp32
@@ -205,7 +205,7 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(const TX* __restrict__ x, 
 }
 
 // A forward call whose operands are bf16 with K a multiple of 64 and that keeps nothing for a backward pass multiplies them as
-// they are: no scales, no copy of W (20011 x 512: 12 us of 75), the rows that count copied one behind the other.
+// they are: no scales, no copy of W (2048 x 512 x 20011: 75 -> 64 us), the rows that count copied one behind the other.
 __global__ __launch_bounds__(256) void ce_list_kernel(const int64_t* __restrict__ target, int64_t ignore, int N, int V, RowList rows,
                                                       float* __restrict__ rowloss, int64_t* __restrict__ pred) {
   list_rows(target, ignore, N, V, rows, rowloss, pred);

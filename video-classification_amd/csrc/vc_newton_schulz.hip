@@ -7,8 +7,8 @@
 // and stored twice), bound by the matrix pipes for large matrices and by the chain of launches for small ones, so all
 // matrices of a call share each launch, three a step and a join where a reduction is cut.
 //   4096 x 4096: S 210 + 9 us, P 212 + 10, update 389 (1.06 PFLOP/s of fp16 products); 5 steps 3.9 ms
-//   52 matrices of a ResNet-50 (64 to 2048 rows): 195 us a step, 0.97 ms in all
-//   4 matrices of up to 256 x 1152, on 64 x 64 tiles: 24 us a step -- six microseconds a launch, most of them latency
+//   52 matrices of a ResNet-50 (64 to 2048 rows): 195 us a step, 0.95 - 1.01 ms in all
+//   4 matrices of up to 256 x 1152, on 64 x 64 tiles: 23 us a step -- six microseconds a launch, most of them latency
 //
 // Precision: a gradient's small singular values are amplified by a^steps (485 for the usual coefficients) and with them the
 // rounding of X, so bf16 products leave errors of 1 % of the largest entry for random matrices and 50 % for matrices of
