@@ -327,11 +327,17 @@ __device__ __forceinline__ void f16_split8(const F8& v, f16x8& hi, f16x8& lo) {
   }
 }
 
-// Workgroup -> tile: consecutive workgroups of one XCD (every eighth) walk bands of eight tile rows, so that the rows of A
-// and B they share stay in that XCD's L2.
-__device__ __forceinline__ void g16_tile(int id, int total, int tm, int tn, int& m, int& n) {
+// Workgroup -> tile (of a slice of the reduction): consecutive workgroups of one XCD (every eighth) walk bands of eight tile
+// rows, slice after slice, so that the rows of A and B they share stay in that XCD's L2.
+__device__ __forceinline__ void g16_tile(int id, int slices, int tm, int tn, int& slice, int& m, int& n) {
+  const int tiles = tm * tn, total = tiles * slices;
   const int q = total >> 3, r = total & 7, xcd = id & 7, idx = id >> 3;
-  const int v = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + idx;
+  int v = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + idx;
+  slice = 0;
+  if (slices > 1) {
+    slice = v / tiles;
+    v -= slice * tiles;
+  }
   const int band = v / (8 * tn), first = band * 8, rows = tm - first < 8 ? tm - first : 8;
   const int w = v - band * 8 * tn;
   m = first + w % rows;

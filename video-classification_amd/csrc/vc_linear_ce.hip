@@ -240,7 +240,7 @@ struct CeArgs {
   const float* bl;   // bias log2(e), -inf behind the last class
   const int* target; // of the packed rows
   const int* exps;
-  int N, V, ld, db_bf16;
+  int N, V, K, ld, db_bf16;
   int tiles_v;
 
   __device__ __forceinline__ int rows() const { return exps[2]; }
@@ -248,7 +248,8 @@ struct CeArgs {
   __device__ __forceinline__ bool tile(int& tv, int& tn) const {
     const int tiles_n = max(1, (rows() + GM - 1) / GM), total = tiles_v * tiles_n;
     if ((int)blockIdx.x >= total) return false;
-    g16_tile(blockIdx.x, total, tiles_v, tiles_n, tv, tn);
+    int slice;
+    g16_tile(blockIdx.x, 1, tiles_v, tiles_n, slice, tv, tn);
     return true;
   }
 };
@@ -260,7 +261,7 @@ __device__ __forceinline__ void logit_tile(const CeArgs& a, int v0, int n0, f16*
   typedef G16<PW, PX, ROW, ROW, 4, BF> G;
   G::zero(acc);
   G::run(acc, Op16{a.w + (int64_t)v0 * a.ld, (int64_t)a.V * a.ld, a.ld, a.V - v0, 0},
-         Op16{a.x + (int64_t)n0 * a.ld, (int64_t)a.N * a.ld, a.ld, a.rows() - n0, 0}, 0, a.ld, smem);
+         Op16{a.x + (int64_t)n0 * a.ld, (int64_t)a.N * a.ld, a.ld, a.rows() - n0, 0}, 0, (a.K + G::BK - 1) / G::BK * G::BK, smem);
   const float* bl = a.bl + v0 + (threadIdx.x >> 7) * 64 + ((threadIdx.x & 63) >> 4) * 4;
 #pragma unroll
   for (int i = 0; i < 4; ++i) bias[i] = *reinterpret_cast<const f32x4*>(bl + i * 16);
@@ -705,7 +706,7 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
     tn = id % g.tiles_n;
     split = 0;
   } else
-    g16_tile(blockIdx.x - split * tiles, tiles, tiles_m, g.tiles_n, tm, tn);
+    g16_tile(blockIdx.x, splits, tiles_m, g.tiles_n, split, tm, tn);
   const int m0 = tm * GM, n0 = tn * GM;
   f32x4 acc[4][4];
   G::zero(acc);
@@ -1031,7 +1032,7 @@ int vc_linear_ce_fwd(int xdtype, int wdtype, const void* x, const void* w, const
   else if (wdtype == VC_F32) pack_go<bf16, float>(p, x, w, bias, N, V, K, target, ignore_index, row_loss, pred, sv, ws, stream);
   else pack_go<bf16, bf16>(p, x, w, bias, N, V, K, target, ignore_index, row_loss, pred, sv, ws, stream);
   CeArgs a{raw ? (const f16*)w : (const f16*)(sv + p.o_wp), (const f16*)(sv + p.o_xp), (const float*)(sv + p.o_bl),
-           list.target, (const int*)(sv + p.o_exps), N, V, p.ld,
+           list.target, (const int*)(sv + p.o_exps), N, V, K, p.ld,
            wdtype == VC_BF16, ceil_div(V, GM)};
   float4* part = (float4*)(ws + p.f_part);
   float* zt = (float*)(ws + p.f_zt);
@@ -1078,7 +1079,7 @@ int vc_linear_ce_bwd(int xdtype, int wdtype, float smoothing, int mean,
   for (int c = 0; c < p.pieces; ++c) {
     const int vbeg = c * p.piece;
     const int vcols = p.piece < ceil_div(V - vbeg, GM) * GM ? p.piece : ceil_div(V - vbeg, GM) * GM;
-    CeArgs a{wp, xp, (const float*)(sv + p.o_bl), (const int*)(sv + p.o_target), exps, N, V, p.ld, wdtype == VC_BF16, vcols / GM};
+    CeArgs a{wp, xp, (const float*)(sv + p.o_bl), (const int*)(sv + p.o_target), exps, N, V, K, p.ld, wdtype == VC_BF16, vcols / GM};
     float* dbq = db ? dbp : nullptr;
     if (p.pw == 2) grad_go<2, 2, 2>(a, lse, rs, smoothing, vbeg, vcols, dn, dbq, fac, db, accumulate & 2, stream);
     else if (p.pd == 2) grad_go<1, 1, 2>(a, lse, rs, smoothing, vbeg, vcols, dn, dbq, fac, db, accumulate & 2, stream);

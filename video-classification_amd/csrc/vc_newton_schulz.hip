@@ -401,8 +401,8 @@ __global__ __launch_bounds__(G_THREADS, 2) void ns_update_kernel(const NsMat* __
   const NsMat t = table[i];
   const NsView w(t, parity);
   const int tiles_m = (t.m + G::T - 1) / G::T, tiles_n = (t.n + G::T - 1) / G::T;
-  int tm, tn;
-  g16_tile(blockIdx.x - t.first[BY_UPDATE], tiles_m * tiles_n, tiles_m, tiles_n, tm, tn);
+  int tm, tn, slice;
+  g16_tile(blockIdx.x - t.first[BY_UPDATE], 1, tiles_m, tiles_n, slice, tm, tn);
   const int m0 = tm * G::T, n0 = tn * G::T;
   const int64_t pp = (int64_t)t.m * w.ldm, px = (int64_t)t.m * w.ldn;
   const f16* x = ws + w.x;
