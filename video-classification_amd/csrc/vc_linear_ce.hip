@@ -676,7 +676,8 @@ struct MmArgs {
   int tiles_m, tiles_n, splits;
   int piece;                   // dx: classes of a whole piece, whose slices every piece takes
   const int* order;            // dx: where its packed rows go
-  float* part;                 // [splits][M, of dx: rows that count][Nn], or null: write out
+  float* part;                 // [splits][M, of dx: rows that count][pitch], or null: write out
+  int pitch;                   // of part (dx: a multiple of 8) or out
   int add;                     // add to what part / out hold
   void* out;                   // [M][Nn]
   CeFac fac;
@@ -727,7 +728,7 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
   const int lane = threadIdx.x & 63, q = lane >> 4, l15 = lane & 15;
   const int wave = threadIdx.x >> 6, wc = wave >> 1, wr = wave & 1;
   const float f = g.part ? 1.f : mm_factor(g.fac, g.exps, g.which);
-  float* part = g.part ? g.part + (int64_t)split * (KM == ROW ? rows : g.M) * g.Nn : nullptr;
+  float* part = g.part ? g.part + (int64_t)split * (KM == ROW ? rows : g.M) * g.pitch : nullptr;
   const bool vec = g.vec;
   if (!part)
 #pragma unroll
@@ -740,7 +741,7 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int row = m0 + wr * 64 + j * 16 + l15, r = min(row, g.M - 1);
-    at[j] = (int64_t)(KM == ROW && !part ? g.order[r] : r) * g.Nn;
+    at[j] = (int64_t)(KM == ROW && !part ? g.order[r] : r) * g.pitch;
     if (row >= live)
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -751,7 +752,7 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int64_t o = at[j] + min(n0 + wc * 64 + i * 16 + q * 4, g.Nn - 4);
+        const int64_t o = at[j] + min(n0 + wc * 64 + i * 16 + q * 4, g.pitch - 4);
         if (part) acc[i][j] += *reinterpret_cast<const f32x4*>(part + o);
         else if constexpr (sizeof(T) == 4) acc[i][j] += *reinterpret_cast<const f32x4*>((const float*)g.out + o);
         else {
@@ -770,7 +771,7 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
       const int64_t o = at[j] + col;
       const f32x4 v = acc[i][j];
       if (vec) {
-        if (col >= g.Nn) continue;
+        if (col >= g.pitch) continue;
         if (part) *reinterpret_cast<f32x4*>(part + o) = v;
         else if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4*>((float*)g.out + o) = v;
         else *reinterpret_cast<bf16x4*>((bf16*)g.out + o) = bf16x4{(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
@@ -799,12 +800,13 @@ __global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ pa
   const int rows = exps[2];
   int splits, len;
   slices(max(1, (rows + GM - 1) / GM) * ((K + GM - 1) / GM), piece, splits, len);
-  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), n = (int64_t)rows * K;
+  const int pitch = (K + 7) / 8 * 8;
+  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), n = (int64_t)rows * pitch;
   const int r = (int)(unit / per), c0 = (int)(unit - (int64_t)r * per) * 512 + (threadIdx.x & 63) * (vec ? 8 : 1);
   if (r >= N) return;
   const bool live = r < rows;
   const float f = mm_factor(fac, exps, 1);
-  const float* p = part + (int64_t)r * K;
+  const float* p = part + (int64_t)r * pitch;
   T* o = out + (int64_t)order[r] * K;
   if (vec) {
     if (c0 >= K) return;
@@ -915,7 +917,7 @@ Plan make_plan(int xf32, int wf32, int N, int V, int K) {
   p.b_db = take((int64_t)tn * V * 4);
   // dx in slices: fewer rows that count take more of them, s <= 512 / (row tiles x tk), so s x rows stays below this
   const int64_t most = 512 * GM / tk > N ? 512 * GM / tk : N;
-  p.b_px = (p.pieces > 1 || p.sx > 1) ? take((most < 16ll * N ? most : 16ll * N) * K * 4) : -1;
+  p.b_px = (p.pieces > 1 || p.sx > 1) ? take((most < 16ll * N ? most : 16ll * N) * ((K + 7) / 8 * 8) * 4) : -1;
   p.b_pw = p.sw > 1 ? take((int64_t)p.sw * p.piece * K * 4) : -1;
   p.bwd = o;
   return p;
@@ -1086,7 +1088,7 @@ int vc_linear_ce_bwd(int xdtype, int wdtype, float smoothing, int mean,
     else grad_go<1, 1, 1>(a, lse, rs, smoothing, vbeg, vcols, dn, dbq, fac, db, accumulate & 2, stream);
     const int rows = vcols < V - vbeg ? vcols : V - vbeg;
     MmArgs g{};
-    g.Nn = K;
+    g.Nn = g.pitch = K;
     g.tiles_n = tk;
     g.fac = fac;
     g.exps = exps;
@@ -1103,7 +1105,8 @@ int vc_linear_ce_bwd(int xdtype, int wdtype, float smoothing, int mean,
       g.add = c > 0;
       g.out = dx;
       g.which = 1;
-      g.vec = K % 4 == 0 && ((uintptr_t)dx & 15) == 0;
+      if (g.part) g.pitch = (K + 7) / 8 * 8;
+      g.vec = g.part || (K % 4 == 0 && ((uintptr_t)dx & 15) == 0);
       mm_terms<ROW>(p.pw, p.pdx, g, xdtype == VC_BF16, stream);
     }
     if (dw) {
@@ -1114,6 +1117,7 @@ int vc_linear_ce_bwd(int xdtype, int wdtype, float smoothing, int mean,
       g.k = pad64(N);
       g.tiles_m = ceil_div(rows, GM);
       g.splits = p.sw;
+      g.pitch = K;
       g.part = p.b_pw >= 0 ? (float*)(ws + p.b_pw) : nullptr;
       g.add = g.part ? 0 : accumulate & 1;
       g.out = out;
