@@ -160,10 +160,13 @@ __device__ __forceinline__ void pack_rows(const T* __restrict__ src, f16* __rest
   if (c0 >= ld) return;
   const T* s = src + (order ? order[row] : row) * (int64_t)K;
   float v[8];
-  if (c0 + 8 <= K && ((uintptr_t)(s + c0) & 15) == 0) {
-    const F8 t = load8(s + c0);
+  if (c0 + 8 <= K) {
+    struct __attribute__((packed, aligned(sizeof(T)))) Row8 {
+      T v[8];
+    };
+    const Row8 t = *reinterpret_cast<const Row8*>(s + c0);  // wide loads whatever the alignment of the row
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = t.v[i];
+    for (int i = 0; i < 8; ++i) v[i] = to_f32(t.v[i]);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = c0 + i < K ? to_f32(s[c0 + i]) : 0.f;
@@ -683,7 +686,6 @@ struct MmArgs {
   CeFac fac;
   const int* exps;             // exps[2] = rows that count: rows of dx that are worked, reduction length of dW
   int which;                   // whose scale exponent the column side carries
-  int vec;                     // rows of the result start on 16-byte (fp32) / 8-byte (bf16) boundaries
 };
 
 __device__ __forceinline__ float mm_factor(const CeFac& fac, const int* exps, int which) {
@@ -729,7 +731,6 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
   const int wave = threadIdx.x >> 6, wc = wave >> 1, wr = wave & 1;
   const float f = g.part ? 1.f : mm_factor(g.fac, g.exps, g.which);
   float* part = g.part ? g.part + (int64_t)split * (KM == ROW ? rows : g.M) * g.pitch : nullptr;
-  const bool vec = g.vec;
   if (!part)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -746,17 +747,22 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
+  // Rows of any length: four results are one access of the result's own alignment, the last few of a row one by one.
+  typedef f32x4 u32x4 __attribute__((aligned(4)));
+  typedef bf16x4 u16x4 __attribute__((aligned(2)));
   // what is added to comes first: the stores could alias these loads and would hold them back
-  if (vec && g.add) {
+  if (g.add) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int64_t o = at[j] + min(n0 + wc * 64 + i * 16 + q * 4, g.pitch - 4);
-        if (part) acc[i][j] += *reinterpret_cast<const f32x4*>(part + o);
-        else if constexpr (sizeof(T) == 4) acc[i][j] += *reinterpret_cast<const f32x4*>((const float*)g.out + o);
+        const int col = n0 + wc * 64 + i * 16 + q * 4;
+        if (col > g.pitch - 4) continue;
+        const int64_t o = at[j] + col;
+        if (part) acc[i][j] += *reinterpret_cast<const u32x4*>(part + o);
+        else if constexpr (sizeof(T) == 4) acc[i][j] += *reinterpret_cast<const u32x4*>((const float*)g.out + o);
         else {
-          const bf16x4 r = *reinterpret_cast<const bf16x4*>((const bf16*)g.out + o);
+          const bf16x4 r = *reinterpret_cast<const u16x4*>((const bf16*)g.out + o);
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[i][j][e] += (float)r[e];
         }
@@ -770,15 +776,14 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
       const int col = n0 + wc * 64 + i * 16 + q * 4;  // four results of one row
       const int64_t o = at[j] + col;
       const f32x4 v = acc[i][j];
-      if (vec) {
-        if (col >= g.pitch) continue;
-        if (part) *reinterpret_cast<f32x4*>(part + o) = v;
-        else if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4*>((float*)g.out + o) = v;
-        else *reinterpret_cast<bf16x4*>((bf16*)g.out + o) = bf16x4{(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
+      if (col <= g.pitch - 4) {
+        if (part) *reinterpret_cast<u32x4*>(part + o) = v;
+        else if constexpr (sizeof(T) == 4) *reinterpret_cast<u32x4*>((float*)g.out + o) = v;
+        else *reinterpret_cast<u16x4*>((bf16*)g.out + o) = bf16x4{(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
       } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (col + e >= g.Nn) break;
+        for (int e = 0; e < 3; ++e) {
+          if (col + e >= g.pitch) break;
           if (part) part[o + e] = g.add ? part[o + e] + v[e] : v[e];
           else {
             T* out = (T*)g.out + o + e;
@@ -1106,7 +1111,6 @@ int vc_linear_ce_bwd(int xdtype, int wdtype, float smoothing, int mean,
       g.out = dx;
       g.which = 1;
       if (g.part) g.pitch = (K + 7) / 8 * 8;
-      g.vec = g.part || (K % 4 == 0 && ((uintptr_t)dx & 15) == 0);
       mm_terms<ROW>(p.pw, p.pdx, g, xdtype == VC_BF16, stream);
     }
     if (dw) {
@@ -1122,7 +1126,6 @@ int vc_linear_ce_bwd(int xdtype, int wdtype, float smoothing, int mean,
       g.add = g.part ? 0 : accumulate & 1;
       g.out = out;
       g.which = 0;
-      g.vec = K % 4 == 0 && ((uintptr_t)dw & 15) == 0;
       mm_terms<COL>(p.px, p.pdw, g, wdtype == VC_BF16, stream);
       if (g.part) reduce_go(g.part, p.sw, (int64_t)rows * K, fac, exps, 0, accumulate & 1, out, wdtype == VC_BF16, stream);
     }
