@@ -521,3 +521,41 @@ def test_bf16_without_gradients_keeps_the_whole_range(cuda):
     keep = torch.arange(200, device=cuda) != 7
     assert torch.equal(got[keep], alone[keep])
     assert float((got.double() - want)[keep].abs().max()) < 1e-4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("types,N,K,V", [("bf16", 1500, 128, 9000), ("mixed", 260, 72, 300), ("f32", 300, 40, 700)])
+def test_replays_follow_the_rows_that_count(cuda, types, N, K, V):
+    """How many rows count is read on the device: one captured step serves every mask, from none to all rows."""
+    from video_classification_amd import ops
+    x, w, b, t = make(N, K, V, types, seed=21)
+    xs, ts = x.clone().requires_grad_(True), t.clone()
+    w.grad, b.grad, xs.grad = torch.zeros_like(w), torch.zeros_like(b), torch.zeros_like(xs)
+
+    def step():
+        for g in (w.grad, b.grad, xs.grad):
+            g.zero_()
+        loss = ops.linear_cross_entropy(xs, w, b, ts)
+        loss.backward()
+        with torch.no_grad():
+            rows = ops.linear_cross_entropy(xs, w, b, ts, reduction="none")
+        return loss.detach(), rows
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, rows = step()
+    for k, share in enumerate((0.0, 0.9, 0.5, 1.0, 0.0, 0.3)):
+        drop = torch.rand(N, generator=torch.Generator().manual_seed(k)) < share
+        ts.copy_(torch.where(drop.to(cuda), torch.full_like(t, -100), t.roll(k)))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [loss.clone(), rows.clone(), xs.grad.clone(), w.grad.clone(), b.grad.clone()]
+        want = step()
+        want = [want[0], want[1], xs.grad, w.grad, b.grad]
+        for g, e in zip(got, want):
+            assert torch.equal(g, e)
