@@ -21,6 +21,10 @@ import torch.distributed as dist
 from . import ops
 from .trainer import forward_for
 
+# A process group's watchdog thread queries the events of earlier collectives whenever it likes; in the default (global) mode
+# such a query fails while any thread captures, and the watchdog ends the process.
+CAPTURE_MODE = "thread_local"
+
 
 class GraphedTrainStep:
     def __init__(self, model, optimizer, criterion, x_example, y_example, warmup=3, phased=True):
@@ -51,7 +55,7 @@ class GraphedTrainStep:
         self.graphs = []
         try:
             g0 = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(g0):
+            with torch.cuda.graph(g0, capture_error_mode=CAPTURE_MODE):
                 self.opt.flat.zero_grad()
                 out = forward_for(model, criterion, self.x)
                 self.loss = criterion(out, self.y)
@@ -70,7 +74,8 @@ class GraphedTrainStep:
             for k in range(len(cuts) - 1, -1, -1):
                 cur[0] += 1
                 gk = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(gk, pool=g0.pool()):  # one memory pool: activations of phase 0 are freed here
+                # one memory pool: activations of phase 0 are freed here
+                with torch.cuda.graph(gk, pool=g0.pool(), capture_error_mode=CAPTURE_MODE):
                     if k > 0:
                         grad = torch.autograd.grad([cuts[k]], [cuts[k - 1]], [grad])[0]
                     else:
@@ -150,7 +155,7 @@ class GraphedInference:
             torch.cuda.current_stream().wait_stream(side)
             torch.cuda.synchronize()
             self.graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(self.graph):
+            with torch.cuda.graph(self.graph, capture_error_mode=CAPTURE_MODE):
                 self.out = model(self.x)
 
     def __call__(self, x):
