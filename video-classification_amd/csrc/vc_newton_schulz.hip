@@ -7,7 +7,7 @@
 // and stored twice), bound by the matrix pipes for large matrices and by the chain of launches for small ones, so all
 // matrices of a call share each launch, three a step and a join where a reduction is cut.
 //   4096 x 4096: S 210 + 9 us, P 212 + 10, update 389 (1.06 PFLOP/s of fp16 products); 5 steps 3.9 ms
-//   52 matrices of a ResNet-50 (64 to 2048 rows): 195 us a step, 0.95 - 1.01 ms in all
+//   52 matrices of a ResNet-50 (64 to 2048 rows): 190 us a step, 0.97 ms in all
 //   4 matrices of up to 256 x 1152, on 64 x 64 tiles: 23 us a step -- six microseconds a launch, most of them latency
 //
 // Precision: a gradient's small singular values are amplified by a^steps (485 for the usual coefficients) and with them the
@@ -27,11 +27,12 @@ namespace {
 
 constexpr int NS_MAX = 64;        // matrices per launch
 constexpr int NORM_CHUNK = 1 << 14;
-// Calls with up to this many operations a step work on 64 x 64 tiles, which are four times as many and a quarter as long,
-// the others on 128 x 128, which load half as much per product.  64 against 128, us: four matrices up to 256 x 1152 (0.3 G)
-// 131 / 214, 1024^2 (4 G) 215 / 335, two of them 323 / 381, 1024 x 4096 (14 G) 446 / 429, 1536^2 (14 G) 511 / 480, 2048^2
-// (34 G) 880 / 753.
-constexpr double NS_SMALL_WORK = 10e9;
+// Launches with up to this many products (m^2 n for S, m^3 for P, 2 m^2 n for the update) work on 64 x 64 tiles, which are four
+// times as many and a quarter as long, the others on 128 x 128, which load half as much per product.  64 against 128, us,
+// joins included: S of 1024^2 (1.1 G) 13 / 17, 512 x 4608 (1.2 G) 17 / 23, 1536^2 (3.6 G) 30 / 26, 1024 x 4096 (4.3 G) 36 /
+// 29; P of 1024 rows (1.1 G) 14 / 19, the ResNet-50 set (2.8 G) 25 / 31, 1536^2 30 / 27; updates of 1024^2 (2.1 G) 15 / 30,
+// 512 x 4608 (2.4 G) 20 / 20, 1536^2 (7.2 G) 46 / 44, 1024 x 4096 (8.6 G) 44 / 37.
+constexpr double NS_SMALL_SYM = 3e9, NS_SMALL_UPDATE = 5e9;
 
 // What a launch numbers its workgroups by, matrix after matrix.
 enum { BY_NORM, BY_INIT, BY_UPDATE, BY_S, BY_P, BY_JOIN_S, BY_JOIN_P, KINDS };
@@ -652,10 +653,10 @@ struct NsLayout {
   NsMat mat[NS_MAX];
   int64_t blocks[KINDS];
   int64_t norms, part, bufs, bytes;
-  int tile;  // 128, or 64
+  int tile_s, tile_p, tile_u;  // 128 or 64
   NsLayout(const int* rows, const int* cols, int count) {
     int64_t at = 0;
-    double work = 0;
+    double ws = 0, wp = 0;
     for (int i = 0; i < count; ++i) {
       NsMat& t = mat[i];
       t = NsMat{};
@@ -664,16 +665,21 @@ struct NsLayout {
       t.n = t.tall ? rows[i] : cols[i];
       t.at = at;
       at = NsView(t, 0).end;
-      work += (double)t.m * t.m * (3.0 * t.n + t.m);
+      ws += (double)t.m * t.m * t.n;
+      wp += (double)t.m * t.m * t.m;
     }
-    tile = work <= NS_SMALL_WORK ? 64 : 128;
-    const int64_t ps = cut_sym(mat, count, 0, tile), pp = cut_sym(mat, count, 1, tile);
+    tile_s = ws <= NS_SMALL_SYM ? 64 : 128;
+    tile_p = wp <= NS_SMALL_SYM ? 64 : 128;
+    tile_u = 2 * ws <= NS_SMALL_UPDATE ? 64 : 128;
+    const int64_t ps = cut_sym(mat, count, 0, tile_s) * tile_s * tile_s, pp = cut_sym(mat, count, 1, tile_p) * tile_p * tile_p;
     for (int k = 0; k < KINDS; ++k) {
       blocks[k] = 0;
       for (int i = 0; i < count; ++i) {
         NsMat& t = mat[i];
         t.first[k] = (int)blocks[k];
-        const NsMat::Cut& c = t.cut[k == BY_P || k == BY_JOIN_P];
+        const bool sq = k == BY_P || k == BY_JOIN_P;
+        const NsMat::Cut& c = t.cut[sq];
+        const int tile = k == BY_UPDATE ? tile_u : sq ? tile_p : tile_s;
         blocks[k] += k == BY_NORM     ? ceil_div64((int64_t)t.m * t.n, NORM_CHUNK)
                      : k == BY_INIT   ? (int64_t)(up64(t.m) / 64) * (up64(t.n) / 64)
                      : k == BY_UPDATE ? (int64_t)ceil_div(t.m, tile) * ceil_div(t.n, tile)
@@ -683,7 +689,7 @@ struct NsLayout {
     }
     norms = NS_MAX * (int64_t)(sizeof(NsMat) + sizeof(NsScale));
     part = norms + up128(blocks[BY_NORM] * 8);
-    bufs = part + (ps > pp ? ps : pp) * tile * tile * 4;
+    bufs = part + (ps > pp ? ps : pp) * 4;
     bytes = bufs + at * 2;
   }
 };
@@ -775,16 +781,21 @@ int vc_newton_schulz(int dtype, int count, const void* const* g, void* const* ou
       st.b = coeffs[3 * k + 1];
       st.c = coeffs[3 * k + 2];
       st.last = k == steps - 1;
-      auto step = [&](auto tb) {
+      auto sym = [&](auto square, auto tb) {
+        constexpr bool SQ = decltype(square)::value;
         constexpr int TB = decltype(tb)::value;
-        launch(BY_S, ns_sym_kernel<false, TB>, G_THREADS, ws, sc, st, k & 1, part);
-        if (l.blocks[BY_JOIN_S]) launch(BY_JOIN_S, ns_sym_join_kernel<false, TB>, G_THREADS, ws, sc, st, k & 1, part);
-        launch(BY_P, ns_sym_kernel<true, TB>, G_THREADS, ws, sc, st, k & 1, part);
-        if (l.blocks[BY_JOIN_P]) launch(BY_JOIN_P, ns_sym_join_kernel<true, TB>, G_THREADS, ws, sc, st, k & 1, part);
-        launch(BY_UPDATE, bf ? ns_update_kernel<bf16, TB> : ns_update_kernel<float, TB>, G_THREADS, ws, sc, st, k & 1);
+        launch(SQ ? BY_P : BY_S, ns_sym_kernel<SQ, TB>, G_THREADS, ws, sc, st, k & 1, part);
+        const int join = SQ ? BY_JOIN_P : BY_JOIN_S;
+        if (l.blocks[join]) launch(join, ns_sym_join_kernel<SQ, TB>, G_THREADS, ws, sc, st, k & 1, part);
       };
-      if (l.tile == 64) step(std::integral_constant<int, 2>());
-      else step(std::integral_constant<int, 4>());
+      const std::integral_constant<int, 2> t64;
+      const std::integral_constant<int, 4> t128;
+      if (l.tile_s == 64) sym(std::false_type(), t64);
+      else sym(std::false_type(), t128);
+      if (l.tile_p == 64) sym(std::true_type(), t64);
+      else sym(std::true_type(), t128);
+      if (l.tile_u == 64) launch(BY_UPDATE, bf ? ns_update_kernel<bf16, 2> : ns_update_kernel<float, 2>, G_THREADS, ws, sc, st, k & 1);
+      else launch(BY_UPDATE, bf ? ns_update_kernel<bf16, 4> : ns_update_kernel<float, 4>, G_THREADS, ws, sc, st, k & 1);
     }
   }
   flush();
