@@ -13,8 +13,8 @@
 // Tiles of 64 x 64 (TB = 2) serve launches that would leave most of the chip idle: a quarter of the work per k-step and in the
 // epilogue, four stages in flight instead of two.
 //
-// Four waves in a 2 x 2 grid own 64 x 64 (32 x 32) each.  Two LDS stages of (PA + PB) x 128 x BK elements (BK = 64 for single terms,
-// 32 otherwise: at most 32 KiB a stage), so that two workgroups share a CU.  ROW stages permute the 16-byte chunks of a
+// Four waves in a 2 x 2 grid own 64 x 64 (32 x 32) each.  Two LDS stages of (PA + PB) x 128 x BK elements (BK = 64 for single
+// terms, 32 otherwise: at most 32 KiB a stage), so that two workgroups share a CU.  ROW stages permute the 16-byte chunks of a
 // row so that the 16 rows of a fragment read fall into 16 different slots of the 256-byte bank row; COL stages permute
 // the 32-byte blocks of a row so that the eight rows of a transposing read fall on different groups of banks.  Stages
 // are filled by LDS-DMA requests in opaque assembly (with the builtin the compiler waits for every outstanding request
@@ -23,8 +23,8 @@
 // Measured: 1.0 PFLOP/s of products in one term (8192 x 1024 x 8192: 132 us) and 1.06 of the three products in two terms
 // (4096^3: 389 us, 353 TFLOP/s of fp32 accuracy), where the library's fp16 product of 8192^3 reaches 1.38 and its fp32
 // product 0.153.  Bound by the matrix pipes at the clock they leave (62 % of the busy CUs' cycles, 1.84 - 1.98 GHz) and by
-// what surrounds a tile: prologue and epilogue of 8 to 16 k-steps.  Tried and slower: 256 x 128 tiles, four stages, three workgroups per CU, tiles chained in one
-// workgroup.
+// what surrounds a tile: prologue and epilogue of 8 to 16 k-steps.  Tried on the large tile and slower: 256 x 128, four stages,
+// three workgroups per CU, tiles chained in one workgroup.
 #pragma once
 #include "vc_common.h"
 
