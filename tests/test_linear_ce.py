@@ -559,3 +559,41 @@ def test_replays_follow_the_rows_that_count(cuda, types, N, K, V):
         want = [want[0], want[1], xs.grad, w.grad, b.grad]
         for g, e in zip(got, want):
             assert torch.equal(g, e)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("types", list(TYPES))
+@pytest.mark.parametrize("e", [0, 12, 40])
+def test_ties_of_large_logits(cuda, types, e):
+    """Logits that are whole multiples of 2^e, so that from e = 12 on a row's probability falls in equal shares on the classes that
+    tie for its maximum: the maximum takes nothing from the sum, however large it is.
+
+    Every product and every logit is exact; the maximum and the target's logit meet a rounding each on their way through
+    log2 (2^-22 of the larger with the factors'), the shares the error of exp2 and log2 (2^-20)."""
+    from video_classification_amd import ops
+    xd, wd = TYPES[types]
+    N, K, V = 96, 32, 160
+    g = torch.Generator().manual_seed(3)
+    x = (torch.randint(-3, 4, (N, K), generator=g) * 2.0 ** (e // 2)).to(xd).cuda()
+    w = torch.randint(-2, 3, (V, K), generator=g) * 2.0 ** (e - e // 2)
+    w[80:] = w[:80]  # every maximum is met twice
+    w = nn.Parameter(w.to(wd).cuda())
+    t = torch.randint(0, V, (N,), generator=g).cuda()
+    x64, w64 = x.double(), w.detach().double()
+    z = x64 @ w64.t()
+    p = torch.softmax(z, dim=1)
+    d = p.clone()
+    d[torch.arange(N), t] -= 1
+    xg = x.clone().requires_grad_(True)
+    rows = ops.linear_cross_entropy(xg, w, None, t, reduction="none")
+    rows.sum().backward()
+    want = torch.nn.functional.cross_entropy(z, t, reduction="none")
+    assert ((rows.double() - want).abs() <= 2.0 ** -20 + 2.0 ** -22 * (z.max(1).values.abs() + z[torch.arange(N), t].abs())).all()
+    # a share's error: 2^-20, and where the shares are unequal (e = 0) that of the logits in log2, 2^-22 of the largest
+    share = p * (2.0 ** -20 + (2.0 ** -21 * float(z.abs().max()) if e == 0 else 0.0))
+    for got, want, A, M, P, dt, n in ((xg.grad, d @ w64, d.abs(), w64.abs(), share, xd, V),
+                                      (w.grad, d.t() @ x64, d.abs().t(), x64.abs(), share.t(), wd, N)):
+        term = (2.0 ** -22 if dt == torch.float32 else FEW_ROWS) + 2.0 ** -21 + (3 * n / 32 + 8) * 2.0 ** -23
+        # fp16's smallest step is 2^-24 and d is scaled by 2^15: whatever the terms, half a step is 2^-40
+        floor = 2.0 ** -40 * (torch.ones_like(A) @ M)
+        assert ((got.double() - want).abs() <= term * (A @ M) + P @ M + floor + half(dt) * want.abs()).all()

@@ -394,23 +394,25 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_stats_kernel(CeArgs a, float4
     }
 }
 
-// Per packed row, from its joined statistics: lse (in units of log2); at its place in the call: loss (NaN for a target outside
-// [0, V)) and arg-max.
+// Per packed row, from its joined statistics: the maximum and the log2 of the sum, apart (next to a maximum of 2^24 and more
+// the other one would vanish in their sum, and the probabilities with it); at its place in the call: loss (NaN for a target
+// outside [0, V)) and arg-max.
 struct CeRows {
   const float* zt;
   const int *target, *order, *exps;
   int N, V, tiles_v;
   float smooth;
-  float *lse, *rowloss;
+  float2* lse;
+  float* rowloss;
   int64_t* pred;
 };
 __device__ __forceinline__ float row_out(const CeRows& k, int n, const Stat& s) {
-  const float l = (s.m == -INFINITY ? 0.f : s.m) + log2f(s.s);
-  k.lse[n] = l;
+  const float m = s.m == -INFINITY ? 0.f : s.m, l = log2f(s.s);
+  k.lse[n] = make_float2(m, l);
   float loss = NAN;
   if (k.target[n] >= 0) {
-    const float d = l - k.zt[n];
-    loss = LN2 * (k.smooth > 0.f ? (1.f - k.smooth) * d + k.smooth * (l - s.z / (float)k.V) : d);
+    const float d = m - k.zt[n];
+    loss = LN2 * (l + (k.smooth > 0.f ? (1.f - k.smooth) * d + k.smooth * (m - s.z / (float)k.V) : d));
   }
   const int at = k.order[n];
   k.rowloss[at] = loss;
@@ -536,7 +538,7 @@ __device__ __forceinline__ void bias_out(T* db, float s, const CeFac& fac, int a
 // One 128 x 128 tile of d for the classes [vbeg, vbeg + vcols), as dn[n][vcols] in PD terms scaled by 2^15, and its column
 // sums dbpart[tile n][v] (db itself where there is one row tile).
 template <int PW, int PX, int PD>
-__global__ __launch_bounds__(G_THREADS, 2) void ce_grad_kernel(CeArgs a, const float* __restrict__ lse,
+__global__ __launch_bounds__(G_THREADS, 2) void ce_grad_kernel(CeArgs a, const float2* __restrict__ lse,
                                                                const float* __restrict__ rs, float smooth, int vbeg,
                                                                int vcols, f16* __restrict__ dn,
                                                                float* __restrict__ dbpart, CeFac fac, void* db, int add) {
@@ -560,12 +562,14 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_grad_kernel(CeArgs a, const f
   const int64_t plane = (int64_t)a.N * vcols;
   const int rows = a.rows();
   int target[4];
-  float weight[4], low[4];  // 2^(z - low) is the scaled probability
+  float weight[4], top[4], low[4];  // 2^((z - top) + low) is the scaled probability
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int n = n0 + wn * 64 + j * 16 + l15;
     target[j] = row_target(a, n);
-    low[j] = lse[max(min(n, rows - 1), 0)] - 15.f;
+    const float2 s = lse[max(min(n, rows - 1), 0)];
+    top[j] = s.x;
+    low[j] = 15.f - s.y;
     weight[j] = n < rows ? 1.f : 0.f;
     if (target[j] < 0) low[j] = NAN;
   }
@@ -577,13 +581,13 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_grad_kernel(CeArgs a, const f
     }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float w = weight[j], l = low[j];
+    const float w = weight[j], m = top[j], l = low[j];
     const int hit = lane_class(target[j], v0);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        acc[i][j][r] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], scale, bias[i][r]) - l);
+        acc[i][j][r] = __builtin_amdgcn_exp2f((fmaf(acc[i][j][r], scale, bias[i][r]) - m) + l);
     if (smooth > 0.f)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -907,7 +911,7 @@ Plan make_plan(int xf32, int wf32, int N, int V, int K) {
   p.o_bl = take((int64_t)all * 4);
   p.o_order = take((int64_t)N * 4);
   p.o_target = take((int64_t)N * 4);
-  p.o_lse = take((int64_t)N * 4);
+  p.o_lse = take((int64_t)N * 8);
   p.o_total = take(16);
   p.saved = o;
   o = 0;
@@ -979,7 +983,7 @@ void stats_go(const CeArgs& a, bool more, float4* part, float* zt, hipStream_t s
   else hipLaunchKernelGGL((ce_stats_kernel<PW, PX, false, BF>), grid, blk, 0, st, a, part, zt);
 }
 template <int PW, int PX, int PD>
-void grad_go(const CeArgs& a, const float* lse, const float* rs, float smooth, int vbeg, int vcols, f16* dn, float* dbp,
+void grad_go(const CeArgs& a, const float2* lse, const float* rs, float smooth, int vbeg, int vcols, f16* dn, float* dbp,
              const CeFac& fac, void* db, int add, hipStream_t st) {
   hipLaunchKernelGGL((ce_grad_kernel<PW, PX, PD>), dim3(a.tiles_v * ceil_div(a.N, GM)), dim3(G_THREADS), 0, st, a, lse, rs, smooth,
                      vbeg, vcols, dn, dbp, fac, db, add);
@@ -1047,7 +1051,7 @@ int vc_linear_ce_fwd(int xdtype, int wdtype, const void* x, const void* w, const
   if (raw) stats_go<1, 1, true>(a, more, part, zt, stream);
   else if (p.pw == 2) stats_go<2, 2>(a, more, part, zt, stream);
   else stats_go<1, 1>(a, more, part, zt, stream);
-  const CeRows rows{zt, a.target, (const int*)(sv + p.o_order), a.exps, N, V, a.tiles_v, smoothing, (float*)(sv + p.o_lse), row_loss, pred};
+  const CeRows rows{zt, a.target, (const int*)(sv + p.o_order), a.exps, N, V, a.tiles_v, smoothing, (float2*)(sv + p.o_lse), row_loss, pred};
   float* total = (float*)(sv + p.o_total);
   const bool sums = loss || correct;
   if (sums && N <= 1024 && a.tiles_v <= 16) {
@@ -1077,7 +1081,7 @@ int vc_linear_ce_bwd(int xdtype, int wdtype, float smoothing, int mean,
   f16* dn = (f16*)(ws + p.b_dn);
   const int* exps = (const int*)(sv + p.o_exps);
   const int* order = (const int*)(sv + p.o_order);
-  const float* lse = (const float*)(sv + p.o_lse);
+  const float2* lse = (const float2*)(sv + p.o_lse);
   float *rs = (float*)(ws + p.b_rs), *big = (float*)(ws + p.b_fac), *dbp = (float*)(ws + p.b_db);
   const CeFac fac{per_row ? big : nullptr, dloss, mean ? (const float*)(sv + p.o_total) : nullptr};
   const int tn = ceil_div(N, GM), tk = ceil_div(K, GM);
