@@ -597,3 +597,125 @@ def test_ties_of_large_logits(cuda, types, e):
         # fp16's smallest step is 2^-24 and d is scaled by 2^15: whatever the terms, half a step is 2^-40
         floor = 2.0 ** -40 * (torch.ones_like(A) @ M)
         assert ((got.double() - want).abs() <= term * (A @ M) + P @ M + floor + half(dt) * want.abs()).all()
+
+
+def check_each(types, x, w, b, t, rows, dx, dw, db, weight, skip=()):
+    """Like `check`, with every logit's own error bound: rows and classes of any magnitude side by side.  skip: rows whose
+    logits overflow, with weight 0."""
+    xd, wd = TYPES[types]
+    N, V, K = x.shape[0], w.shape[0], x.shape[1]
+    live = torch.ones(N, dtype=torch.bool, device=x.device)
+    live[list(skip)] = False
+    x64, w64 = x.double() * live[:, None], w.detach().double()
+    z, S = x64 @ w64.t() + b.detach().double(), x64.abs() @ w64.abs().t() + b.detach().double().abs()
+    lse = torch.logsumexp(z, dim=1)
+    p = torch.exp(z - lse[:, None])
+    dz = ((3 * K / 32 + 4) * 2.0 ** -23 + 2.0 ** -21) * S
+    mid = (p * dz).sum(1)
+    at = torch.arange(N, device=x.device)
+    want = lse - z[at, t]
+    tol = 2 * (mid + dz[at, t]) + 2.0 ** -20 * (1 + lse.abs() + want.abs())
+    err = (rows.double() - want).abs()
+    assert (err <= tol)[live].all(), float((err - tol)[live].max())
+    d = p.clone()
+    d[at, t] -= 1
+    d = d * (weight * live)[:, None]
+    off = (2 * p * (1 - p).clamp_min(0) * (dz + mid[:, None]) + 2.0 ** -20 * p) * (weight * live)[:, None]
+    for got, want, A, M, P, dt, length in ((dx, d @ w64, d.abs(), w64.abs(), off, xd, V),
+                                           (dw, d.t() @ x64, d.abs().t(), x64.abs(), off.t(), wd, N)):
+        # joins of a sum: of 32 fp16 products each, or (rows of their own scale) one rounding per fp32 product
+        term = (2.0 ** -22 if dt == torch.float32 else FEW_ROWS) + 2.0 ** -21 + (length + 8) * 2.0 ** -23
+        # fp16's smallest step is 2^-24 and d is scaled by 2^15: half a step is 2^-40, or all of a smaller value
+        tol = term * (A @ M) + A.clamp_max(2.0 ** -40) @ M + P @ M + half(dt) * want.abs() + 1e-37
+        err = (got.double() - want).abs()
+        assert (err <= tol).all(), float((err / tol).max())
+    tol = off.sum(0) + (N / 16 + 16) * U * d.abs().sum(0) + half(wd) * d.sum(0).abs() + 1e-37
+    assert ((db.double() - d.sum(0)).abs() <= tol).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("types", list(TYPES))
+@pytest.mark.parametrize("N,K,V", [(200, 64, 300), (77, 72, 130), (1500, 40, 700)])
+@pytest.mark.parametrize("where", ["row", "class", "both", "near", "small row", "overflow"])
+def test_magnitudes_of_rows_and_classes_side_by_side(cuda, types, N, K, V, where):
+    """One row of x, or one class's weights, far larger than the others takes no precision from them, with gradients as
+    without."""
+    from video_classification_amd import ops
+    x, w, b, t = make(N, K, V, types, seed=13)
+    weight = torch.ones(N, device=cuda, dtype=torch.float64)
+    with torch.no_grad():
+        if where in ("row", "both"):
+            x[7] *= 2.0 ** 40
+        if where in ("class", "both"):
+            w[11] *= 2.0 ** 40
+        if where == "near":  # within one scale's reach
+            x[7] *= 2.0 ** 14
+            w[11] *= 2.0 ** 14
+        if where == "small row":
+            x[:-1] *= 2.0 ** 60
+            w.mul_(2.0 ** -60)
+        if where == "overflow":
+            x[7], weight[7] = 3e38, 0.0
+    xg = x.clone().requires_grad_(True)
+    rows = ops.linear_cross_entropy(xg, w, b, t, reduction="none")
+    rows.backward(weight.float())
+    check_each(types, x, w, b, t, rows.detach(), xg.grad, w.grad, b.grad, weight, skip=[7] if where == "overflow" else [])
+    with torch.no_grad():
+        again = ops.linear_cross_entropy(x, w, b, t, reduction="none")
+    keep = torch.ones(N, dtype=torch.bool, device=cuda)
+    keep[7] = where != "overflow"
+    scale = (rows.detach().abs() + again.abs())[keep]
+    assert ((rows.detach() - again).abs()[keep] <= 2.0 ** -10 * (1 + scale)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("types,N,K,V", [("bf16", 3000, 64, 13001), ("f32", 200, 520, 4099)])
+def test_magnitudes_in_pieces_and_slices(cuda, types, N, K, V):
+    """The same where the classes come in pieces and the reductions in slices, next to a call without such rows."""
+    from video_classification_amd import ops
+    x, w, b, t = make(N, K, V, types, seed=14)
+    one = torch.ones(N, device=cuda, dtype=torch.float64)
+    for scale in (2.0 ** 40, 1.0):
+        with torch.no_grad():
+            big, wide = x.clone(), nn.Parameter(w.detach().clone())
+            big[7] *= scale
+            wide[11] *= scale
+        b.grad = None
+        xg = big.clone().requires_grad_(True)
+        rows = ops.linear_cross_entropy(xg, wide, b, t, reduction="none")
+        rows.sum().backward()
+        check_each(types, big, wide, b, t, rows.detach(), xg.grad, wide.grad, b.grad, one)
+
+
+@pytest.mark.gpu
+def test_replays_follow_the_magnitudes(cuda):
+    """Whether rows have scales of their own is found on the device: one captured step serves both."""
+    from video_classification_amd import ops
+    x, w, b, t = make(300, 96, 500, "bf16", seed=15)
+    xs = x.clone().requires_grad_(True)
+    w.grad, b.grad, xs.grad = torch.zeros_like(w), torch.zeros_like(b), torch.zeros_like(xs)
+
+    def step():
+        for g in (w.grad, b.grad, xs.grad):
+            g.zero_()
+        loss = ops.linear_cross_entropy(xs, w, b, t)
+        loss.backward()
+        return loss.detach()
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = step()
+    for k in (0, 40, 0, 30, 0):
+        with torch.no_grad():
+            xs.copy_(x)
+            xs[3] *= 2.0 ** k
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [loss.clone(), xs.grad.clone(), w.grad.clone(), b.grad.clone()]
+        for g, e in zip(got, [step(), xs.grad, w.grad, b.grad]):
+            assert torch.equal(g, e)

@@ -14,10 +14,11 @@
 // over its four products; 2048 x 512 x 20011 forward: 64 us, 54 of them the statistics (0.8 PFLOP/s).
 //
 // All products run on fp16 terms (vc_gemm16.h).  x and W are scaled by one power of two each (from their largest finite
-// magnitude): bf16 values are exact in one term over 29 binades and within 2^-40 of the largest magnitude below that, fp32
-// values take two terms (22 bits).  An fp32 master weight next to bf16 activations takes one term (11 bits, against the
-// 8 of a bf16 copy).  d is at most 1 in magnitude and is scaled by 2^15: one term (2^-11 of the value) where the gradient
-// it makes is bf16, two where it is fp32.
+// magnitude), but for rows whose own largest value lies more than 16 binades below it, which are scaled by themselves: no row
+// takes precision from another one.  bf16 values are exact in one term over 29 binades and within 2^-23 of their row's largest
+// magnitude below that, fp32 values take two terms (22 bits).  An fp32 master weight next to bf16 activations takes one
+// term (11 bits, against the 8 of a bf16 copy).  d is at most 1 in magnitude and is scaled by 2^15: one term (2^-11 of
+// the value) where the gradient it makes is bf16, two where it is fp32.
 #include "vc_gemm16.h"
 
 namespace {
@@ -31,42 +32,63 @@ __device__ __forceinline__ float finite_mag(float v) {
 }
 
 template <typename T>
-__device__ __forceinline__ float amax_part(const T* p, int64_t rows, int K, const int64_t* target, int64_t ignore, int block,
-                                           int nblocks) {
-  float m = 0.f;
-  if (!target) {
-    const int64_t total = rows * K, head = ((uintptr_t)p & 15) ? 0 : total / 8 * 8;
-    for (int64_t i = ((int64_t)block * 256 + threadIdx.x) * 8; i < head; i += (int64_t)nblocks * 256 * 8) {
-      const F8 v = load8(p + i);
+struct __attribute__((packed, aligned(sizeof(T)))) Row8 {  // eight values in one wide load whatever their alignment
+  T v[8];
+};
+
+// rowmax[r] = largest finite magnitude of row r (not of rows that do not count); returns that of all rows this lane met.  As
+// many lanes per row as it has groups of eight values, up to a wave, and four rows at once, so that their loads overlap
+// (65536 + 8192 rows of 1024 in bf16: 40 us, 45 one by one).
+template <typename T>
+__device__ __forceinline__ float amax_rows(const T* p, int64_t rows, int K, const int64_t* target, int64_t ignore,
+                                           float* rowmax, int block, int nblocks) {
+  constexpr int U = 4;
+  int lanes = 1;
+  while (lanes < 64 && lanes * 8 < K) lanes <<= 1;
+  const int lane = threadIdx.x & 63, k0 = (lane & (lanes - 1)) * 8, per = 64 / lanes;
+  const int64_t step = (int64_t)nblocks * 4 * per;  // rows between those of a lane
+  float most = 0.f;
+  for (int64_t first = ((int64_t)block * 4 + (threadIdx.x >> 6)) * per; first < rows; first += U * step) {
+    bool on[U];
+    const T* row[U];
+    float m[U];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) m = fmaxf(m, finite_mag(v.v[e]));
+    for (int u = 0; u < U; ++u) {
+      const int64_t r = first + lane / lanes + u * step;
+      on[u] = r < rows && !(target && target[r] == ignore);
+      row[u] = p + (on[u] ? r * K : 0);  // row 0 in place of one that does not count: its values are dropped
+      m[u] = 0.f;
     }
-    for (int64_t i = head + (int64_t)block * 256 + threadIdx.x; i < total; i += (int64_t)nblocks * 256)
-      m = fmaxf(m, finite_mag(to_f32(p[i])));
-  } else {
-    for (int64_t r = block * 4 + (threadIdx.x >> 6); r < rows; r += nblocks * 4) {
-      if (target[r] == ignore) continue;
-      const T* row = p + r * K;
-      int k = threadIdx.x & 63;
-      if (K % 8 == 0 && ((uintptr_t)p & 15) == 0) {
-        for (k *= 8; k < K; k += 512) {
-          const F8 v = load8(row + k);
+    int k = k0;
+    for (; k + 8 <= K; k += lanes * 8) {
+      Row8<T> v[U];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) m = fmaxf(m, finite_mag(v.v[e]));
-        }
-      } else {
-#pragma unroll 4
-        for (; k < K; k += 64) m = fmaxf(m, finite_mag(to_f32(row[k])));
-      }
+      for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const Row8<T>*>(row[u] + k);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m[u] = fmaxf(m[u], finite_mag(to_f32(v[u].v[e])));
+    }
+    for (; k < K; ++k)  // the lane with the rows' last, partial group
+#pragma unroll
+      for (int u = 0; u < U; ++u) m[u] = fmaxf(m[u], finite_mag(to_f32(row[u][k])));
+    for (int o = 1; o < lanes; o <<= 1)
+#pragma unroll
+      for (int u = 0; u < U; ++u) m[u] = fmaxf(m[u], __shfl_xor(m[u], o, 64));
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (!on[u]) continue;
+      if (k0 == 0) rowmax[first + lane / lanes + u * step] = m[u];
+      most = fmaxf(most, m[u]);
     }
   }
-  return m;
+  return most;
 }
 
 // The rows of a call in the order they are packed: order[0 .. count) = the rows that count, in order, then the others;
 // target[k] = class of the k-th of them, -1 if there is no such class.
 struct RowList {
-  int *order, *target, *count;
+  int *order, *target, *count;  // count[1], count[2]: cleared here, set where a row of x / of W has a scale of its own
 };
 
 // One workgroup, 4096 rows at a time.  Rows that do not count get their loss (0) and prediction (0) here.
@@ -110,7 +132,10 @@ __device__ __forceinline__ void list_rows(const int64_t* __restrict__ target, in
     }
     base += __shfl(upto, 63, 64);
   }
-  if (threadIdx.x == 0) *l.count = base;
+  if (threadIdx.x == 0) {
+    l.count[0] = base;
+    l.count[1] = l.count[2] = 0;
+  }
 }
 
 // amax[0 .. xb) / [AMAX_MOST ..] = largest finite magnitudes met by the xb blocks of x / the next ones' of W; the last block
@@ -119,15 +144,16 @@ template <typename TX, typename TW>
 __global__ __launch_bounds__(256) void ce_amax_kernel(const TX* __restrict__ x, const TW* __restrict__ w, int N, int V,
                                                       int K, const int64_t* __restrict__ target, int64_t ignore,
                                                       float* __restrict__ amax, int xb, RowList rows,
-                                                      float* __restrict__ rowloss, int64_t* __restrict__ pred) {
+                                                      float* __restrict__ rowloss, int64_t* __restrict__ pred,
+                                                      float* __restrict__ xmax, float* __restrict__ wmax) {
   __shared__ float sm[4];
   const int b = blockIdx.x, wb = (int)gridDim.x - 1 - xb;
   if (b == xb + wb) {
     list_rows(target, ignore, N, V, rows, rowloss, pred);
     return;
   }
-  float m = b < xb ? amax_part(x, N, K, target, ignore, b, xb)
-                   : amax_part(w, V, K, (const int64_t*)nullptr, 0, b - xb, wb);
+  float m = b < xb ? amax_rows(x, N, K, target, ignore, xmax, b, xb)
+                   : amax_rows(w, V, K, (const int64_t*)nullptr, 0, wmax, b - xb, wb);
   m = wave_max(m);
   if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
   __syncthreads();
@@ -146,25 +172,36 @@ __device__ __forceinline__ int scale_exp(const float* amax, int parts, float* sm
 }
 
 // ---- packing -----------------------------------------------------------------------------------------------------
-// Amax and packing pass over x and W once each: 36 + 63 us for (8192 + 65536) x 1024 in bf16 (4.2 and 4.8 TB/s), 2 % of the
+// Amax and packing pass over x and W once each: 40 + 70 us for (8192 + 65536) x 1024 in bf16 (3.8 and 4.3 TB/s), 2 % of the
 // call.
 //
-// dst[plane][row][ld] = terms of src[order[row]][k] 2^e (order null: row), zeros behind K.  A wave per row and 512 columns.
+// A row whose largest value lies more than this many binades below the operand's is scaled by itself.  Up to there the
+// operand's scale keeps 2^-23 of the row's own largest value: half of fp16's last step, 2^-25, next to at least 2^(14 - 16).
+constexpr int OWN_SCALE = 16;
+
+// dst[plane][row][ld] = terms of src[order[row]][k] 2^e (order null: row), zeros behind K; exps[row] = e, e0 or the row's own
+// scale, and then *own = 1.  A wave per row and 512 columns.
 template <typename T>
 __device__ __forceinline__ void pack_rows(const T* __restrict__ src, f16* __restrict__ dst, int64_t plane, int rows, int K,
-                                          int ld, int planes, int e, const int* order, int64_t unit) {
+                                          int ld, int planes, int e0, const int* order, int64_t unit,
+                                          const float* __restrict__ rowmax, int* __restrict__ exps, int* __restrict__ own) {
   const int per = (ld + 511) / 512;
   const int64_t row = unit / per;
   if (row >= rows) return;
   const int c0 = (int)(unit - row * per) * 512 + (threadIdx.x & 63) * 8;
   if (c0 >= ld) return;
-  const T* s = src + (order ? order[row] : row) * (int64_t)K;
+  const int64_t from = order ? order[row] : row;
+  const T* s = src + from * K;
+  const float most = rowmax[from];
+  int e = most > 0.f ? 14 - ilogbf(most) : e0;
+  if (e - e0 <= OWN_SCALE) e = e0;
+  if (c0 == 0) {
+    exps[row] = e;
+    if (e != e0) *own = 1;
+  }
   float v[8];
   if (c0 + 8 <= K) {
-    struct __attribute__((packed, aligned(sizeof(T)))) Row8 {
-      T v[8];
-    };
-    const Row8 t = *reinterpret_cast<const Row8*>(s + c0);  // wide loads whatever the alignment of the row
+    const Row8<T> t = *reinterpret_cast<const Row8<T>*>(s + c0);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = to_f32(t.v[i]);
   } else {
@@ -185,7 +222,7 @@ __device__ __forceinline__ void pack_rows(const T* __restrict__ src, f16* __rest
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
-// exps[0] / [1] = scale exponents of x / W, [2] = rows that count; the first `xblocks` workgroups pack x, the others W and the bias: bl = bias
+// exps[0] / [1] = scale exponents of x / W, [2] = rows that count, [3] / [4] = whether rows of x / W have their own; the first `xblocks` workgroups pack x, the others W and the bias: bl = bias
 // log2(e) over whole tiles of classes, -inf behind the last one, which leaves the epilogues of the products four plain
 // vector loads (clamped and converted there, these cost a fifth of a tile's time).
 template <typename TX, typename TW>
@@ -193,15 +230,17 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(const TX* __restrict__ x, 
                                                       int K, int ld, int px, int pw, const int* __restrict__ order,
                                                       const float* __restrict__ amax, f16* __restrict__ xp,
                                                       f16* __restrict__ wp, int* __restrict__ exps, int xblocks, int xb,
-                                                      int wb, const TW* __restrict__ bias, float* __restrict__ bl) {
+                                                      int wb, const TW* __restrict__ bias, float* __restrict__ bl,
+                                                      const float* __restrict__ xmax, const float* __restrict__ wmax,
+                                                      int* __restrict__ ex, int* __restrict__ ew) {
   __shared__ float sm[4];
   const bool isx = (int)blockIdx.x < xblocks;
   const int e = scale_exp(isx ? amax : amax + AMAX_MOST, isx ? xb : wb, sm);
   if (threadIdx.x == 0 && ((int)blockIdx.x == 0 || (int)blockIdx.x == xblocks)) exps[isx ? 0 : 1] = e;
-  const int64_t unit = (int64_t)(isx ? blockIdx.x : blockIdx.x - xblocks) * 4 + (threadIdx.x >> 6);
-  if (isx) pack_rows(x, xp, (int64_t)N * ld, exps[2], K, ld, px, e, order, unit);
+  const int64_t unit = (int64_t)(isx ? blockIdx.x : blockIdx.x - xblocks) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (isx) pack_rows(x, xp, (int64_t)N * ld, exps[2], K, ld, px, e, order, unit, xmax, ex, exps + 3);
   else {
-    pack_rows(w, wp, (int64_t)V * ld, V, K, ld, pw, e, (const int*)nullptr, unit);
+    pack_rows(w, wp, (int64_t)V * ld, V, K, ld, pw, e, (const int*)nullptr, unit, wmax, ew, exps + 4);
     const int64_t v = (int64_t)(blockIdx.x - xblocks) * 256 + threadIdx.x;  // four rows or more per workgroup: all classes
     if (v < (V + GM - 1) / GM * GM) bl[v] = v >= V ? -INFINITY : bias ? to_f32(bias[v]) * LOG2E : 0.f;
   }
@@ -243,6 +282,7 @@ struct CeArgs {
   const float* bl;   // bias log2(e), -inf behind the last class
   const int* target; // of the packed rows
   const int* exps;
+  const int *ex, *ew;  // scale exponents of the packed rows and of the classes
   int N, V, K, ld, db_bf16;
   int tiles_v;
 
@@ -268,16 +308,24 @@ __device__ __forceinline__ void logit_tile(const CeArgs& a, int v0, int n0, f16*
   const float* bl = a.bl + v0 + (threadIdx.x >> 7) * 64 + ((threadIdx.x & 63) >> 4) * 4;
 #pragma unroll
   for (int i = 0; i < 4; ++i) bias[i] = *reinterpret_cast<const f32x4*>(bl + i * 16);
-  int es = -(a.exps[0] + a.exps[1]);
-  if (es < -120 || es > 120) {  // operands of extreme magnitude: two factors
-    const float f = ldexpf(1.f, es / 2);
+  const int es = -(a.exps[0] + a.exps[1]);
+  if (!BF && (a.exps[3] | a.exps[4] || es < -120 || es > 120)) {  // scales by rows and classes, or beyond one factor's range
+    const int lane = threadIdx.x & 63, n = n0 + (threadIdx.x >> 6 & 1) * 64 + (lane & 15);
+    const int v = v0 + (threadIdx.x >> 7) * 64 + (lane >> 4) * 4;
+    int er[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) er[j] = a.ex[max(min(n + j * 16, a.rows() - 1), 0)];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] *= f;
-    es -= es / 2;
-  }
-  scale = ldexpf(LOG2E, es);
+      for (int r = 0; r < 4; ++r) {
+        const int ec = a.ew[min(v + i * 16 + r, a.V - 1)];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j][r] = ldexpf(acc[i][j][r], -(er[j] + ec));
+      }
+    scale = LOG2E;
+  } else
+    scale = ldexpf(LOG2E, es);
 }
 
 // position of class t among this lane's 16 of a tile column (i * 4 + r), or -1
@@ -690,10 +738,46 @@ struct MmArgs {
   CeFac fac;
   const int* exps;             // exps[2] = rows that count: rows of dx that are worked, reduction length of dW
   int which;                   // whose scale exponent the column side carries
+  const int* own;              // the column side's scale exponents along the reduction, for exps[3 + which]
 };
 
 __device__ __forceinline__ float mm_factor(const CeFac& fac, const int* exps, int which) {
-  return ldexpf(fac.get(), -15 - exps[which]);
+  return exps[3 + which] ? fac.get() : ldexpf(fac.get(), -15 - exps[which]);
+}
+
+// The product where the column side's scales differ along the reduction (some rows of x or of W lie more than 2^16 below the
+// largest): its values as they are, on the fp32 matrix instructions, whose range holds all of them.  Operands come straight
+// from memory: a step of 4096 x 768 x 16384 in bf16 takes 3.2 ms (rows) or 4.1 (classes) instead of 0.58; data with such rows
+// is not what training usually meets.
+template <int PC, int PM, int KM>
+__device__ __forceinline__ void own_product(f32x4 (&acc)[4][4], const Op16& c, const Op16& m, const int* own, int k0, int k1) {
+  const int lane = threadIdx.x & 63, q = lane >> 4, l15 = lane & 15;
+  const int wave = threadIdx.x >> 6, wc = wave >> 1, wr = wave & 1;
+  for (int k = k0; k < k1; k += 4) {
+    const int kk = k + q;
+    const bool on = kk < c.n;  // the reduction's true length
+    const int e = on ? -own[kk] : 0;
+    float fc[4], fm[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int col = c.side + (wc * 4 + i) * 16 + l15;
+      fc[i] = 0.f;
+      if (on && col < c.ld) {
+        const f16* p = c.p + (int64_t)kk * c.ld + col;
+        fc[i] = ldexpf(PC == 2 ? (float)p[0] + (float)p[c.plane] : (float)p[0], e);
+      }
+      const int row = (wr * 4 + i) * 16 + l15;
+      fm[i] = 0.f;
+      if (on && (KM == ROW ? row < m.n : m.side + row < m.ld)) {
+        const f16* p = KM == ROW ? m.p + (int64_t)row * m.ld + kk : m.p + (int64_t)kk * m.ld + m.side + row;
+        fm[i] = (PM == 2 ? (float)p[0] + (float)p[m.plane] : (float)p[0]) * (1.f / D_SCALE);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fc[i], fm[j], acc[i][j], 0, 0, 0);
+  }
 }
 
 template <int PC, int PM, int KM, typename T>
@@ -730,7 +814,10 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
     m.side = m0;
     m.n = c.n = rows;
   }
-  if (!idle) G::run(acc, c, m, k0, k1, smem);
+  if (!idle) {
+    if (g.exps[3 + g.which]) own_product<PC, PM, KM>(acc, c, m, g.own, k0, k1);
+    else G::run(acc, c, m, k0, k1, smem);
+  }
   const int lane = threadIdx.x & 63, q = lane >> 4, l15 = lane & 15;
   const int wave = threadIdx.x >> 6, wc = wave >> 1, wr = wave & 1;
   const float f = g.part ? 1.f : mm_factor(g.fac, g.exps, g.which);
@@ -872,10 +959,10 @@ struct Plan {
   int pdx, pdw, pd;            // terms of d for dx and dW, and the larger of the two
   int piece, pieces;           // classes of a piece
   int sx, sw;                  // slices of the reductions of dx (per piece, if all rows count) and dW
-  // forward workspace (saved for backward): packed x, packed W, exponents and count, bias, row list, lse, total
-  int64_t o_xp, o_wp, o_exps, o_bl, o_order, o_target, o_lse, o_total, saved;
+  // forward workspace (saved for backward): packed x, packed W, exponents and count, bias, row list, lse, total, scales
+  int64_t o_xp, o_wp, o_exps, o_bl, o_order, o_target, o_lse, o_total, o_ex, o_ew, saved;
   // forward scratch
-  int64_t f_amax, f_part, f_zt, fwd;
+  int64_t f_amax, f_part, f_zt, f_xmax, f_wmax, fwd;
   // backward scratch
   int64_t b_rs, b_fac, b_dn, b_db, b_px, b_pw, bwd;
 };
@@ -907,17 +994,21 @@ Plan make_plan(int xf32, int wf32, int N, int V, int K) {
   };
   p.o_xp = take((int64_t)p.px * N * p.ld * 2);
   p.o_wp = take((int64_t)p.pw * V * p.ld * 2);
-  p.o_exps = take(16);
+  p.o_exps = take(32);
   p.o_bl = take((int64_t)all * 4);
   p.o_order = take((int64_t)N * 4);
   p.o_target = take((int64_t)N * 4);
   p.o_lse = take((int64_t)N * 8);
   p.o_total = take(16);
+  p.o_ex = take((int64_t)N * 4);
+  p.o_ew = take((int64_t)V * 4);
   p.saved = o;
   o = 0;
   p.f_amax = take(2 * AMAX_MOST * 4);
   p.f_part = take((int64_t)ceil_div(V, GM) * N * 16);
   p.f_zt = take((int64_t)N * 4);
+  p.f_xmax = take((int64_t)N * 4);
+  p.f_wmax = take((int64_t)V * 4);
   p.fwd = o;
   o = 0;
   p.b_rs = take((int64_t)N * 4);
@@ -952,7 +1043,7 @@ int check_ce(const char* who, int xdtype, int wdtype, int N, int V, int K, float
 template <typename TX, typename TW>
 void pack_go(const Plan& p, const void* x, const void* w, const void* bias, int N, int V, int K, const int64_t* target, int64_t ignore,
              float* rowloss, int64_t* pred, char* saved, char* ws, hipStream_t st) {
-  float* amax = (float*)(ws + p.f_amax);
+  float *amax = (float*)(ws + p.f_amax), *xmax = (float*)(ws + p.f_xmax), *wmax = (float*)(ws + p.f_wmax);
   const int per = ceil_div(p.ld, 512);
   const int xb = (int)ceil_div64((int64_t)N * per, 4), wb = (int)ceil_div64((int64_t)V * per, 4);
   auto blocks = [](int64_t elems) {  // of one vector per thread where that is enough blocks
@@ -962,10 +1053,11 @@ void pack_go(const Plan& p, const void* x, const void* w, const void* bias, int 
   const int xa = blocks((int64_t)N * K), wa = blocks((int64_t)V * K);
   hipLaunchKernelGGL((ce_amax_kernel<TX, TW>), dim3(xa + wa + 1), dim3(256), 0, st, (const TX*)x, (const TW*)w, N, V, K,
                      target, ignore, amax, xa, RowList{(int*)(saved + p.o_order), (int*)(saved + p.o_target), (int*)(saved + p.o_exps) + 2},
-                     rowloss, pred);
+                     rowloss, pred, xmax, wmax);
   hipLaunchKernelGGL((ce_pack_kernel<TX, TW>), dim3(xb + wb), dim3(256), 0, st, (const TX*)x, (const TW*)w, N, V, K, p.ld,
                      p.px, p.pw, (const int*)(saved + p.o_order), amax, (f16*)(saved + p.o_xp), (f16*)(saved + p.o_wp),
-                     (int*)(saved + p.o_exps), xb, xa, wa, (const TW*)bias, (float*)(saved + p.o_bl));
+                     (int*)(saved + p.o_exps), xb, xa, wa, (const TW*)bias, (float*)(saved + p.o_bl), xmax, wmax,
+                     (int*)(saved + p.o_ex), (int*)(saved + p.o_ew));
 }
 
 template <int PC, int PM, int KM>
@@ -1043,7 +1135,7 @@ int vc_linear_ce_fwd(int xdtype, int wdtype, const void* x, const void* w, const
   else if (wdtype == VC_F32) pack_go<bf16, float>(p, x, w, bias, N, V, K, target, ignore_index, row_loss, pred, sv, ws, stream);
   else pack_go<bf16, bf16>(p, x, w, bias, N, V, K, target, ignore_index, row_loss, pred, sv, ws, stream);
   CeArgs a{raw ? (const f16*)w : (const f16*)(sv + p.o_wp), (const f16*)(sv + p.o_xp), (const float*)(sv + p.o_bl),
-           list.target, (const int*)(sv + p.o_exps), N, V, K, p.ld,
+           list.target, (const int*)(sv + p.o_exps), (const int*)(sv + p.o_ex), (const int*)(sv + p.o_ew), N, V, K, p.ld,
            wdtype == VC_BF16, ceil_div(V, GM)};
   float4* part = (float4*)(ws + p.f_part);
   float* zt = (float*)(ws + p.f_zt);
@@ -1081,6 +1173,7 @@ int vc_linear_ce_bwd(int xdtype, int wdtype, float smoothing, int mean,
   f16* dn = (f16*)(ws + p.b_dn);
   const int* exps = (const int*)(sv + p.o_exps);
   const int* order = (const int*)(sv + p.o_order);
+  const int *ex = (const int*)(sv + p.o_ex), *ew = (const int*)(sv + p.o_ew);
   const float2* lse = (const float2*)(sv + p.o_lse);
   float *rs = (float*)(ws + p.b_rs), *big = (float*)(ws + p.b_fac), *dbp = (float*)(ws + p.b_db);
   const CeFac fac{per_row ? big : nullptr, dloss, mean ? (const float*)(sv + p.o_total) : nullptr};
@@ -1090,7 +1183,7 @@ int vc_linear_ce_bwd(int xdtype, int wdtype, float smoothing, int mean,
   for (int c = 0; c < p.pieces; ++c) {
     const int vbeg = c * p.piece;
     const int vcols = p.piece < ceil_div(V - vbeg, GM) * GM ? p.piece : ceil_div(V - vbeg, GM) * GM;
-    CeArgs a{wp, xp, (const float*)(sv + p.o_bl), (const int*)(sv + p.o_target), exps, N, V, K, p.ld, wdtype == VC_BF16, vcols / GM};
+    CeArgs a{wp, xp, (const float*)(sv + p.o_bl), (const int*)(sv + p.o_target), exps, ex, ew, N, V, K, p.ld, wdtype == VC_BF16, vcols / GM};
     float* dbq = db ? dbp : nullptr;
     if (p.pw == 2) grad_go<2, 2, 2>(a, lse, rs, smoothing, vbeg, vcols, dn, dbq, fac, db, accumulate & 2, stream);
     else if (p.pd == 2) grad_go<1, 1, 2>(a, lse, rs, smoothing, vbeg, vcols, dn, dbq, fac, db, accumulate & 2, stream);
@@ -1114,6 +1207,7 @@ int vc_linear_ce_bwd(int xdtype, int wdtype, float smoothing, int mean,
       g.add = c > 0;
       g.out = dx;
       g.which = 1;
+      g.own = ew + vbeg;
       if (g.part) g.pitch = (K + 7) / 8 * 8;
       mm_terms<ROW>(p.pw, p.pdx, g, xdtype == VC_BF16, stream);
     }
@@ -1130,6 +1224,7 @@ int vc_linear_ce_bwd(int xdtype, int wdtype, float smoothing, int mean,
       g.add = g.part ? 0 : accumulate & 1;
       g.out = out;
       g.which = 0;
+      g.own = ex;
       mm_terms<COL>(p.px, p.pdw, g, wdtype == VC_BF16, stream);
       if (g.part) reduce_go(g.part, p.sw, (int64_t)rows * K, fac, exps, 0, accumulate & 1, out, wdtype == VC_BF16, stream);
     }

@@ -1426,8 +1426,10 @@ def linear_cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoot
     int64 of x's leading shape.  Rows whose target is `ignore_index` count for nothing, are not read and cost no products;
     any other target outside [0, V) makes the loss NaN.  reduction: "mean" over the rows that count (0 if there are none),
     "sum", or "none" (a loss per row, 0 where ignored).  The loss is float32; gradients of weight and bias, which have to be
-    leaves, are accumulated into .grad.  Values of x and of the weight are resolved to 2^-39 of the largest finite one of
-    each, and with "none" a row's gradient to 2^-39 of the largest upstream gradient.  stats: a dict that receives "pred"
+    leaves, are accumulated into .grad.  Products take bfloat16 values as they are and float32 ones in 22 bits, but a float32
+    weight next to bfloat16 rows in 11 (a bfloat16 copy has 8; pass float32 rows for 22); every row of x, and of the
+    weight, down to 2^-23 of its largest finite magnitude.  With "none" a row's gradient is resolved to 2^-39 of the largest
+    upstream gradient.  stats: a dict that receives "pred"
     (arg-max per row, 0 where ignored) and "correct" (rows that count and are right).  At most 2^22 rows, 2^22 classes and
     K = 2^20."""
     _require_cuda(x, "linear_cross_entropy")
