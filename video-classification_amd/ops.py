@@ -11,6 +11,7 @@ import functools
 import os
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -1448,6 +1449,7 @@ def linear_cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoot
         raise ValueError(f"linear_cross_entropy: label_smoothing {label_smoothing} outside [0, 1]")
     if reduction not in CE_REDUCTIONS:
         raise ValueError(f"linear_cross_entropy: reduction must be one of {CE_REDUCTIONS}, not {reduction!r}")
+    _no_tangents("linear_cross_entropy", x, weight, bias)
     _leaf_params("linear_cross_entropy", weight, bias)
     _same_device("linear_cross_entropy", x, weight, bias, target)
     if target.numel() > 1 << 22 or weight.shape[0] > 1 << 22 or weight.shape[1] > 1 << 20:
@@ -1729,6 +1731,16 @@ def _wants_grad(*tensors):
     return False
 
 
+def _no_tangents(what, *tensors):
+    """Refuses forward-mode derivatives: the kernels carry no tangents, and a call that needs no gradients bypasses the
+    autograd function that would say so."""
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what}: forward-mode derivatives are not implemented, only backward passes are")
+
+
 def _capturing(t):
     return t.is_cuda and torch.cuda.is_current_stream_capturing()
 
@@ -1927,6 +1939,7 @@ def group_norm(x, gn, act="none", residual=None):
         raise ValueError(f"group_norm: act must be one of {sorted(GN_ACTS)}, not {act!r}")
     L.dtype_code(x.dtype)
     weight, bias = gn.weight, gn.bias
+    _no_tangents("group_norm", x, residual, weight, bias)
     _leaf_params("group_norm", weight, bias)
     if x.dim() < 2 or x.shape[-1] != gn.num_channels:
         raise RuntimeError(f"group_norm: input of shape {tuple(x.shape)} does not end in {gn.num_channels} channels")
@@ -2120,6 +2133,7 @@ def newton_schulz(g, steps=5, coeffs=NS_COEFFS, eps=1e-7, inplace=False):
             raise TypeError(f"newton_schulz: matrices of {first.dtype} and {t.dtype} in one call")
         if inplace and (not t.is_contiguous() or (t.requires_grad and torch.is_grad_enabled())):
             raise RuntimeError("newton_schulz: in place needs dense tensors outside the autograd graph")
+    _no_tangents("newton_schulz", *items)
     code = L.dtype_code(first.dtype)
     _same_device("newton_schulz", first, *items)
     for t in items:
