@@ -7,6 +7,7 @@ into libvc_hip.  Parameter gradients are accumulated by the kernels directly int
 (fp32), so the autograd functions return ``None`` for parameter inputs.
 """
 import contextlib
+import ctypes
 import functools
 import os
 
@@ -1825,9 +1826,12 @@ def _f32_param(what, p):
 
 
 # Autograd orders the backward passes of forward calls on different streams at a parameter's gradient node; the parameters
-# of these operators have none, so passes that write gradients follow each other here.  Per device: handle and stream of the
-# last such pass, and for a stream that is not torch's own, which may be gone by the next one, an event behind it.
+# of these operators have none, so passes that write gradients follow each other here.  Per device: handle of the stream of
+# the last such pass, and what the next one waits for: the default stream itself, which nobody captures on, or behind any
+# other stream an event on a stream of our own.  By the time it is asked for, another thread may be capturing on the pass's
+# stream: an event recorded then would lie in its graph, and one recorded on it before makes HIP invalidate the capture.
 _last_writer = {}
+_marks = {}
 
 
 def _before_grads(dev, *grads):
@@ -1848,8 +1852,25 @@ def _after_grads(dev):
     if (last is not None and last[0] == handle and last[2] is None) or torch.cuda.is_current_stream_capturing():
         return
     stream = torch.cuda.current_stream(dev)
-    foreign = stream.stream_id != 0 and stream.stream_id == stream.cuda_stream
-    _last_writer[dev.index] = handle, stream, stream.record_event() if foreign else None
+    if stream.stream_id == 0:
+        _last_writer[dev.index] = handle, stream, None
+        return
+    if dev.index not in _marks:
+        _marks[dev.index] = _own_stream(dev), torch.cuda.Event(), torch.cuda.Event()
+    own, passed, mark = _marks[dev.index]
+    passed.record(stream)
+    own.wait_event(passed)
+    mark.record(own)
+    # the handle of a stream that is not torch's may come back as another stream's: not remembered
+    _last_writer[dev.index] = None if stream.stream_id == stream.cuda_stream else handle, stream, mark
+
+
+def _own_stream(dev):
+    """A stream that no one else gets: torch hands out those of its pool in turn."""
+    handle = ctypes.c_void_p()
+    with _on(dev):
+        L.check(L.lib().hipStreamCreateWithFlags(ctypes.byref(handle), 1), "hipStreamCreateWithFlags")
+    return torch.cuda.ExternalStream(handle.value, device=dev)
 
 
 def _grad_target(p):
