@@ -347,3 +347,22 @@ def test_runs_of_samples_cover_them_once():
         runs = list(ops._gn_runs(n, 24))
         assert sum(k for _, k, _ in runs) == n and all(0 < k <= 65535 and o == 24 * a for a, k, o in runs)
         assert [a for a, _, _ in runs] == [sum(k for _, k, _ in runs[:i]) for i in range(len(runs))]
+
+
+@pytest.mark.gpu
+def test_parameter_gradients_of_many_samples(cuda):
+    """One value per sample and channel, 65535 times the same: the join of the samples adds nothing but the rounding of its
+    result (half a step, 2^-24), and of the two runs' sums where the gradients are added to."""
+    from video_classification_amd import ops
+    N, C = 65535, 16
+    gn = nn.GroupNorm(2, C).to(cuda)
+    x = torch.arange(C, device=cuda, dtype=torch.float32).repeat(N, 1)
+    dy = torch.full((N, C), 0.1, device=cuda)
+    for times in (1, 2):
+        ops.group_norm(x, gn).backward(dy)
+        want = times * N * dy[0].double()
+        assert ((gn.bias.grad.double() - want).abs() <= times * U * want).all()
+        xh = ops.group_norm(x[:1], nn.GroupNorm(2, C, affine=False)).double()[0]
+        want = times * N * dy[0].double() * xh
+        # dy * xhat is rounded once per sample, the same way in each
+        assert ((gn.weight.grad.double() - want).abs() <= (times + 2) * U * want.abs()).all()

@@ -719,3 +719,20 @@ def test_replays_follow_the_magnitudes(cuda):
         got = [loss.clone(), xs.grad.clone(), w.grad.clone(), b.grad.clone()]
         for g, e in zip(got, [step(), xs.grad, w.grad, b.grad]):
             assert torch.equal(g, e)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("types", list(TYPES))
+def test_bias_gradient_of_many_rows(cuda, types):
+    """Rows that are all alike: every tile of 128 rows has the sums of a call of 128 rows, bit for bit, and 10000 of them add
+    nothing but the rounding of the result, and of the tile's sum in the smaller call's own type."""
+    from video_classification_amd import ops
+    grads = []
+    for n in (128, 1280000):
+        x, t = torch.zeros(n, 8, device=cuda, dtype=TYPES[types][0]), torch.zeros(n, dtype=torch.int64, device=cuda)
+        w = nn.Parameter(torch.zeros(3, 8, device=cuda, dtype=TYPES[types][1]))
+        b = nn.Parameter(torch.tensor([0.5, 0.1, -0.3], device=cuda).to(w.dtype))
+        ops.linear_cross_entropy(x, w, b, t, reduction="sum").backward()
+        grads.append(b.grad.double())
+    want = 10000 * grads[0]
+    assert ((grads[1] - want).abs() <= 2 * half(TYPES[types][1]) * want.abs()).all()

@@ -331,25 +331,25 @@ __global__ __launch_bounds__(64) void gn_bwd_join_kernel(Cover k, const float* _
 }
 
 // dgamma[c] (+)= sum_n B_c, dbeta[c] (+)= sum_n A_c (added to where bit 0 / bit 1 of `add` is set): 64 channels x 4 runs of
-// samples per block, runs joined in order
+// samples per block, runs joined in order, in doubles: a run is up to 16384 samples long
 __global__ __launch_bounds__(GT) void gn_bwd_params_kernel(const float* __restrict__ ab, float* __restrict__ dgamma,
                                                            float* __restrict__ dbeta, int N, int C, int add) {
-  __shared__ float sa[4][64], sb[4][64];
+  __shared__ double sa[4][64], sb[4][64];
   const int e = threadIdx.x & 63, run = threadIdx.x >> 6;
   const int c = blockIdx.x * 64 + e;
-  float a = 0.f, b = 0.f;
+  double a = 0.0, b = 0.0;
   if (c < C)
 #pragma unroll 4
     for (int n = run; n < N; n += 4) {
-      a += ab[(size_t)n * 2 * C + c];
-      b += ab[(size_t)n * 2 * C + C + c];
+      a += (double)ab[(size_t)n * 2 * C + c];
+      b += (double)ab[(size_t)n * 2 * C + C + c];
     }
   sa[run][e] = a;
   sb[run][e] = b;
   __syncthreads();
   if (run == 0 && c < C) {
-    if (dbeta) dbeta[c] = (add & 2 ? dbeta[c] : 0.f) + ((sa[0][e] + sa[1][e]) + (sa[2][e] + sa[3][e]));
-    if (dgamma) dgamma[c] = (add & 1 ? dgamma[c] : 0.f) + ((sb[0][e] + sb[1][e]) + (sb[2][e] + sb[3][e]));
+    if (dbeta) dbeta[c] = (add & 2 ? dbeta[c] : 0.f) + (float)((sa[0][e] + sa[1][e]) + (sa[2][e] + sa[3][e]));
+    if (dgamma) dgamma[c] = (add & 1 ? dgamma[c] : 0.f) + (float)((sb[0][e] + sb[1][e]) + (sb[2][e] + sb[3][e]));
   }
 }
 

@@ -695,17 +695,17 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_grad_kernel(CeArgs a, const f
   }
 }
 
-// db[v] (+)= fac sum over the row tiles of dbpart[tile][v]
+// db[v] (+)= fac sum over the row tiles of dbpart[tile][v], up to 32768 of them and therefore in doubles
 template <typename T>
 __global__ __launch_bounds__(256) void ce_bias_kernel(const float* __restrict__ dbpart, const int* __restrict__ exps, int V,
                                                       CeFac fac, int add, T* __restrict__ db) {
   const int tiles = max(1, (exps[2] + GM - 1) / GM);
   const int v = blockIdx.x * 256 + threadIdx.x;
   if (v >= V) return;
-  float s = 0.f;
+  double s = 0.0;
 #pragma unroll 4
-  for (int t = 0; t < tiles; ++t) s += dbpart[(int64_t)t * V + v];
-  bias_out(db + v, s, fac, add);
+  for (int t = 0; t < tiles; ++t) s += (double)dbpart[(int64_t)t * V + v];
+  bias_out(db + v, (float)s, fac, add);
 }
 
 // slices of a reduction of length k (a multiple of 64) over `tiles` output tiles: two workgroups per CU where the slices
