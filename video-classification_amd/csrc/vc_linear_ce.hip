@@ -576,9 +576,18 @@ __device__ __forceinline__ float row16_sum(float v) {  // over the 16 lanes of a
   return v;
 }
 
+// fac 2^e as a factor of [1/2, 1) and an exponent: applied one after the other, neither underflows where their product, a
+// gradient of tiny operands, does not.
+struct Factor {
+  float f;
+  int e;
+  __device__ __forceinline__ Factor(float fac, int exp) : f(__builtin_amdgcn_frexp_mantf(fac)), e(exp + __builtin_amdgcn_frexp_expf(fac)) {}
+  __device__ __forceinline__ float operator()(float v) const { return ldexpf(v * f, e); }
+};
+
 template <typename T>
 __device__ __forceinline__ void bias_out(T* db, float s, const CeFac& fac, int add) {
-  *db = from_f32<T>((add ? to_f32(*db) : 0.f) + s * (fac.get() / D_SCALE));
+  *db = from_f32<T>((add ? to_f32(*db) : 0.f) + Factor(fac.get(), -15)(s));  // of D_SCALE
 }
 
 // 8192 x 1024 against a piece of 8192 classes: 154 us, 0.89 PFLOP/s; the tile leaves through LDS in rows of 256 bytes.
@@ -741,8 +750,8 @@ struct MmArgs {
   const int* own;              // the column side's scale exponents along the reduction, for exps[3 + which]
 };
 
-__device__ __forceinline__ float mm_factor(const CeFac& fac, const int* exps, int which) {
-  return exps[3 + which] ? fac.get() : ldexpf(fac.get(), -15 - exps[which]);
+__device__ __forceinline__ Factor mm_factor(const CeFac& fac, const int* exps, int which) {
+  return Factor(fac.get(), exps[3 + which] ? 0 : -15 - exps[which]);
 }
 
 // The product where the column side's scales differ along the reduction (some rows of x or of W lie more than 2^16 below the
@@ -820,13 +829,16 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
   }
   const int lane = threadIdx.x & 63, q = lane >> 4, l15 = lane & 15;
   const int wave = threadIdx.x >> 6, wc = wave >> 1, wr = wave & 1;
-  const float f = g.part ? 1.f : mm_factor(g.fac, g.exps, g.which);
   float* part = g.part ? g.part + (int64_t)split * (KM == ROW ? rows : g.M) * g.pitch : nullptr;
-  if (!part)
+  if (!part) {
+    const Factor f = mm_factor(g.fac, g.exps, g.which);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] *= f;
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = f(acc[i][j][e]);
+  }
   // dx: packed rows go to their places, those that do not count as zeros
   const int live = KM == ROW ? rows : g.M, end = KM == ROW && part ? rows : g.M;
   int64_t at[4];
@@ -901,7 +913,7 @@ __global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ pa
   const int r = (int)(unit / per), c0 = (int)(unit - (int64_t)r * per) * 512 + (threadIdx.x & 63) * (vec ? 8 : 1);
   if (r >= N) return;
   const bool live = r < rows;
-  const float f = mm_factor(fac, exps, 1);
+  const Factor f = mm_factor(fac, exps, 1);
   const float* p = part + (int64_t)r * pitch;
   T* o = out + (int64_t)order[r] * K;
   if (vec) {
@@ -917,7 +929,7 @@ __global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ pa
         for (int e = 0; e < 8; ++e) s.v[e] += v.v[e];
       }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s.v[e] *= f;
+    for (int e = 0; e < 8; ++e) s.v[e] = f(s.v[e]);
     if (!live)
 #pragma unroll
       for (int e = 0; e < 8; ++e) s.v[e] = 0.f;
@@ -932,7 +944,7 @@ __global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ pa
         for (int e = 0; e < 8; ++e) s[e] += p[k * n + min(c0 + e * 64, K - 1)];
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (c0 + e * 64 < K) o[c0 + e * 64] = from_f32<T>(live ? s[e] * f : 0.f);
+      if (c0 + e * 64 < K) o[c0 + e * 64] = from_f32<T>(live ? f(s[e]) : 0.f);
   }
 }
 
@@ -940,12 +952,12 @@ __global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ pa
 template <typename T>
 __global__ __launch_bounds__(256) void ce_reduce_kernel(const float* __restrict__ part, int slices, int64_t n,
                                                         CeFac fac, const int* __restrict__ exps, int which, int add, T* __restrict__ out) {
-  const float f = mm_factor(fac, exps, which);
+  const Factor f = mm_factor(fac, exps, which);
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
     float s = 0.f;
 #pragma unroll 4
     for (int k = 0; k < slices; ++k) s += part[k * n + i];
-    s *= f;
+    s = f(s);
     out[i] = from_f32<T>(add ? to_f32(out[i]) + s : s);
   }
 }
