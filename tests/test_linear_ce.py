@@ -763,3 +763,15 @@ def test_gradients_of_tiny_magnitude(cuda, types, xs, ws, gs, N, K, V):
         g = p.grad.double() / scale
         got.append(g + (want - g).clamp(-half_step, half_step))
     check(ref, types, None, *got, one_term=FEW_ROWS)
+
+
+def test_refuses_what_no_launch_can_hold():
+    """A launch has fewer than 2^32 threads: sizes beyond that are refused before the first one, with a reason."""
+    from video_classification_amd import _lib as L, ops
+    for n, v, k, why in ((1 << 20, 1 << 18, 64, "tiles of logits"), (1 << 22, 1 << 22, 8, "tiles of logits"),
+                         (1 << 17, 1 << 19, 1 << 17, "pieces of 512"), (1 << 20, 7, 1 << 15, "pieces of 512")):
+        for what in (0, 1, 2, 4):
+            assert L.query("vc_linear_ce_bytes", what, 1, 1, n, v, k) == -1
+            with pytest.raises(RuntimeError, match=why):
+                ops._size("vc_linear_ce_bytes", what, 1, 1, n, v, k)
+    assert ops._size("vc_linear_ce_bytes", 0, 1, 1, (1 << 20) - 128, 1 << 18, 64) > 0

@@ -308,7 +308,7 @@ bool pick(Slab& k, int esize, int N, int S, int C, int G, int64_t most) {
   k.lg = lg;
   k.slabs = cv >> lg;
   k.gspan = span;
-  return (int64_t)N * k.slabs < (1ll << 31);
+  return (int64_t)N * k.slabs < (1ll << 23);  // a launch holds fewer than 2^32 threads, 512 to a slab
 }
 
 #define BY_GROUPS(cpg, ...)                                          \

@@ -1046,8 +1046,11 @@ int check_ce(const char* who, int xdtype, int wdtype, int N, int V, int K, float
   // 128 rows of an operand have to fit a 32-bit buffer descriptor, tiles a grid
   VC_CHECK_SHAPE(K <= (1 << 20) && N <= (1 << 22) && V <= (1 << 22), "%s: N, V or K too large (at most 2^22, 2^22, 2^20)",
                  who);
-  VC_CHECK_SHAPE((int64_t)ceil_div(N, GM) * ceil_div(V, GM) < (1ll << 31) - 1 &&
-                     ((int64_t)N + V) * ceil_div(K, 512) < (1ll << 33) - 8, "%s: too many tiles", who);
+  // a launch holds fewer than 2^32 threads
+  VC_CHECK_SHAPE((int64_t)ceil_div(N, GM) * ceil_div(V, GM) < (1 << 24), "%s: %d rows against %d classes are more than 2^24 tiles of logits",
+                 who, N, V);
+  VC_CHECK_SHAPE(((int64_t)N + V) * ceil_div(K, 512) < (1 << 26) - 8, "%s: %d rows and %d classes of %d are more than 2^26 pieces of 512 to pack",
+                 who, N, V, K);
   VC_CHECK_ARG(smooth >= 0.f && smooth <= 1.f, "%s: label smoothing %g outside [0, 1]", who, (double)smooth);
   return VC_OK;
 }

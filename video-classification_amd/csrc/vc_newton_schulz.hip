@@ -755,7 +755,8 @@ int vc_newton_schulz(int dtype, int count, const void* const* g, void* const* ou
     }
     if (!n) break;  // the rest was small
     NsLayout l(r, c, n);
-    for (int k = 0; k < KINDS; ++k) VC_CHECK_SHAPE(l.blocks[k] < (1ll << 31), "vc_newton_schulz: too many tiles");
+    for (int k = 0; k < KINDS; ++k)  // a launch holds fewer than 2^32 threads
+      VC_CHECK_SHAPE(l.blocks[k] < (1 << 24), "vc_newton_schulz: the matrices of a launch are more than 2^24 tiles");
     double* norms = (double*)((char*)workspace + l.norms);
     float* part = (float*)((char*)workspace + l.part);
     f16* ws = (f16*)((char*)workspace + l.bufs);

@@ -1432,8 +1432,8 @@ def linear_cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoot
     weight next to bfloat16 rows in 11 (a bfloat16 copy has 8; pass float32 rows for 22); every row of x, and of the
     weight, down to 2^-23 of its largest finite magnitude.  With "none" a row's gradient is resolved to 2^-39 of the largest
     upstream gradient.  stats: a dict that receives "pred"
-    (arg-max per row, 0 where ignored) and "correct" (rows that count and are right).  At most 2^22 rows, 2^22 classes and
-    K = 2^20."""
+    (arg-max per row, 0 where ignored) and "correct" (rows that count and are right).  At most 2^22 rows, 2^22 classes,
+    K = 2^20, 2^38 logits and 2^35 values in x and the weight together."""
     _require_cuda(x, "linear_cross_entropy")
     xd, wd = L.dtype_code(x.dtype), L.dtype_code(weight.dtype)
     if xd == L.VC_F32 and wd != L.VC_F32:
@@ -1776,8 +1776,11 @@ def _addr(t, offset=0):
 
 @functools.lru_cache(maxsize=1024)
 def _size(name, *ints):
-    """A size query of the library, which depends on its arguments alone."""
-    return L.query(name, *ints)
+    """A size query of the library, which depends on its arguments alone; raises where the library refuses the sizes."""
+    n = L.query(name, *ints)
+    if n < 0:
+        raise RuntimeError(L.last_error())
+    return n
 
 
 def _same_device(what, first, *rest):
