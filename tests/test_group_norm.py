@@ -386,3 +386,20 @@ def test_more_slabs_than_a_launch_holds(cuda):
     # next to the corner of ReLU a rounding decides about a whole gradient; elsewhere the norm's gradient holds to 1e-5
     err = (xg.grad[pick].double() - x64.grad).abs()
     assert float((err > 1e-4).double().mean()) < 1e-3
+
+
+# Groups of 1 to 64 channels in slabs of one group and of several, as wide as a line (many samples) or narrowed (few), with the
+# register counts of every size of the one-pass kernels; the layers of a ResNet trunk with 32 groups.
+SLABS = [((300, 49, 64), 64), ((300, 49, 64), 32), ((300, 49, 64), 16), ((300, 49, 64), 8), ((300, 9, 128), 4),
+         ((40, 9, 256), 16), ((16, 25, 1024), 32), ((8, 16, 2048), 32), ((2, 49, 512), 8), ((1, 120, 64), 1),
+         ((1, 510, 64), 1), ((1, 1020, 32), 1), ((1, 9001, 8), 1), ((1, 9001, 8), 4), ((1, 9001, 8), 8), ((2, 4500, 16), 1),
+         ((1, 3000, 32), 1), ((1, 1700, 64), 1), ((2, 1, 56, 56, 256), 32), ((3, 1, 28, 28, 512), 32), ((4, 1, 14, 14, 1024), 32),
+         ((5, 1, 7, 7, 2048), 32), ((270, 768), 32)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("act,use_res", [("none", False), ("relu", True), ("silu", True), ("gelu", False)])
+@pytest.mark.parametrize("shape,groups", SLABS)
+def test_slabs(cuda, dt, act, use_res, shape, groups):
+    test_forward_backward(cuda, dt, act, use_res, shape, groups)

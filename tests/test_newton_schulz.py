@@ -248,3 +248,35 @@ def test_large_tiles(cuda, dt):
     unit = (4 + 3 * 2100 ** 0.5 / 16) * 2.0 ** -22
     tol = sum(C[0] ** (5 - k) * unit * float(n) for k, n in enumerate(norms)) + torch.finfo(DT[dt]).eps / 2 * float(want.norm())
     assert float((outs[0].double() - want).norm()) <= tol
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("m,n", [(4033, 4040), (4100, 4000)])
+def test_last_round_of_a_large_matrix(cuda, dt, m, n):
+    """More than 512 tiles of a symmetric product: those of the last round are cut along the reduction, the others are whole."""
+    from video_classification_amd import ops
+    g = gaussian(m, n, 5).to(DT[dt]).to(cuda)
+    out = ops.newton_schulz(g)
+    want, norms = reference(g)
+    unit = (4 + 3 * max(m, n) ** 0.5 / 16) * 2.0 ** -22
+    tol = sum(C[0] ** (5 - k) * unit * float(v) for k, v in enumerate(norms)) + torch.finfo(DT[dt]).eps / 2 * float(want.norm())
+    assert float((out.double() - want).norm()) <= tol
+    # every entry, for a wrong tile could hide in the norm of them all: 485 times a step's 16 x 2^-22 is 2^-9, the result's own
+    # rounding another 2^-9, relative to entries of the largest's size
+    assert float((out.double() - want).abs().max()) <= 2.0 ** -7 * float(want.abs().max())
+    assert torch.equal(out, ops.newton_schulz(g))
+
+
+@pytest.mark.gpu
+def test_bits_repeat_for_the_same_set(cuda):
+    """The same matrices in the same call give the same bits, cut reductions or not; in other company the reductions may be cut
+    elsewhere, and the results agree within the tolerance only."""
+    from video_classification_amd import ops
+    shapes = [(64, 576), (128, 1152), (256, 2304), (512, 4608), (512, 512), (1000, 64)]
+    mats = [gaussian(m, n, i).to(cuda) for i, (m, n) in enumerate(shapes)]
+    first, second = ops.newton_schulz(mats), ops.newton_schulz(mats)
+    for a, b, g in zip(first, second, mats):
+        assert torch.equal(a, b)
+        close(a, g)
+        close(ops.newton_schulz(g), g)

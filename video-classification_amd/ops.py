@@ -2130,7 +2130,9 @@ def newton_schulz(g, steps=5, coeffs=NS_COEFFS, eps=1e-7, inplace=False):
     g: a tensor [..., m, n], or a list or tuple of such tensors of any shapes (all of one type, float32 or bfloat16, on one
     device); all their matrices go through the same launches.  coeffs: (a, b, c), or `steps` such triples.  Returns new
     tensors of g's structure, shapes and type, or with `inplace` the tensors of g themselves (dense, sharing no memory);
-    products are carried at float32 accuracy whatever the type.  Not differentiable: gradients are its input."""
+    products are carried at float32 accuracy whatever the type.  The same set of matrices gives the same bits every time; a
+    matrix in other company may differ in its last ones.  Coefficients and steps may let singular values grow to 16 at most, and
+    by a factor of at most 8192 (the default ones: up to seven steps).  Not differentiable: gradients are its input."""
     single = isinstance(g, torch.Tensor)
     items = [g] if single else list(g)
     if not items:
