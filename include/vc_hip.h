@@ -362,8 +362,8 @@ int vc_ce_fwd_bwd(int grad_dtype, const float* logits, int ld, const int64_t* ta
  * fwd: row_loss [N] (0 for ignored rows), loss (nullable, one float), pred [N] (nullable, lowest arg-max, 0 for ignored
  *   rows) and correct (nullable).  saved: vc_linear_ce_bytes(0, ..) bytes that backward reads; workspace: vc_linear_ce_bytes(1, ..),
  *   or with saved = null, for a call without a backward pass, vc_linear_ce_bytes(4, ..).
- * bwd: dloss = upstream gradient of the mean or sum, or with per_row of every row's loss (each resolved to 2^-39 of the
- *   largest); dx, dw and db (each nullable) are written, or added to where bit 0 (dw) / bit 1 (db) of `accumulate` is
+ * bwd: dloss = upstream gradient of the mean or sum, or with per_row of every row's loss (a row's gradient is resolved to
+ *   2^-24 of its own); dx, dw and db (each nullable) are written, or added to where bit 0 (dw) / bit 1 (db) of `accumulate` is
  *   set; workspace: vc_linear_ce_bytes(2, ..).
  * Buffers 256-byte aligned, contents of the workspaces irrelevant before and after; every sum has a fixed order. */
 int64_t vc_linear_ce_bytes(int what, int xdtype, int wdtype, int N, int V, int K);

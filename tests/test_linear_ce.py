@@ -619,14 +619,18 @@ def check_each(types, x, w, b, t, rows, dx, dw, db, weight, skip=()):
     assert (err <= tol)[live].all(), float((err - tol)[live].max())
     d = p.clone()
     d[at, t] -= 1
+    # fp16's smallest step is 2^-24 and d is scaled by 2^15: half a step is 2^-40 of the row's weight (of the largest one where
+    # they are within 2^16 of each other), or all of a smaller value
+    size = (weight * live).abs()
+    unit = size if size[size > 0].min() < 2.0 ** -16 * size.max() else size.max().expand(N)
+    floor = torch.minimum(d.abs() * size[:, None], 2.0 ** -40 * unit[:, None])
     d = d * (weight * live)[:, None]
-    off = (2 * p * (1 - p).clamp_min(0) * (dz + mid[:, None]) + 2.0 ** -20 * p) * (weight * live)[:, None]
-    for got, want, A, M, P, dt, length in ((dx, d @ w64, d.abs(), w64.abs(), off, xd, V),
-                                           (dw, d.t() @ x64, d.abs().t(), x64.abs(), off.t(), wd, N)):
+    off = (2 * p * (1 - p).clamp_min(0) * (dz + mid[:, None]) + 2.0 ** -20 * p) * size[:, None]
+    for got, want, A, F, M, P, dt, length in ((dx, d @ w64, d.abs(), floor, w64.abs(), off, xd, V),
+                                              (dw, d.t() @ x64, d.abs().t(), floor.t(), x64.abs(), off.t(), wd, N)):
         # joins of a sum: of 32 fp16 products each, or (rows of their own scale) one rounding per fp32 product
         term = (2.0 ** -22 if dt == torch.float32 else FEW_ROWS) + 2.0 ** -21 + (length + 8) * 2.0 ** -23
-        # fp16's smallest step is 2^-24 and d is scaled by 2^15: half a step is 2^-40, or all of a smaller value
-        tol = term * (A @ M) + A.clamp_max(2.0 ** -40) @ M + P @ M + half(dt) * want.abs() + 1e-37
+        tol = term * (A @ M) + F @ M + P @ M + half(dt) * want.abs() + 1e-37
         err = (got.double() - want).abs()
         assert (err <= tol).all(), float((err / tol).max())
     tol = off.sum(0) + (N / 16 + 16) * U * d.abs().sum(0) + half(wd) * d.sum(0).abs() + 1e-37
@@ -775,3 +779,20 @@ def test_refuses_what_no_launch_can_hold():
             with pytest.raises(RuntimeError, match=why):
                 ops._size("vc_linear_ce_bytes", what, 1, 1, n, v, k)
     assert ops._size("vc_linear_ce_bytes", 0, 1, 1, (1 << 20) - 128, 1 << 18, 64) > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("types", list(TYPES))
+@pytest.mark.parametrize("N,K,V", [(200, 64, 300), (1500, 40, 700), (90, 520, 4099)])
+@pytest.mark.parametrize("e", [10, 40, -140])
+def test_upstream_gradients_side_by_side(cuda, types, N, K, V, e):
+    """One row's upstream gradient 2^e times the others', and one of zero: no row's gradient takes precision from another."""
+    from video_classification_amd import ops
+    x, w, b, t = make(N, K, V, types, seed=17)
+    weight = torch.full((N,), -1 / 3, device=cuda)
+    weight[7], weight[20] = 2.0 ** e, 0.0
+    xg = x.clone().requires_grad_(True)
+    rows = ops.linear_cross_entropy(xg, w, b, t, reduction="none")
+    rows.backward(weight)
+    check_each(types, x, w, b, t, rows.detach(), xg.grad, w.grad, b.grad, weight.double())
+    assert not xg.grad[20].any()

@@ -540,7 +540,9 @@ __global__ __launch_bounds__(1024) void ce_total_kernel(CeRows k, const float4* 
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------------
-// Per-row upstream gradients: rs[k] = weight of packed row k relative to the largest one, fac[0] = that largest weight.
+// Per-row upstream gradients: rs[k] = weight of packed row k relative to the largest one, fac[0] = that largest weight, fac[1] = 0.
+// If a weight other than 0 lies more than 2^16 below the largest, rs[k] = the weight itself, fac[0] = fac[1] = 1: d is kept without
+// the weights, which dx takes on as it is written, and dW in its product.
 __global__ __launch_bounds__(1024) void ce_weights_kernel(const float* __restrict__ g, const int* __restrict__ order,
                                                           const int* __restrict__ exps, float* __restrict__ rs,
                                                           float* __restrict__ fac) {
@@ -554,8 +556,17 @@ __global__ __launch_bounds__(1024) void ce_weights_kernel(const float* __restric
   big = sm[0];
   for (int i = 1; i < 16; ++i) big = fmaxf(big, sm[i]);
   if (!(big > 0.f)) big = 1.f;
-  for (int k = threadIdx.x; k < rows; k += 1024) rs[k] = g[order[k]] / big;
-  if (threadIdx.x == 0) fac[0] = big;
+  int own = 0;
+  for (int k = threadIdx.x; k < rows; k += 1024) {
+    const float w = fabsf(g[order[k]]);
+    own |= w > 0.f && w < ldexpf(big, -OWN_SCALE);
+  }
+  own = __syncthreads_or(own);
+  for (int k = threadIdx.x; k < rows; k += 1024) rs[k] = own ? g[order[k]] : g[order[k]] / big;
+  if (threadIdx.x == 0) {
+    fac[0] = own ? 1.f : big;
+    fac[1] = own ? 1.f : 0.f;
+  }
 }
 
 constexpr float D_SCALE = 32768.f;  // of d's fp16 terms, and of dbpart
@@ -565,6 +576,8 @@ struct CeFac {
   const float* fac;    // per-row weights
   const float* g;      // else the one gradient,
   const float* total;  // of a mean (the counted rows) or, null, of a sum
+  // whether d is kept without the rows' weights
+  __device__ __forceinline__ bool own() const { return fac && fac[1] != 0.f; }
   __device__ __forceinline__ float get() const { return fac ? fac[0] : total ? g[0] / fmaxf(total[0], 1.f) : g[0]; }
 };
 
@@ -636,9 +649,12 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_grad_kernel(CeArgs a, const f
       const int n = n0 + wn * 64 + j * 16 + l15;
       if (n < rows) weight[j] = rs[n];
     }
+  const bool own = fac.own();
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float w = weight[j], m = top[j], l = low[j];
+    const float m = top[j], l = low[j];
+    const bool live = weight[j] != 0.f;  // a row without weight vanishes whatever it holds
+    const float w = own ? 1.f : weight[j], wb = own ? weight[j] : 1.f;  // of d and, beyond that, of the bias's gradient
     const int hit = lane_class(target[j], v0);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -655,13 +671,12 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_grad_kernel(CeArgs a, const f
 #pragma unroll
       for (int e = 0; e < 16; ++e)
         if (e == hit) acc[e >> 2][j][e & 3] -= (1.f - smooth) * D_SCALE;
-    const bool live = w != 0.f;  // a row without weight vanishes whatever it holds
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         acc[i][j][r] = live ? acc[i][j][r] * w : 0.f;
-        col[i][r] += acc[i][j][r];
+        col[i][r] = fmaf(acc[i][j][r], wb, col[i][r]);
       }
   }
   float* tile = reinterpret_cast<float*>(smem);
@@ -748,24 +763,31 @@ struct MmArgs {
   const int* exps;             // exps[2] = rows that count: rows of dx that are worked, reduction length of dW
   int which;                   // whose scale exponent the column side carries
   const int* own;              // the column side's scale exponents along the reduction, for exps[3 + which]
+  const float* rs;             // the rows' weights, for fac.own()
 };
 
+// whether the product goes by own_product: the column side has scales of its own along the reduction, or is to take the
+// rows' weights (dW)
+__device__ __forceinline__ bool mm_own(const CeFac& fac, const int* exps, int which) {
+  return exps[3 + which] || (which == 0 && fac.own());
+}
 __device__ __forceinline__ Factor mm_factor(const CeFac& fac, const int* exps, int which) {
-  return Factor(fac.get(), exps[3 + which] ? 0 : -15 - exps[which]);
+  return Factor(fac.get(), mm_own(fac, exps, which) ? 0 : -15 - exps[which]);
 }
 
-// The product where the column side's scales differ along the reduction (some rows of x or of W lie more than 2^16 below the
-// largest): its values as they are, on the fp32 matrix instructions, whose range holds all of them.  Operands come straight
+// The product where the column side's scales, or for dW the rows' weights, differ along the reduction (some rows of x or of W, or
+// some upstream gradients, lie more than 2^16 below the largest): its values as they are, on the fp32 matrix instructions, whose range holds all of them.  Operands come straight
 // from memory: a step of 4096 x 768 x 16384 in bf16 takes 3.2 ms (rows) or 4.1 (classes) instead of 0.58; data with such rows
 // is not what training usually meets.
 template <int PC, int PM, int KM>
-__device__ __forceinline__ void own_product(f32x4 (&acc)[4][4], const Op16& c, const Op16& m, const int* own, int k0, int k1) {
+__device__ __forceinline__ void own_product(f32x4 (&acc)[4][4], const Op16& c, const Op16& m, const int* own, const float* rs, int k0, int k1) {
   const int lane = threadIdx.x & 63, q = lane >> 4, l15 = lane & 15;
   const int wave = threadIdx.x >> 6, wc = wave >> 1, wr = wave & 1;
   for (int k = k0; k < k1; k += 4) {
     const int kk = k + q;
     const bool on = kk < c.n;  // the reduction's true length
     const int e = on ? -own[kk] : 0;
+    const float w = on && rs ? rs[kk] : 1.f;
     float fc[4], fm[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -779,7 +801,7 @@ __device__ __forceinline__ void own_product(f32x4 (&acc)[4][4], const Op16& c, c
       fm[i] = 0.f;
       if (on && (KM == ROW ? row < m.n : m.side + row < m.ld)) {
         const f16* p = KM == ROW ? m.p + (int64_t)row * m.ld + kk : m.p + (int64_t)kk * m.ld + m.side + row;
-        fm[i] = (PM == 2 ? (float)p[0] + (float)p[m.plane] : (float)p[0]) * (1.f / D_SCALE);
+        fm[i] = (PM == 2 ? (float)p[0] + (float)p[m.plane] : (float)p[0]) * (1.f / D_SCALE) * w;
       }
     }
 #pragma unroll
@@ -824,7 +846,7 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
     m.n = c.n = rows;
   }
   if (!idle) {
-    if (g.exps[3 + g.which]) own_product<PC, PM, KM>(acc, c, m, g.own, k0, k1);
+    if (mm_own(g.fac, g.exps, g.which)) own_product<PC, PM, KM>(acc, c, m, g.own, KM == COL && g.fac.own() ? g.rs : nullptr, k0, k1);
     else G::run(acc, c, m, k0, k1, smem);
   }
   const int lane = threadIdx.x & 63, q = lane >> 4, l15 = lane & 15;
@@ -838,6 +860,13 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[i][j][e] = f(acc[i][j][e]);
+    if (KM == ROW && g.fac.own())
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float w = g.rs[max(min(m0 + wr * 64 + j * 16 + l15, rows - 1), 0)];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i][j] *= w;
+      }
   }
   // dx: packed rows go to their places, those that do not count as zeros
   const int live = KM == ROW ? rows : g.M, end = KM == ROW && part ? rows : g.M;
@@ -902,8 +931,8 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
 // 512 columns.
 template <typename T>
 __global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ part, int piece, int N, int K, CeFac fac,
-                                                    const int* __restrict__ exps, const int* __restrict__ order, int vec,
-                                                    T* __restrict__ out) {
+                                                    const int* __restrict__ exps, const int* __restrict__ order,
+                                                    const float* __restrict__ rs, int vec, T* __restrict__ out) {
   const int per = (K + 511) / 512;
   const int rows = exps[2];
   int splits, len;
@@ -914,6 +943,7 @@ __global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ pa
   if (r >= N) return;
   const bool live = r < rows;
   const Factor f = mm_factor(fac, exps, 1);
+  const float w = live && fac.own() ? rs[r] : 1.f;
   const float* p = part + (int64_t)r * pitch;
   T* o = out + (int64_t)order[r] * K;
   if (vec) {
@@ -929,7 +959,7 @@ __global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ pa
         for (int e = 0; e < 8; ++e) s.v[e] += v.v[e];
       }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s.v[e] = f(s.v[e]);
+    for (int e = 0; e < 8; ++e) s.v[e] = f(s.v[e]) * w;
     if (!live)
 #pragma unroll
       for (int e = 0; e < 8; ++e) s.v[e] = 0.f;
@@ -944,7 +974,7 @@ __global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ pa
         for (int e = 0; e < 8; ++e) s[e] += p[k * n + min(c0 + e * 64, K - 1)];
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (c0 + e * 64 < K) o[c0 + e * 64] = from_f32<T>(live ? f(s[e]) : 0.f);
+      if (c0 + e * 64 < K) o[c0 + e * 64] = from_f32<T>(live ? f(s[e]) * w : 0.f);
   }
 }
 
@@ -1101,12 +1131,12 @@ void mm_terms(int pc, int pm, const MmArgs& g, int out_bf16, hipStream_t st) {
   else if (pc == 1) mm_go<1, 2, KM>(g, out_bf16, st);
   else mm_go<2, 2, KM>(g, out_bf16, st);
 }
-void dx_go(const float* part, int piece, int N, int K, const CeFac& fac, const int* exps, const int* order, void* dx,
-           int out_bf16, hipStream_t st) {
+void dx_go(const float* part, int piece, int N, int K, const CeFac& fac, const int* exps, const int* order, const float* rs,
+           void* dx, int out_bf16, hipStream_t st) {
   const dim3 grid((unsigned)ceil_div64((int64_t)N * ceil_div(K, 512), 4));
   const int vec = K % 8 == 0 && ((uintptr_t)dx & 15) == 0;
-  if (out_bf16) hipLaunchKernelGGL((ce_dx_kernel<bf16>), grid, dim3(256), 0, st, part, piece, N, K, fac, exps, order, vec, (bf16*)dx);
-  else hipLaunchKernelGGL((ce_dx_kernel<float>), grid, dim3(256), 0, st, part, piece, N, K, fac, exps, order, vec, (float*)dx);
+  if (out_bf16) hipLaunchKernelGGL((ce_dx_kernel<bf16>), grid, dim3(256), 0, st, part, piece, N, K, fac, exps, order, rs, vec, (bf16*)dx);
+  else hipLaunchKernelGGL((ce_dx_kernel<float>), grid, dim3(256), 0, st, part, piece, N, K, fac, exps, order, rs, vec, (float*)dx);
 }
 void reduce_go(const float* part, int slices, int64_t n, const CeFac& fac, const int* exps, int which, int add, void* out,
                int out_bf16, hipStream_t st) {
@@ -1209,6 +1239,7 @@ int vc_linear_ce_bwd(int xdtype, int wdtype, float smoothing, int mean,
     g.tiles_n = tk;
     g.fac = fac;
     g.exps = exps;
+    g.rs = rs;
     if (dx) {
       g.c = Op16{wp + (int64_t)vbeg * p.ld, (int64_t)V * p.ld, p.ld, rows, 0};
       g.m = Op16{dn, (int64_t)N * vcols, vcols, N, 0};
@@ -1245,7 +1276,7 @@ int vc_linear_ce_bwd(int xdtype, int wdtype, float smoothing, int mean,
     }
   }
   if (dx && p.b_px >= 0)
-    dx_go((const float*)(ws + p.b_px), p.piece, N, K, fac, exps, order, dx, xdtype == VC_BF16, stream);
+    dx_go((const float*)(ws + p.b_px), p.piece, N, K, fac, exps, order, rs, dx, xdtype == VC_BF16, stream);
   if (db && tn > 1) {
     if (wdtype == VC_BF16)
       hipLaunchKernelGGL((ce_bias_kernel<bf16>), dim3(ceil_div(V, 256)), dim3(256), 0, stream, dbp, exps, V, fac,

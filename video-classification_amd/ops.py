@@ -1430,10 +1430,9 @@ def linear_cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoot
     "sum", or "none" (a loss per row, 0 where ignored).  The loss is float32; gradients of weight and bias, which have to be
     leaves, are accumulated into .grad.  Products take bfloat16 values as they are and float32 ones in 22 bits, but a float32
     weight next to bfloat16 rows in 11 (a bfloat16 copy has 8; pass float32 rows for 22); every row of x, and of the
-    weight, down to 2^-23 of its largest finite magnitude.  With "none" a row's gradient is resolved to 2^-39 of the largest
-    upstream gradient.  stats: a dict that receives "pred"
-    (arg-max per row, 0 where ignored) and "correct" (rows that count and are right).  At most 2^22 rows, 2^22 classes,
-    K = 2^20, 2^38 logits and 2^35 values in x and the weight together."""
+    weight, down to 2^-23 of its largest finite magnitude, a row's gradient down to 2^-24 of its upstream one.  stats: a
+    dict that receives "pred" (arg-max per row, 0 where ignored) and "correct" (rows that count and are right).  At most 2^22
+    rows, 2^22 classes, K = 2^20, 2^38 logits and 2^35 values in x and the weight together."""
     _require_cuda(x, "linear_cross_entropy")
     xd, wd = L.dtype_code(x.dtype), L.dtype_code(weight.dtype)
     if xd == L.VC_F32 and wd != L.VC_F32:
