@@ -356,7 +356,7 @@ int vc_ce_fwd_bwd(int grad_dtype, const float* logits, int ld, const int64_t* ta
  * and nn.CrossEntropyLoss in one, for label sets whose logits should not be kept; no counterpart in the reference).
  * x [N][K] (xdtype), w [V][K], bias [V] nullable, db [V], dw [V][K] (wdtype), dx [N][K] (xdtype); fp32 x needs fp32 w;
  * N and V up to 2^22, K up to 2^20, N V up to 2^38 and (N + V) K up to 2^35.  Products take bf16 values as they are, fp32 values in 22 bits, an fp32 w next to bf16 x
- * in 11 (a bf16 copy has 8), each row of x and of w down to 2^-23 of its largest finite magnitude.  Rows with
+ * in 11 (a bf16 copy has 8), each row of x and of w down to 2^-23 of its largest finite magnitude; a finite bias beyond 2.3e38 in magnitude counts as that.  Rows with
  * target == ignore_index count for nothing, are not read, and cost no products; a target outside [0, V) makes its row's loss and
  * gradients NaN.  mean: divide by the rows that count (by 1 if there are none).
  * fwd: row_loss [N] (0 for ignored rows), loss (nullable, one float), pred [N] (nullable, lowest arg-max, 0 for ignored

@@ -796,3 +796,45 @@ def test_upstream_gradients_side_by_side(cuda, types, N, K, V, e):
     rows.backward(weight)
     check_each(types, x, w, b, t, rows.detach(), xg.grad, w.grad, b.grad, weight.double())
     assert not xg.grad[20].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("types", list(TYPES))
+@pytest.mark.parametrize("N,K,V", [(50, 64, 300), (70, 40, 128), (3, 8, 5)])
+def test_nothing_left_by_lowest_values(cuda, types, N, K, V):
+    """Every class at the type's lowest value: next to it no logit counts, the probabilities are all 1 / V; with a single class
+    beside it that one takes all, and a target among the masked ones has a finite loss."""
+    from video_classification_amd import ops
+    x, w, b, t = make(N, K, V, types, seed=18)
+    low = torch.finfo(b.dtype).min
+    x64, w64 = x.double(), w.detach().double()
+    at = torch.arange(N, device=cuda)
+    for spared in (None, 2):
+        with torch.no_grad():
+            b.fill_(low)
+            if spared is not None:
+                b[spared] = 0.25
+        w.grad = b.grad = None
+        xg = x.clone().requires_grad_(True)
+        stats = {}
+        rows = ops.linear_cross_entropy(xg, w, b, t, reduction="none", stats=stats)
+        rows.sum().backward()
+        p = torch.full((N, V), 1.0 / V, device=cuda, dtype=torch.float64)
+        if spared is None:
+            assert ((rows.double() - torch.log(torch.tensor(float(V)))).abs() <= 2.0 ** -20 * 6).all()
+        else:
+            p.zero_()
+            p[:, spared] = 1
+            masked = t != spared
+            assert torch.isfinite(rows).all() and (rows[masked] > 2e38).all() and (rows[~masked].abs() <= 2.0 ** -20).all()
+        assert (stats["pred"] == (0 if spared is None else spared)).all()
+        d = p.clone()
+        d[at, t] -= 1
+        off = 2.0 ** -20 * p
+        for got, want, A, M, P, dt, n in ((xg.grad, d @ w64, d.abs(), w64.abs(), off, xg.dtype, V),
+                                          (w.grad, d.t() @ x64, d.abs().t(), x64.abs(), off.t(), w.dtype, N)):
+            term = (2.0 ** -22 if dt == torch.float32 else FEW_ROWS) + 2.0 ** -21 + (3 * n / 32 + 8) * 2.0 ** -23
+            assert ((got.double() - want).abs() <= term * (A @ M) + P @ M + half(dt) * want.abs()).all()
+        assert ((b.grad.double() - d.sum(0)).abs() <= off.sum(0) + (N / 16 + 16) * U * d.abs().sum(0) + half(b.dtype) * d.sum(0).abs()).all()
+        with torch.no_grad():
+            assert torch.allclose(ops.linear_cross_entropy(x, w, b, t, reduction="none"), rows.detach(), rtol=1e-6, atol=1e-6)

@@ -222,6 +222,14 @@ __device__ __forceinline__ void pack_rows(const T* __restrict__ src, f16* __rest
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
+// bias log2(e); a finite one stays finite (a mask of the type's lowest value is no -inf: a row that it leaves nothing else
+// spreads its probability evenly)
+template <typename T>
+__device__ __forceinline__ float bias_log2(T b) {
+  const float v = to_f32(b) * LOG2E, most = 3.4028235e38f;
+  return fabsf(to_f32(b)) <= most ? fminf(fmaxf(v, -most), most) : v;
+}
+
 // exps[0] / [1] = scale exponents of x / W, [2] = rows that count, [3] / [4] = whether rows of x / W have their own; the first `xblocks` workgroups pack x, the others W and the bias: bl = bias
 // log2(e) over whole tiles of classes, -inf behind the last one, which leaves the epilogues of the products four plain
 // vector loads (clamped and converted there, these cost a fifth of a tile's time).
@@ -242,7 +250,7 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(const TX* __restrict__ x, 
   else {
     pack_rows(w, wp, (int64_t)V * ld, V, K, ld, pw, e, (const int*)nullptr, unit, wmax, ew, exps + 4);
     const int64_t v = (int64_t)(blockIdx.x - xblocks) * 256 + threadIdx.x;  // four rows or more per workgroup: all classes
-    if (v < (V + GM - 1) / GM * GM) bl[v] = v >= V ? -INFINITY : bias ? to_f32(bias[v]) * LOG2E : 0.f;
+    if (v < (V + GM - 1) / GM * GM) bl[v] = v >= V ? -INFINITY : bias ? bias_log2(bias[v]) : 0.f;
   }
 }
 
@@ -257,7 +265,7 @@ __global__ __launch_bounds__(256) void ce_copy_kernel(const bf16* __restrict__ x
                                                       const bf16* __restrict__ bias, float* __restrict__ bl) {
   if (blockIdx.x == 0 && threadIdx.x < 2) exps[threadIdx.x] = 0;
   const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
-  for (int64_t v = first; v < (V + GM - 1) / GM * GM; v += step) bl[v] = v >= V ? -INFINITY : bias ? to_f32(bias[v]) * LOG2E : 0.f;
+  for (int64_t v = first; v < (V + GM - 1) / GM * GM; v += step) bl[v] = v >= V ? -INFINITY : bias ? bias_log2(bias[v]) : 0.f;
   const int per = K / 8;
   const int64_t total = (int64_t)exps[2] * per;
   const bool vec = ((uintptr_t)x & 15) == 0;
