@@ -355,17 +355,18 @@ int vc_ce_fwd_bwd(int grad_dtype, const float* logits, int ld, const int64_t* ta
 /* Softmax cross entropy of a linear classifier z = x W^T + b without the logit matrix (the last nn.Linear of a decoder
  * and nn.CrossEntropyLoss in one, for label sets whose logits should not be kept; no counterpart in the reference).
  * x [N][K] (xdtype), w [V][K], bias [V] nullable, db [V], dw [V][K] (wdtype), dx [N][K] (xdtype); fp32 x needs fp32 w;
- * N and V up to 2^22, K up to 2^20, N V up to 2^38 and (N + V) K up to 2^35.  Products take bf16 values as they are, fp32 values in 22 bits, an fp32 w next to bf16 x
- * in 11 (a bf16 copy has 8), each row of x and of w down to 2^-23 of its largest finite magnitude; a finite bias beyond 2.3e38 in magnitude counts as that.  Rows with
- * target == ignore_index count for nothing, are not read, and cost no products; a target outside [0, V) makes its row's loss and
- * gradients NaN.  mean: divide by the rows that count (by 1 if there are none).
+ * N and V up to 2^22, K up to 2^20, N V up to 2^38 and (N + V) K up to 2^35.  Products take bf16 values as they are, fp32
+ * values in 22 bits, an fp32 w next to bf16 x in 11 (a bf16 copy has 8), each row of x and of w down to 2^-23 of its largest
+ * finite magnitude; a finite bias beyond 2.3e38 in magnitude counts as that.  Rows with target == ignore_index count for
+ * nothing, are not read, and cost no products; a target outside [0, V) makes its row's loss and gradients NaN.  mean: divide
+ * by the rows that count (by 1 if there are none).
  * fwd: row_loss [N] (0 for ignored rows), loss (nullable, one float), pred [N] (nullable, lowest arg-max, 0 for ignored
  *   rows) and correct (nullable).  saved: vc_linear_ce_bytes(0, ..) bytes that backward reads; workspace: vc_linear_ce_bytes(1, ..),
  *   or with saved = null, for a call without a backward pass, vc_linear_ce_bytes(4, ..).
  * bwd: dloss = upstream gradient of the mean or sum, or with per_row of every row's loss (a row's gradient is resolved to
  *   2^-24 of its own); dx, dw and db (each nullable) are written, or added to where bit 0 (dw) / bit 1 (db) of `accumulate` is
  *   set; workspace: vc_linear_ce_bytes(2, ..).
- * Buffers 256-byte aligned, contents of the workspaces irrelevant before and after; every sum has a fixed order. */
+ * saved and workspace 256-byte aligned, contents of the workspaces irrelevant before and after; every sum has a fixed order. */
 int64_t vc_linear_ce_bytes(int what, int xdtype, int wdtype, int N, int V, int K);
 int vc_linear_ce_fwd(int xdtype, int wdtype, const void* x, const void* w, const void* bias, const int64_t* target,
                      int64_t ignore_index, float smoothing, int mean, float* row_loss, float* loss, int64_t* pred,
