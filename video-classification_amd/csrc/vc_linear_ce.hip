@@ -10,8 +10,8 @@
 //
 // 2 N V K operations forward, 6 N V K backward (the logits once more, dx, dW): bound by the matrix pipes for the sizes where
 // time matters, which is why the logits are recomputed rather than kept: N x V fp32 logits written and read cost as much
-// as the product at K = 1024 and gigabytes of memory.  8192 x 1024 x 65536 in bf16: 4.39 ms forward and backward, 1.0 PFLOP/s
-// over its four products; 2048 x 512 x 20011 forward: 64 us, 54 of them the statistics (0.8 PFLOP/s).
+// as the product at K = 1024 and gigabytes of memory.  8192 x 1024 x 65536 in bf16: 4.4 - 4.7 ms forward and backward by
+// card, 1.0 PFLOP/s over its four products; 2048 x 512 x 20011 forward: 65 us, 54 of them the statistics (0.8 PFLOP/s).
 //
 // All products run on fp16 terms (vc_gemm16.h).  x and W are scaled by one power of two each (from their largest finite
 // magnitude), but for rows whose own largest value lies more than 16 binades below it, which are scaled by themselves: no row
@@ -52,14 +52,19 @@ __device__ __forceinline__ float amax_rows(const T* p, int64_t rows, int K, cons
     bool on[U];
     const T* row[U];
     float m[U];
+    const T* some = nullptr;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t r = first + lane / lanes + u * step;
       on[u] = r < rows && !(target && target[r] == ignore);
-      row[u] = p + (on[u] ? r * K : 0);  // row 0 in place of one that does not count: its values are dropped
+      row[u] = p + r * K;
+      if (on[u]) some = row[u];
       m[u] = 0.f;
     }
-    int k = k0;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (!on[u]) row[u] = some;  // another row in place of one that does not count, whose values are dropped
+    int k = some ? k0 : K;
     for (; k + 8 <= K; k += lanes * 8) {
       Row8<T> v[U];
 #pragma unroll
@@ -359,7 +364,7 @@ __device__ __forceinline__ void stat_join(Stat& a, const Stat& b) {
   a.m = m;
   a.z += b.z;
 }
-// 1.0 PFLOP/s at K = 1024 (1.08 ms for 8192 x 65536), 0.8 at K = 512, where eight k-steps carry the same epilogue: 64
+// 1.0 PFLOP/s at K = 1024 (1.08 - 1.16 ms for 8192 x 65536), 0.8 at K = 512, where eight k-steps carry the same epilogue: 64
 // exponentials a thread and the joins, the maximum first, so that they cost no exponentials of their own.
 //
 // part[vt][n] = (max, sum, sum z, arg) of the tile, zt[n] = the target's logit.  MORE: also sum z and arg (label smoothing,
@@ -611,7 +616,7 @@ __device__ __forceinline__ void bias_out(T* db, float s, const CeFac& fac, int a
   *db = from_f32<T>((add ? to_f32(*db) : 0.f) + Factor(fac.get(), -15)(s));  // of D_SCALE
 }
 
-// 8192 x 1024 against a piece of 8192 classes: 154 us, 0.89 PFLOP/s; the tile leaves through LDS in rows of 256 bytes.
+// 8192 x 1024 against a piece of 8192 classes: 154 - 166 us, 0.83 - 0.89 PFLOP/s; the tile leaves through LDS in rows of 256 bytes.
 //
 // One 128 x 128 tile of d for the classes [vbeg, vbeg + vcols), as dn[n][vcols] in PD terms scaled by 2^15, and its column
 // sums dbpart[tile n][v] (db itself where there is one row tile).
@@ -754,9 +759,9 @@ __host__ __device__ inline void slices(int tiles, int k, int& s, int& per) {
 }
 
 // out[m][c] = factor * sum over the reduction of (row side)[m] (column side)[c]: dx = d W and dW = d^T x.  Operands that lie
-// along the reduction the wrong way are read from LDS with transposing reads, so nothing is stored twice.  139 and 132 us
-// for a piece of 8192 classes of 8192 x 1024 (1.0 PFLOP/s); fp32 dW of bf16 rows, d in two terms: 94 us per piece of
-// 8192 classes at K = 768 and three quarters of 4096 rows.
+// along the reduction the wrong way are read from LDS with transposing reads, so nothing is stored twice.  137 - 147 and
+// 132 - 140 us by card for a piece of 8192 classes of 8192 x 1024 (1.0 PFLOP/s); fp32 dW of bf16 rows, d in two terms: 88 - 100 us
+// per piece of 8192 classes at K = 768 and three quarters of 4096 rows.
 struct MmArgs {
   Op16 c, m;                   // column side (W or x, COL) and row side (d: ROW for dx, COL for dW), at their corners
   int M, Nn, k;                // rows and columns of the result, reduction length of dx (a multiple of 64)
