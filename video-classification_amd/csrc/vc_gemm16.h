@@ -60,8 +60,9 @@ __device__ __forceinline__ i32x4_t g16_desc(const f16* p, unsigned bytes) {
 
 enum { ROW = 0, COL = 1 };
 
-// One operand of a tile.  ROW: p = the tile's first row, n = rows from there on.  COL: p = row 0 of the matrix, side = the
-// tile's first column, n = rows (the true length of the reduction).
+// One operand of a tile, of one row at least: an empty descriptor and the scalar offset of a k-step are not to meet, for the
+// range check may subtract one from the other.  ROW: p = the tile's first row, n = rows from there on.  COL: p = row 0 of the
+// matrix, side = the tile's first column, n = rows (the true length of the reduction).
 struct Op16 {
   const f16* p;
   int64_t plane;

@@ -316,8 +316,9 @@ __device__ __forceinline__ void logit_tile(const CeArgs& a, int v0, int n0, f16*
                                            f32x4 (&bias)[4], float& scale) {
   typedef G16<PW, PX, ROW, ROW, 4, BF> G;
   G::zero(acc);
-  G::run(acc, Op16{a.w + (int64_t)v0 * a.ld, (int64_t)a.V * a.ld, a.ld, a.V - v0, 0},
-         Op16{a.x + (int64_t)n0 * a.ld, (int64_t)a.N * a.ld, a.ld, a.rows() - n0, 0}, 0, (a.K + G::BK - 1) / G::BK * G::BK, smem);
+  if (a.rows() > n0)  // not where no row counts: G16 reads operands of one row at least
+    G::run(acc, Op16{a.w + (int64_t)v0 * a.ld, (int64_t)a.V * a.ld, a.ld, a.V - v0, 0},
+           Op16{a.x + (int64_t)n0 * a.ld, (int64_t)a.N * a.ld, a.ld, a.rows() - n0, 0}, 0, (a.K + G::BK - 1) / G::BK * G::BK, smem);
   const float* bl = a.bl + v0 + (threadIdx.x >> 7) * 64 + ((threadIdx.x & 63) >> 4) * 4;
 #pragma unroll
   for (int i = 0; i < 4; ++i) bias[i] = *reinterpret_cast<const f32x4*>(bl + i * 16);
@@ -858,7 +859,7 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
     m.side = m0;
     m.n = c.n = rows;
   }
-  if (!idle) {
+  if (!idle && rows > (KM == ROW ? m0 : 0)) {  // not where no row counts
     if (mm_own(g.fac, g.exps, g.which)) own_product<PC, PM, KM>(acc, c, m, g.own, KM == COL && g.fac.own() ? g.rs : nullptr, k0, k1);
     else G::run(acc, c, m, k0, k1, smem);
   }
