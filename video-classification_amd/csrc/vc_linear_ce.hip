@@ -235,8 +235,8 @@ __device__ __forceinline__ float bias_log2(T b) {
   return fabsf(to_f32(b)) <= most ? fminf(fmaxf(v, -most), most) : v;
 }
 
-// exps[0] / [1] = scale exponents of x / W, [2] = rows that count, [3] / [4] = whether rows of x / W have their own; the first `xblocks` workgroups pack x, the others W and the bias: bl = bias
-// log2(e) over whole tiles of classes, -inf behind the last one, which leaves the epilogues of the products four plain
+// exps[0] / [1] = scale exponents of x / W, [2] = rows that count, [3] / [4] = whether rows of x / W have their own; the first
+// `xblocks` workgroups pack x, the others W and the bias: bl = bias log2(e) over whole tiles of classes, -inf behind the last one, which leaves the epilogues of the products four plain
 // vector loads (clamped and converted there, these cost a fifth of a tile's time).
 template <typename TX, typename TW>
 __global__ __launch_bounds__(256) void ce_pack_kernel(const TX* __restrict__ x, const TW* __restrict__ w, int N, int V,
@@ -790,11 +790,12 @@ __device__ __forceinline__ Factor mm_factor(const CeFac& fac, const int* exps, i
 }
 
 // The product where the column side's scales, or for dW the rows' weights, differ along the reduction (some rows of x or of W, or
-// some upstream gradients, lie more than 2^16 below the largest): its values as they are, on the fp32 matrix instructions, whose range holds all of them.  Operands come straight
-// from memory: a step of 4096 x 768 x 16384 in bf16 takes 3.2 ms (rows) or 4.1 (classes) instead of 0.58; data with such rows
-// is not what training usually meets.
+// some upstream gradients, lie more than 2^16 below the largest): its values as they are, on the fp32 matrix instructions,
+// whose range holds all of them.  Operands come straight from memory: a step of 4096 x 768 x 16384 in bf16 takes 3.2 ms
+// (rows) or 4.1 (classes) instead of 0.58; data with such rows is not what training usually meets.
 template <int PC, int PM, int KM>
-__device__ __forceinline__ void own_product(f32x4 (&acc)[4][4], const Op16& c, const Op16& m, const int* own, const float* rs, int k0, int k1) {
+__device__ __forceinline__ void own_product(f32x4 (&acc)[4][4], const Op16& c, const Op16& m, const int* own, const float* rs,
+                                            int k0, int k1) {
   const int lane = threadIdx.x & 63, q = lane >> 4, l15 = lane & 15;
   const int wave = threadIdx.x >> 6, wc = wave >> 1, wr = wave & 1;
   for (int k = k0; k < k1; k += 4) {
@@ -1091,10 +1092,10 @@ int check_ce(const char* who, int xdtype, int wdtype, int N, int V, int K, float
   VC_CHECK_SHAPE(K <= (1 << 20) && N <= (1 << 22) && V <= (1 << 22), "%s: N, V or K too large (at most 2^22, 2^22, 2^20)",
                  who);
   // a launch holds fewer than 2^32 threads
-  VC_CHECK_SHAPE((int64_t)ceil_div(N, GM) * ceil_div(V, GM) < (1 << 24), "%s: %d rows against %d classes are more than 2^24 tiles of logits",
-                 who, N, V);
-  VC_CHECK_SHAPE(((int64_t)N + V) * ceil_div(K, 512) < (1 << 26) - 8, "%s: %d rows and %d classes of %d are more than 2^26 pieces of 512 to pack",
-                 who, N, V, K);
+  VC_CHECK_SHAPE((int64_t)ceil_div(N, GM) * ceil_div(V, GM) < (1 << 24),
+                 "%s: %d rows against %d classes are more than 2^24 tiles of logits", who, N, V);
+  VC_CHECK_SHAPE(((int64_t)N + V) * ceil_div(K, 512) < (1 << 26) - 8,
+                 "%s: %d rows and %d classes of %d are more than 2^26 pieces of 512 to pack", who, N, V, K);
   VC_CHECK_ARG(smooth >= 0.f && smooth <= 1.f, "%s: label smoothing %g outside [0, 1]", who, (double)smooth);
   return VC_OK;
 }
