@@ -236,8 +236,9 @@ __device__ __forceinline__ float bias_log2(T b) {
 }
 
 // exps[0] / [1] = scale exponents of x / W, [2] = rows that count, [3] / [4] = whether rows of x / W have their own; the first
-// `xblocks` workgroups pack x, the others W and the bias: bl = bias log2(e) over whole tiles of classes, -inf behind the last one, which leaves the epilogues of the products four plain
-// vector loads (clamped and converted there, these cost a fifth of a tile's time).
+// `xblocks` workgroups pack x, the others W and the bias: bl = bias log2(e) over whole tiles of classes, -inf behind the last
+// one, which leaves the epilogues of the products four plain vector loads (clamped and converted there, these cost a fifth of
+// a tile's time).
 template <typename TX, typename TW>
 __global__ __launch_bounds__(256) void ce_pack_kernel(const TX* __restrict__ x, const TW* __restrict__ w, int N, int V,
                                                       int K, int ld, int px, int pw, const int* __restrict__ order,
@@ -554,9 +555,9 @@ __global__ __launch_bounds__(1024) void ce_total_kernel(CeRows k, const float4* 
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------------
-// Per-row upstream gradients: rs[k] = weight of packed row k relative to the largest one, fac[0] = that largest weight, fac[1] = 0.
-// If a weight other than 0 lies more than 2^16 below the largest, rs[k] = the weight itself, fac[0] = fac[1] = 1: d is kept without
-// the weights, which dx takes on as it is written, and dW in its product.
+// Per-row upstream gradients: rs[k] = weight of packed row k relative to the largest one, fac[0] = that largest weight, fac[1] =
+// 0.  If a weight other than 0 lies more than 2^16 below the largest, rs[k] = the weight itself, fac[0] = fac[1] = 1: d is kept
+// without the weights, which dx takes on as it is written, and dW in its product.
 __global__ __launch_bounds__(1024) void ce_weights_kernel(const float* __restrict__ g, const int* __restrict__ order,
                                                           const int* __restrict__ exps, float* __restrict__ rs,
                                                           float* __restrict__ fac) {
@@ -861,7 +862,8 @@ __global__ __launch_bounds__(G_THREADS, 2) void ce_mm_kernel(MmArgs g) {
     m.n = c.n = rows;
   }
   if (!idle && rows > (KM == ROW ? m0 : 0)) {  // not where no row counts
-    if (mm_own(g.fac, g.exps, g.which)) own_product<PC, PM, KM>(acc, c, m, g.own, KM == COL && g.fac.own() ? g.rs : nullptr, k0, k1);
+    if (mm_own(g.fac, g.exps, g.which))
+      own_product<PC, PM, KM>(acc, c, m, g.own, KM == COL && g.fac.own() ? g.rs : nullptr, k0, k1);
     else G::run(acc, c, m, k0, k1, smem);
   }
   const int lane = threadIdx.x & 63, q = lane >> 4, l15 = lane & 15;
